@@ -21,7 +21,7 @@ ELA_ERR_INTERNAL = 5
 PATH_AUTO, PATH_CTA, PATH_GRID, PATH_CLUSTER = 0, 1, 2, 3
 TIE_HIGHEST_ROW, TIE_LOWEST_ROW = 0, 1  # ELA_TIE_*: election rule among bids within 1e-5
 
-# Every symbol include/ela_auction.h declares, with (restype, argtypes).
+# Every symbol include/ela_auction.h and include/ela_expert.h declare, with (restype, argtypes).
 _c = ctypes
 SIGNATURES = {
     "ela_auction_version": (_c.c_int, []),
@@ -53,6 +53,34 @@ SIGNATURES = {
     "ela_auction_compute_bids": (_c.c_int, [
         _c.c_void_p, _c.c_int, _c.c_int64, _c.c_int64, _c.c_int64, _c.c_int64, _c.c_int64, _c.c_void_p,
         _c.c_void_p, _c.c_double, _c.c_void_p, _c.c_void_p, _c.c_void_p]),
+    "ela_expert_plan_workspace_bytes": (_c.c_size_t, [_c.c_int64, _c.c_int64]),
+    "ela_expert_plan": (_c.c_int, [
+        _c.c_void_p, _c.c_int, _c.c_int64, _c.c_int64, _c.c_void_p, _c.c_void_p, _c.c_void_p, _c.c_void_p,
+        _c.c_size_t, _c.c_void_p]),
+    "ela_expert_dispatch": (_c.c_int, [
+        _c.c_void_p, _c.c_int, _c.c_int64, _c.c_int64, _c.c_int64, _c.c_int64, _c.c_void_p, _c.c_void_p, _c.c_int64,
+        _c.c_void_p, _c.c_void_p]),
+    "ela_expert_combine": (_c.c_int, [
+        _c.c_void_p, _c.c_int, _c.c_int64, _c.c_int64, _c.c_int64, _c.c_int64, _c.c_void_p, _c.c_void_p, _c.c_int64,
+        _c.c_void_p, _c.c_int, _c.c_void_p, _c.c_void_p]),
+    "ela_expert_combine_grad": (_c.c_int, [
+        _c.c_void_p, _c.c_void_p, _c.c_int, _c.c_int64, _c.c_int64, _c.c_int64, _c.c_int64, _c.c_int64, _c.c_void_p,
+        _c.c_void_p, _c.c_int64, _c.c_void_p, _c.c_int, _c.c_void_p, _c.c_void_p, _c.c_void_p]),
+    "ela_expert_linear_workspace_bytes": (_c.c_size_t, [
+        _c.c_int, _c.c_int64, _c.c_int64, _c.c_int64, _c.c_int64, _c.c_int]),
+    "ela_expert_linear": (_c.c_int, [
+        _c.c_void_p, _c.c_void_p, _c.c_void_p, _c.c_void_p, _c.c_void_p, _c.c_int, _c.c_int64, _c.c_int64, _c.c_int64,
+        _c.c_int64, _c.c_int64, _c.c_int64, _c.c_int64, _c.c_int64, _c.c_int, _c.c_void_p, _c.c_void_p, _c.c_void_p,
+        _c.c_size_t, _c.c_void_p]),
+    "ela_expert_linear_grad_act": (_c.c_int, [
+        _c.c_void_p, _c.c_void_p, _c.c_void_p, _c.c_int, _c.c_int64, _c.c_int64, _c.c_int64, _c.c_int, _c.c_void_p,
+        _c.c_void_p, _c.c_void_p, _c.c_size_t, _c.c_void_p]),
+    "ela_expert_linear_grad_input": (_c.c_int, [
+        _c.c_void_p, _c.c_void_p, _c.c_void_p, _c.c_int, _c.c_int64, _c.c_int64, _c.c_int64, _c.c_int64, _c.c_int64,
+        _c.c_int64, _c.c_void_p, _c.c_void_p, _c.c_size_t, _c.c_void_p]),
+    "ela_expert_linear_grad_weight": (_c.c_int, [
+        _c.c_void_p, _c.c_void_p, _c.c_void_p, _c.c_int, _c.c_int64, _c.c_int64, _c.c_int64, _c.c_int64, _c.c_int64,
+        _c.c_void_p, _c.c_void_p, _c.c_size_t, _c.c_void_p]),
     "ela_auction_set_wait_limit_ns": (None, [_c.c_uint64]),
     "ela_auction_debug_skip_arrive": (None, [_c.c_int]),
 }

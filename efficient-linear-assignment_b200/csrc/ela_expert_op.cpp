@@ -1,0 +1,388 @@
+// ela_expert_op.cpp -- the expert-layer operators as C++ torch operators over
+// the C ABI (include/ela_expert.h), with their autograd.
+//
+//   ela_native::expert_plan(expert, num_experts) -> (offsets, position, source)
+//   ela_native::expert_dispatch(x, position, offsets) -> rows
+//   ela_native::expert_combine(y, position, offsets, weights?) -> out
+//   ela_native::expert_linear(x, weight, bias?, residual?, offsets?, activation) -> y
+//
+// As in ela_torch_op.cpp: device guard, outputs and workspaces from the caching
+// allocator, the current stream, no synchronisation.  Autograd is here rather
+// than in Python because a small call is bound by host time.  The backward
+// passes launch kernels that autograd does not see, so asking for a gradient of
+// a gradient (create_graph) raises.
+#include <torch/library.h>
+#include <torch/csrc/autograd/custom_function.h>
+#include <ATen/ATen.h>
+#include <ATen/core/dispatch/Dispatcher.h>
+#include <c10/cuda/CUDAGuard.h>
+#include <c10/cuda/CUDAStream.h>
+
+#include <tuple>
+
+#include "ela_expert.h"
+
+namespace {
+
+using at::Tensor;
+using torch::autograd::AutogradContext;
+using torch::autograd::variable_list;
+typedef std::optional<Tensor> OptTensor;
+
+int code_of(const Tensor& t) {
+    switch (t.scalar_type()) {
+    case at::kFloat: return ELA_DTYPE_F32;
+    case at::kHalf: return ELA_DTYPE_F16;
+    case at::kBFloat16: return ELA_DTYPE_BF16;
+    default: return -1;
+    }
+}
+
+void check_rc(int rc, const char* where) {
+    TORCH_CHECK(rc == ELA_OK, where, ": ", ela_status_string(rc), " (status ", rc, ")");
+}
+
+void* stream_of(const Tensor& t) { return c10::cuda::getCurrentCUDAStream(t.device().index()).stream(); }
+const void* ptr(const OptTensor& t) { return t.has_value() ? t->data_ptr() : nullptr; }
+void* ptr(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
+
+// Unit stride inside a row; any (non-negative) distance between rows.
+Tensor rows_of(const Tensor& t) {
+    return (t.size(-1) <= 1 || t.stride(-1) == 1) && (t.size(0) <= 1 || t.stride(0) >= t.size(-1)) ? t : t.contiguous();
+}
+int64_t ld(const Tensor& t) { return t.size(0) > 1 ? t.stride(0) : t.size(-1); }
+
+Tensor workspace(size_t bytes, const Tensor& like) {
+    return bytes ? at::empty({(int64_t)bytes}, like.options().dtype(at::kByte)) : Tensor();
+}
+
+void no_second_derivative() {
+    TORCH_CHECK(!at::GradMode::is_enabled(), "the expert operators have no second derivative (create_graph=True)");
+}
+
+// ---- plan
+std::tuple<Tensor, Tensor, Tensor> plan(const Tensor& expert_in, int64_t E) {
+    TORCH_CHECK(expert_in.is_cuda(), "expert_plan needs a CUDA tensor (there is no CPU path)");
+    TORCH_CHECK(expert_in.scalar_type() == at::kInt || expert_in.scalar_type() == at::kLong, "expert must be int32 or int64");
+    c10::cuda::CUDAGuard guard(expert_in.device());
+    const Tensor expert = expert_in.contiguous();
+    const auto opt = expert.options().dtype(at::kInt);
+    Tensor offsets = at::empty({E + 1}, opt), source = at::empty({expert.numel()}, opt);
+    Tensor position = at::empty(expert.dim() == 1 ? at::IntArrayRef({expert.numel(), 1}) : expert.sizes(), opt);
+    const size_t bytes = ela_expert_plan_workspace_bytes(expert.numel(), E);
+    Tensor ws = workspace(bytes, expert);
+    check_rc(ela_expert_plan(expert.data_ptr(), (int)expert.element_size(), expert.numel(), E, offsets.data_ptr<int32_t>(),
+                             position.data_ptr<int32_t>(), source.data_ptr<int32_t>(), ptr(ws), bytes, stream_of(expert)),
+             "ela_expert_plan");
+    return {offsets, position, source};
+}
+
+void check_plan(const Tensor& like, const Tensor& position, const Tensor& offsets) {
+    TORCH_CHECK(position.scalar_type() == at::kInt && offsets.scalar_type() == at::kInt && position.dim() == 2 &&
+                    offsets.dim() == 1 && offsets.numel() >= 2 && position.is_contiguous() && offsets.is_contiguous() &&
+                    position.device() == like.device() && offsets.device() == like.device(),
+                "the plan's position (T,k) and offsets (E+1,) must be contiguous int32 on the rows' device");
+}
+
+// ---- dispatch and combine
+Tensor dispatch_raw(const Tensor& x_in, const Tensor& position, const Tensor& offsets) {
+    TORCH_CHECK(x_in.is_cuda(), "expert_dispatch needs a CUDA tensor (there is no CPU path)");
+    const int code = code_of(x_in);
+    TORCH_CHECK(code >= 0, "unsupported dtype ", x_in.scalar_type());
+    check_plan(x_in, position, offsets);
+    TORCH_CHECK(x_in.dim() == 2 && x_in.size(0) == position.size(0), "x must be (T, H) with the plan's T");
+    c10::cuda::CUDAGuard guard(x_in.device());
+    const Tensor x = rows_of(x_in);
+    Tensor rows = at::empty({position.numel(), x.size(1)}, x.options());
+    check_rc(ela_expert_dispatch(x.data_ptr(), code, x.size(0), position.size(1), x.size(1), ld(x),
+                                 position.data_ptr<int32_t>(), offsets.data_ptr<int32_t>(), offsets.numel() - 1,
+                                 rows.data_ptr(), stream_of(x)),
+             "ela_expert_dispatch");
+    return rows;
+}
+
+Tensor combine_raw(const Tensor& y_in, const Tensor& position, const Tensor& offsets, const OptTensor& weights) {
+    TORCH_CHECK(y_in.is_cuda(), "expert_combine needs a CUDA tensor (there is no CPU path)");
+    const int code = code_of(y_in);
+    TORCH_CHECK(code >= 0, "unsupported dtype ", y_in.scalar_type());
+    check_plan(y_in, position, offsets);
+    TORCH_CHECK(y_in.dim() == 2 && y_in.size(0) == position.numel(), "y must be (T*k, H)");
+    if (weights.has_value())
+        TORCH_CHECK(weights->sizes() == position.sizes() && weights->device() == y_in.device() &&
+                        (weights->scalar_type() == at::kFloat || weights->scalar_type() == y_in.scalar_type()),
+                    "weights must be (T, k), float32 or y's dtype");
+    c10::cuda::CUDAGuard guard(y_in.device());
+    const Tensor y = rows_of(y_in);
+    const OptTensor w = weights.has_value() ? OptTensor(weights->contiguous()) : OptTensor();
+    Tensor out = at::empty({position.size(0), y.size(1)}, y.options());
+    check_rc(ela_expert_combine(y.data_ptr(), code, position.size(0), position.size(1), y.size(1), ld(y),
+                                position.data_ptr<int32_t>(), offsets.data_ptr<int32_t>(), offsets.numel() - 1, ptr(w),
+                                w.has_value() ? code_of(*w) : ELA_DTYPE_F32, out.data_ptr(), stream_of(y)),
+             "ela_expert_combine");
+    return out;
+}
+
+// (dy, dweights); the one that is not needed comes back empty
+std::tuple<Tensor, Tensor> combine_grad_raw(const Tensor& dout_in, const OptTensor& y_in, const Tensor& position,
+                                            const Tensor& offsets, const OptTensor& weights, bool need_y, bool need_w) {
+    const Tensor dout = rows_of(dout_in);
+    const OptTensor y = y_in.has_value() ? OptTensor(rows_of(*y_in)) : OptTensor();
+    const OptTensor w = weights.has_value() ? OptTensor(weights->contiguous()) : OptTensor();
+    c10::cuda::CUDAGuard guard(dout.device());
+    Tensor dy = at::empty({need_y ? position.numel() : 0, dout.size(1)}, dout.options());
+    Tensor dw = need_w ? at::empty(position.sizes(), w->options()) : at::empty({0}, dout.options());
+    check_rc(ela_expert_combine_grad(dout.data_ptr(), ptr(y), code_of(dout), position.size(0), position.size(1),
+                                     dout.size(1), ld(dout), y.has_value() ? ld(*y) : 0, position.data_ptr<int32_t>(),
+                                     offsets.data_ptr<int32_t>(), offsets.numel() - 1, ptr(w),
+                                     w.has_value() ? code_of(*w) : ELA_DTYPE_F32, need_y ? dy.data_ptr() : nullptr,
+                                     need_w ? dw.data_ptr() : nullptr, stream_of(dout)),
+             "ela_expert_combine_grad");
+    return {dy, dw};
+}
+
+// ---- linear
+struct LinearSizes {
+    int64_t R, E, K, N;
+    Tensor x, w;  // unit stride inside rows
+    int64_t stride_e, ldw;
+};
+
+Tensor weight_rows(const Tensor& w) {
+    const Tensor v = w.dim() == 2 ? w.unsqueeze(0) : w;
+    const bool ok = (v.size(2) <= 1 || v.stride(2) == 1) && (v.size(1) <= 1 || v.stride(1) >= v.size(2)) &&
+                    (v.size(0) <= 1 || v.stride(0) >= 0);
+    return ok ? v : v.contiguous();
+}
+
+LinearSizes linear_sizes(const Tensor& x, const Tensor& weight, const OptTensor& bias, const OptTensor& residual,
+                         const OptTensor& offsets) {
+    TORCH_CHECK(x.is_cuda(), "expert_linear needs CUDA tensors (there is no CPU path)");
+    TORCH_CHECK(x.scalar_type() == at::kHalf || x.scalar_type() == at::kBFloat16, "x must be float16 or bfloat16");
+    TORCH_CHECK(x.dim() == 2 && (weight.dim() == 2 || weight.dim() == 3), "x must be (R, K), weight (E, N, K) or (N, K)");
+    LinearSizes s;
+    s.x = rows_of(x);
+    s.w = weight_rows(weight);
+    s.R = x.size(0);
+    s.E = s.w.size(0);
+    s.K = x.size(1);
+    s.N = s.w.size(1);
+    s.stride_e = s.E > 1 ? s.w.stride(0) : 0;
+    s.ldw = s.N > 1 ? s.w.stride(1) : s.K;
+    auto same = [&](const Tensor& t) { return t.scalar_type() == x.scalar_type() && t.device() == x.device(); };
+    TORCH_CHECK(s.w.size(2) == s.K && same(weight), "weight must be (E, N, K) or (N, K) in x's dtype and device");
+    if (bias.has_value()) TORCH_CHECK(bias->numel() == s.E * s.N && same(*bias), "bias must be (E, N) in x's dtype and device");
+    if (residual.has_value())
+        TORCH_CHECK(residual->dim() == 2 && residual->size(0) == s.R && residual->size(1) == s.N && same(*residual),
+                    "residual must be (R, N) in x's dtype and device");
+    if (offsets.has_value())
+        TORCH_CHECK(offsets->scalar_type() == at::kInt && offsets->is_contiguous() && offsets->numel() == s.E + 1 &&
+                        offsets->device() == x.device(), "offsets must be contiguous int32 (E+1,) on x's device");
+    TORCH_CHECK(offsets.has_value() || s.E == 1, "offsets are needed for more than one expert");
+    return s;
+}
+
+int aligned(const Tensor& t, int64_t ldt, int64_t stride_e = 0) {
+    const int64_t es = t.element_size();
+    return reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0 && ldt * es % 16 == 0 && stride_e * es % 16 == 0;
+}
+
+const int32_t* off_ptr(const OptTensor& o) { return o.has_value() ? o->data_ptr<int32_t>() : nullptr; }
+
+std::tuple<Tensor, Tensor> linear_raw(const Tensor& x, const Tensor& weight, const OptTensor& bias,
+                                      const OptTensor& residual, const OptTensor& offsets, int64_t act, bool want_z) {
+    c10::cuda::CUDAGuard guard(x.device());
+    const LinearSizes s = linear_sizes(x, weight, bias, residual, offsets);
+    const OptTensor b = bias.has_value() ? OptTensor(bias->contiguous()) : OptTensor();
+    const OptTensor r = residual.has_value() ? OptTensor(rows_of(*residual)) : OptTensor();
+    Tensor y = at::empty({s.R, s.N}, s.x.options());
+    Tensor z = at::empty({want_z ? s.R : 0, s.N}, s.x.options());  // rows of no expert stay unwritten
+    const int al = aligned(s.x, ld(s.x)) && aligned(s.w, s.ldw, s.stride_e);
+    const size_t bytes = ela_expert_linear_workspace_bytes(ELA_LINEAR_FORWARD, s.R, s.E, s.K, s.N, al);
+    Tensor ws = workspace(bytes, x);
+    check_rc(ela_expert_linear(s.x.data_ptr(), s.w.data_ptr(), ptr(b), ptr(r), off_ptr(offsets), code_of(x), s.R, s.E, s.K,
+                               s.N, ld(s.x), s.stride_e, s.ldw, r.has_value() ? ld(*r) : 0, (int)act, y.data_ptr(), want_z ? z.data_ptr() : nullptr,
+                               ptr(ws), bytes, stream_of(x)),
+             "ela_expert_linear");
+    return {y, z};
+}
+
+// The gradients asked for; the others come back empty.
+std::tuple<Tensor, Tensor, Tensor> linear_grad_raw(const Tensor& dy_in, const OptTensor& z, const OptTensor& x_in,
+                                                   const OptTensor& weight, const OptTensor& offsets, int64_t act,
+                                                   at::IntArrayRef wsizes, at::IntArrayRef bsizes, bool need_x,
+                                                   bool need_w, bool need_b) {
+    const Tensor dy = dy_in.contiguous();
+    c10::cuda::CUDAGuard guard(dy.device());
+    const int64_t R = dy.size(0), N = dy.size(1), K = wsizes.back(), E = wsizes.size() == 3 ? wsizes[0] : 1;
+    const int code = code_of(dy);
+    void* stream = stream_of(dy);
+    Tensor dx = at::empty({need_x ? R : 0, K}, dy.options());
+    Tensor dw = need_w ? at::empty(wsizes, dy.options()) : at::empty({0}, dy.options());
+    Tensor db = need_b ? at::empty(bsizes, dy.options()) : at::empty({0}, dy.options());
+    Tensor dz = dy;
+    if (need_b || act != ELA_ACT_NONE) {
+        const bool write = act != ELA_ACT_NONE && (need_x || need_w);
+        if (write) dz = at::empty_like(dy);
+        const size_t bytes = ela_expert_linear_workspace_bytes(ELA_LINEAR_GRAD_ACT, R, E, K, N, 1);
+        Tensor ws = workspace(bytes, dy);
+        check_rc(ela_expert_linear_grad_act(dy.data_ptr(), ptr(z), off_ptr(offsets), code, R, E, N, (int)act,
+                                            write ? dz.data_ptr() : nullptr, need_b ? db.data_ptr() : nullptr, ptr(ws),
+                                            bytes, stream),
+                 "ela_expert_linear_grad_act");
+    }
+    if (need_x) {
+        const Tensor w = weight_rows(*weight);
+        const int64_t se = E > 1 ? w.stride(0) : 0, ldw = N > 1 ? w.stride(1) : K;
+        const size_t bytes = ela_expert_linear_workspace_bytes(ELA_LINEAR_GRAD_INPUT, R, E, K, N,
+                                                               aligned(dz, N) && aligned(w, ldw, se));
+        Tensor ws = workspace(bytes, dy);
+        check_rc(ela_expert_linear_grad_input(dz.data_ptr(), w.data_ptr(), off_ptr(offsets), code, R, E, K, N, se, ldw,
+                                              dx.data_ptr(), ptr(ws), bytes, stream),
+                 "ela_expert_linear_grad_input");
+    }
+    if (need_w) {
+        const Tensor x = rows_of(*x_in);
+        const size_t bytes = ela_expert_linear_workspace_bytes(ELA_LINEAR_GRAD_WEIGHT, R, E, K, N,
+                                                               aligned(dz, N) && aligned(x, ld(x)));
+        Tensor ws = workspace(bytes, dy);
+        check_rc(ela_expert_linear_grad_weight(dz.data_ptr(), x.data_ptr(), off_ptr(offsets), code, R, E, K, N, ld(x),
+                                               dw.data_ptr(), ptr(ws), bytes, stream),
+                 "ela_expert_linear_grad_weight");
+    }
+    return {dx, dw, db};
+}
+
+Tensor linear_cuda(const Tensor& x, const Tensor& weight, const OptTensor& bias, const OptTensor& residual,
+                   const OptTensor& offsets, int64_t act) {
+    return std::get<0>(linear_raw(x, weight, bias, residual, offsets, act, false));
+}
+
+// ---- autograd: every pass is a registered operator, so that traced graphs see them
+template <typename F> auto op(const char* name) {
+    return c10::Dispatcher::singleton().findSchemaOrThrow(name, "").typed<F>();
+}
+OptTensor opt(const Tensor& t) { return t.defined() ? OptTensor(t) : OptTensor(); }
+Tensor given(const OptTensor& t) { return t.has_value() ? *t : Tensor(); }
+
+Tensor call_dispatch(const Tensor& x, const Tensor& position, const Tensor& offsets) {
+    static auto f = op<Tensor(const Tensor&, const Tensor&, const Tensor&)>("ela_native::expert_dispatch");
+    return f.call(x, position, offsets);
+}
+Tensor call_combine(const Tensor& y, const Tensor& position, const Tensor& offsets, const OptTensor& weights) {
+    static auto f = op<Tensor(const Tensor&, const Tensor&, const Tensor&, const OptTensor&)>("ela_native::expert_combine");
+    return f.call(y, position, offsets, weights);
+}
+
+struct Dispatch : torch::autograd::Function<Dispatch> {
+    static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& position, const Tensor& offsets) {
+        at::AutoDispatchBelowADInplaceOrView below;
+        ctx->save_for_backward({position, offsets});
+        return call_dispatch(x, position, offsets);
+    }
+    static variable_list backward(AutogradContext* ctx, variable_list grads) {
+        no_second_derivative();
+        const auto saved = ctx->get_saved_variables();
+        return {call_combine(grads[0], saved[0], saved[1], OptTensor()), Tensor(), Tensor()};
+    }
+};
+
+struct Combine : torch::autograd::Function<Combine> {
+    static Tensor forward(AutogradContext* ctx, const Tensor& y, const Tensor& position, const Tensor& offsets,
+                          const OptTensor& weights) {
+        const bool need_w = weights.has_value() && weights->requires_grad();
+        at::AutoDispatchBelowADInplaceOrView below;
+        ctx->save_for_backward({need_w ? y : Tensor(), position, offsets, given(weights)});
+        return call_combine(y, position, offsets, weights);
+    }
+    static variable_list backward(AutogradContext* ctx, variable_list grads) {
+        no_second_derivative();
+        static auto f = op<std::tuple<Tensor, Tensor>(const Tensor&, const OptTensor&, const Tensor&, const Tensor&,
+                                                      const OptTensor&, bool, bool)>("ela_native::expert_combine_grad");
+        const auto saved = ctx->get_saved_variables();
+        const bool need_y = ctx->needs_input_grad(0), need_w = saved[0].defined() && ctx->needs_input_grad(3);
+        auto g = f.call(grads[0], opt(saved[0]), saved[1], saved[2], opt(saved[3]), need_y, need_w);
+        return {need_y ? std::get<0>(g) : Tensor(), Tensor(), Tensor(), need_w ? std::get<1>(g) : Tensor()};
+    }
+};
+
+struct Linear : torch::autograd::Function<Linear> {
+    static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& weight, const OptTensor& bias,
+                          const OptTensor& residual, const OptTensor& offsets, int64_t act) {
+        static auto f = op<std::tuple<Tensor, Tensor>(const Tensor&, const Tensor&, const OptTensor&, const OptTensor&,
+                                                      const OptTensor&, int64_t, bool)>("ela_native::expert_linear_z");
+        const bool gx = x.requires_grad(), gw = weight.requires_grad(), gb = bias.has_value() && bias->requires_grad();
+        at::AutoDispatchBelowADInplaceOrView below;
+        const bool want_z = act != ELA_ACT_NONE && (gx || gw || gb);
+        auto out = f.call(x, weight, bias, residual, offsets, act, want_z);
+        ctx->save_for_backward({gw ? x : Tensor(), gx ? weight : Tensor(), want_z ? std::get<1>(out) : Tensor(),
+                                given(offsets)});
+        ctx->saved_data["act"] = act;
+        ctx->saved_data["residual"] = residual.has_value();
+        ctx->saved_data["wsizes"] = weight.sizes().vec();
+        ctx->saved_data["bsizes"] = bias.has_value() ? bias->sizes().vec() : std::vector<int64_t>{};
+        return std::get<0>(out);
+    }
+    static variable_list backward(AutogradContext* ctx, variable_list grads) {
+        no_second_derivative();
+        static auto f = op<std::tuple<Tensor, Tensor, Tensor>(const Tensor&, const OptTensor&, const OptTensor&,
+                                                              const OptTensor&, const OptTensor&, int64_t,
+                                                              at::IntArrayRef, at::IntArrayRef, bool, bool, bool)>(
+            "ela_native::expert_linear_grad");
+        const auto saved = ctx->get_saved_variables();
+        const auto wsizes = ctx->saved_data["wsizes"].toIntVector(), bsizes = ctx->saved_data["bsizes"].toIntVector();
+        const bool need_x = ctx->needs_input_grad(0), need_w = ctx->needs_input_grad(1),
+                   need_b = !bsizes.empty() && ctx->needs_input_grad(2);
+        const int residual_at = bsizes.empty() ? 2 : 3;  // an absent bias has no edge
+        variable_list out(6);
+        if (ctx->saved_data["residual"].toBool() && ctx->needs_input_grad(residual_at)) out[3] = grads[0];
+        if (!need_x && !need_w && !need_b) return out;
+        auto g = f.call(grads[0], opt(saved[2]), opt(saved[0]), opt(saved[1]), opt(saved[3]),
+                        ctx->saved_data["act"].toInt(), wsizes, bsizes, need_x, need_w, need_b);
+        if (need_x) out[0] = std::get<0>(g);
+        if (need_w) out[1] = std::get<1>(g);
+        if (need_b) out[2] = std::get<2>(g);
+        return out;
+    }
+};
+
+Tensor dispatch_autograd(const Tensor& x, const Tensor& position, const Tensor& offsets) {
+    return Dispatch::apply(x, position, offsets);
+}
+Tensor combine_autograd(const Tensor& y, const Tensor& position, const Tensor& offsets, const OptTensor& weights) {
+    return Combine::apply(y, position, offsets, weights);
+}
+Tensor linear_autograd(const Tensor& x, const Tensor& weight, const OptTensor& bias, const OptTensor& residual,
+                       const OptTensor& offsets, int64_t act) {
+    return Linear::apply(x, weight, bias, residual, offsets, act);
+}
+
+}  // namespace
+
+TORCH_LIBRARY_FRAGMENT(ela_native, m) {
+    m.def("expert_plan(Tensor expert, int num_experts) -> (Tensor, Tensor, Tensor)");
+    m.def("expert_dispatch(Tensor x, Tensor position, Tensor offsets) -> Tensor");
+    m.def("expert_combine(Tensor y, Tensor position, Tensor offsets, Tensor? weights) -> Tensor");
+    m.def("expert_combine_grad(Tensor dout, Tensor? y, Tensor position, Tensor offsets, Tensor? weights, "
+          "bool need_y, bool need_w) -> (Tensor, Tensor)");
+    m.def("expert_linear(Tensor x, Tensor weight, Tensor? bias, Tensor? residual, Tensor? offsets, int activation) -> Tensor");
+    m.def("expert_linear_z(Tensor x, Tensor weight, Tensor? bias, Tensor? residual, Tensor? offsets, int activation, "
+          "bool want_z) -> (Tensor, Tensor)");
+    m.def("expert_linear_grad(Tensor dy, Tensor? z, Tensor? x, Tensor? weight, Tensor? offsets, int activation, "
+          "int[] wsizes, int[] bsizes, bool need_x, bool need_w, bool need_b) -> (Tensor, Tensor, Tensor)");
+}
+
+TORCH_LIBRARY_IMPL(ela_native, CUDA, m) {
+    m.impl("expert_plan", &plan);
+    m.impl("expert_dispatch", &dispatch_raw);
+    m.impl("expert_combine", &combine_raw);
+    m.impl("expert_combine_grad", &combine_grad_raw);
+    m.impl("expert_linear", &linear_cuda);
+    m.impl("expert_linear_z", &linear_raw);
+    m.impl("expert_linear_grad", &linear_grad_raw);
+}
+
+TORCH_LIBRARY_IMPL(ela_native, AutogradCUDA, m) {
+    m.impl("expert_dispatch", &dispatch_autograd);
+    m.impl("expert_combine", &combine_autograd);
+    m.impl("expert_linear", &linear_autograd);
+}
