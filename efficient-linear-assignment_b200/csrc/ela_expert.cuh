@@ -20,11 +20,13 @@ template <> struct El<float> {
 };
 template <> struct El<__half> {
     static constexpr int W = 8;
+    static constexpr bool BF16 = false;
     static __device__ __forceinline__ float to(__half v) { return __half2float(v); }
     static __device__ __forceinline__ __half from(float v) { return __float2half_rn(v); }
 };
 template <> struct El<__nv_bfloat16> {
     static constexpr int W = 8;
+    static constexpr bool BF16 = true;
     static __device__ __forceinline__ float to(__nv_bfloat16 v) { return __bfloat162float(v); }
     static __device__ __forceinline__ __nv_bfloat16 from(float v) { return __float2bfloat16_rn(v); }
 };

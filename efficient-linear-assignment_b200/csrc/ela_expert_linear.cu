@@ -1,117 +1,58 @@
 // ela_expert_linear.cu -- the product with each expert's weights and its
 // gradient (include/ela_expert.h).
 //
-// Three products share one form, C[m,n] = sum_k A(m,k) B(n,k):
-//   forward       C = z  (rows x N):  A = x rows,  B = W_e rows,     sum over K
-//   input grad    C = dx (rows x K):  A = dz rows, B = W_e columns,  sum over N
-//   weight grad   C = dW_e (N x K):   A = dz columns, B = x columns, sum over the expert's rows
+// The three products (forward, input gradient, weight gradient) are one
+// tensor-core kernel, ela_expert_mma.cuh; here are their entry points, the copies
+// of operands that TMA cannot address, and the gradient of the activation with the
+// bias gradient.
 
 #include "ela_expert.cuh"
+#include "ela_expert_mma.cuh"
 
 namespace ela_expert {
 
-// ------------------------------------------------- the product, simple form
-// A 64 x 64 tile of C per CTA, fp32 sums in registers, operands of any stride
-// staged 16 deep in shared memory.
-#define ELA_TILE 64
-#define ELA_DEPTH 16
+constexpr unsigned long long LINEAR_WAIT_NS = 2000000000ull;  // limit of every device-side wait
 
-struct Operand {
+// Rows of any stride and alignment copied to rows a multiple of 16 bytes apart
+// (TMA's rule for strides and base).  Bits are moved, types do not matter.
+__global__ void __launch_bounds__(256) realign_kernel(const uint16_t* src, int64_t rows, int64_t cols, int64_t ld,
+                                                      int64_t rows_per_matrix, int64_t stride_e, uint16_t* dst, int64_t ldd) {
+    for (int64_t r = blockIdx.x; r < rows; r += gridDim.x) {
+        const uint16_t* s = src + r / rows_per_matrix * stride_e + r % rows_per_matrix * ld;
+        uint16_t* d = dst + r * ldd;
+        for (int64_t c = threadIdx.x; c < cols; c += blockDim.x) d[c] = s[c];
+    }
+}
+
+inline int64_t round8(int64_t n) { return (n + 7) / 8 * 8; }
+inline size_t round256(size_t n) { return (n + 255) / 256 * 256; }
+
+// A matrix operand: (matrices, rows, cols), 16-bit.
+struct Matrix {
     const void* p;
-    int64_t s_mn, s_k, s_e;  // distance along m (or n), along k, between experts
+    int64_t matrices, rows, cols, ld, stride_e;
+    size_t padded_bytes() const { return round256((size_t)(matrices * rows * round8(cols)) * 2); }
+    bool ok() const { return aligned16(p, ld * 2) && (matrices == 1 || stride_e * 2 % 16 == 0); }
 };
 
-template <typename T, int ACT>
-__device__ __forceinline__ void finish(float z, int64_t at, const T* bias, int64_t bias_at, const T* residual,
-                                       int64_t res_at, T* y, T* zout) {
-    if (bias) z += El<T>::to(bias[bias_at]);
-    if (zout) zout[at] = El<T>::from(z);
-    float v = act_value<ACT>(z);
-    if (residual) v += El<T>::to(residual[res_at]);
-    y[at] = El<T>::from(v);
+// The matrix itself where TMA can read it, else its copy in the workspace.
+inline int readable(Matrix& m, char*& ws, size_t& left, cudaStream_t st) {
+    if (m.ok()) return ELA_OK;
+    const size_t need = m.padded_bytes();
+    if (!ws || left < need) return ELA_ERR_ARGUMENT;
+    const int64_t rows = m.matrices * m.rows, ld = round8(m.cols);
+    realign_kernel<<<(unsigned)(rows < 4096 ? rows : 4096), 256, 0, st>>>((const uint16_t*)m.p, rows, m.cols, m.ld, m.rows, m.stride_e,
+                                                                         (uint16_t*)ws, ld);
+    m.p = ws;
+    m.ld = ld;
+    m.stride_e = m.rows * ld;
+    ws += need;
+    left -= need;
+    return launch_status();
 }
-
-// ROWS: C's rows are the expert's rows (forward, input grad); else the sum runs over them.
-template <typename T, int ACT, bool ROWS>
-__global__ void __launch_bounds__(256) simple_kernel(Operand A, Operand B, const int32_t* offsets, int R, int E, int M,
-                                                     int N, int K, const T* bias, const T* residual, int64_t ldr,
-                                                     T* C, T* zout) {
-    __shared__ float as[ELA_DEPTH][ELA_TILE + 1], bs[ELA_DEPTH][ELA_TILE + 1];
-    __shared__ int s_e, s_m;
-    int e, m0, r0, r1;
-    if (ROWS) {  // blockIdx.y counts the experts' row tiles
-        if (threadIdx.x == 0) {
-            int tile = blockIdx.y, f = 0, m = 0;
-            for (; f < E; ++f) {
-                int a, b;
-                expert_rows(offsets, f, R, a, b);
-                const int tiles = (b - a + ELA_TILE - 1) / ELA_TILE;
-                if (tile < tiles) { m = a + tile * ELA_TILE; break; }
-                tile -= tiles;
-            }
-            s_e = f;
-            s_m = m;
-        }
-        __syncthreads();
-        e = s_e;
-        m0 = s_m;
-        if (e >= E) return;
-        expert_rows(offsets, e, R, r0, r1);
-    } else {
-        e = blockIdx.z;
-        m0 = blockIdx.y * ELA_TILE;
-        expert_rows(offsets, e, R, r0, r1);
-    }
-    const int n0 = blockIdx.x * ELA_TILE;
-    const int m_end = ROWS ? r1 : M;
-    const int k_begin = ROWS ? 0 : r0, k_end = ROWS ? K : r1;
-    const T* a = reinterpret_cast<const T*>(A.p) + (int64_t)e * A.s_e;
-    const T* b = reinterpret_cast<const T*>(B.p) + (int64_t)e * B.s_e;
-    const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
-    float acc[4][4] = {};
-    for (int k0 = k_begin; k0 < k_end; k0 += ELA_DEPTH) {
-        for (int i = threadIdx.x; i < ELA_TILE * ELA_DEPTH; i += 256) {
-            const int mn = A.s_k == 1 ? i / ELA_DEPTH : i % ELA_TILE, k = A.s_k == 1 ? i % ELA_DEPTH : i / ELA_TILE;
-            as[k][mn] = m0 + mn < m_end && k0 + k < k_end ? El<T>::to(a[(m0 + mn) * A.s_mn + (k0 + k) * A.s_k]) : 0.f;
-        }
-        for (int i = threadIdx.x; i < ELA_TILE * ELA_DEPTH; i += 256) {
-            const int mn = B.s_k == 1 ? i / ELA_DEPTH : i % ELA_TILE, k = B.s_k == 1 ? i % ELA_DEPTH : i / ELA_TILE;
-            bs[k][mn] = n0 + mn < N && k0 + k < k_end ? El<T>::to(b[(n0 + mn) * B.s_mn + (k0 + k) * B.s_k]) : 0.f;
-        }
-        __syncthreads();
-#pragma unroll
-        for (int k = 0; k < ELA_DEPTH; ++k) {
-            float av[4], bv[4];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) { av[i] = as[k][ty * 4 + i]; bv[i] = bs[k][tx * 4 + i]; }
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-#pragma unroll
-                for (int j = 0; j < 4; ++j) acc[i][j] = fmaf(av[i], bv[j], acc[i][j]);
-        }
-        __syncthreads();
-    }
-    T* c = C + (ROWS ? 0 : (int64_t)e * M * N);
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const int m = m0 + ty * 4 + i, n = n0 + tx * 4 + j;
-            if (m < m_end && n < N)
-                finish<T, ACT>(acc[i][j], (int64_t)m * N + n, bias, (int64_t)e * N + n, residual, (int64_t)m * ldr + n, c, zout);
-        }
-}
-
-// Rows of no expert: the residual, or 0.
-template <typename T>
-__global__ void __launch_bounds__(256) rest_kernel(const int32_t* offsets, int E, int R, int N, const T* residual,
-                                                   int64_t ldr, T* y) {
-    const int first = clampi(offsets[0], 0, R), last = clampi(offsets[E], 0, R);
-    for (int r = blockIdx.x; r < R; r += gridDim.x) {
-        if (r >= first && r < last) { r = last - 1 - (last - 1 - r) % (int)gridDim.x; continue; }
-        for (int n = threadIdx.x; n < N; n += blockDim.x)
-            y[(int64_t)r * N + n] = residual ? residual[(int64_t)r * ldr + n] : El<T>::from(0.f);
-    }
+inline bool map_of(CUtensorMap* map, int dtype, const Matrix& m, int box_cols, int box_rows, bool three) {
+    const int64_t se = m.matrices > 1 ? m.stride_e : round8(m.ld * m.rows);
+    return make_map(map, dtype, m.p, m.cols, m.rows, m.matrices, m.ld, se, box_cols, box_rows, three ? 3 : 2);
 }
 
 // dz = dy * act'(z) and the bias gradient: a CTA owns 32 columns of an expert;
@@ -144,7 +85,28 @@ inline bool linear_sizes_ok(int dtype, int64_t R, int64_t E, int64_t K, int64_t 
     return (dtype == ELA_DTYPE_F16 || dtype == ELA_DTYPE_BF16) && R >= 0 && R <= (1ll << 30) && E >= 1 &&
            E <= ELA_EXPERT_MAX && K >= 1 && K <= (1ll << 30) && N >= 1 && N <= (1ll << 30) && (offsets || E == 1);
 }
-inline unsigned tiles(int64_t n) { return (unsigned)((n + ELA_TILE - 1) / ELA_TILE); }
+inline bool aligned8(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 7u) == 0; }
+
+// Parameters of a pass whose columns are the experts' rows: F features out, contraction length K.
+inline MmaParams row_pass(const int32_t* offsets, int64_t R, int64_t E, int64_t F, int64_t K) {
+    MmaParams p = {};
+    p.offsets = offsets;
+    p.R = (int)R; p.E = (int)E; p.F = (int)F; p.K = (int)K;
+    p.bn = columns_per_tile(R, E);
+    // boxes as tall as an expert's share of the rows, so that few rows do not load many
+    int64_t share = (R + E - 1) / E;
+    p.bbox = 16;
+    while (p.bbox < p.bn && p.bbox < share) p.bbox *= 2;
+    p.stages = stages_for(p.bn);
+    p.f_tiles = (int)((F + MMA_F - 1) / MMA_F);
+    p.wait_ns = LINEAR_WAIT_NS;
+    return p;
+}
+// At least as many tiles as the offsets can make.
+inline int64_t row_tiles(const MmaParams& p) {
+    const int64_t by_rows = p.R / p.bn + (p.E < p.R ? p.E : p.R);
+    return (by_rows > 0 ? by_rows : 1) * p.f_tiles;
+}
 
 #define ELA_BY_TYPE(dtype, ...)                               \
     if ((dtype) == ELA_DTYPE_F16) { typedef __half T_; __VA_ARGS__; } \
@@ -163,27 +125,48 @@ using namespace ela_expert;
 
 extern "C" {
 
-size_t ela_expert_linear_workspace_bytes(int, int64_t, int64_t, int64_t, int64_t, int) { return 0; }
+size_t ela_expert_linear_workspace_bytes(int pass, int64_t R, int64_t E, int64_t K, int64_t N, int aligned) {
+    if (aligned || pass == ELA_LINEAR_GRAD_ACT) return 0;
+    const Matrix x = {nullptr, 1, R, K, 0, 0}, w = {nullptr, E, N, K, 0, 0}, dz = {nullptr, 1, R, N, 0, 0};
+    return pass == ELA_LINEAR_FORWARD ? x.padded_bytes() + w.padded_bytes()
+         : pass == ELA_LINEAR_GRAD_INPUT ? dz.padded_bytes() + w.padded_bytes()
+                                         : dz.padded_bytes() + x.padded_bytes();
+}
+
+int ela_expert_status(int* status) {
+    if (!status) return ELA_ERR_ARGUMENT;
+    const int zero = ELA_OK;
+    if (cudaMemcpyFromSymbol(status, g_expert_error, sizeof(int)) != cudaSuccess) return ELA_ERR_CUDA;
+    if (*status != ELA_OK && cudaMemcpyToSymbol(g_expert_error, &zero, sizeof(int)) != cudaSuccess) return ELA_ERR_CUDA;
+    return ELA_OK;
+}
 
 int ela_expert_linear(const void* x, const void* weight, const void* bias, const void* residual,
                       const int32_t* offsets, int dtype, int64_t R, int64_t E, int64_t K, int64_t N, int64_t ldx,
-                      int64_t stride_e, int64_t ldw, int64_t ldr, int activation, void* y, void* z, void*, size_t,
-                      void* stream) {
+                      int64_t stride_e, int64_t ldw, int64_t ldr, int activation, void* y, void* z, void* workspace,
+                      size_t workspace_bytes, void* stream) {
     if (!linear_sizes_ok(dtype, R, E, K, N, offsets) || activation < 0 || activation > ELA_ACT_SILU || ldx < 0 ||
         stride_e < 0 || ldw < 0 || ldr < 0)
         return ELA_ERR_ARGUMENT;
     if (R == 0) return ELA_OK;
     if (!x || !weight || !y) return ELA_ERR_ARGUMENT;
     cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-    const Operand A = {x, ldx, 1, 0}, B = {weight, ldw, 1, stride_e};
-    const dim3 grid(tiles(N), tiles(R) + (unsigned)(E - 1));
-    ELA_BY_TYPE(dtype, {
-        if (offsets)
-            rest_kernel<T_><<<(unsigned)(R < 592 ? R : 592), 256, 0, st>>>(offsets, (int)E, (int)R, (int)N, (const T_*)residual, ldr, (T_*)y);
-        ELA_BY_ACT(activation, (simple_kernel<T_, A_, true><<<grid, 256, 0, st>>>(A, B, offsets, (int)R, (int)E, (int)R, (int)N, (int)K,
-                                (const T_*)bias, (const T_*)residual, ldr, (T_*)y, (T_*)z)))
-    })
-    return launch_status();
+    char* ws = reinterpret_cast<char*>(workspace);
+    Matrix mx = {x, 1, R, K, ldx, 0}, mw = {weight, E, N, K, ldw, stride_e};
+    int rc = readable(mx, ws, workspace_bytes, st);
+    if (rc == ELA_OK) rc = readable(mw, ws, workspace_bytes, st);
+    if (rc != ELA_OK) return rc;
+    MmaParams p = row_pass(offsets, R, E, N, K);
+    p.bias = bias;
+    p.residual = residual;
+    p.ldr = ldr;
+    p.out = y;
+    p.z = z;
+    p.vec = N % 4 == 0 && aligned8(y) && (!z || aligned8(z)) && (!residual || (aligned8(residual) && ldr % 4 == 0));
+    CUtensorMap a, b;
+    if (!map_of(&a, dtype, mw, MMA_KB, MMA_F, true) || !map_of(&b, dtype, mx, MMA_KB, p.bbox, false)) return ELA_ERR_CUDA;
+    ELA_BY_TYPE(dtype, { ELA_BY_ACT(activation, rc = (mma_launch<PASS_FORWARD, T_, A_>(a, b, p, row_tiles(p), st))) })
+    return rc;
 }
 
 int ela_expert_linear_grad_act(const void* dy, const void* z, const int32_t* offsets, int dtype, int64_t R,
@@ -202,36 +185,52 @@ int ela_expert_linear_grad_act(const void* dy, const void* z, const int32_t* off
 }
 
 int ela_expert_linear_grad_input(const void* dz, const void* weight, const int32_t* offsets, int dtype, int64_t R,
-                                 int64_t E, int64_t K, int64_t N, int64_t stride_e, int64_t ldw, void* dx, void*,
-                                 size_t, void* stream) {
+                                 int64_t E, int64_t K, int64_t N, int64_t stride_e, int64_t ldw, void* dx,
+                                 void* workspace, size_t workspace_bytes, void* stream) {
     if (!linear_sizes_ok(dtype, R, E, K, N, offsets) || stride_e < 0 || ldw < 0) return ELA_ERR_ARGUMENT;
     if (R == 0) return ELA_OK;
     if (!dz || !weight || !dx) return ELA_ERR_ARGUMENT;
     cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-    const Operand A = {dz, N, 1, 0}, B = {weight, 1, ldw, stride_e};
-    const dim3 grid(tiles(K), tiles(R) + (unsigned)(E - 1));
-    ELA_BY_TYPE(dtype, {
-        if (offsets)
-            rest_kernel<T_><<<(unsigned)(R < 592 ? R : 592), 256, 0, st>>>(offsets, (int)E, (int)R, (int)K, (const T_*)nullptr, 0, (T_*)dx);
-        simple_kernel<T_, ELA_ACT_NONE, true><<<grid, 256, 0, st>>>(A, B, offsets, (int)R, (int)E, (int)R, (int)K, (int)N,
-                                                                    (const T_*)nullptr, (const T_*)nullptr, 0, (T_*)dx, (T_*)nullptr);
-    })
-    return launch_status();
+    char* ws = reinterpret_cast<char*>(workspace);
+    Matrix mz = {dz, 1, R, N, N, 0}, mw = {weight, E, N, K, ldw, stride_e};
+    int rc = readable(mz, ws, workspace_bytes, st);
+    if (rc == ELA_OK) rc = readable(mw, ws, workspace_bytes, st);
+    if (rc != ELA_OK) return rc;
+    MmaParams p = row_pass(offsets, R, E, K, N);
+    p.out = dx;
+    p.vec = K % 4 == 0 && aligned8(dx);
+    CUtensorMap a, b;
+    if (!map_of(&a, dtype, mw, 64, MMA_KB, true) || !map_of(&b, dtype, mz, MMA_KB, p.bbox, false)) return ELA_ERR_CUDA;
+    ELA_BY_TYPE(dtype, { rc = (mma_launch<PASS_INPUT, T_, ELA_ACT_NONE>(a, b, p, row_tiles(p), st)); })
+    return rc;
 }
 
 int ela_expert_linear_grad_weight(const void* dz, const void* x, const int32_t* offsets, int dtype, int64_t R,
-                                  int64_t E, int64_t K, int64_t N, int64_t ldx, void* dweight, void*, size_t,
-                                  void* stream) {
+                                  int64_t E, int64_t K, int64_t N, int64_t ldx, void* dweight, void* workspace,
+                                  size_t workspace_bytes, void* stream) {
     if (!linear_sizes_ok(dtype, R, E, K, N, offsets) || ldx < 0) return ELA_ERR_ARGUMENT;
     if (!dweight || (R > 0 && (!dz || !x))) return ELA_ERR_ARGUMENT;
     cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-    const Operand A = {dz, 1, N, 0}, B = {x, 1, ldx, 0};
-    const dim3 grid(tiles(K), tiles(N), (unsigned)E);
-    ELA_BY_TYPE(dtype, {
-        simple_kernel<T_, ELA_ACT_NONE, false><<<grid, 256, 0, st>>>(A, B, offsets, (int)R, (int)E, (int)N, (int)K, (int)R,
-                                                                     (const T_*)nullptr, (const T_*)nullptr, 0, (T_*)dweight, (T_*)nullptr);
-    })
-    return launch_status();
+    if (R == 0) return cudaMemsetAsync(dweight, 0, (size_t)(E * N * K) * 2, st) == cudaSuccess ? ELA_OK : ELA_ERR_CUDA;
+    char* ws = reinterpret_cast<char*>(workspace);
+    Matrix mz = {dz, 1, R, N, N, 0}, mx = {x, 1, R, K, ldx, 0};
+    int rc = readable(mz, ws, workspace_bytes, st);
+    if (rc == ELA_OK) rc = readable(mx, ws, workspace_bytes, st);
+    if (rc != ELA_OK) return rc;
+    MmaParams p = {};
+    p.offsets = offsets;
+    p.R = (int)R; p.E = (int)E; p.F = (int)K; p.C = (int)N;
+    p.bn = MMA_C;
+    p.stages = stages_for(p.bn);
+    p.f_tiles = (int)((K + MMA_F - 1) / MMA_F);
+    p.c_tiles = (int)((N + MMA_C - 1) / MMA_C);
+    p.out = dweight;
+    p.vec = K % 4 == 0 && aligned8(dweight);
+    p.wait_ns = LINEAR_WAIT_NS;
+    CUtensorMap a, b;
+    if (!map_of(&a, dtype, mx, 64, MMA_KB, false) || !map_of(&b, dtype, mz, 64, MMA_KB, false)) return ELA_ERR_CUDA;
+    ELA_BY_TYPE(dtype, { rc = (mma_launch<PASS_WEIGHT, T_, ELA_ACT_NONE>(a, b, p, E * p.f_tiles * p.c_tiles, st)); })
+    return rc;
 }
 
 }  // extern "C"

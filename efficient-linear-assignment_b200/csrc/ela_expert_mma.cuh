@@ -1,0 +1,509 @@
+// ela_expert_mma.cuh -- the tensor-core product behind ela_expert_linear and its
+// gradients (included by ela_expert_linear.cu).
+//
+// One persistent kernel computes out[c][f] = sum_k A(f,k) B(c,k), f contiguous in
+// memory, in tiles of 128 features f by up to 256 columns c:
+//
+//   pass           f (128 TMEM lanes)     c (MMA N)            k
+//   forward        output feature n       row of the expert    input feature
+//   input grad     input feature          row of the expert    output feature
+//   weight grad    input feature          output feature       row of the expert
+//
+// The rows of an expert are the MMA's N side, whose extent is a multiple of 16
+// chosen per instruction: the last tile of an expert costs what its rows need, so
+// a generating step of a few rows and a long prompt run the same kernel, and the
+// weights, the side with whole tiles, fill the 128 lanes.
+//
+// Operands are K-major where k is contiguous in memory (x and W in the forward
+// pass, dz in the input gradient) and MN-major where it is not (W in the input
+// gradient, both sides of the weight gradient); both come as 128-byte-swizzled TMA
+// boxes, so no operand is ever transposed in memory.  Rows that belong to the next
+// expert are harmless on the N side (their columns are not stored); in the weight
+// gradient, where rows are summed over, the last block's rows past the expert are
+// zeroed in shared memory, on both sides, since 0 * NaN is not 0.
+//
+// Roles: warp 0 issues the TMA loads, warp 1 the MMAs, warp 2 owns the TMEM
+// allocation, warps 4-7 run the epilogue while the next tile's MMAs fill the other
+// half of TMEM (2 x 256 columns).  The epilogue stages 32 columns at a time in
+// shared memory to turn "thread = feature" into rows of 128 consecutive features:
+// bias, activation and residual are applied there in fp32, and a warp stores one
+// row's 256 bytes at once.
+#pragma once
+
+#include <cuda.h>
+#include <cudaTypedefs.h>
+
+#include "ela_expert.cuh"
+
+namespace ela_expert {
+
+enum { PASS_FORWARD = 0, PASS_INPUT = 1, PASS_WEIGHT = 2 };
+
+constexpr int MMA_F = 128;              // features per tile (TMEM lanes)
+constexpr int MMA_C = 256;              // most columns per tile
+constexpr int MMA_KB = 64;              // k per stage: 128 bytes, one swizzle span
+constexpr int MMA_A_BYTES = MMA_F * MMA_KB * 2;
+constexpr int MMA_STAGING = 32 * MMA_F * 4;  // one chunk of 32 columns, fp32
+constexpr int MMA_MAX_STAGES = 10;
+constexpr int MMA_THREADS = 256;
+constexpr int MMA_SMEM = 227 * 1024;
+constexpr int MMA_SMEM_FIXED = 2 * MMA_STAGING + 1024;  // staging, alignment of the first stage
+constexpr int MMA_GROUP = 16;           // column tiles walked together, for L2 reuse of both operands
+
+struct MmaParams {
+    const int32_t* offsets;
+    int R, E, F, C, K;      // C: columns of the weight gradient; K: contraction length of the row passes
+    int bn, bbox, stages;   // columns per tile; rows per TMA box of the column operand; pipeline depth
+    int f_tiles, c_tiles;   // c_tiles: weight gradient only
+    int vec;                // 4 features at a time may be loaded and stored together
+    const void* bias;
+    const void* residual;
+    int64_t ldr;
+    void* out;
+    void* z;
+    unsigned long long wait_ns;
+};
+
+// Sticky error of the kernels below (a wait that ran out), read by ela_expert_status.
+__device__ int g_expert_error;
+
+// ------------------------------------------------------------- PTX wrappers
+__device__ __forceinline__ uint32_t saddr(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
+__device__ __forceinline__ void bar_init(uint64_t* b, int count) {
+    asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(saddr(b)), "r"(count) : "memory");
+}
+__device__ __forceinline__ void bar_expect(uint64_t* b, uint32_t bytes) {
+    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(saddr(b)), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void bar_arrive(uint64_t* b) {
+    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(saddr(b)) : "memory");
+}
+// Bounded wait for the phase of this parity; false when the limit ran out or another role gave up.
+__device__ __forceinline__ bool bar_wait(uint64_t* b, uint32_t parity, unsigned long long limit_ns,
+                                         const volatile int* abort) {
+    const uint32_t a = saddr(b);
+    unsigned long long t0 = 0;
+    for (uint32_t spins = 1;; ++spins) {
+        uint32_t done;
+        asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+                     : "=r"(done) : "r"(a), "r"(parity) : "memory");
+        if (done) return true;
+        if ((spins & 15u) == 0) {
+            unsigned long long t;
+            asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));
+            if (t0 == 0) t0 = t;
+            if (*abort || t - t0 > limit_ns) return false;
+        }
+    }
+}
+// The same for a whole warp: one lane polls, all get its answer.
+__device__ __forceinline__ bool warp_wait(uint64_t* b, uint32_t parity, unsigned long long limit_ns,
+                                          const volatile int* abort) {
+    int ok = 0;
+    if ((threadIdx.x & 31) == 0) ok = bar_wait(b, parity, limit_ns, abort);
+    ok = __shfl_sync(~0u, ok, 0);
+    __syncwarp();
+    return ok;
+}
+__device__ __forceinline__ void tma_2d(void* dst, const CUtensorMap* map, int x, int y, uint64_t* bar) {
+    asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];"
+                 ::"r"(saddr(dst)), "l"(map), "r"(saddr(bar)), "r"(x), "r"(y) : "memory");
+}
+__device__ __forceinline__ void tma_3d(void* dst, const CUtensorMap* map, int x, int y, int z, uint64_t* bar) {
+    asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];"
+                 ::"r"(saddr(dst)), "l"(map), "r"(saddr(bar)), "r"(x), "r"(y), "r"(z) : "memory");
+}
+__device__ __forceinline__ void mma_commit(uint64_t* b) {
+    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(saddr(b)) : "memory");
+}
+__device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void mma_issue(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool accumulate) {
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+                 "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
+                 ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"((uint32_t)accumulate) : "memory");
+}
+__device__ __forceinline__ void tmem_ld32(uint32_t addr, float* v) {
+    uint32_t* r = reinterpret_cast<uint32_t*>(v);
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+                 "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+                   "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
+                   "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]),
+                   "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+                 : "r"(addr));
+    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+}
+
+// Shared-memory operand descriptors, 128-byte swizzle (layout type 2, version 1).
+// K-major: 8-row groups 1024 bytes apart; the k steps of 16 advance the start by 32 bytes.
+// MN-major: blocks of 64 along MN 8192 bytes apart (one TMA box each), groups of 8
+// along k 1024 bytes apart; the k steps of 16 advance the start by 2048 bytes.
+__device__ __forceinline__ uint64_t operand_desc(uint32_t addr, bool k_major) {
+    const uint64_t lead = k_major ? 1 : 8192 >> 4, stride = 1024 >> 4;
+    return (uint64_t)((addr >> 4) & 0x3fff) | (lead << 16) | (stride << 32) | (1ull << 46) | (2ull << 61);
+}
+template <typename T> __device__ __forceinline__ uint32_t instr_desc(int n, bool a_k_major, bool b_k_major) {
+    const uint32_t ab = sizeof(T) == 2 && El<T>::BF16 ? 1u : 0u;
+    return (1u << 4) | (ab << 7) | (ab << 10) | ((a_k_major ? 0u : 1u) << 15) | ((b_k_major ? 0u : 1u) << 16) |
+           ((uint32_t)(n >> 3) << 17) | ((uint32_t)(MMA_F >> 4) << 24);
+}
+
+// ------------------------------------------------------------- tile order
+struct Tile {
+    int e, f0, c0, nc;  // expert, first feature, first column, columns
+    int k0, nk;         // contraction range (weight gradient: the expert's rows)
+};
+
+// Tile number -> tile.  Row passes: experts in order; within an expert, groups of
+// MMA_GROUP column tiles, feature tiles within a group, columns innermost.  The
+// number of tiles depends on the offsets, which only the device knows, so every
+// role walks them by itself, 32 experts at a time (one a lane; the whole warp calls).
+template <int PASS> struct Order {
+    const MmaParams& p;
+    int block, first, last, tiles, incl, before;
+    __device__ __forceinline__ explicit Order(const MmaParams& q) : p(q), block(0), before(0) { if (PASS != PASS_WEIGHT) load(); }
+    __device__ __forceinline__ void load() {
+        const int lane = threadIdx.x & 31, e = block + lane;
+        first = last = 0;
+        if (e < p.E) expert_rows(p.offsets, e, p.R, first, last);
+        tiles = (last - first + p.bn - 1) / p.bn * p.f_tiles;
+        incl = tiles;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int v = __shfl_up_sync(~0u, incl, o);
+            if (lane >= o) incl += v;
+        }
+    }
+    __device__ __forceinline__ bool get(int t, Tile& out) {
+        if constexpr (PASS == PASS_WEIGHT) {
+            const int per = p.f_tiles * p.c_tiles;
+            out.e = t / per;
+            if (out.e >= p.E) return false;
+            int local = t % per;
+            const int group = local / (MMA_GROUP * p.f_tiles), g = min(MMA_GROUP, p.c_tiles - group * MMA_GROUP);
+            local -= group * MMA_GROUP * p.f_tiles;
+            out.f0 = local / g * MMA_F;
+            out.c0 = (group * MMA_GROUP + local % g) * MMA_C;
+            out.nc = min(MMA_C, p.C - out.c0);
+            int r0, r1;
+            expert_rows(p.offsets, out.e, p.R, r0, r1);
+            out.k0 = r0;
+            out.nk = r1 - r0;
+            return true;
+        } else {
+            while (t >= before + __shfl_sync(~0u, incl, 31)) {
+                before += __shfl_sync(~0u, incl, 31);
+                block += 32;
+                if (block >= p.E) return false;
+                load();
+            }
+            const int l = __ffs(__ballot_sync(~0u, before + incl > t)) - 1;
+            int local = t - before - __shfl_sync(~0u, incl - tiles, l);
+            const int r0 = __shfl_sync(~0u, first, l), r1 = __shfl_sync(~0u, last, l);
+            const int ct = (r1 - r0 + p.bn - 1) / p.bn;
+            const int group = local / (MMA_GROUP * p.f_tiles), g = min(MMA_GROUP, ct - group * MMA_GROUP);
+            local -= group * MMA_GROUP * p.f_tiles;
+            out.e = block + l;
+            out.f0 = local / g * MMA_F;
+            out.c0 = r0 + (group * MMA_GROUP + local % g) * p.bn;
+            out.nc = min(p.bn, r1 - out.c0);
+            out.k0 = 0;
+            out.nk = p.K;
+            return true;
+        }
+    }
+};
+
+// ------------------------------------------------------------- epilogue
+// Four consecutive features of one column: z = v + bias, y = act(z) + residual.
+template <typename T, int ACT>
+__device__ __forceinline__ void finish4(float4 v, const float* bias, const MmaParams& p, int64_t c, int f) {
+    T* out = reinterpret_cast<T*>(p.out) + c * p.F + f;
+    T* zout = p.z ? reinterpret_cast<T*>(p.z) + c * p.F + f : nullptr;
+    const T* res = p.residual ? reinterpret_cast<const T*>(p.residual) + c * p.ldr + f : nullptr;
+    float q[4] = {v.x + bias[0], v.y + bias[1], v.z + bias[2], v.w + bias[3]};
+    struct alignas(8) T4 { T v[4]; } o;
+    if (p.vec) {
+        if (zout) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) o.v[i] = El<T>::from(q[i]);
+            *reinterpret_cast<T4*>(zout) = o;
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) q[i] = act_value<ACT>(q[i]);
+        if (res) {
+            const T4 r = *reinterpret_cast<const T4*>(res);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) q[i] += El<T>::to(r.v[i]);
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) o.v[i] = El<T>::from(q[i]);
+        *reinterpret_cast<T4*>(out) = o;
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            if (f + i < p.F) {
+                if (zout) zout[i] = El<T>::from(q[i]);
+                out[i] = El<T>::from(act_value<ACT>(q[i]) + (res ? El<T>::to(res[i]) : 0.f));
+            }
+    }
+}
+
+template <int PASS, typename T, int ACT>
+__global__ void __launch_bounds__(MMA_THREADS, 1) mma_kernel(const __grid_constant__ CUtensorMap map_a,
+                                                             const __grid_constant__ CUtensorMap map_b,
+                                                             const MmaParams p) {
+    constexpr bool A_K_MAJOR = PASS == PASS_FORWARD, B_K_MAJOR = PASS != PASS_WEIGHT;
+    extern __shared__ unsigned char smem_raw[];
+    __shared__ __align__(8) uint64_t full[MMA_MAX_STAGES], empty[MMA_MAX_STAGES], tfull[2], tempty[2], drained;
+    __shared__ uint32_t s_tmem;
+    __shared__ int s_abort;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
+    const int stage_bytes = MMA_A_BYTES + p.bn * MMA_KB * 2;
+    float* staging = reinterpret_cast<float*>(smem + (size_t)p.stages * stage_bytes);
+    const volatile int* abort = &s_abort;
+
+    if (warp == 2) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(saddr(&s_tmem)) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    if (tid == 0) {
+        s_abort = 0;
+        for (int s = 0; s < p.stages; ++s) { bar_init(&full[s], 1); bar_init(&empty[s], 1); }
+        for (int b = 0; b < 2; ++b) { bar_init(&tfull[b], 1); bar_init(&tempty[b], 4); }
+        bar_init(&drained, 1);
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    fence_before();
+    __syncthreads();
+    fence_after();
+    const uint32_t tmem = s_tmem;
+    auto give_up = [&]() {
+        *(volatile int*)&s_abort = 1;
+        atomicExch(&g_expert_error, ELA_ERR_TIMEOUT);
+    };
+
+    uint32_t issued = 0;  // stages loaded (thread 0)
+    if (warp == 0) {  // ---- loads
+        Order<PASS> order(p);
+        Tile t;
+        int s = 0;
+        uint32_t phase = 0;
+        bool ok = true;
+        for (int n = blockIdx.x; ok && order.get(n, t); n += gridDim.x) {
+            const int blocks = (t.nk + MMA_KB - 1) / MMA_KB;
+            // column operand: boxes of p.bbox rows (K-major) or of 64 columns (MN-major)
+            const int nc16 = (t.nc + 15) & ~15;
+            const int boxes = B_K_MAJOR ? (nc16 + p.bbox - 1) / p.bbox : (nc16 + 63) / 64;
+            const int box_bytes = B_K_MAJOR ? p.bbox * MMA_KB * 2 : 64 * MMA_KB * 2;
+            for (int kb = 0; kb < blocks && ok; ++kb) {
+                if (lane == 0) {
+                    ok = bar_wait(&empty[s], phase ^ 1, p.wait_ns, abort);
+                    if (ok) {
+                        unsigned char* a = smem + (size_t)s * stage_bytes;
+                        unsigned char* b = a + MMA_A_BYTES;
+                        const int k = t.k0 + kb * MMA_KB;
+                        bar_expect(&full[s], MMA_A_BYTES + boxes * box_bytes);
+                        if (PASS == PASS_FORWARD) {
+                            tma_3d(a, &map_a, k, t.f0, t.e, &full[s]);
+                        } else {
+                            for (int h = 0; h < 2; ++h)
+                                if (PASS == PASS_INPUT) tma_3d(a + h * 8192, &map_a, t.f0 + h * 64, k, t.e, &full[s]);
+                                else tma_2d(a + h * 8192, &map_a, t.f0 + h * 64, k, &full[s]);
+                        }
+                        for (int i = 0; i < boxes; ++i)
+                            if (B_K_MAJOR) tma_2d(b + i * box_bytes, &map_b, k, t.c0 + i * p.bbox, &full[s]);
+                            else tma_2d(b + i * box_bytes, &map_b, t.c0 + i * 64, k, &full[s]);
+                        ++issued;
+                    } else {
+                        give_up();
+                    }
+                }
+                ok = __shfl_sync(~0u, (int)ok, 0);
+                if (++s == p.stages) { s = 0; phase ^= 1; }
+            }
+        }
+    } else if (warp == 1) {  // ---- products
+        Order<PASS> order(p);
+        Tile t;
+        int s = 0, it = 0;
+        uint32_t phase = 0;
+        bool ok = true;
+        for (int n = blockIdx.x; ok && order.get(n, t); n += gridDim.x) {
+            const int blocks = (t.nk + MMA_KB - 1) / MMA_KB;
+            if (blocks == 0) continue;  // an expert without rows: the epilogue writes its zeros
+            const int half = it & 1;
+            const uint32_t d = tmem + half * MMA_C;
+            const uint32_t idesc = instr_desc<T>((t.nc + 15) & ~15, A_K_MAJOR, B_K_MAJOR);
+            ok = warp_wait(&tempty[half], ((it >> 1) & 1) ^ 1, p.wait_ns, abort);
+            for (int kb = 0; kb < blocks && ok; ++kb) {
+                ok = warp_wait(&full[s], phase, p.wait_ns, abort);
+                if (!ok) break;
+                fence_after();
+                unsigned char* a = smem + (size_t)s * stage_bytes;
+                const int left = t.nk - kb * MMA_KB;
+                const int steps = left >= MMA_KB ? 4 : (left + 15) >> 4;
+                if (PASS == PASS_WEIGHT && left < steps * 16) {  // rows of the next expert: zeros
+                    const int c_boxes = (((t.nc + 15) & ~15) + 63) / 64, pieces = (steps * 16 - left) * 8;
+                    for (int i = lane; i < (2 + c_boxes) * pieces; i += 32) {
+                        const int box = i / pieces, r = i % pieces;  // A's two boxes, then B's, 8192 bytes each
+                        *reinterpret_cast<uint4*>(a + (size_t)box * 8192 + left * 128 + r * 16) = make_uint4(0, 0, 0, 0);
+                    }
+                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                    __syncwarp();
+                }
+                if (lane == 0) {
+                    const uint64_t ad = operand_desc(saddr(a), A_K_MAJOR), bd = operand_desc(saddr(a) + MMA_A_BYTES, B_K_MAJOR);
+                    for (int j = 0; j < steps; ++j)
+                        mma_issue(d, ad + j * (A_K_MAJOR ? 2 : 128), bd + j * (B_K_MAJOR ? 2 : 128), idesc, kb + j > 0);
+                    mma_commit(&empty[s]);
+                    if (kb == blocks - 1) mma_commit(&tfull[half]);
+                }
+                __syncwarp();
+                if (++s == p.stages) { s = 0; phase ^= 1; }
+            }
+            ++it;
+        }
+        if (!ok && lane == 0) give_up();
+    } else if (warp >= 4) {  // ---- epilogue
+        const int w = warp - 4, et = tid - 128;
+        if (PASS != PASS_WEIGHT && p.offsets) {  // rows of no expert: the residual, or 0
+            const int lo = clampi(p.offsets[0], 0, p.R), hi = clampi(p.offsets[p.E], 0, p.R);
+            for (int r = blockIdx.x; r < p.R; r += gridDim.x) {
+                if (r >= lo && r < hi) { r = hi - 1 - (hi - 1 - r) % (int)gridDim.x; continue; }
+                for (int f = et; f < p.F; f += 128)
+                    reinterpret_cast<T*>(p.out)[(int64_t)r * p.F + f] =
+                        p.residual ? reinterpret_cast<const T*>(p.residual)[r * p.ldr + f] : El<T>::from(0.f);
+            }
+        }
+        Order<PASS> order(p);
+        Tile t;
+        int it = 0;
+        for (int n = blockIdx.x; order.get(n, t); n += gridDim.x) {
+            const bool product = t.nk > 0;
+            const int half = it & 1;
+            if (product) {
+                // all four warps go on or give up together: they share barriers below
+                const int ok = bar_wait(&tfull[half], (it >> 1) & 1, p.wait_ns, abort);
+                int all;
+                asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %1, 0;\n\tbarrier.cta.red.and.pred q, 1, 128, p;\n\t"
+                             "selp.b32 %0, 1, 0, q;\n\t}" : "=r"(all) : "r"(ok) : "memory");
+                if (!all) { give_up(); break; }
+                fence_after();
+            }
+            const int f = t.f0 + 4 * lane;
+            float bias[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                bias[i] = PASS == PASS_FORWARD && p.bias && f + i < p.F
+                              ? El<T>::to(reinterpret_cast<const T*>(p.bias)[(int64_t)t.e * p.F + f + i]) : 0.f;
+            const int64_t c_base = PASS == PASS_WEIGHT ? (int64_t)t.e * p.C + t.c0 : t.c0;
+            for (int c = 0; c < t.nc; c += 32) {
+                float* st = staging + ((c >> 5) & 1) * (32 * MMA_F);
+                if (product) {
+                    float v[32];
+                    __syncwarp();
+                    tmem_ld32(tmem + ((uint32_t)(32 * w) << 16) + half * MMA_C + c, v);
+                    if (c + 32 >= t.nc) {  // the accumulator's half is free for the tile after next
+                        fence_before();
+                        __syncwarp();
+                        if (lane == 0) bar_arrive(&tempty[half]);
+                    }
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) st[i * MMA_F + 32 * w + lane] = v[i];
+                    asm volatile("barrier.cta.sync 1, 128;" ::: "memory");
+                }
+                for (int i = w; i < 32 && c + i < t.nc; i += 4) {
+                    const float4 v = product ? *reinterpret_cast<const float4*>(st + i * MMA_F + 4 * lane) : make_float4(0, 0, 0, 0);
+                    if (f < p.F) finish4<T, ACT>(v, bias, p, c_base + c + i, f);
+                }
+            }
+            // the next tile's first chunk reuses a staging buffer: all reads are done
+            if (product) asm volatile("barrier.cta.sync 1, 128;" ::: "memory");
+            it += product;
+        }
+    }
+    __syncthreads();
+    if (s_abort) {  // loads and products in flight end before the CTA gives back its memory
+        int never = 0;
+        if (tid == 0) {
+            const uint32_t last = issued < (uint32_t)p.stages ? issued : p.stages;
+            for (uint32_t i = issued - last; i < issued; ++i)
+                bar_wait(&full[i % p.stages], (i / p.stages) & 1, p.wait_ns, &never);
+        }
+        if (tid == 32) {
+            mma_commit(&drained);
+            bar_wait(&drained, 0, p.wait_ns, &never);
+        }
+        __syncthreads();
+    }
+    fence_after();
+    if (warp == 2) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
+}
+
+// ------------------------------------------------------------- host side
+inline PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
+    static PFN_cuTensorMapEncodeTiled_v12000 fn = [] {
+        void* f = nullptr;
+        cudaDriverEntryPointQueryResult found;
+        if (cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &f, 12000, cudaEnableDefault, &found) != cudaSuccess ||
+            found != cudaDriverEntryPointSuccess)
+            f = nullptr;
+        return reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(f);
+    }();
+    return fn;
+}
+
+// A (d2, d1, d0) tensor of 16-bit elements, strides s1 and s2 in elements, read in
+// boxes of b0 x b1 with 128-byte swizzle; what lies outside reads as 0.
+inline bool make_map(CUtensorMap* map, int dtype, const void* base, int64_t d0, int64_t d1, int64_t d2, int64_t s1,
+                     int64_t s2, int b0, int b1, int rank) {
+    const auto fn = encode_fn();
+    if (!fn) return false;
+    const cuuint64_t dims[3] = {(cuuint64_t)d0, (cuuint64_t)d1, (cuuint64_t)d2};
+    const cuuint64_t strides[2] = {(cuuint64_t)s1 * 2, (cuuint64_t)s2 * 2};
+    const cuuint32_t box[3] = {(cuuint32_t)b0, (cuuint32_t)b1, 1}, step[3] = {1, 1, 1};
+    return fn(map, dtype == ELA_DTYPE_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, rank,
+              const_cast<void*>(base), dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE,
+              CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+inline int sm_count() {
+    static int counts[64] = {};
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 0;
+    if (counts[dev] == 0) {
+        int n = 0;
+        if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) return 0;
+        counts[dev] = n;
+    }
+    return counts[dev];
+}
+
+template <int PASS, typename T, int ACT>
+int mma_launch(const CUtensorMap& a, const CUtensorMap& b, const MmaParams& p, int64_t max_tiles, cudaStream_t st) {
+    auto kern = mma_kernel<PASS, T, ACT>;
+    const int sms = sm_count();
+    if (sms == 0 || cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, MMA_SMEM - 1024) != cudaSuccess)
+        return ELA_ERR_CUDA;
+    const int grid = (int)(max_tiles < sms ? max_tiles : sms);
+    kern<<<grid, MMA_THREADS, MMA_SMEM - 1024, st>>>(a, b, p);
+    return launch_status();
+}
+
+// Columns per tile of the row passes: the least of 32, 64, 128, 256 that holds an
+// expert's share of the rows.  A smaller tile leaves more of the shared memory to
+// stages of the weights (9 of 20 KB at 32, 4 of 48 KB at 256), which is what a few
+// rows per expert wait for.
+inline int columns_per_tile(int64_t R, int64_t E) {
+    const int64_t share = (R + E - 1) / E;
+    return share <= 32 ? 32 : share <= 64 ? 64 : share <= 128 ? 128 : 256;
+}
+inline int stages_for(int bn) {
+    const int n = (MMA_SMEM - 1024 - MMA_SMEM_FIXED) / (MMA_A_BYTES + bn * MMA_KB * 2);
+    return n < MMA_MAX_STAGES ? n : MMA_MAX_STAGES;
+}
+
+}  // namespace ela_expert

@@ -150,7 +150,7 @@ struct LinearSizes {
 Tensor weight_rows(const Tensor& w) {
     const Tensor v = w.dim() == 2 ? w.unsqueeze(0) : w;
     const bool ok = (v.size(2) <= 1 || v.stride(2) == 1) && (v.size(1) <= 1 || v.stride(1) >= v.size(2)) &&
-                    (v.size(0) <= 1 || v.stride(0) >= 0);
+                    (v.size(0) <= 1 || v.stride(0) > 0);
     return ok ? v : v.contiguous();
 }
 

@@ -18,6 +18,7 @@ the last rows, is dispatched as zeros and adds nothing to the combined token.
 """
 from __future__ import annotations
 
+import ctypes
 from typing import NamedTuple, Optional
 
 import torch
@@ -148,6 +149,15 @@ def expert_linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Te
     elif offsets.dtype != torch.int32 or tuple(offsets.shape) != (E + 1,) or offsets.device != x.device:
         raise ValueError("expert_linear: offsets must be int32 (E+1,) on x's device")
     return _native().expert_linear(x, weight, bias, residual, offsets, ACTIVATIONS[activation])
+
+
+def expert_check() -> None:
+    """Raise AuctionError if a product on the current device gave up a wait since
+    the last check (its results are then incomplete).  Waits for the device; the
+    operators themselves never do."""
+    status = ctypes.c_int(0)
+    _lib.check(_lib.load().ela_expert_status(ctypes.byref(status)), "ela_expert_status")
+    _lib.check(status.value, "expert_linear kernel")
 
 
 def _register_fakes() -> None:

@@ -121,6 +121,13 @@ int ela_expert_linear_grad_weight(const void* dz, const void* x, const int32_t* 
                                   int64_t E, int64_t K, int64_t N, int64_t ldx, void* dweight, void* workspace,
                                   size_t workspace_bytes, void* stream);
 
+/*
+ * Error of the linear kernels on the current device since the last call: ELA_OK, or
+ * ELA_ERR_TIMEOUT when a device-side wait ran out (the results of that call are
+ * incomplete).  Waits for the device and clears the error.
+ */
+int ela_expert_status(int* status);
+
 #ifdef __cplusplus
 }
 #endif
