@@ -50,20 +50,42 @@ __device__ __forceinline__ void expert_rows(const int32_t* offsets, int e, int R
     r1 = offsets ? clampi(__ldg(offsets + e + 1), r0, R) : R;
 }
 
+// Complementary error function of x / sqrt(2) for x >= 0: Abramowitz and Stegun
+// 7.1.26, a polynomial in t = 1 / (1 + 0.3275911 x / sqrt(2)) times exp(-x^2 / 2)
+// (absolute error of erf below 1.5e-7); gauss receives the exponential.  Two special
+// function calls and no branch, where erff takes a divergent one and 1 + erf cancels
+// in the negative tail.
+__device__ __forceinline__ float erfc_sqrt2(float x, float& gauss) {
+    const float t = __fdividef(1.f, fmaf(0.3275911f * 0.70710678f, x, 1.f));
+    gauss = __expf(-0.5f * x * x);
+    float q = fmaf(1.061405429f, t, -1.453152027f);
+    q = fmaf(q, t, 1.421413741f);
+    q = fmaf(q, t, -0.284496736f);
+    q = fmaf(q, t, 0.254829592f);
+    return q * t * gauss;
+}
+
 // Activation and its derivative, fp32.
 template <int ACT> __device__ __forceinline__ float act_value(float z) {
     if (ACT == ELA_ACT_RELU) return z < 0.f ? 0.f : z;  // NaN stays NaN
-    if (ACT == ELA_ACT_GELU) return 0.5f * z * (1.f + erff(z * 0.70710678118654752f));
-    if (ACT == ELA_ACT_SILU) return z / (1.f + __expf(-z));
+    if (ACT == ELA_ACT_GELU) {
+        float g;
+        const float tail = 0.5f * erfc_sqrt2(fabsf(z), g);  // 1 - Phi(|z|)
+        return z * (z < 0.f ? tail : 1.f - tail);
+    }
+    if (ACT == ELA_ACT_SILU) return __fdividef(z, 1.f + __expf(-z));
     return z;
 }
 template <int ACT> __device__ __forceinline__ float act_slope(float z) {
     if (ACT == ELA_ACT_RELU) return z > 0.f ? 1.f : 0.f;
-    if (ACT == ELA_ACT_GELU)  // Phi(z) + z * phi(z)
-        return 0.5f * (1.f + erff(z * 0.70710678118654752f)) + z * __expf(-0.5f * z * z) * 0.39894228040143268f;
+    if (ACT == ELA_ACT_GELU) {  // Phi(z) + z * phi(z)
+        float g;
+        const float tail = 0.5f * erfc_sqrt2(fabsf(z), g);
+        return fmaf(z * 0.39894228040143268f, g, z < 0.f ? tail : 1.f - tail);
+    }
     if (ACT == ELA_ACT_SILU) {
-        const float q = 1.f / (1.f + __expf(-z));
-        return q * (1.f + z * (1.f - q));
+        const float q = __fdividef(1.f, 1.f + __expf(-z));
+        return q * fmaf(z, 1.f - q, 1.f);
     }
     return 1.f;
 }

@@ -93,12 +93,12 @@ inline MmaParams row_pass(const int32_t* offsets, int64_t R, int64_t E, int64_t 
     p.offsets = offsets;
     p.R = (int)R; p.E = (int)E; p.F = (int)F; p.K = (int)K;
     p.bn = columns_per_tile(R, E);
-    // boxes as tall as an expert's share of the rows, so that few rows do not load many
+    // boxes as tall as half an expert's share of the rows, so that few rows do not load many
     int64_t share = (R + E - 1) / E;
     p.bbox = 16;
-    while (p.bbox < p.bn && p.bbox < share) p.bbox *= 2;
+    while (p.bbox < p.bn / 2 && 2 * p.bbox < share) p.bbox *= 2;  // each CTA of a pair loads half
     p.stages = stages_for(p.bn);
-    p.f_tiles = (int)((F + MMA_F - 1) / MMA_F);
+    p.f_tiles = (int)((F + MMA_PAIR_F - 1) / MMA_PAIR_F);
     p.wait_ns = LINEAR_WAIT_NS;
     return p;
 }
@@ -222,7 +222,7 @@ int ela_expert_linear_grad_weight(const void* dz, const void* x, const int32_t* 
     p.R = (int)R; p.E = (int)E; p.F = (int)K; p.C = (int)N;
     p.bn = MMA_C;
     p.stages = stages_for(p.bn);
-    p.f_tiles = (int)((K + MMA_F - 1) / MMA_F);
+    p.f_tiles = (int)((K + MMA_PAIR_F - 1) / MMA_PAIR_F);
     p.c_tiles = (int)((N + MMA_C - 1) / MMA_C);
     p.out = dweight;
     p.vec = K % 4 == 0 && aligned8(dweight);

@@ -2,14 +2,19 @@
 // gradients (included by ela_expert_linear.cu).
 //
 // One persistent kernel computes out[c][f] = sum_k A(f,k) B(c,k), f contiguous in
-// memory, in tiles of 128 features f by up to 256 columns c:
+// memory.  A pair of CTAs (cluster of 2, tcgen05 cta_group::2) owns a tile of 256
+// features f by up to 256 columns c: each CTA loads 128 of the features and half of
+// the columns, and keeps the accumulators of its 128 features by all columns.
 //
-//   pass           f (128 TMEM lanes)     c (MMA N)            k
+//   pass           f (TMEM lanes)         c (MMA N)            k
 //   forward        output feature n       row of the expert    input feature
 //   input grad     input feature          row of the expert    output feature
 //   weight grad    input feature          output feature       row of the expert
 //
-// The rows of an expert are the MMA's N side, whose extent is a multiple of 16
+// Why a pair: one CTA's 128 x 256 tile loads 48 KB per 64 k, and the L2 then sets the
+// rate; half of the columns per CTA makes it 32 KB for the same products.
+//
+// The rows of an expert are the MMA's N side, whose extent is a multiple of 32
 // chosen per instruction: the last tile of an expert costs what its rows need, so
 // a generating step of a few rows and a long prompt run the same kernel, and the
 // weights, the side with whole tiles, fill the 128 lanes.
@@ -22,12 +27,14 @@
 // gradient, where rows are summed over, the last block's rows past the expert are
 // zeroed in shared memory, on both sides, since 0 * NaN is not 0.
 //
-// Roles: warp 0 issues the TMA loads, warp 1 the MMAs, warp 2 owns the TMEM
-// allocation, warps 4-7 run the epilogue while the next tile's MMAs fill the other
-// half of TMEM (2 x 256 columns).  The epilogue stages 32 columns at a time in
-// shared memory to turn "thread = feature" into rows of 128 consecutive features:
-// bias, activation and residual are applied there in fp32, and a warp stores one
-// row's 256 bytes at once.
+// Roles, in each CTA: warp 0 issues the TMA loads of the CTA's halves, which count on
+// the first CTA's barriers; warp 1 of the first CTA issues the MMAs of the pair; warp 2
+// owns the TMEM allocation; warps 4-11 run the epilogue while the next tile's MMAs fill
+// the other half of TMEM (2 x 256 columns).  The epilogue stages 16 columns at a time in
+// shared memory to turn "thread = feature" into rows of 128 consecutive features: bias,
+// activation and residual are applied there in fp32, and a warp stores one row's 256
+// bytes at once.  The residual of a chunk is loaded before its accumulators are waited
+// for, since one warp per scheduler and residual row would otherwise wait for memory.
 #pragma once
 
 #include <cuda.h>
@@ -39,15 +46,18 @@ namespace ela_expert {
 
 enum { PASS_FORWARD = 0, PASS_INPUT = 1, PASS_WEIGHT = 2 };
 
-constexpr int MMA_F = 128;              // features per tile (TMEM lanes)
+constexpr int MMA_F = 128;              // features per CTA (TMEM lanes)
+constexpr int MMA_PAIR_F = 256;         // features per tile
 constexpr int MMA_C = 256;              // most columns per tile
 constexpr int MMA_KB = 64;              // k per stage: 128 bytes, one swizzle span
 constexpr int MMA_A_BYTES = MMA_F * MMA_KB * 2;
-constexpr int MMA_STAGING = 32 * MMA_F * 4;  // one chunk of 32 columns, fp32
+constexpr int MMA_CHUNK = 16;           // columns an epilogue group stages at a time
+constexpr int MMA_STAGING = MMA_CHUNK * MMA_F * 4;  // one chunk, fp32
+constexpr int MMA_GROUPS = 2;           // epilogue groups of four warps
 constexpr int MMA_MAX_STAGES = 10;
-constexpr int MMA_THREADS = 256;
+constexpr int MMA_THREADS = 128 + MMA_GROUPS * 128;
 constexpr int MMA_SMEM = 227 * 1024;
-constexpr int MMA_SMEM_FIXED = 2 * MMA_STAGING + 1024;  // staging, alignment of the first stage
+constexpr int MMA_SMEM_FIXED = MMA_GROUPS * 2 * MMA_STAGING + 1024;  // staging, alignment of the first stage
 constexpr int MMA_GROUP = 16;           // column tiles walked together, for L2 reuse of both operands
 
 struct MmaParams {
@@ -72,11 +82,34 @@ __device__ __forceinline__ uint32_t saddr(const void* p) { return (uint32_t)__cv
 __device__ __forceinline__ void bar_init(uint64_t* b, int count) {
     asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(saddr(b)), "r"(count) : "memory");
 }
+// The address of the same object in the pair's first CTA.
+__device__ __forceinline__ uint32_t leader_addr(const void* p) {
+    uint32_t r;
+    asm("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(r) : "r"(saddr(p)));
+    return r;
+}
 __device__ __forceinline__ void bar_expect(uint64_t* b, uint32_t bytes) {
     asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(saddr(b)), "r"(bytes) : "memory");
 }
+// Arrivals on another CTA's barrier.  Where the barrier orders TMEM or loads alone, the
+// arrival is relaxed: a release at cluster scope is a fence that costs hundreds of cycles.
+__device__ __forceinline__ void bar_arrive_at(uint32_t addr) {
+    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(addr) : "memory");
+}
+__device__ __forceinline__ void bar_arrive_relaxed_at(uint32_t addr) {
+    asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(addr) : "memory");
+}
 __device__ __forceinline__ void bar_arrive(uint64_t* b) {
     asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(saddr(b)) : "memory");
+}
+// True in one lane of a converged warp.
+__device__ __forceinline__ bool elect_one() {
+    uint32_t yes;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(yes));
+    return yes;
+}
+__device__ __forceinline__ void cluster_sync() {
+    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 // Bounded wait for the phase of this parity; false when the limit ran out or another role gave up.
 __device__ __forceinline__ bool bar_wait(uint64_t* b, uint32_t parity, unsigned long long limit_ns,
@@ -96,41 +129,32 @@ __device__ __forceinline__ bool bar_wait(uint64_t* b, uint32_t parity, unsigned 
         }
     }
 }
-// The same for a whole warp: one lane polls, all get its answer.
-__device__ __forceinline__ bool warp_wait(uint64_t* b, uint32_t parity, unsigned long long limit_ns,
-                                          const volatile int* abort) {
-    int ok = 0;
-    if ((threadIdx.x & 31) == 0) ok = bar_wait(b, parity, limit_ns, abort);
-    ok = __shfl_sync(~0u, ok, 0);
-    __syncwarp();
-    return ok;
+// bar: shared::cluster address; it may be the pair's other CTA's.
+__device__ __forceinline__ void tma_2d(void* dst, const CUtensorMap* map, int x, int y, uint32_t bar) {
+    asm volatile("cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];"
+                 ::"r"(saddr(dst)), "l"(map), "r"(bar), "r"(x), "r"(y) : "memory");
 }
-__device__ __forceinline__ void tma_2d(void* dst, const CUtensorMap* map, int x, int y, uint64_t* bar) {
-    asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];"
-                 ::"r"(saddr(dst)), "l"(map), "r"(saddr(bar)), "r"(x), "r"(y) : "memory");
+__device__ __forceinline__ void tma_3d(void* dst, const CUtensorMap* map, int x, int y, int z, uint32_t bar) {
+    asm volatile("cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];"
+                 ::"r"(saddr(dst)), "l"(map), "r"(bar), "r"(x), "r"(y), "r"(z) : "memory");
 }
-__device__ __forceinline__ void tma_3d(void* dst, const CUtensorMap* map, int x, int y, int z, uint64_t* bar) {
-    asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];"
-                 ::"r"(saddr(dst)), "l"(map), "r"(saddr(bar)), "r"(x), "r"(y), "r"(z) : "memory");
-}
+// Arrives on the barrier of this place in both CTAs when the products issued so far are done.
 __device__ __forceinline__ void mma_commit(uint64_t* b) {
-    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(saddr(b)) : "memory");
+    asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;"
+                 ::"r"(saddr(b)), "h"((uint16_t)3) : "memory");
 }
 __device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void mma_issue(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool accumulate) {
     asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-                 "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
+                 "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}"
                  ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"((uint32_t)accumulate) : "memory");
 }
-__device__ __forceinline__ void tmem_ld32(uint32_t addr, float* v) {
+__device__ __forceinline__ void tmem_ld16(uint32_t addr, float* v) {
     uint32_t* r = reinterpret_cast<uint32_t*>(v);
-    asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
-                 "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
                  : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
-                   "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
-                   "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]),
-                   "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+                   "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
                  : "r"(addr));
     asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 }
@@ -146,7 +170,7 @@ __device__ __forceinline__ uint64_t operand_desc(uint32_t addr, bool k_major) {
 template <typename T> __device__ __forceinline__ uint32_t instr_desc(int n, bool a_k_major, bool b_k_major) {
     const uint32_t ab = sizeof(T) == 2 && El<T>::BF16 ? 1u : 0u;
     return (1u << 4) | (ab << 7) | (ab << 10) | ((a_k_major ? 0u : 1u) << 15) | ((b_k_major ? 0u : 1u) << 16) |
-           ((uint32_t)(n >> 3) << 17) | ((uint32_t)(MMA_F >> 4) << 24);
+           ((uint32_t)(n >> 3) << 17) | ((uint32_t)(MMA_PAIR_F >> 4) << 24);
 }
 
 // ------------------------------------------------------------- tile order
@@ -183,7 +207,7 @@ template <int PASS> struct Order {
             int local = t % per;
             const int group = local / (MMA_GROUP * p.f_tiles), g = min(MMA_GROUP, p.c_tiles - group * MMA_GROUP);
             local -= group * MMA_GROUP * p.f_tiles;
-            out.f0 = local / g * MMA_F;
+            out.f0 = local / g * MMA_PAIR_F;
             out.c0 = (group * MMA_GROUP + local % g) * MMA_C;
             out.nc = min(MMA_C, p.C - out.c0);
             int r0, r1;
@@ -205,7 +229,7 @@ template <int PASS> struct Order {
             const int group = local / (MMA_GROUP * p.f_tiles), g = min(MMA_GROUP, ct - group * MMA_GROUP);
             local -= group * MMA_GROUP * p.f_tiles;
             out.e = block + l;
-            out.f0 = local / g * MMA_F;
+            out.f0 = local / g * MMA_PAIR_F;
             out.c0 = r0 + (group * MMA_GROUP + local % g) * p.bn;
             out.nc = min(p.bn, r1 - out.c0);
             out.k0 = 0;
@@ -216,68 +240,81 @@ template <int PASS> struct Order {
 };
 
 // ------------------------------------------------------------- epilogue
+template <typename T> struct alignas(8) Four { T v[4]; };
+
+// Four consecutive features of one row of the residual (zeros without one).
+template <typename T>
+__device__ __forceinline__ Four<T> residual4(const MmaParams& p, int64_t c, int f) {
+    Four<T> r = {};
+    const T* at = reinterpret_cast<const T*>(p.residual) + c * p.ldr + f;
+    if (p.vec) {
+        r = *reinterpret_cast<const Four<T>*>(at);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            if (f + i < p.F) r.v[i] = at[i];
+    }
+    return r;
+}
+
 // Four consecutive features of one column: z = v + bias, y = act(z) + residual.
 template <typename T, int ACT>
-__device__ __forceinline__ void finish4(float4 v, const float* bias, const MmaParams& p, int64_t c, int f) {
+__device__ __forceinline__ void finish4(float4 v, const float* bias, const Four<T>& res, const MmaParams& p, int64_t c, int f) {
     T* out = reinterpret_cast<T*>(p.out) + c * p.F + f;
     T* zout = p.z ? reinterpret_cast<T*>(p.z) + c * p.F + f : nullptr;
-    const T* res = p.residual ? reinterpret_cast<const T*>(p.residual) + c * p.ldr + f : nullptr;
-    float q[4] = {v.x + bias[0], v.y + bias[1], v.z + bias[2], v.w + bias[3]};
-    struct alignas(8) T4 { T v[4]; } o;
+    const float q[4] = {v.x + bias[0], v.y + bias[1], v.z + bias[2], v.w + bias[3]};
+    Four<T> y, z;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        z.v[i] = El<T>::from(q[i]);
+        y.v[i] = El<T>::from(act_value<ACT>(q[i]) + El<T>::to(res.v[i]));
+    }
     if (p.vec) {
-        if (zout) {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) o.v[i] = El<T>::from(q[i]);
-            *reinterpret_cast<T4*>(zout) = o;
-        }
-#pragma unroll
-        for (int i = 0; i < 4; ++i) q[i] = act_value<ACT>(q[i]);
-        if (res) {
-            const T4 r = *reinterpret_cast<const T4*>(res);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) q[i] += El<T>::to(r.v[i]);
-        }
-#pragma unroll
-        for (int i = 0; i < 4; ++i) o.v[i] = El<T>::from(q[i]);
-        *reinterpret_cast<T4*>(out) = o;
+        if (zout) *reinterpret_cast<Four<T>*>(zout) = z;
+        *reinterpret_cast<Four<T>*>(out) = y;
     } else {
 #pragma unroll
         for (int i = 0; i < 4; ++i)
             if (f + i < p.F) {
-                if (zout) zout[i] = El<T>::from(q[i]);
-                out[i] = El<T>::from(act_value<ACT>(q[i]) + (res ? El<T>::to(res[i]) : 0.f));
+                if (zout) zout[i] = z.v[i];
+                out[i] = y.v[i];
             }
     }
 }
 
 template <int PASS, typename T, int ACT>
-__global__ void __launch_bounds__(MMA_THREADS, 1) mma_kernel(const __grid_constant__ CUtensorMap map_a,
-                                                             const __grid_constant__ CUtensorMap map_b,
-                                                             const MmaParams p) {
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(MMA_THREADS, 1)
+    mma_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const MmaParams p) {
     constexpr bool A_K_MAJOR = PASS == PASS_FORWARD, B_K_MAJOR = PASS != PASS_WEIGHT;
     extern __shared__ unsigned char smem_raw[];
-    __shared__ __align__(8) uint64_t full[MMA_MAX_STAGES], empty[MMA_MAX_STAGES], tfull[2], tempty[2], drained;
+    // full, tempty, patched: the first CTA's are used; empty, tfull, landed: each CTA its own
+    __shared__ __align__(8) uint64_t full[MMA_MAX_STAGES], empty[MMA_MAX_STAGES], tfull[2], tempty[2], landed, patched, drained;
     __shared__ uint32_t s_tmem;
     __shared__ int s_abort;
+    __shared__ uint32_t s_issued;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int rank = blockIdx.x & 1, pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
     unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
-    const int stage_bytes = MMA_A_BYTES + p.bn * MMA_KB * 2;
+    const int stage_bytes = MMA_A_BYTES + p.bn / 2 * MMA_KB * 2;
     float* staging = reinterpret_cast<float*>(smem + (size_t)p.stages * stage_bytes);
     const volatile int* abort = &s_abort;
 
     if (warp == 2) {
-        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(saddr(&s_tmem)) : "memory");
-        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+        asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(saddr(&s_tmem)) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
     }
     if (tid == 0) {
         s_abort = 0;
         for (int s = 0; s < p.stages; ++s) { bar_init(&full[s], 1); bar_init(&empty[s], 1); }
-        for (int b = 0; b < 2; ++b) { bar_init(&tfull[b], 1); bar_init(&tempty[b], 4); }
+        for (int b = 0; b < 2; ++b) { bar_init(&tfull[b], 1); bar_init(&tempty[b], 2 * 4 * MMA_GROUPS); }
+        bar_init(&landed, 1);
+        bar_init(&patched, 1);
         bar_init(&drained, 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     fence_before();
     __syncthreads();
+    cluster_sync();  // the barriers of both CTAs are there before either is signalled
     fence_after();
     const uint32_t tmem = s_tmem;
     auto give_up = [&]() {
@@ -285,95 +322,139 @@ __global__ void __launch_bounds__(MMA_THREADS, 1) mma_kernel(const __grid_consta
         atomicExch(&g_expert_error, ELA_ERR_TIMEOUT);
     };
 
-    uint32_t issued = 0;  // stages loaded (thread 0)
-    if (warp == 0) {  // ---- loads
+    uint32_t issued = 0;  // stages loaded (by the loading lane)
+    if (warp == 0) {  // ---- loads of this CTA's features and its half of the columns
         Order<PASS> order(p);
         Tile t;
         int s = 0;
-        uint32_t phase = 0;
+        uint32_t phase = 0, landings = 0;
         bool ok = true;
-        for (int n = blockIdx.x; ok && order.get(n, t); n += gridDim.x) {
-            const int blocks = (t.nk + MMA_KB - 1) / MMA_KB;
+        for (int n = pair; ok && order.get(n, t); n += pairs) {
+            const int f0 = t.f0 + rank * MMA_F;
             // column operand: boxes of p.bbox rows (K-major) or of 64 columns (MN-major)
-            const int nc16 = (t.nc + 15) & ~15;
-            const int boxes = B_K_MAJOR ? (nc16 + p.bbox - 1) / p.bbox : (nc16 + 63) / 64;
+            const int half = ((t.nc + 31) & ~31) >> 1, c0 = t.c0 + rank * half;
+            const int boxes = B_K_MAJOR ? (half + p.bbox - 1) / p.bbox : (half + 63) / 64;
             const int box_bytes = B_K_MAJOR ? p.bbox * MMA_KB * 2 : 64 * MMA_KB * 2;
-            for (int kb = 0; kb < blocks && ok; ++kb) {
-                if (lane == 0) {
+            const uint32_t bytes = MMA_A_BYTES + boxes * box_bytes;
+            // Rows of the next expert in the last block of a sum over rows: that block's
+            // loads land on a barrier of this CTA, the rows are zeroed, then the stage is full.
+            const int tail = PASS == PASS_WEIGHT ? t.nk % MMA_KB : 0, blocks = (t.nk + MMA_KB - 1) / MMA_KB;
+            const bool patch = (tail & 15) != 0;
+            auto load = [&](int k, uint32_t bar) {  // one thread; into stage s
+                unsigned char* a = smem + (size_t)s * stage_bytes;
+                unsigned char* b = a + MMA_A_BYTES;
+                if (PASS == PASS_FORWARD) {
+                    tma_3d(a, &map_a, k, f0, t.e, bar);
+                } else {
+                    for (int h = 0; h < 2; ++h)
+                        if (PASS == PASS_INPUT) tma_3d(a + h * 8192, &map_a, f0 + h * 64, k, t.e, bar);
+                        else tma_2d(a + h * 8192, &map_a, f0 + h * 64, k, bar);
+                }
+                for (int i = 0; i < boxes; ++i)
+                    if (B_K_MAJOR) tma_2d(b + i * box_bytes, &map_b, k, c0 + i * p.bbox, bar);
+                    else tma_2d(b + i * box_bytes, &map_b, c0 + i * 64, k, bar);
+                ++issued;
+            };
+            const int plain = blocks - patch;
+            if (elect_one()) {
+                for (int kb = 0; kb < plain; ++kb) {
+                    ok = bar_wait(&empty[s], phase ^ 1, p.wait_ns, abort);
+                    if (!ok) break;
+                    if (rank == 0) bar_expect(&full[s], 2 * bytes);  // the pair's
+                    load(t.k0 + kb * MMA_KB, leader_addr(&full[s]));
+                    if (++s == p.stages) { s = 0; phase ^= 1; }
+                }
+                if (patch && ok) {
                     ok = bar_wait(&empty[s], phase ^ 1, p.wait_ns, abort);
                     if (ok) {
-                        unsigned char* a = smem + (size_t)s * stage_bytes;
-                        unsigned char* b = a + MMA_A_BYTES;
-                        const int k = t.k0 + kb * MMA_KB;
-                        bar_expect(&full[s], MMA_A_BYTES + boxes * box_bytes);
-                        if (PASS == PASS_FORWARD) {
-                            tma_3d(a, &map_a, k, t.f0, t.e, &full[s]);
-                        } else {
-                            for (int h = 0; h < 2; ++h)
-                                if (PASS == PASS_INPUT) tma_3d(a + h * 8192, &map_a, t.f0 + h * 64, k, t.e, &full[s]);
-                                else tma_2d(a + h * 8192, &map_a, t.f0 + h * 64, k, &full[s]);
-                        }
-                        for (int i = 0; i < boxes; ++i)
-                            if (B_K_MAJOR) tma_2d(b + i * box_bytes, &map_b, k, t.c0 + i * p.bbox, &full[s]);
-                            else tma_2d(b + i * box_bytes, &map_b, t.c0 + i * 64, k, &full[s]);
-                        ++issued;
+                        bar_expect(&landed, bytes);
+                        load(t.k0 + plain * MMA_KB, saddr(&landed));
+                        ok = bar_wait(&landed, landings & 1, p.wait_ns, abort);
+                    }
+                }
+                if (!ok) give_up();
+            }
+            // the elected lane's place in the ring, to all (elect_one names the same lane again)
+            const int who = __ffs(__ballot_sync(~0u, elect_one())) - 1;
+            ok = __shfl_sync(~0u, (int)ok, who);
+            s = __shfl_sync(~0u, s, who);
+            phase = __shfl_sync(~0u, phase, who);
+            __syncwarp();
+            if (patch && ok) {
+                ++landings;
+                unsigned char* a = smem + (size_t)s * stage_bytes;
+                const int pieces = (16 - (tail & 15)) * 8;  // A's two boxes, then B's, 8192 bytes each
+                for (int i = lane; i < (2 + boxes) * pieces; i += 32)
+                    *reinterpret_cast<uint4*>(a + (size_t)(i / pieces) * 8192 + tail * 128 + i % pieces * 16) = make_uint4(0, 0, 0, 0);
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                __syncwarp();
+                if (lane == 0) {
+                    if (rank == 1) {
+                        bar_arrive_at(leader_addr(&patched));
                     } else {
-                        give_up();
+                        ok = bar_wait(&patched, (landings - 1) & 1, p.wait_ns, abort);
+                        asm volatile("fence.acq_rel.cluster;" ::: "memory");
+                        if (ok) bar_arrive(&full[s]);
+                        else give_up();
                     }
                 }
                 ok = __shfl_sync(~0u, (int)ok, 0);
                 if (++s == p.stages) { s = 0; phase ^= 1; }
             }
         }
-    } else if (warp == 1) {  // ---- products
+        s_issued = 0;
+        __syncwarp();
+        if (issued) s_issued = issued;
+    } else if (warp == 1 && rank == 0) {  // ---- products of the pair
         Order<PASS> order(p);
         Tile t;
         int s = 0, it = 0;
         uint32_t phase = 0;
         bool ok = true;
-        for (int n = blockIdx.x; ok && order.get(n, t); n += gridDim.x) {
+        const uint64_t a_desc = operand_desc(saddr(smem), A_K_MAJOR), b_desc = operand_desc(saddr(smem) + MMA_A_BYTES, B_K_MAJOR);
+        constexpr int A_STEP = A_K_MAJOR ? 2 : 128, B_STEP = B_K_MAJOR ? 2 : 128;  // 16 k, in 16-byte units
+        for (int n = pair; ok && order.get(n, t); n += pairs) {
             const int blocks = (t.nk + MMA_KB - 1) / MMA_KB;
             if (blocks == 0) continue;  // an expert without rows: the epilogue writes its zeros
-            const int half = it & 1;
-            const uint32_t d = tmem + half * MMA_C;
-            const uint32_t idesc = instr_desc<T>((t.nc + 15) & ~15, A_K_MAJOR, B_K_MAJOR);
-            ok = warp_wait(&tempty[half], ((it >> 1) & 1) ^ 1, p.wait_ns, abort);
-            for (int kb = 0; kb < blocks && ok; ++kb) {
-                ok = warp_wait(&full[s], phase, p.wait_ns, abort);
-                if (!ok) break;
+            if (elect_one()) {
+                const int half = it & 1;
+                const uint32_t d = tmem + half * MMA_C;
+                const uint32_t idesc = instr_desc<T>((t.nc + 31) & ~31, A_K_MAJOR, B_K_MAJOR);
+                ok = bar_wait(&tempty[half], ((it >> 1) & 1) ^ 1, p.wait_ns, abort);
                 fence_after();
-                unsigned char* a = smem + (size_t)s * stage_bytes;
-                const int left = t.nk - kb * MMA_KB;
-                const int steps = left >= MMA_KB ? 4 : (left + 15) >> 4;
-                if (PASS == PASS_WEIGHT && left < steps * 16) {  // rows of the next expert: zeros
-                    const int c_boxes = (((t.nc + 15) & ~15) + 63) / 64, pieces = (steps * 16 - left) * 8;
-                    for (int i = lane; i < (2 + c_boxes) * pieces; i += 32) {
-                        const int box = i / pieces, r = i % pieces;  // A's two boxes, then B's, 8192 bytes each
-                        *reinterpret_cast<uint4*>(a + (size_t)box * 8192 + left * 128 + r * 16) = make_uint4(0, 0, 0, 0);
+                for (int kb = 0; kb < blocks && ok; ++kb) {
+                    ok = bar_wait(&full[s], phase, p.wait_ns, abort);
+                    if (!ok) break;
+                    fence_after();
+                    const uint64_t off = (uint32_t)(s * stage_bytes) >> 4;
+                    const int left = t.nk - kb * MMA_KB;
+                    if (left >= MMA_KB) {
+#pragma unroll
+                        for (int j = 0; j < 4; ++j)
+                            mma_issue(d, a_desc + off + j * A_STEP, b_desc + off + j * B_STEP, idesc, kb + j > 0);
+                    } else {
+                        for (int j = 0; j < (left + 15) >> 4; ++j)
+                            mma_issue(d, a_desc + off + j * A_STEP, b_desc + off + j * B_STEP, idesc, kb + j > 0);
                     }
-                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-                    __syncwarp();
-                }
-                if (lane == 0) {
-                    const uint64_t ad = operand_desc(saddr(a), A_K_MAJOR), bd = operand_desc(saddr(a) + MMA_A_BYTES, B_K_MAJOR);
-                    for (int j = 0; j < steps; ++j)
-                        mma_issue(d, ad + j * (A_K_MAJOR ? 2 : 128), bd + j * (B_K_MAJOR ? 2 : 128), idesc, kb + j > 0);
                     mma_commit(&empty[s]);
-                    if (kb == blocks - 1) mma_commit(&tfull[half]);
+                    if (++s == p.stages) { s = 0; phase ^= 1; }
                 }
-                __syncwarp();
-                if (++s == p.stages) { s = 0; phase ^= 1; }
+                if (ok) mma_commit(&tfull[half]);
+                else give_up();
             }
+            const int who = __ffs(__ballot_sync(~0u, elect_one())) - 1;
+            ok = __shfl_sync(~0u, (int)ok, who);
+            s = __shfl_sync(~0u, s, who);
+            phase = __shfl_sync(~0u, phase, who);
             ++it;
         }
-        if (!ok && lane == 0) give_up();
     } else if (warp >= 4) {  // ---- epilogue
-        const int w = warp - 4, et = tid - 128;
-        if (PASS != PASS_WEIGHT && p.offsets) {  // rows of no expert: the residual, or 0
-            const int lo = clampi(p.offsets[0], 0, p.R), hi = clampi(p.offsets[p.E], 0, p.R);
+        const int w = warp & 3, group = (warp - 4) >> 2;
+        if constexpr (PASS != PASS_WEIGHT) {  // rows of no expert: the residual, or 0
+            const int lo = p.offsets ? clampi(p.offsets[0], 0, p.R) : 0, hi = p.offsets ? clampi(p.offsets[p.E], 0, p.R) : p.R;
             for (int r = blockIdx.x; r < p.R; r += gridDim.x) {
                 if (r >= lo && r < hi) { r = hi - 1 - (hi - 1 - r) % (int)gridDim.x; continue; }
-                for (int f = et; f < p.F; f += 128)
+                for (int f = tid - 128; f < p.F; f += MMA_GROUPS * 128)
                     reinterpret_cast<T*>(p.out)[(int64_t)r * p.F + f] =
                         p.residual ? reinterpret_cast<const T*>(p.residual)[r * p.ldr + f] : El<T>::from(0.f);
             }
@@ -381,66 +462,89 @@ __global__ void __launch_bounds__(MMA_THREADS, 1) mma_kernel(const __grid_consta
         Order<PASS> order(p);
         Tile t;
         int it = 0;
-        for (int n = blockIdx.x; order.get(n, t); n += gridDim.x) {
+        for (int n = pair; order.get(n, t); n += pairs) {
             const bool product = t.nk > 0;
             const int half = it & 1;
-            if (product) {
-                // all four warps go on or give up together: they share barriers below
-                const int ok = bar_wait(&tfull[half], (it >> 1) & 1, p.wait_ns, abort);
-                int all;
-                asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %1, 0;\n\tbarrier.cta.red.and.pred q, 1, 128, p;\n\t"
-                             "selp.b32 %0, 1, 0, q;\n\t}" : "=r"(all) : "r"(ok) : "memory");
-                if (!all) { give_up(); break; }
-                fence_after();
-            }
-            const int f = t.f0 + 4 * lane;
+            const int f = t.f0 + rank * MMA_F + 4 * lane;
             float bias[4];
 #pragma unroll
             for (int i = 0; i < 4; ++i)
                 bias[i] = PASS == PASS_FORWARD && p.bias && f + i < p.F
                               ? El<T>::to(reinterpret_cast<const T*>(p.bias)[(int64_t)t.e * p.F + f + i]) : 0.f;
             const int64_t c_base = PASS == PASS_WEIGHT ? (int64_t)t.e * p.C + t.c0 : t.c0;
-            for (int c = 0; c < t.nc; c += 32) {
-                float* st = staging + ((c >> 5) & 1) * (32 * MMA_F);
-                if (product) {
-                    float v[32];
-                    __syncwarp();
-                    tmem_ld32(tmem + ((uint32_t)(32 * w) << 16) + half * MMA_C + c, v);
-                    if (c + 32 >= t.nc) {  // the accumulator's half is free for the tile after next
-                        fence_before();
-                        __syncwarp();
-                        if (lane == 0) bar_arrive(&tempty[half]);
-                    }
+            const int c_first = group * MMA_CHUNK;
+            // a warp's columns of a chunk are w, w+4, w+8, w+12
+            Four<T> res[MMA_CHUNK / 4] = {};
+            auto load_residual = [&](int c) {
+                if (PASS != PASS_FORWARD || !p.residual || f >= p.F) return;
 #pragma unroll
-                    for (int i = 0; i < 32; ++i) st[i * MMA_F + 32 * w + lane] = v[i];
-                    asm volatile("barrier.cta.sync 1, 128;" ::: "memory");
-                }
-                for (int i = w; i < 32 && c + i < t.nc; i += 4) {
-                    const float4 v = product ? *reinterpret_cast<const float4*>(st + i * MMA_F + 4 * lane) : make_float4(0, 0, 0, 0);
-                    if (f < p.F) finish4<T, ACT>(v, bias, p, c_base + c + i, f);
-                }
+                for (int i = 0; i < MMA_CHUNK / 4; ++i)
+                    if (c + w + 4 * i < t.nc) res[i] = residual4<T>(p, c_base + c + w + 4 * i, f);
+            };
+            load_residual(c_first);
+            if (product) {
+                // the group's warps go on or give up together: they share barriers below
+                const int ok = bar_wait(&tfull[half], (it >> 1) & 1, p.wait_ns, abort);
+                int all;
+                asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %1, 0;\n\tbarrier.cta.red.and.pred q, %2, 128, p;\n\t"
+                             "selp.b32 %0, 1, 0, q;\n\t}" : "=r"(all) : "r"(ok), "r"(1 + group) : "memory");
+                if (!all) { give_up(); break; }
+                fence_after();
             }
-            // the next tile's first chunk reuses a staging buffer: all reads are done
-            if (product) asm volatile("barrier.cta.sync 1, 128;" ::: "memory");
+            int flip = 0;
+            for (int c = c_first; c < t.nc; c += MMA_GROUPS * MMA_CHUNK, flip ^= 1) {
+                float* st = staging + (group * 2 + flip) * (MMA_CHUNK * MMA_F);
+                if (product) {
+                    float v[MMA_CHUNK];
+                    __syncwarp();
+                    tmem_ld16(tmem + ((uint32_t)(32 * w) << 16) + half * MMA_C + c, v);
+#pragma unroll
+                    for (int i = 0; i < MMA_CHUNK; ++i) st[i * MMA_F + 32 * w + lane] = v[i];
+                    asm volatile("barrier.cta.sync %0, 128;" ::"r"(1 + group) : "memory");
+                }
+                if (f < p.F) {
+#pragma unroll
+                    for (int i = 0; i < MMA_CHUNK / 4; ++i) {
+                        const int col = w + 4 * i;
+                        if (c + col < t.nc) {
+                            const float4 v = product ? *reinterpret_cast<const float4*>(st + col * MMA_F + 4 * lane) : make_float4(0, 0, 0, 0);
+                            finish4<T, ACT>(v, bias, res[i], p, c_base + c + col, f);
+                        }
+                    }
+                }
+                if (c + MMA_GROUPS * MMA_CHUNK < t.nc) load_residual(c + MMA_GROUPS * MMA_CHUNK);
+            }
+            if (product) {
+                // this half of TMEM is free for the tile after next, and the staging for the next
+                fence_before();
+                asm volatile("barrier.cta.sync %0, 128;" ::"r"(1 + group) : "memory");
+                if (lane == 0) bar_arrive_relaxed_at(leader_addr(&tempty[half]));
+            }
             it += product;
         }
     }
     __syncthreads();
     if (s_abort) {  // loads and products in flight end before the CTA gives back its memory
         int never = 0;
-        if (tid == 0) {
-            const uint32_t last = issued < (uint32_t)p.stages ? issued : p.stages;
-            for (uint32_t i = issued - last; i < issued; ++i)
+        if (tid == 0 && rank == 0) {
+            const uint32_t last = s_issued < (uint32_t)p.stages ? s_issued : p.stages;
+            for (uint32_t i = s_issued - last; i < s_issued; ++i)
                 bar_wait(&full[i % p.stages], (i / p.stages) & 1, p.wait_ns, &never);
         }
-        if (tid == 32) {
+        if (tid == 32 && rank == 0) {
             mma_commit(&drained);
             bar_wait(&drained, 0, p.wait_ns, &never);
         }
+        if (tid == 0) {  // the other CTA's loads count on barriers that it cannot wait for
+            unsigned long long t0, t1;
+            asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t0));
+            do asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t1)); while (t1 - t0 < 1000000ull);
+        }
         __syncthreads();
     }
+    cluster_sync();  // neither CTA leaves while the other may signal it or read its shared memory
     fence_after();
-    if (warp == 2) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
+    if (warp == 2) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
 }
 
 // ------------------------------------------------------------- host side
@@ -488,21 +592,21 @@ int mma_launch(const CUtensorMap& a, const CUtensorMap& b, const MmaParams& p, i
     const int sms = sm_count();
     if (sms == 0 || cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, MMA_SMEM - 1024) != cudaSuccess)
         return ELA_ERR_CUDA;
-    const int grid = (int)(max_tiles < sms ? max_tiles : sms);
+    const int grid = 2 * (int)(max_tiles < sms / 2 ? max_tiles : sms / 2);
     kern<<<grid, MMA_THREADS, MMA_SMEM - 1024, st>>>(a, b, p);
     return launch_status();
 }
 
 // Columns per tile of the row passes: the least of 32, 64, 128, 256 that holds an
 // expert's share of the rows.  A smaller tile leaves more of the shared memory to
-// stages of the weights (9 of 20 KB at 32, 4 of 48 KB at 256), which is what a few
+// stages of the weights (10 of 18 KB at 32, 6 of 32 KB at 256), which is what a few
 // rows per expert wait for.
 inline int columns_per_tile(int64_t R, int64_t E) {
     const int64_t share = (R + E - 1) / E;
     return share <= 32 ? 32 : share <= 64 ? 64 : share <= 128 ? 128 : 256;
 }
 inline int stages_for(int bn) {
-    const int n = (MMA_SMEM - 1024 - MMA_SMEM_FIXED) / (MMA_A_BYTES + bn * MMA_KB * 2);
+    const int n = (MMA_SMEM - 1024 - MMA_SMEM_FIXED) / (MMA_A_BYTES + bn / 2 * MMA_KB * 2);
     return n < MMA_MAX_STAGES ? n : MMA_MAX_STAGES;
 }
 
