@@ -62,7 +62,9 @@ def build_op(force: bool = False) -> str:
            "-I", os.path.join(tdir, "include"), "-I", os.path.join(tdir, "include", "torch", "csrc", "api", "include"),
            "-I", cuda_inc, "-I", INCLUDE, *OP_SOURCES, "-o", OP_OUT + ".tmp", "-L", PKG_DIR, "-lela_auction",
            "-L", os.path.join(tdir, "lib"), "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_cuda", "-ltorch",
-           "-Wl,-rpath,$ORIGIN"]
+           # the shared C++ runtime that torch uses, by name: a compiler that links its own static copy
+           # brings a second set of locale facets, and formatting a number in an error message then crashes
+           "-nostdlib++", "-l:libstdc++.so.6", "-Wl,-rpath,$ORIGIN"]
     subprocess.run(cmd, check=True)
     os.replace(OP_OUT + ".tmp", OP_OUT)
     return OP_OUT

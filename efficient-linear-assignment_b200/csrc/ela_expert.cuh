@@ -7,6 +7,8 @@
 #include <cuda_bf16.h>
 #include <stdint.h>
 
+#include <atomic>
+
 #include "ela_expert.h"
 
 namespace ela_expert {
@@ -31,8 +33,7 @@ template <> struct El<__nv_bfloat16> {
     static __device__ __forceinline__ __nv_bfloat16 from(float v) { return __float2bfloat16_rn(v); }
 };
 
-// W consecutive elements: 16 bytes when VEC, else one element at a time (rows
-// that are not 16-byte aligned).
+// W consecutive elements, 16 bytes.
 template <typename T> struct alignas(16) Pack { T v[El<T>::W]; };
 
 __host__ inline int dtype_bytes(int dtype) {
@@ -42,6 +43,29 @@ __host__ inline bool aligned16(const void* p, int64_t ld_bytes = 0) {
     return (reinterpret_cast<uintptr_t>(p) & 15u) == 0 && ld_bytes % 16 == 0;
 }
 __host__ inline int launch_status() { return cudaGetLastError() == cudaSuccess ? ELA_OK : ELA_ERR_CUDA; }
+
+inline int sm_count() {
+    static int counts[64] = {};
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 0;
+    if (counts[dev] == 0) {
+        int n = 0;
+        if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) return 0;
+        counts[dev] = n;
+    }
+    return counts[dev];
+}
+
+// Lets a kernel use this much dynamic shared memory; asked of the driver once per kernel and device.
+template <auto KERNEL> __host__ inline bool allow_smem(int bytes) {
+    static std::atomic<bool> done[64];
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return false;
+    if (done[dev].load(std::memory_order_relaxed)) return true;
+    if (cudaFuncSetAttribute(KERNEL, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess) return false;
+    done[dev].store(true, std::memory_order_relaxed);
+    return true;
+}
 
 // Rows of expert e, kept inside [0, R] whatever the offsets hold.
 __device__ __forceinline__ int clampi(int v, int lo, int hi) { return v < lo ? lo : v > hi ? hi : v; }

@@ -452,7 +452,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(MMA_THREADS, 1)
         const int w = warp & 3, group = (warp - 4) >> 2;
         if constexpr (PASS != PASS_WEIGHT) {  // rows of no expert: the residual, or 0
             const int lo = p.offsets ? clampi(p.offsets[0], 0, p.R) : 0, hi = p.offsets ? clampi(p.offsets[p.E], 0, p.R) : p.R;
-            for (int r = blockIdx.x; r < p.R; r += gridDim.x) {
+            for (int r = blockIdx.x; r < p.R; r += (int)gridDim.x) {
                 if (r >= lo && r < hi) { r = hi - 1 - (hi - 1 - r) % (int)gridDim.x; continue; }
                 for (int f = tid - 128; f < p.F; f += MMA_GROUPS * 128)
                     reinterpret_cast<T*>(p.out)[(int64_t)r * p.F + f] =
@@ -574,24 +574,11 @@ inline bool make_map(CUtensorMap* map, int dtype, const void* base, int64_t d0, 
               CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-inline int sm_count() {
-    static int counts[64] = {};
-    int dev = 0;
-    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 0;
-    if (counts[dev] == 0) {
-        int n = 0;
-        if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) return 0;
-        counts[dev] = n;
-    }
-    return counts[dev];
-}
-
 template <int PASS, typename T, int ACT>
 int mma_launch(const CUtensorMap& a, const CUtensorMap& b, const MmaParams& p, int64_t max_tiles, cudaStream_t st) {
     auto kern = mma_kernel<PASS, T, ACT>;
     const int sms = sm_count();
-    if (sms == 0 || cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, MMA_SMEM - 1024) != cudaSuccess)
-        return ELA_ERR_CUDA;
+    if (sms == 0 || !allow_smem<&mma_kernel<PASS, T, ACT>>(MMA_SMEM - 1024)) return ELA_ERR_CUDA;
     const int grid = 2 * (int)(max_tiles < sms / 2 ? max_tiles : sms / 2);
     kern<<<grid, MMA_THREADS, MMA_SMEM - 1024, st>>>(a, b, p);
     return launch_status();

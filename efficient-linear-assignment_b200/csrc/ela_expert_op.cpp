@@ -6,10 +6,11 @@
 //   ela_native::expert_combine(y, position, offsets, weights?) -> out
 //   ela_native::expert_linear(x, weight, bias?, residual?, offsets?, activation) -> y
 //
-// As in ela_torch_op.cpp: device guard, outputs and workspaces from the caching
-// allocator, the current stream, no synchronisation.  Autograd is here rather
-// than in Python because a small call is bound by host time.  The backward
-// passes launch kernels that autograd does not see, so asking for a gradient of
+// Arguments are checked here, with Python's TypeError and ValueError, and host tensors
+// are refused by CPU kernels that raise: the Python functions only forward, since a
+// small call is bound by host time.  As in ela_torch_op.cpp: device guard, outputs and workspaces from the caching
+// allocator, the current stream, no synchronisation.  Autograd is here for
+// the same reason.  The backward passes launch kernels that autograd does not see, so asking for a gradient of
 // a gradient (create_graph) raises.
 #include <torch/library.h>
 #include <torch/csrc/autograd/custom_function.h>
@@ -38,6 +39,8 @@ int code_of(const Tensor& t) {
     }
 }
 
+[[noreturn]] void refuse(const char* name) { TORCH_CHECK(false, name, " needs CUDA tensors (there is no CPU path)"); }
+
 void check_rc(int rc, const char* where) {
     TORCH_CHECK(rc == ELA_OK, where, ": ", ela_status_string(rc), " (status ", rc, ")");
 }
@@ -62,13 +65,16 @@ void no_second_derivative() {
 
 // ---- plan
 std::tuple<Tensor, Tensor, Tensor> plan(const Tensor& expert_in, int64_t E) {
-    TORCH_CHECK(expert_in.is_cuda(), "expert_plan needs a CUDA tensor (there is no CPU path)");
-    TORCH_CHECK(expert_in.scalar_type() == at::kInt || expert_in.scalar_type() == at::kLong, "expert must be int32 or int64");
+    TORCH_CHECK_TYPE(expert_in.scalar_type() == at::kInt || expert_in.scalar_type() == at::kLong,
+                     "expert_plan: expert must be int32 or int64, not ", expert_in.scalar_type());
+    TORCH_CHECK_VALUE(expert_in.dim() == 1 || expert_in.dim() == 2, "expert_plan: expert must be (T,) or (T, k)");
+    TORCH_CHECK_VALUE(E >= 1 && E <= ELA_EXPERT_MAX, "expert_plan: num_experts must be 1..", ELA_EXPERT_MAX);
+    TORCH_CHECK_VALUE(expert_in.numel() <= INT32_MAX, "expert_plan: more than 2^31 - 1 choices");
     c10::cuda::CUDAGuard guard(expert_in.device());
     const Tensor expert = expert_in.contiguous();
     const auto opt = expert.options().dtype(at::kInt);
     Tensor offsets = at::empty({E + 1}, opt), source = at::empty({expert.numel()}, opt);
-    Tensor position = at::empty(expert.dim() == 1 ? at::IntArrayRef({expert.numel(), 1}) : expert.sizes(), opt);
+    Tensor position = at::empty({expert.size(0), expert.dim() == 1 ? 1 : expert.size(1)}, opt);
     const size_t bytes = ela_expert_plan_workspace_bytes(expert.numel(), E);
     Tensor ws = workspace(bytes, expert);
     check_rc(ela_expert_plan(expert.data_ptr(), (int)expert.element_size(), expert.numel(), E, offsets.data_ptr<int32_t>(),
@@ -77,20 +83,20 @@ std::tuple<Tensor, Tensor, Tensor> plan(const Tensor& expert_in, int64_t E) {
     return {offsets, position, source};
 }
 
-void check_plan(const Tensor& like, const Tensor& position, const Tensor& offsets) {
-    TORCH_CHECK(position.scalar_type() == at::kInt && offsets.scalar_type() == at::kInt && position.dim() == 2 &&
-                    offsets.dim() == 1 && offsets.numel() >= 2 && position.is_contiguous() && offsets.is_contiguous() &&
-                    position.device() == like.device() && offsets.device() == like.device(),
-                "the plan's position (T,k) and offsets (E+1,) must be contiguous int32 on the rows' device");
+void check_rows(const char* name, const Tensor& rows, int64_t want, const Tensor& position, const Tensor& offsets) {
+    if (!rows.is_cuda()) refuse(name);
+    TORCH_CHECK_TYPE(code_of(rows) >= 0, name, ": unsupported dtype ", rows.scalar_type());
+    TORCH_CHECK_VALUE(position.scalar_type() == at::kInt && offsets.scalar_type() == at::kInt && position.dim() == 2 &&
+                          offsets.dim() == 1 && offsets.numel() >= 2 && position.is_contiguous() && offsets.is_contiguous() &&
+                          position.device() == rows.device() && offsets.device() == rows.device(),
+                      name, ": the plan's position (T, k) and offsets (E+1,) must be contiguous int32 on the rows' device");
+    TORCH_CHECK_VALUE(rows.dim() == 2 && rows.size(0) == want, name, ": a matrix of ", want, " rows is needed");
 }
 
 // ---- dispatch and combine
 Tensor dispatch_raw(const Tensor& x_in, const Tensor& position, const Tensor& offsets) {
-    TORCH_CHECK(x_in.is_cuda(), "expert_dispatch needs a CUDA tensor (there is no CPU path)");
+    check_rows("expert_dispatch", x_in, position.dim() == 2 ? position.size(0) : -1, position, offsets);
     const int code = code_of(x_in);
-    TORCH_CHECK(code >= 0, "unsupported dtype ", x_in.scalar_type());
-    check_plan(x_in, position, offsets);
-    TORCH_CHECK(x_in.dim() == 2 && x_in.size(0) == position.size(0), "x must be (T, H) with the plan's T");
     c10::cuda::CUDAGuard guard(x_in.device());
     const Tensor x = rows_of(x_in);
     Tensor rows = at::empty({position.numel(), x.size(1)}, x.options());
@@ -102,15 +108,14 @@ Tensor dispatch_raw(const Tensor& x_in, const Tensor& position, const Tensor& of
 }
 
 Tensor combine_raw(const Tensor& y_in, const Tensor& position, const Tensor& offsets, const OptTensor& weights) {
-    TORCH_CHECK(y_in.is_cuda(), "expert_combine needs a CUDA tensor (there is no CPU path)");
+    check_rows("expert_combine", y_in, position.numel(), position, offsets);
     const int code = code_of(y_in);
-    TORCH_CHECK(code >= 0, "unsupported dtype ", y_in.scalar_type());
-    check_plan(y_in, position, offsets);
-    TORCH_CHECK(y_in.dim() == 2 && y_in.size(0) == position.numel(), "y must be (T*k, H)");
-    if (weights.has_value())
-        TORCH_CHECK(weights->sizes() == position.sizes() && weights->device() == y_in.device() &&
-                        (weights->scalar_type() == at::kFloat || weights->scalar_type() == y_in.scalar_type()),
-                    "weights must be (T, k), float32 or y's dtype");
+    if (weights.has_value()) {
+        TORCH_CHECK_TYPE(weights->scalar_type() == at::kFloat || weights->scalar_type() == y_in.scalar_type(),
+                         "expert_combine: weights must be float32 or y's dtype, not ", weights->scalar_type());
+        TORCH_CHECK_VALUE((weights->sizes() == position.sizes() || (weights->dim() == 1 && position.size(1) == 1 && weights->size(0) == position.size(0))) &&
+                              weights->device() == y_in.device(), "expert_combine: weights must be (T, k) on y's device");
+    }
     c10::cuda::CUDAGuard guard(y_in.device());
     const Tensor y = rows_of(y_in);
     const OptTensor w = weights.has_value() ? OptTensor(weights->contiguous()) : OptTensor();
@@ -130,7 +135,7 @@ std::tuple<Tensor, Tensor> combine_grad_raw(const Tensor& dout_in, const OptTens
     const OptTensor w = weights.has_value() ? OptTensor(weights->contiguous()) : OptTensor();
     c10::cuda::CUDAGuard guard(dout.device());
     Tensor dy = at::empty({need_y ? position.numel() : 0, dout.size(1)}, dout.options());
-    Tensor dw = need_w ? at::empty(position.sizes(), w->options()) : at::empty({0}, dout.options());
+    Tensor dw = need_w ? at::empty(w->sizes(), w->options()) : at::empty({0}, dout.options());
     check_rc(ela_expert_combine_grad(dout.data_ptr(), ptr(y), code_of(dout), position.size(0), position.size(1),
                                      dout.size(1), ld(dout), y.has_value() ? ld(*y) : 0, position.data_ptr<int32_t>(),
                                      offsets.data_ptr<int32_t>(), offsets.numel() - 1, ptr(w),
@@ -156,9 +161,18 @@ Tensor weight_rows(const Tensor& w) {
 
 LinearSizes linear_sizes(const Tensor& x, const Tensor& weight, const OptTensor& bias, const OptTensor& residual,
                          const OptTensor& offsets) {
-    TORCH_CHECK(x.is_cuda(), "expert_linear needs CUDA tensors (there is no CPU path)");
-    TORCH_CHECK(x.scalar_type() == at::kHalf || x.scalar_type() == at::kBFloat16, "x must be float16 or bfloat16");
-    TORCH_CHECK(x.dim() == 2 && (weight.dim() == 2 || weight.dim() == 3), "x must be (R, K), weight (E, N, K) or (N, K)");
+    if (!x.is_cuda()) refuse("expert_linear");
+    TORCH_CHECK_TYPE(x.scalar_type() == at::kHalf || x.scalar_type() == at::kBFloat16,
+                     "expert_linear: x must be float16 or bfloat16, not ", x.scalar_type());
+    auto operand = [&](const char* name, const Tensor& t) {
+        TORCH_CHECK_TYPE(t.scalar_type() == x.scalar_type(), "expert_linear: ", name, " must be ", x.scalar_type(), ", not ", t.scalar_type());
+        TORCH_CHECK_VALUE(t.device() == x.device(), "expert_linear: ", name, " must be on x's device");
+    };
+    operand("weight", weight);
+    TORCH_CHECK_VALUE(x.dim() == 2 && (weight.dim() == 2 || weight.dim() == 3) && weight.size(-1) == x.size(1),
+                      "expert_linear: x must be (R, K), weight (E, N, K) or (N, K)");
+    TORCH_CHECK_VALUE(weight.numel() > 0 && (weight.dim() == 2 || weight.size(0) <= ELA_EXPERT_MAX),
+                      "expert_linear: E must be 1..", ELA_EXPERT_MAX, ", N and K at least 1");
     LinearSizes s;
     s.x = rows_of(x);
     s.w = weight_rows(weight);
@@ -168,16 +182,22 @@ LinearSizes linear_sizes(const Tensor& x, const Tensor& weight, const OptTensor&
     s.N = s.w.size(1);
     s.stride_e = s.E > 1 ? s.w.stride(0) : 0;
     s.ldw = s.N > 1 ? s.w.stride(1) : s.K;
-    auto same = [&](const Tensor& t) { return t.scalar_type() == x.scalar_type() && t.device() == x.device(); };
-    TORCH_CHECK(s.w.size(2) == s.K && same(weight), "weight must be (E, N, K) or (N, K) in x's dtype and device");
-    if (bias.has_value()) TORCH_CHECK(bias->numel() == s.E * s.N && same(*bias), "bias must be (E, N) in x's dtype and device");
-    if (residual.has_value())
-        TORCH_CHECK(residual->dim() == 2 && residual->size(0) == s.R && residual->size(1) == s.N && same(*residual),
-                    "residual must be (R, N) in x's dtype and device");
+    if (bias.has_value()) {
+        operand("bias", *bias);
+        TORCH_CHECK_VALUE(weight.dim() == 3 ? bias->dim() == 2 && bias->size(0) == s.E && bias->size(1) == s.N
+                                            : bias->dim() == 1 && bias->size(0) == s.N,
+                          "expert_linear: bias must be (E, N), or (N,) for one matrix");
+    }
+    if (residual.has_value()) {
+        operand("residual", *residual);
+        TORCH_CHECK_VALUE(residual->dim() == 2 && residual->size(0) == s.R && residual->size(1) == s.N,
+                          "expert_linear: residual must be (R, N)");
+    }
     if (offsets.has_value())
-        TORCH_CHECK(offsets->scalar_type() == at::kInt && offsets->is_contiguous() && offsets->numel() == s.E + 1 &&
-                        offsets->device() == x.device(), "offsets must be contiguous int32 (E+1,) on x's device");
-    TORCH_CHECK(offsets.has_value() || s.E == 1, "offsets are needed for more than one expert");
+        TORCH_CHECK_VALUE(offsets->scalar_type() == at::kInt && offsets->is_contiguous() && offsets->dim() == 1 &&
+                              offsets->numel() == s.E + 1 && offsets->device() == x.device(),
+                          "expert_linear: offsets must be contiguous int32 (E+1,) on x's device");
+    TORCH_CHECK_VALUE(offsets.has_value() || s.E == 1, "expert_linear: offsets are needed for more than one expert");
     return s;
 }
 
@@ -190,8 +210,8 @@ const int32_t* off_ptr(const OptTensor& o) { return o.has_value() ? o->data_ptr<
 
 std::tuple<Tensor, Tensor> linear_raw(const Tensor& x, const Tensor& weight, const OptTensor& bias,
                                       const OptTensor& residual, const OptTensor& offsets, int64_t act, bool want_z) {
-    c10::cuda::CUDAGuard guard(x.device());
     const LinearSizes s = linear_sizes(x, weight, bias, residual, offsets);
+    c10::cuda::CUDAGuard guard(x.device());
     const OptTensor b = bias.has_value() ? OptTensor(bias->contiguous()) : OptTensor();
     const OptTensor r = residual.has_value() ? OptTensor(rows_of(*residual)) : OptTensor();
     Tensor y = at::empty({s.R, s.N}, s.x.options());
@@ -345,14 +365,33 @@ struct Linear : torch::autograd::Function<Linear> {
     }
 };
 
+// Without a gradient to prepare, the operator itself: the graph's bookkeeping costs more
+// host time than a small call's kernel.
+bool tracked(const Tensor& t) { return t.requires_grad() && at::GradMode::is_enabled(); }
+bool tracked(const OptTensor& t) { return t.has_value() && tracked(*t); }
+
 Tensor dispatch_autograd(const Tensor& x, const Tensor& position, const Tensor& offsets) {
+    if (!tracked(x)) {
+        at::AutoDispatchBelowADInplaceOrView below;
+        return call_dispatch(x, position, offsets);
+    }
     return Dispatch::apply(x, position, offsets);
 }
 Tensor combine_autograd(const Tensor& y, const Tensor& position, const Tensor& offsets, const OptTensor& weights) {
+    if (!tracked(y) && !tracked(weights)) {
+        at::AutoDispatchBelowADInplaceOrView below;
+        return call_combine(y, position, offsets, weights);
+    }
     return Combine::apply(y, position, offsets, weights);
 }
 Tensor linear_autograd(const Tensor& x, const Tensor& weight, const OptTensor& bias, const OptTensor& residual,
                        const OptTensor& offsets, int64_t act) {
+    if (!tracked(x) && !tracked(weight) && !tracked(bias) && !tracked(residual)) {
+        static auto f = op<Tensor(const Tensor&, const Tensor&, const OptTensor&, const OptTensor&, const OptTensor&,
+                                  int64_t)>("ela_native::expert_linear");
+        at::AutoDispatchBelowADInplaceOrView below;
+        return f.call(x, weight, bias, residual, offsets, act);
+    }
     return Linear::apply(x, weight, bias, residual, offsets, act);
 }
 
@@ -379,6 +418,15 @@ TORCH_LIBRARY_IMPL(ela_native, CUDA, m) {
     m.impl("expert_linear", &linear_cuda);
     m.impl("expert_linear_z", &linear_raw);
     m.impl("expert_linear_grad", &linear_grad_raw);
+}
+
+TORCH_LIBRARY_IMPL(ela_native, CPU, m) {
+    m.impl("expert_plan", [](const Tensor&, int64_t) -> std::tuple<Tensor, Tensor, Tensor> { refuse("expert_plan"); });
+    m.impl("expert_dispatch", [](const Tensor&, const Tensor&, const Tensor&) -> Tensor { refuse("expert_dispatch"); });
+    m.impl("expert_combine", [](const Tensor&, const Tensor&, const Tensor&, const OptTensor&) -> Tensor { refuse("expert_combine"); });
+    m.impl("expert_linear", [](const Tensor&, const Tensor&, const OptTensor&, const OptTensor&, const OptTensor&, int64_t) -> Tensor {
+        refuse("expert_linear");
+    });
 }
 
 TORCH_LIBRARY_IMPL(ela_native, AutogradCUDA, m) {

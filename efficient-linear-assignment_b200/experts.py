@@ -10,7 +10,8 @@ these operators take the tokens there and back:
     out  = expert_combine(h, plan, weights)          # back, weighted and summed
 
 All of them are C++ torch operators (csrc/ela_expert_op.cpp) over the C ABI of
-include/ela_expert.h: current stream, no synchronisation, no data-dependent
+include/ela_expert.h, which also checks the arguments (TypeError, ValueError,
+RuntimeError for host tensors): current stream, no synchronisation, no data-dependent
 sizes, so the whole layer can be captured in a CUDA graph.  Dispatch, combine
 and linear are differentiable (once).  A choice outside [0, num_experts), such
 as the solver's -1 for an unassigned row, belongs to no expert: it takes one of
@@ -27,9 +28,7 @@ from . import _lib
 from .solver import _native_op
 
 ACTIVATIONS = {"none": 0, "relu": 1, "gelu": 2, "silu": 3}
-MAX_EXPERTS = 4096
-
-_DTYPES = (torch.float32, torch.float16, torch.bfloat16)
+MAX_EXPERTS = 4096  # ELA_EXPERT_MAX
 
 
 class ExpertPlan(NamedTuple):
@@ -48,51 +47,26 @@ _ops = None
 
 
 def _native():
+    """The operators' overloads (loaded once: the lookup by name costs host time)."""
     global _ops
     if _ops is None:
         _native_op()  # loads the operator library
-        _ops = torch.ops.ela_native
+        n = torch.ops.ela_native
+        _ops = (n.expert_plan.default, n.expert_dispatch.default, n.expert_combine.default, n.expert_linear.default)
     return _ops
-
-
-def _need_cuda(name: str, t: torch.Tensor) -> None:
-    if t.device.type != "cuda":
-        raise RuntimeError(f"{name} needs CUDA tensors (there is no CPU path)")
 
 
 def expert_plan(expert: torch.Tensor, num_experts: int) -> ExpertPlan:
     """Stable sort of the choices ``expert`` (T,) or (T, k), int32 or int64, by
     expert.  Choices outside [0, num_experts) go last."""
-    _need_cuda("expert_plan", expert)
-    if expert.dtype not in (torch.int32, torch.int64):
-        raise TypeError(f"expert must be int32 or int64, not {expert.dtype}")
-    if expert.dim() not in (1, 2):
-        raise ValueError("expert must be (T,) or (T, k)")
-    if not 1 <= num_experts <= MAX_EXPERTS:
-        raise ValueError(f"num_experts must be 1..{MAX_EXPERTS}")
-    if expert.numel() >= 1 << 31:
-        raise ValueError("more than 2^31 - 1 choices")
-    return ExpertPlan(*_native().expert_plan(expert, num_experts))
-
-
-def _check_plan(name: str, plan: ExpertPlan, t: torch.Tensor) -> None:
-    _need_cuda(name, t)
-    if t.dtype not in _DTYPES:
-        raise TypeError(f"{name}: unsupported dtype {t.dtype}")
-    if t.dim() != 2:
-        raise ValueError(f"{name}: rows must be a matrix")
-    if plan.position.dim() != 2 or plan.position.dtype != torch.int32 or plan.offsets.dtype != torch.int32:
-        raise ValueError(f"{name}: plan.position must be int32 (T, k), plan.offsets int32 (E+1,)")
+    return ExpertPlan._make((_ops or _native())[0](expert, num_experts))
 
 
 def expert_dispatch(x: torch.Tensor, plan: ExpertPlan) -> torch.Tensor:
     """Token rows ``x`` (T, H) in expert order, (T*k, H): row r is the token of
     slot ``plan.source[r]``; rows of no expert are zeros.  fp32, fp16 or bf16.
     Backward: each token's gradients summed in fp32, rounded once."""
-    _check_plan("expert_dispatch", plan, x)
-    if x.shape[0] != plan.position.shape[0]:
-        raise ValueError(f"expert_dispatch: x has {x.shape[0]} tokens, the plan {plan.position.shape[0]}")
-    return _native().expert_dispatch(x, plan.position, plan.offsets)
+    return (_ops or _native())[1](x, plan[1], plan[0])
 
 
 def expert_combine(y: torch.Tensor, plan: ExpertPlan, weights: Optional[torch.Tensor] = None) -> torch.Tensor:
@@ -100,17 +74,7 @@ def expert_combine(y: torch.Tensor, plan: ExpertPlan, weights: Optional[torch.Te
     choices of weight times row, in fp32, rounded once.  weights (T, k) (or (T,)
     when k is 1), float32 or y's dtype; None: 1.  Choices of no expert add
     nothing.  Backward: gradients of y and of weights."""
-    _check_plan("expert_combine", plan, y)
-    if y.shape[0] != plan.position.numel():
-        raise ValueError(f"expert_combine: y has {y.shape[0]} rows, the plan {plan.position.numel()}")
-    if weights is not None:
-        if weights.dtype != torch.float32 and weights.dtype != y.dtype:
-            raise TypeError(f"expert_combine: weights must be float32 or {y.dtype}, not {weights.dtype}")
-        if weights.dim() == 1 and plan.position.shape[1] == 1:
-            weights = weights.unsqueeze(1)
-        if weights.shape != plan.position.shape or weights.device != y.device:
-            raise ValueError("expert_combine: weights must be (T, k) on y's device")
-    return _native().expert_combine(y, plan.position, plan.offsets, weights)
+    return (_ops or _native())[2](y, plan[1], plan[0], weights)
 
 
 def expert_linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] = None,
@@ -124,31 +88,10 @@ def expert_linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Te
     is the one expert's).  Rows of no expert get the residual, or 0.  fp16 or
     bf16; sums in fp32 on the tensor cores, one rounding at the end.  Backward:
     gradients of x, weight, bias and residual."""
-    _need_cuda("expert_linear", x)
-    if x.dtype not in (torch.float16, torch.bfloat16):
-        raise TypeError(f"expert_linear: x must be float16 or bfloat16, not {x.dtype}")
-    if activation not in ACTIVATIONS:
+    code = ACTIVATIONS.get(activation)
+    if code is None:
         raise ValueError(f"expert_linear: unknown activation '{activation}'. Options: {list(ACTIVATIONS)}")
-    if x.dim() != 2 or weight.dim() not in (2, 3) or weight.shape[-1] != x.shape[1]:
-        raise ValueError("expert_linear: x must be (R, K), weight (E, N, K) or (N, K)")
-    E, N = (weight.shape[0] if weight.dim() == 3 else 1), weight.shape[-2]
-    if min(E, N, x.shape[1]) < 1 or E > MAX_EXPERTS:
-        raise ValueError(f"expert_linear: E must be 1..{MAX_EXPERTS}, N and K at least 1")
-    for name, t in (("weight", weight), ("bias", bias), ("residual", residual)):
-        if t is not None and t.dtype != x.dtype:
-            raise TypeError(f"expert_linear: {name} must be {x.dtype}, not {t.dtype}")
-        if t is not None and t.device != x.device:
-            raise ValueError(f"expert_linear: {name} must be on x's device")
-    if bias is not None and tuple(bias.shape) != ((E, N) if weight.dim() == 3 else (N,)):
-        raise ValueError("expert_linear: bias must be (E, N), or (N,) for one matrix")
-    if residual is not None and tuple(residual.shape) != (x.shape[0], N):
-        raise ValueError("expert_linear: residual must be (R, N)")
-    if offsets is None:
-        if E != 1:
-            raise ValueError("expert_linear: offsets are needed for more than one expert")
-    elif offsets.dtype != torch.int32 or tuple(offsets.shape) != (E + 1,) or offsets.device != x.device:
-        raise ValueError("expert_linear: offsets must be int32 (E+1,) on x's device")
-    return _native().expert_linear(x, weight, bias, residual, offsets, ACTIVATIONS[activation])
+    return (_ops or _native())[3](x, weight, bias, residual, offsets, code)
 
 
 def expert_check() -> None:
