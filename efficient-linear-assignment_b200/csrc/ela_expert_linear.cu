@@ -186,7 +186,7 @@ inline bool linear_sizes_ok(int dtype, int64_t R, int64_t E, int64_t K, int64_t 
     return (dtype == ELA_DTYPE_F16 || dtype == ELA_DTYPE_BF16) && R >= 0 && R <= (1ll << 30) && E >= 1 &&
            E <= ELA_EXPERT_MAX && K >= 1 && K <= (1ll << 30) && N >= 1 && N <= (1ll << 30) && (offsets || E == 1);
 }
-inline bool aligned8(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 7u) == 0; }
+inline bool aligned4(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 3u) == 0; }
 
 // Parameters of a pass whose columns are the experts' rows: F features out, contraction length K.
 inline MmaParams row_pass(const int32_t* offsets, int64_t R, int64_t E, int64_t F, int64_t K) {
@@ -198,7 +198,7 @@ inline MmaParams row_pass(const int32_t* offsets, int64_t R, int64_t E, int64_t 
     int64_t share = (R + E - 1) / E;
     p.bbox = 16;
     while (p.bbox < p.bn / 2 && 2 * p.bbox < share) p.bbox *= 2;  // each CTA of a pair loads half
-    p.stages = stages_for(p.bn);
+    p.stages = stages_for(p.bn, E);
     p.f_tiles = (int)((F + MMA_PAIR_F - 1) / MMA_PAIR_F);
     p.wait_ns = LINEAR_WAIT_NS;
     return p;
@@ -267,7 +267,7 @@ int ela_expert_linear(const void* x, const void* weight, const void* bias, const
     p.ldr = ldr;
     p.out = y;
     p.z = z;
-    p.vec = N % 4 == 0 && aligned8(y) && (!z || aligned8(z)) && (!residual || (aligned8(residual) && ldr % 4 == 0));
+    p.vec = N % 2 == 0 && aligned4(y) && (!z || aligned4(z)) && (!residual || (aligned4(residual) && ldr % 2 == 0));
     CUtensorMap a, b;
     if (!map_of(&a, dtype, mw, MMA_KB, MMA_F, true) || !map_of(&b, dtype, mx, MMA_KB, p.bbox, false)) return ELA_ERR_CUDA;
     ELA_BY_TYPE(dtype, { ELA_BY_ACT(activation, rc = (mma_launch<PASS_FORWARD, T_, A_>(a, b, p, row_tiles(p), st))) })
@@ -314,7 +314,7 @@ int ela_expert_linear_grad_input(const void* dz, const void* weight, const int32
     if (rc != ELA_OK) return rc;
     MmaParams p = row_pass(offsets, R, E, K, N);
     p.out = dx;
-    p.vec = K % 4 == 0 && aligned8(dx);
+    p.vec = K % 2 == 0 && aligned4(dx);
     CUtensorMap a, b;
     if (!map_of(&a, dtype, mw, 64, MMA_KB, true) || !map_of(&b, dtype, mz, MMA_KB, p.bbox, false)) return ELA_ERR_CUDA;
     ELA_BY_TYPE(dtype, { rc = (mma_launch<PASS_INPUT, T_, ELA_ACT_NONE>(a, b, p, row_tiles(p), st)); })
@@ -337,11 +337,11 @@ int ela_expert_linear_grad_weight(const void* dz, const void* x, const int32_t* 
     p.offsets = offsets;
     p.R = (int)R; p.E = (int)E; p.F = (int)K; p.C = (int)N;
     p.bn = MMA_C;
-    p.stages = stages_for(p.bn);
+    p.stages = stages_for(p.bn, E);
     p.f_tiles = (int)((K + MMA_PAIR_F - 1) / MMA_PAIR_F);
     p.c_tiles = (int)((N + MMA_C - 1) / MMA_C);
     p.out = dweight;
-    p.vec = K % 4 == 0 && aligned8(dweight);
+    p.vec = K % 2 == 0 && aligned4(dweight);
     p.wait_ns = LINEAR_WAIT_NS;
     CUtensorMap a, b;
     if (!map_of(&a, dtype, mx, 64, MMA_KB, false) || !map_of(&b, dtype, mz, 64, MMA_KB, false)) return ELA_ERR_CUDA;

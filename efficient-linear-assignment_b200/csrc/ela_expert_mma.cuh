@@ -30,11 +30,13 @@
 // Roles, in each CTA: warp 0 issues the TMA loads of the CTA's halves, which count on
 // the first CTA's barriers; warp 1 of the first CTA issues the MMAs of the pair; warp 2
 // owns the TMEM allocation; warps 4-11 run the epilogue while the next tile's MMAs fill
-// the other half of TMEM (2 x 256 columns).  The epilogue stages 16 columns at a time in
-// shared memory to turn "thread = feature" into rows of 128 consecutive features: bias,
-// activation and residual are applied there in fp32, and a warp stores one row's 256
-// bytes at once.  The residual of a chunk is loaded before its accumulators are waited
-// for, since one warp per scheduler and residual row would otherwise wait for memory.
+// the other half of TMEM (2 x 256 columns).  A warp reads 32 columns of its 32 features
+// at a time, one feature a lane; bias, activation and residual are applied in fp32, and
+// two neighbouring lanes swap halves so that each stores two consecutive features of
+// one column: a store instruction writes 64 bytes of two columns, whole sectors, with
+// no staging in shared memory and no barrier between the warps (staging fp32 chunks to
+// store 256 bytes a row took about 12k cycles a tile, more than the products of a sum
+// over 1024).  The residual of a chunk is loaded before its accumulators are waited for.
 #pragma once
 
 #include <cuda.h>
@@ -51,13 +53,12 @@ constexpr int MMA_PAIR_F = 256;         // features per tile
 constexpr int MMA_C = 256;              // most columns per tile
 constexpr int MMA_KB = 64;              // k per stage: 128 bytes, one swizzle span
 constexpr int MMA_A_BYTES = MMA_F * MMA_KB * 2;
-constexpr int MMA_CHUNK = 16;           // columns an epilogue group stages at a time
-constexpr int MMA_STAGING = MMA_CHUNK * MMA_F * 4;  // one chunk, fp32
-constexpr int MMA_GROUPS = 2;           // epilogue groups of four warps
+constexpr int MMA_CHUNK = 32;           // columns an epilogue warp takes at a time
+constexpr int MMA_GROUPS = 2;           // epilogue warps per 32 TMEM lanes
 constexpr int MMA_MAX_STAGES = 10;
 constexpr int MMA_THREADS = 128 + MMA_GROUPS * 128;
 constexpr int MMA_SMEM = 227 * 1024;
-constexpr int MMA_SMEM_FIXED = MMA_GROUPS * 2 * MMA_STAGING + 1024;  // staging, alignment of the first stage
+constexpr int MMA_SMEM_FIXED = 1024;    // alignment of the first stage
 constexpr int MMA_GROUP = 16;           // column tiles walked together, for L2 reuse of both operands
 
 struct MmaParams {
@@ -65,7 +66,7 @@ struct MmaParams {
     int R, E, F, C, K;      // C: columns of the weight gradient; K: contraction length of the row passes
     int bn, bbox, stages;   // columns per tile; rows per TMA box of the column operand; pipeline depth
     int f_tiles, c_tiles;   // c_tiles: weight gradient only
-    int vec;                // 4 features at a time may be loaded and stored together
+    int vec;                // two consecutive features may be loaded and stored together
     const void* bias;
     const void* residual;
     int64_t ldr;
@@ -150,11 +151,14 @@ __device__ __forceinline__ void mma_issue(uint32_t d, uint64_t a, uint64_t b, ui
                  "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}"
                  ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"((uint32_t)accumulate) : "memory");
 }
-__device__ __forceinline__ void tmem_ld16(uint32_t addr, float* v) {
+__device__ __forceinline__ void tmem_ld32(uint32_t addr, float* v) {
     uint32_t* r = reinterpret_cast<uint32_t*>(v);
-    asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+                 "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
                  : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
-                   "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+                   "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
+                   "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]),
+                   "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
                  : "r"(addr));
     asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 }
@@ -176,110 +180,132 @@ template <typename T> __device__ __forceinline__ uint32_t instr_desc(int n, bool
 // ------------------------------------------------------------- tile order
 struct Tile {
     int e, f0, c0, nc;  // expert, first feature, first column, columns
-    int k0, nk;         // contraction range (weight gradient: the expert's rows)
+    int k0, nk;         // contraction range (weight gradient: rows of the expert)
 };
 
-// Tile number -> tile.  Row passes: experts in order; within an expert, groups of
-// MMA_GROUP column tiles, feature tiles within a group, columns innermost.  The
-// number of tiles depends on the offsets, which only the device knows, so every
-// role walks them by itself, 32 experts at a time (one a lane; the whole warp calls).
-template <int PASS> struct Order {
-    const MmaParams& p;
-    int block, first, last, tiles, incl, before;
-    __device__ __forceinline__ explicit Order(const MmaParams& q) : p(q), block(0), before(0) { if (PASS != PASS_WEIGHT) load(); }
-    __device__ __forceinline__ void load() {
-        const int lane = threadIdx.x & 31, e = block + lane;
-        first = last = 0;
-        if (e < p.E) expert_rows(p.offsets, e, p.R, first, last);
-        tiles = (last - first + p.bn - 1) / p.bn * p.f_tiles;
-        incl = tiles;
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const int v = __shfl_up_sync(~0u, incl, o);
-            if (lane >= o) incl += v;
-        }
-    }
-    __device__ __forceinline__ bool get(int t, Tile& out) {
-        if constexpr (PASS == PASS_WEIGHT) {
-            const int per = p.f_tiles * p.c_tiles;
-            out.e = t / per;
-            if (out.e >= p.E) return false;
-            int local = t % per;
-            const int group = local / (MMA_GROUP * p.f_tiles), g = min(MMA_GROUP, p.c_tiles - group * MMA_GROUP);
-            local -= group * MMA_GROUP * p.f_tiles;
-            out.f0 = local / g * MMA_PAIR_F;
-            out.c0 = (group * MMA_GROUP + local % g) * MMA_C;
-            out.nc = min(MMA_C, p.C - out.c0);
-            int r0, r1;
-            expert_rows(p.offsets, out.e, p.R, r0, r1);
-            out.k0 = r0;
-            out.nk = r1 - r0;
-            return true;
-        } else {
-            while (t >= before + __shfl_sync(~0u, incl, 31)) {
-                before += __shfl_sync(~0u, incl, 31);
-                block += 32;
-                if (block >= p.E) return false;
-                load();
-            }
-            const int l = __ffs(__ballot_sync(~0u, before + incl > t)) - 1;
-            int local = t - before - __shfl_sync(~0u, incl - tiles, l);
-            const int r0 = __shfl_sync(~0u, first, l), r1 = __shfl_sync(~0u, last, l);
-            const int ct = (r1 - r0 + p.bn - 1) / p.bn;
-            const int group = local / (MMA_GROUP * p.f_tiles), g = min(MMA_GROUP, ct - group * MMA_GROUP);
-            local -= group * MMA_GROUP * p.f_tiles;
-            out.e = block + l;
-            out.f0 = local / g * MMA_PAIR_F;
-            out.c0 = r0 + (group * MMA_GROUP + local % g) * p.bn;
-            out.nc = min(p.bn, r1 - out.c0);
-            out.k0 = 0;
-            out.nk = p.K;
-            return true;
-        }
-    }
+// The experts' rows and row tiles, in shared memory.
+struct Plan {
+    const int *row0, *row1, *tile0;  // [E]; tile0: tiles before expert e (row passes)
+    int tiles;
 };
 
-// ------------------------------------------------------------- epilogue
-template <typename T> struct alignas(8) Four { T v[4]; };
-
-// Four consecutive features of one row of the residual (zeros without one).
-template <typename T>
-__device__ __forceinline__ Four<T> residual4(const MmaParams& p, int64_t c, int f) {
-    Four<T> r = {};
-    const T* at = reinterpret_cast<const T*>(p.residual) + c * p.ldr + f;
-    if (p.vec) {
-        r = *reinterpret_cast<const Four<T>*>(at);
+// Row passes: experts in order; within an expert, groups of MMA_GROUP column tiles,
+// feature tiles within a group, columns innermost.  Weight gradient: the same with the
+// output features as columns.  The offsets, and so the tiles, are only known on the
+// device: every role asks for the tiles by number (the whole warp calls).
+template <int PASS> __device__ __forceinline__ bool get_tile(const MmaParams& p, const Plan& plan, int t, Tile& out) {
+    if (t >= plan.tiles) return false;
+    int local, ct, r0, r1;
+    if constexpr (PASS == PASS_WEIGHT) {
+        ct = p.c_tiles;
+        const int per = p.f_tiles * ct;
+        out.e = t / per;
+        local = t - out.e * per;
     } else {
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-            if (f + i < p.F) r.v[i] = at[i];
+        // the last expert whose tiles start at or before t: 32 probes a step
+        const int lane = threadIdx.x & 31;
+        int lo = 0, n = p.E;
+        while (n > 1) {
+            const int step = (n + 31) >> 5, at = lo + lane * step;
+            const unsigned in = __ballot_sync(~0u, lane * step < n && plan.tile0[at < p.E ? at : p.E - 1] <= t);
+            const int last = 31 - __clz(in);  // (probe 0 always holds)
+            lo += last * step;
+            n = min(step, n - last * step);
+        }
+        out.e = lo;
+        local = t - plan.tile0[lo];
     }
-    return r;
+    r0 = plan.row0[out.e];
+    r1 = plan.row1[out.e];
+    if constexpr (PASS != PASS_WEIGHT) ct = (r1 - r0 + p.bn - 1) / p.bn;
+    const int group = local / (MMA_GROUP * p.f_tiles), g = min(MMA_GROUP, ct - group * MMA_GROUP);
+    local -= group * MMA_GROUP * p.f_tiles;
+    out.f0 = local / g * MMA_PAIR_F;
+    const int c = (group * MMA_GROUP + local % g) * p.bn;
+    if constexpr (PASS == PASS_WEIGHT) {
+        out.c0 = c;
+        out.nc = min(p.bn, p.C - c);
+        out.k0 = r0;
+        out.nk = r1 - r0;
+    } else {
+        out.c0 = r0 + c;
+        out.nc = min(p.bn, r1 - out.c0);
+        out.k0 = 0;
+        out.nk = p.K;
+    }
+    return true;
 }
 
-// Four consecutive features of one column: z = v + bias, y = act(z) + residual.
-template <typename T, int ACT>
-__device__ __forceinline__ void finish4(float4 v, const float* bias, const Four<T>& res, const MmaParams& p, int64_t c, int f) {
-    T* out = reinterpret_cast<T*>(p.out) + c * p.F + f;
-    T* zout = p.z ? reinterpret_cast<T*>(p.z) + c * p.F + f : nullptr;
-    const float q[4] = {v.x + bias[0], v.y + bias[1], v.z + bias[2], v.w + bias[3]};
-    Four<T> y, z;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        z.v[i] = El<T>::from(q[i]);
-        y.v[i] = El<T>::from(act_value<ACT>(q[i]) + El<T>::to(res.v[i]));
-    }
+// ------------------------------------------------------------- epilogue
+// Lanes 2i and 2i+1 hold features f and f+1 of columns c (low half of p) and c+1 (high
+// half).  After the swap the even lane has f, f+1 of column c, the odd lane of column
+// c+1, which is how memory has them; it is its own inverse.
+__device__ __forceinline__ uint32_t swap_pair(uint32_t p, bool odd) {
+    const uint32_t o = __shfl_xor_sync(~0u, p, 1);
+    return __byte_perm(p, o, odd ? 0x3276 : 0x5410);
+}
+template <typename T> __device__ __forceinline__ uint32_t pack2(float lo, float hi);
+template <> __device__ __forceinline__ uint32_t pack2<__half>(float lo, float hi) {
+    const __half2 h = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+template <> __device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float lo, float hi) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+template <typename T> __device__ __forceinline__ float2 unpack2(uint32_t p);
+template <> __device__ __forceinline__ float2 unpack2<__half>(uint32_t p) { return __half22float2(*reinterpret_cast<const __half2*>(&p)); }
+template <> __device__ __forceinline__ float2 unpack2<__nv_bfloat16>(uint32_t p) {
+    return make_float2(__uint_as_float(p << 16), __uint_as_float(p & 0xffff0000u));
+}
+
+// One chunk of a warp: v[j] is feature f (this lane's) of column c + j, j < left.  The
+// lane's residual words are those of swap_pair's layout (loaded by load_residual).
+template <typename T, int ACT, bool Z, bool RES>
+__device__ __forceinline__ void finish(float* v, float bias, const uint32_t* res, const MmaParams& p, int64_t c, int f, int left) {
+    const bool odd = threadIdx.x & 1;
     if (p.vec) {
-        if (zout) *reinterpret_cast<Four<T>*>(zout) = z;
-        *reinterpret_cast<Four<T>*>(out) = y;
-    } else {
+        const int64_t at = (c + odd) * p.F + (f & ~1), step = 2 * (int64_t)p.F;
+        uint32_t* out = reinterpret_cast<uint32_t*>(reinterpret_cast<T*>(p.out) + at);
+        uint32_t* zout = reinterpret_cast<uint32_t*>(reinterpret_cast<T*>(p.z) + at);
+        const int mine = f < p.F ? left - odd : 0;  // (F is even: both lanes of a pair are in or out)
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-            if (f + i < p.F) {
-                if (zout) zout[i] = z.v[i];
-                out[i] = y.v[i];
+        for (int j = 0; j < MMA_CHUNK; j += 2) {
+            float a = v[j] + bias, b = v[j + 1] + bias;
+            if (Z) {
+                const uint32_t w = swap_pair(pack2<T>(a, b), odd);
+                if (j < mine) zout[j / 2 * (step / 2)] = w;
+            }
+            a = act_value<ACT>(a);
+            b = act_value<ACT>(b);
+            if (RES) {
+                const float2 r = unpack2<T>(swap_pair(res[j / 2], odd));
+                a += r.x;
+                b += r.y;
+            }
+            const uint32_t w = swap_pair(pack2<T>(a, b), odd);
+            if (j < mine) out[j / 2 * (step / 2)] = w;
+        }
+    } else if (f < p.F) {
+#pragma unroll
+        for (int j = 0; j < MMA_CHUNK; ++j)
+            if (j < left) {
+                const float a = v[j] + bias;
+                const int64_t at = (c + j) * p.F + f;
+                if (Z) reinterpret_cast<T*>(p.z)[at] = El<T>::from(a);
+                const float r = RES ? El<T>::to(reinterpret_cast<const T*>(p.residual)[(c + j) * p.ldr + f]) : 0.f;
+                reinterpret_cast<T*>(p.out)[at] = El<T>::from(act_value<ACT>(a) + r);
             }
     }
+}
+
+template <typename T>
+__device__ __forceinline__ void load_residual(uint32_t* res, const MmaParams& p, int64_t c, int f, int left) {
+    const bool odd = threadIdx.x & 1;
+    const uint32_t* at = reinterpret_cast<const uint32_t*>(reinterpret_cast<const T*>(p.residual) + (c + odd) * p.ldr + (f & ~1));
+    const int mine = p.vec && f < p.F ? left - odd : 0;
+#pragma unroll
+    for (int j = 0; j < MMA_CHUNK; j += 2) res[j / 2] = j < mine ? __ldg(at + j / 2 * p.ldr) : 0u;
 }
 
 template <int PASS, typename T, int ACT>
@@ -292,11 +318,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(MMA_THREADS, 1)
     __shared__ uint32_t s_tmem;
     __shared__ int s_abort;
     __shared__ uint32_t s_issued;
+    __shared__ int s_tiles;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int rank = blockIdx.x & 1, pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
-    unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
+    // the experts' tables, then the stages, each on a 1024-byte boundary
+    int* table = reinterpret_cast<int*>(smem_raw);
+    unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(table + 3 * p.E) + 1023) & ~(uintptr_t)1023);
     const int stage_bytes = MMA_A_BYTES + p.bn / 2 * MMA_KB * 2;
-    float* staging = reinterpret_cast<float*>(smem + (size_t)p.stages * stage_bytes);
     const volatile int* abort = &s_abort;
 
     if (warp == 2) {
@@ -312,11 +340,29 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(MMA_THREADS, 1)
         bar_init(&drained, 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
+    for (int e = tid; e < p.E; e += MMA_THREADS) expert_rows(p.offsets, e, p.R, table[e], table[p.E + e]);
+    __syncthreads();
+    if (PASS != PASS_WEIGHT && warp == 3) {  // row tiles before each expert
+        int before = 0;
+        for (int e = lane; e - lane < p.E; e += 32) {
+            const int mine = e < p.E ? (table[p.E + e] - table[e] + p.bn - 1) / p.bn * p.f_tiles : 0;
+            int incl = mine;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const int v = __shfl_up_sync(~0u, incl, o);
+                if (lane >= o) incl += v;
+            }
+            if (e < p.E) table[2 * p.E + e] = before + incl - mine;
+            before += __shfl_sync(~0u, incl, 31);
+        }
+        if (lane == 0) s_tiles = before;
+    }
     fence_before();
     __syncthreads();
     cluster_sync();  // the barriers of both CTAs are there before either is signalled
     fence_after();
     const uint32_t tmem = s_tmem;
+    const Plan plan = {table, table + p.E, table + 2 * p.E, PASS == PASS_WEIGHT ? p.E * p.f_tiles * p.c_tiles : s_tiles};
     auto give_up = [&]() {
         *(volatile int*)&s_abort = 1;
         atomicExch(&g_expert_error, ELA_ERR_TIMEOUT);
@@ -324,12 +370,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(MMA_THREADS, 1)
 
     uint32_t issued = 0;  // stages loaded (by the loading lane)
     if (warp == 0) {  // ---- loads of this CTA's features and its half of the columns
-        Order<PASS> order(p);
         Tile t;
         int s = 0;
         uint32_t phase = 0, landings = 0;
         bool ok = true;
-        for (int n = pair; ok && order.get(n, t); n += pairs) {
+        for (int n = pair; ok && get_tile<PASS>(p, plan, n, t); n += pairs) {
             const int f0 = t.f0 + rank * MMA_F;
             // column operand: boxes of p.bbox rows (K-major) or of 64 columns (MN-major)
             const int half = ((t.nc + 31) & ~31) >> 1, c0 = t.c0 + rank * half;
@@ -406,14 +451,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(MMA_THREADS, 1)
         __syncwarp();
         if (issued) s_issued = issued;
     } else if (warp == 1 && rank == 0) {  // ---- products of the pair
-        Order<PASS> order(p);
         Tile t;
         int s = 0, it = 0;
         uint32_t phase = 0;
         bool ok = true;
         const uint64_t a_desc = operand_desc(saddr(smem), A_K_MAJOR), b_desc = operand_desc(saddr(smem) + MMA_A_BYTES, B_K_MAJOR);
         constexpr int A_STEP = A_K_MAJOR ? 2 : 128, B_STEP = B_K_MAJOR ? 2 : 128;  // 16 k, in 16-byte units
-        for (int n = pair; ok && order.get(n, t); n += pairs) {
+        for (int n = pair; ok && get_tile<PASS>(p, plan, n, t); n += pairs) {
             const int blocks = (t.nk + MMA_KB - 1) / MMA_KB;
             if (blocks == 0) continue;  // an expert without rows: the epilogue writes its zeros
             if (elect_one()) {
@@ -459,67 +503,51 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(MMA_THREADS, 1)
                         p.residual ? reinterpret_cast<const T*>(p.residual)[r * p.ldr + f] : El<T>::from(0.f);
             }
         }
-        Order<PASS> order(p);
         Tile t;
         int it = 0;
-        for (int n = pair; order.get(n, t); n += pairs) {
+        bool ok = true;
+        const bool with_z = PASS == PASS_FORWARD && p.z, with_res = PASS == PASS_FORWARD && p.residual;
+        auto accumulators = [&](int half, int it) {  // waits for the tile's products
+            if (lane == 0) ok = bar_wait(&tfull[half], (it >> 1) & 1, p.wait_ns, abort);
+            ok = __shfl_sync(~0u, (int)ok, 0);
+            if (!ok && lane == 0) give_up();
+            __syncwarp();
+            fence_after();
+            return ok;
+        };
+        auto release = [&](int half) {  // this half of TMEM is free for the tile after next
+            fence_before();
+            __syncwarp();
+            if (lane == 0) bar_arrive_relaxed_at(leader_addr(&tempty[half]));
+        };
+        auto write = [&](float* v, float bias, const uint32_t* res, int64_t c, int f, int left) {
+            if (with_z) {
+                if (with_res) finish<T, ACT, true, true>(v, bias, res, p, c, f, left);
+                else finish<T, ACT, true, false>(v, bias, res, p, c, f, left);
+            } else {
+                if (with_res) finish<T, ACT, false, true>(v, bias, res, p, c, f, left);
+                else finish<T, ACT, false, false>(v, bias, res, p, c, f, left);
+            }
+        };
+        for (int n = pair; ok && get_tile<PASS>(p, plan, n, t); n += pairs) {
             const bool product = t.nk > 0;
             const int half = it & 1;
-            const int f = t.f0 + rank * MMA_F + 4 * lane;
-            float bias[4];
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-                bias[i] = PASS == PASS_FORWARD && p.bias && f + i < p.F
-                              ? El<T>::to(reinterpret_cast<const T*>(p.bias)[(int64_t)t.e * p.F + f + i]) : 0.f;
+            const int f = t.f0 + rank * MMA_F + 32 * w + lane;
+            const float bias = PASS == PASS_FORWARD && p.bias && f < p.F
+                                   ? El<T>::to(reinterpret_cast<const T*>(p.bias)[(int64_t)t.e * p.F + f]) : 0.f;
             const int64_t c_base = PASS == PASS_WEIGHT ? (int64_t)t.e * p.C + t.c0 : t.c0;
-            const int c_first = group * MMA_CHUNK;
-            // a warp's columns of a chunk are w, w+4, w+8, w+12
-            Four<T> res[MMA_CHUNK / 4] = {};
-            auto load_residual = [&](int c) {
-                if (PASS != PASS_FORWARD || !p.residual || f >= p.F) return;
-#pragma unroll
-                for (int i = 0; i < MMA_CHUNK / 4; ++i)
-                    if (c + w + 4 * i < t.nc) res[i] = residual4<T>(p, c_base + c + w + 4 * i, f);
-            };
-            load_residual(c_first);
-            if (product) {
-                // the group's warps go on or give up together: they share barriers below
-                const int ok = bar_wait(&tfull[half], (it >> 1) & 1, p.wait_ns, abort);
-                int all;
-                asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %1, 0;\n\tbarrier.cta.red.and.pred q, %2, 128, p;\n\t"
-                             "selp.b32 %0, 1, 0, q;\n\t}" : "=r"(all) : "r"(ok), "r"(1 + group) : "memory");
-                if (!all) { give_up(); break; }
-                fence_after();
+            uint32_t res[MMA_CHUNK / 2];
+            if (with_res) load_residual<T>(res, p, c_base + group * MMA_CHUNK, f, t.nc - group * MMA_CHUNK);
+            if (product && !accumulators(half, it)) break;
+            for (int c = group * MMA_CHUNK; c < t.nc; c += MMA_GROUPS * MMA_CHUNK) {
+                float v[MMA_CHUNK] = {};
+                __syncwarp();
+                if (product) tmem_ld32(tmem + ((uint32_t)(32 * w) << 16) + half * MMA_C + c, v);
+                write(v, bias, res, c_base + c, f, t.nc - c);
+                const int next = c + MMA_GROUPS * MMA_CHUNK;
+                if (with_res && next < t.nc) load_residual<T>(res, p, c_base + next, f, t.nc - next);
             }
-            int flip = 0;
-            for (int c = c_first; c < t.nc; c += MMA_GROUPS * MMA_CHUNK, flip ^= 1) {
-                float* st = staging + (group * 2 + flip) * (MMA_CHUNK * MMA_F);
-                if (product) {
-                    float v[MMA_CHUNK];
-                    __syncwarp();
-                    tmem_ld16(tmem + ((uint32_t)(32 * w) << 16) + half * MMA_C + c, v);
-#pragma unroll
-                    for (int i = 0; i < MMA_CHUNK; ++i) st[i * MMA_F + 32 * w + lane] = v[i];
-                    asm volatile("barrier.cta.sync %0, 128;" ::"r"(1 + group) : "memory");
-                }
-                if (f < p.F) {
-#pragma unroll
-                    for (int i = 0; i < MMA_CHUNK / 4; ++i) {
-                        const int col = w + 4 * i;
-                        if (c + col < t.nc) {
-                            const float4 v = product ? *reinterpret_cast<const float4*>(st + col * MMA_F + 4 * lane) : make_float4(0, 0, 0, 0);
-                            finish4<T, ACT>(v, bias, res[i], p, c_base + c + col, f);
-                        }
-                    }
-                }
-                if (c + MMA_GROUPS * MMA_CHUNK < t.nc) load_residual(c + MMA_GROUPS * MMA_CHUNK);
-            }
-            if (product) {
-                // this half of TMEM is free for the tile after next, and the staging for the next
-                fence_before();
-                asm volatile("barrier.cta.sync %0, 128;" ::"r"(1 + group) : "memory");
-                if (lane == 0) bar_arrive_relaxed_at(leader_addr(&tempty[half]));
-            }
+            if (product) release(half);
             it += product;
         }
     }
@@ -584,17 +612,18 @@ int mma_launch(const CUtensorMap& a, const CUtensorMap& b, const MmaParams& p, i
     return launch_status();
 }
 
-// Columns per tile of the row passes: the least of 32, 64, 128, 256 that holds an
-// expert's share of the rows.  A smaller tile leaves more of the shared memory to
-// stages of the weights (10 of 18 KB at 32, 6 of 32 KB at 256), which is what a few
-// rows per expert wait for.
+// Columns per tile of the row passes: the least of 32, 64, 128, 256 that holds twice an
+// expert's share of the rows (loads are uneven, and an expert in two tiles has its
+// weights loaded twice).  A smaller tile leaves more of the shared memory to stages of
+// the weights (10 of 18 KB at 32, 6 or 7 of 32 KB at 256), which is what a few rows per
+// expert wait for.
 inline int columns_per_tile(int64_t R, int64_t E) {
     const int64_t share = (R + E - 1) / E;
-    return share <= 32 ? 32 : share <= 64 ? 64 : share <= 128 ? 128 : 256;
+    return share <= 16 ? 32 : share <= 32 ? 64 : share <= 64 ? 128 : 256;
 }
-inline int stages_for(int bn) {
-    const int n = (MMA_SMEM - 1024 - MMA_SMEM_FIXED) / (MMA_A_BYTES + bn / 2 * MMA_KB * 2);
-    return n < MMA_MAX_STAGES ? n : MMA_MAX_STAGES;
+inline int stages_for(int bn, int64_t E) {
+    const int64_t n = (MMA_SMEM - 1024 - MMA_SMEM_FIXED - 12 * E) / (MMA_A_BYTES + bn / 2 * MMA_KB * 2);
+    return (int)(n < MMA_MAX_STAGES ? n : MMA_MAX_STAGES);
 }
 
 }  // namespace ela_expert
