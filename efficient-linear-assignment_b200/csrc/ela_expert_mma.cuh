@@ -29,8 +29,8 @@
 //
 // Roles, in each CTA: warp 0 issues the TMA loads of the CTA's halves, which count on
 // the first CTA's barriers; warp 1 of the first CTA issues the MMAs of the pair; warp 2
-// owns the TMEM allocation; warps 4-11 run the epilogue while the next tile's MMAs fill
-// the other half of TMEM (2 x 256 columns).  A warp reads 32 columns of its 32 features
+// owns the TMEM allocation; warps 4-19 run the epilogue while the next tile's MMAs fill
+// the other half of TMEM (2 x 256 columns).  A warp reads 16 columns of its 32 features
 // at a time, one feature a lane; bias, activation and residual are applied in fp32, and
 // two neighbouring lanes swap halves so that each stores two consecutive features of
 // one column: a store instruction writes 64 bytes of two columns, whole sectors, with
@@ -53,8 +53,8 @@ constexpr int MMA_PAIR_F = 256;         // features per tile
 constexpr int MMA_C = 256;              // most columns per tile
 constexpr int MMA_KB = 64;              // k per stage: 128 bytes, one swizzle span
 constexpr int MMA_A_BYTES = MMA_F * MMA_KB * 2;
-constexpr int MMA_CHUNK = 32;           // columns an epilogue warp takes at a time
-constexpr int MMA_GROUPS = 2;           // epilogue warps per 32 TMEM lanes
+constexpr int MMA_CHUNK = 16;           // columns an epilogue warp takes at a time
+constexpr int MMA_GROUPS = 4;           // epilogue warps per 32 TMEM lanes
 constexpr int MMA_MAX_STAGES = 10;
 constexpr int MMA_THREADS = 128 + MMA_GROUPS * 128;
 constexpr int MMA_SMEM = 227 * 1024;
@@ -151,14 +151,11 @@ __device__ __forceinline__ void mma_issue(uint32_t d, uint64_t a, uint64_t b, ui
                  "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}"
                  ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"((uint32_t)accumulate) : "memory");
 }
-__device__ __forceinline__ void tmem_ld32(uint32_t addr, float* v) {
+__device__ __forceinline__ void tmem_ld16(uint32_t addr, float* v) {
     uint32_t* r = reinterpret_cast<uint32_t*>(v);
-    asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
-                 "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
                  : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
-                   "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
-                   "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]),
-                   "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+                   "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
                  : "r"(addr));
     asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 }
@@ -261,20 +258,22 @@ template <> __device__ __forceinline__ float2 unpack2<__nv_bfloat16>(uint32_t p)
 
 // One chunk of a warp: v[j] is feature f (this lane's) of column c + j, j < left.  The
 // lane's residual words are those of swap_pair's layout (loaded by load_residual).
+// Columns are a 32-bit number of bytes apart (F < 2^30 elements of two bytes).
 template <typename T, int ACT, bool Z, bool RES>
 __device__ __forceinline__ void finish(float* v, float bias, const uint32_t* res, const MmaParams& p, int64_t c, int f, int left) {
     const bool odd = threadIdx.x & 1;
     if (p.vec) {
-        const int64_t at = (c + odd) * p.F + (f & ~1), step = 2 * (int64_t)p.F;
-        uint32_t* out = reinterpret_cast<uint32_t*>(reinterpret_cast<T*>(p.out) + at);
-        uint32_t* zout = reinterpret_cast<uint32_t*>(reinterpret_cast<T*>(p.z) + at);
+        const int64_t at = (c + odd) * p.F + (f & ~1);
+        char* out = reinterpret_cast<char*>(reinterpret_cast<T*>(p.out) + at);
+        char* zout = reinterpret_cast<char*>(reinterpret_cast<T*>(p.z) + at);
+        const uint32_t step = (uint32_t)p.F * 2;
         const int mine = f < p.F ? left - odd : 0;  // (F is even: both lanes of a pair are in or out)
 #pragma unroll
         for (int j = 0; j < MMA_CHUNK; j += 2) {
             float a = v[j] + bias, b = v[j + 1] + bias;
             if (Z) {
                 const uint32_t w = swap_pair(pack2<T>(a, b), odd);
-                if (j < mine) zout[j / 2 * (step / 2)] = w;
+                if (j < mine) *reinterpret_cast<uint32_t*>(zout + (uint64_t)step * j) = w;
             }
             a = act_value<ACT>(a);
             b = act_value<ACT>(b);
@@ -284,7 +283,7 @@ __device__ __forceinline__ void finish(float* v, float bias, const uint32_t* res
                 b += r.y;
             }
             const uint32_t w = swap_pair(pack2<T>(a, b), odd);
-            if (j < mine) out[j / 2 * (step / 2)] = w;
+            if (j < mine) *reinterpret_cast<uint32_t*>(out + (uint64_t)step * j) = w;
         }
     } else if (f < p.F) {
 #pragma unroll
@@ -506,6 +505,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(MMA_THREADS, 1)
         Tile t;
         int it = 0;
         bool ok = true;
+        constexpr bool FWD = PASS == PASS_FORWARD;
         const bool with_z = PASS == PASS_FORWARD && p.z, with_res = PASS == PASS_FORWARD && p.residual;
         auto accumulators = [&](int half, int it) {  // waits for the tile's products
             if (lane == 0) ok = bar_wait(&tfull[half], (it >> 1) & 1, p.wait_ns, abort);
@@ -522,10 +522,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(MMA_THREADS, 1)
         };
         auto write = [&](float* v, float bias, const uint32_t* res, int64_t c, int f, int left) {
             if (with_z) {
-                if (with_res) finish<T, ACT, true, true>(v, bias, res, p, c, f, left);
-                else finish<T, ACT, true, false>(v, bias, res, p, c, f, left);
+                if (with_res) finish<T, ACT, FWD, FWD>(v, bias, res, p, c, f, left);
+                else finish<T, ACT, FWD, false>(v, bias, res, p, c, f, left);
             } else {
-                if (with_res) finish<T, ACT, false, true>(v, bias, res, p, c, f, left);
+                if (with_res) finish<T, ACT, false, FWD>(v, bias, res, p, c, f, left);
                 else finish<T, ACT, false, false>(v, bias, res, p, c, f, left);
             }
         };
@@ -542,7 +542,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(MMA_THREADS, 1)
             for (int c = group * MMA_CHUNK; c < t.nc; c += MMA_GROUPS * MMA_CHUNK) {
                 float v[MMA_CHUNK] = {};
                 __syncwarp();
-                if (product) tmem_ld32(tmem + ((uint32_t)(32 * w) << 16) + half * MMA_C + c, v);
+                if (product) tmem_ld16(tmem + ((uint32_t)(32 * w) << 16) + half * MMA_C + c, v);
                 write(v, bias, res, c_base + c, f, t.nc - c);
                 const int next = c + MMA_GROUPS * MMA_CHUNK;
                 if (with_res && next < t.nc) load_residual<T>(res, p, c_base + next, f, t.nc - next);
