@@ -17,7 +17,7 @@ CSRC = os.path.join(PKG_DIR, "csrc")
 SOURCES = {
     "ela_auction.cu": ["ela_implicit.cuh"],
     "ela_expert.cu": ["ela_expert.cuh"],
-    "ela_expert_linear.cu": ["ela_expert.cuh", "ela_expert_mma.cuh"],
+    "ela_expert_linear.cu": ["ela_expert.cuh", "ela_expert_mma.cuh", "ela_expert_stream.cuh"],
 }
 OUT = os.path.join(PKG_DIR, "libela_auction.so")
 INCLUDE = os.path.join(REPO_DIR, "include")

@@ -8,6 +8,7 @@
 
 #include "ela_expert.cuh"
 #include "ela_expert_mma.cuh"
+#include "ela_expert_stream.cuh"
 
 namespace ela_expert {
 
@@ -231,7 +232,7 @@ size_t ela_expert_linear_workspace_bytes(int pass, int64_t R, int64_t E, int64_t
         const int rows = act_block_rows(R, N);
         return (size_t)((R + rows - 1) / rows + E) * N * 4;
     }
-    if (aligned) return 0;
+    if (aligned || (pass == ELA_LINEAR_FORWARD && few_rows(R, E))) return 0;
     const Matrix x = {nullptr, 1, R, K, 0, 0}, w = {nullptr, E, N, K, 0, 0}, dz = {nullptr, 1, R, N, 0, 0};
     return pass == ELA_LINEAR_FORWARD ? x.padded_bytes() + w.padded_bytes()
          : pass == ELA_LINEAR_GRAD_INPUT ? dz.padded_bytes() + w.padded_bytes()
@@ -256,6 +257,15 @@ int ela_expert_linear(const void* x, const void* weight, const void* bias, const
     if (R == 0) return ELA_OK;
     if (!x || !weight || !y) return ELA_ERR_ARGUMENT;
     cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+    if (few_rows(R, E)) {
+        StreamParams q = {x, weight, bias, residual, offsets, (int)R, (int)E, (int)K, (int)N, 0, ldx, stride_e, ldw, ldr, y, z};
+        const uint64_t bits = reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(weight) | (uint64_t)(ldx * 2) | (uint64_t)(ldw * 2) |
+                              (uint64_t)(E > 1 ? stride_e * 2 : 0) | (uint64_t)(K * 2);
+        const int vb = bits % 32 == 0 ? 32 : bits % 16 == 0 ? 16 : bits % 4 == 0 ? 4 : 2;
+        int rc = ELA_OK;
+        ELA_BY_TYPE(dtype, { ELA_BY_ACT(activation, rc = R <= 4 * E || (E == 1 && R <= 8) ? (stream_launch<T_, A_, 1>(q, vb, st)) : (stream_launch<T_, A_, 2>(q, vb, st))) })
+        return rc;
+    }
     char* ws = reinterpret_cast<char*>(workspace);
     Matrix mx = {x, 1, R, K, ldx, 0}, mw = {weight, E, N, K, ldw, stride_e};
     int rc = readable(mx, ws, workspace_bytes, st);

@@ -119,8 +119,8 @@ __device__ __forceinline__ bool bar_wait(uint64_t* b, uint32_t parity, unsigned 
     unsigned long long t0 = 0;
     for (uint32_t spins = 1;; ++spins) {
         uint32_t done;
-        asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
-                     : "=r"(done) : "r"(a), "r"(parity) : "memory");
+        asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+                     : "=r"(done) : "r"(a), "r"(parity), "r"(20000) : "memory");  // sleeps up to 20 us
         if (done) return true;
         if ((spins & 15u) == 0) {
             unsigned long long t;
