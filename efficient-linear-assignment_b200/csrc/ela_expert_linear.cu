@@ -15,13 +15,28 @@ namespace ela_expert {
 constexpr unsigned long long LINEAR_WAIT_NS = 2000000000ull;  // limit of every device-side wait
 
 // Rows of any stride and alignment copied to rows a multiple of 16 bytes apart
-// (TMA's rule for strides and base).  Bits are moved, types do not matter.
-__global__ void __launch_bounds__(256) realign_kernel(const uint16_t* src, int64_t rows, int64_t cols, int64_t ld,
+// (TMA's rule for strides and base).  Bits are moved, types do not matter.  A thread
+// writes 16 bytes; where the source is off a 4-byte boundary it reads the five words
+// around them (no word is touched that does not hold an element of the row).
+__global__ void __launch_bounds__(256) realign_kernel(const uint16_t* src, int64_t rows, int cols, int64_t ld,
                                                       int64_t rows_per_matrix, int64_t stride_e, uint16_t* dst, int64_t ldd) {
-    for (int64_t r = blockIdx.x; r < rows; r += gridDim.x) {
-        const uint16_t* s = src + r / rows_per_matrix * stride_e + r % rows_per_matrix * ld;
-        uint16_t* d = dst + r * ldd;
-        for (int64_t c = threadIdx.x; c < cols; c += blockDim.x) d[c] = s[c];
+    const int pieces = (cols + 7) / 8;
+    const int64_t all = rows * pieces;
+    for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < all; i += (int64_t)gridDim.x * blockDim.x) {
+        const int64_t r = i / pieces;
+        const int c = (int)(i - r * pieces) * 8, left = cols - c;
+        const uint16_t* s = src + r / rows_per_matrix * stride_e + r % rows_per_matrix * ld + c;
+        const bool shift = (reinterpret_cast<uintptr_t>(s) & 3) != 0;
+        const uint32_t* w = reinterpret_cast<const uint32_t*>(s - shift);
+        uint32_t v[5];
+#pragma unroll
+        for (int k = 0; k < 5; ++k) v[k] = 2 * k - shift < left && (k < 4 || shift) ? __ldg(w + k) : 0u;
+        uint4 o;
+        o.x = shift ? __funnelshift_r(v[0], v[1], 16) : v[0];
+        o.y = shift ? __funnelshift_r(v[1], v[2], 16) : v[1];
+        o.z = shift ? __funnelshift_r(v[2], v[3], 16) : v[2];
+        o.w = shift ? __funnelshift_r(v[3], v[4], 16) : v[3];
+        *reinterpret_cast<uint4*>(dst + r * ldd + c) = o;  // (ldd is cols rounded up to 8)
     }
 }
 
@@ -42,7 +57,8 @@ inline int readable(Matrix& m, char*& ws, size_t& left, cudaStream_t st) {
     const size_t need = m.padded_bytes();
     if (!ws || left < need) return ELA_ERR_ARGUMENT;
     const int64_t rows = m.matrices * m.rows, ld = round8(m.cols);
-    realign_kernel<<<(unsigned)(rows < 4096 ? rows : 4096), 256, 0, st>>>((const uint16_t*)m.p, rows, m.cols, m.ld, m.rows, m.stride_e,
+    const int64_t blocks = (rows * (ld / 8) + 255) / 256, most = 8 * (int64_t)sm_count();
+    realign_kernel<<<(unsigned)(blocks < most ? blocks : most), 256, 0, st>>>((const uint16_t*)m.p, rows, (int)m.cols, m.ld, m.rows, m.stride_e,
                                                                          (uint16_t*)ws, ld);
     m.p = ws;
     m.ld = ld;

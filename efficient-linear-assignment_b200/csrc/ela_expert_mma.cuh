@@ -29,7 +29,7 @@
 //
 // Roles, in each CTA: warp 0 issues the TMA loads of the CTA's halves, which count on
 // the first CTA's barriers; warp 1 of the first CTA issues the MMAs of the pair; warp 2
-// owns the TMEM allocation; warps 4-19 run the epilogue while the next tile's MMAs fill
+// owns the TMEM allocation; warp 3 works out the tiles; warps 4-19 run the epilogue while the next tile's MMAs fill
 // the other half of TMEM (2 x 256 columns).  A warp reads 16 columns of its 32 features
 // at a time, one feature a lane; bias, activation and residual are applied in fp32, and
 // two neighbouring lanes swap halves so that each stores two consecutive features of
@@ -59,6 +59,7 @@ constexpr int MMA_MAX_STAGES = 10;
 constexpr int MMA_THREADS = 128 + MMA_GROUPS * 128;
 constexpr int MMA_SMEM = 227 * 1024;
 constexpr int MMA_SMEM_FIXED = 1024;    // alignment of the first stage
+constexpr int MMA_TILES = 4;            // tiles the scheduling warp is ahead
 constexpr int MMA_GROUP = 16;           // column tiles walked together, for L2 reuse of both operands
 
 struct MmaParams {
@@ -189,7 +190,7 @@ struct Plan {
 // Row passes: experts in order; within an expert, groups of MMA_GROUP column tiles,
 // feature tiles within a group, columns innermost.  Weight gradient: the same with the
 // output features as columns.  The offsets, and so the tiles, are only known on the
-// device: every role asks for the tiles by number (the whole warp calls).
+// device.  The whole warp calls.
 template <int PASS> __device__ __forceinline__ bool get_tile(const MmaParams& p, const Plan& plan, int t, Tile& out) {
     if (t >= plan.tiles) return false;
     int local, ct, r0, r1;
@@ -237,9 +238,8 @@ template <int PASS> __device__ __forceinline__ bool get_tile(const MmaParams& p,
 // Lanes 2i and 2i+1 hold features f and f+1 of columns c (low half of p) and c+1 (high
 // half).  After the swap the even lane has f, f+1 of column c, the odd lane of column
 // c+1, which is how memory has them; it is its own inverse.
-__device__ __forceinline__ uint32_t swap_pair(uint32_t p, bool odd) {
-    const uint32_t o = __shfl_xor_sync(~0u, p, 1);
-    return __byte_perm(p, o, odd ? 0x3276 : 0x5410);
+__device__ __forceinline__ uint32_t swap_pair(uint32_t p, uint32_t order) {
+    return __byte_perm(p, __shfl_xor_sync(~0u, p, 1), order);
 }
 template <typename T> __device__ __forceinline__ uint32_t pack2(float lo, float hi);
 template <> __device__ __forceinline__ uint32_t pack2<__half>(float lo, float hi) {
@@ -258,38 +258,43 @@ template <> __device__ __forceinline__ float2 unpack2<__nv_bfloat16>(uint32_t p)
 
 // One chunk of a warp: v[j] is feature f (this lane's) of column c + j, j < left.  The
 // lane's residual words are those of swap_pair's layout (loaded by load_residual).
-// Columns are a 32-bit number of bytes apart (F < 2^30 elements of two bytes).
-template <typename T, int ACT, bool Z, bool RES>
+// Addresses go from pair to pair of columns by one 64-bit addition: written as a product
+// with j they made most of the epilogue's instructions.
+template <typename T, int ACT, bool BIAS, bool Z, bool RES>
 __device__ __forceinline__ void finish(float* v, float bias, const uint32_t* res, const MmaParams& p, int64_t c, int f, int left) {
     const bool odd = threadIdx.x & 1;
+    const uint32_t order = odd ? 0x3276 : 0x5410;
     if (p.vec) {
         const int64_t at = (c + odd) * p.F + (f & ~1);
         char* out = reinterpret_cast<char*>(reinterpret_cast<T*>(p.out) + at);
         char* zout = reinterpret_cast<char*>(reinterpret_cast<T*>(p.z) + at);
-        const uint32_t step = (uint32_t)p.F * 2;
+        const int64_t step = 4 * (int64_t)p.F;
         const int mine = f < p.F ? left - odd : 0;  // (F is even: both lanes of a pair are in or out)
 #pragma unroll
         for (int j = 0; j < MMA_CHUNK; j += 2) {
-            float a = v[j] + bias, b = v[j + 1] + bias;
+            float a = v[j], b = v[j + 1];
+            if (BIAS) { a += bias; b += bias; }
             if (Z) {
-                const uint32_t w = swap_pair(pack2<T>(a, b), odd);
-                if (j < mine) *reinterpret_cast<uint32_t*>(zout + (uint64_t)step * j) = w;
+                const uint32_t w = swap_pair(pack2<T>(a, b), order);
+                if (j < mine) *reinterpret_cast<uint32_t*>(zout) = w;
+                zout += step;
             }
             a = act_value<ACT>(a);
             b = act_value<ACT>(b);
             if (RES) {
-                const float2 r = unpack2<T>(swap_pair(res[j / 2], odd));
+                const float2 r = unpack2<T>(swap_pair(res[j / 2], order));
                 a += r.x;
                 b += r.y;
             }
-            const uint32_t w = swap_pair(pack2<T>(a, b), odd);
-            if (j < mine) *reinterpret_cast<uint32_t*>(out + (uint64_t)step * j) = w;
+            const uint32_t w = swap_pair(pack2<T>(a, b), order);
+            if (j < mine) *reinterpret_cast<uint32_t*>(out) = w;
+            out += step;
         }
     } else if (f < p.F) {
 #pragma unroll
         for (int j = 0; j < MMA_CHUNK; ++j)
             if (j < left) {
-                const float a = v[j] + bias;
+                const float a = BIAS ? v[j] + bias : v[j];
                 const int64_t at = (c + j) * p.F + f;
                 if (Z) reinterpret_cast<T*>(p.z)[at] = El<T>::from(a);
                 const float r = RES ? El<T>::to(reinterpret_cast<const T*>(p.residual)[(c + j) * p.ldr + f]) : 0.f;
@@ -304,7 +309,7 @@ __device__ __forceinline__ void load_residual(uint32_t* res, const MmaParams& p,
     const uint32_t* at = reinterpret_cast<const uint32_t*>(reinterpret_cast<const T*>(p.residual) + (c + odd) * p.ldr + (f & ~1));
     const int mine = p.vec && f < p.F ? left - odd : 0;
 #pragma unroll
-    for (int j = 0; j < MMA_CHUNK; j += 2) res[j / 2] = j < mine ? __ldg(at + j / 2 * p.ldr) : 0u;
+    for (int j = 0; j < MMA_CHUNK; j += 2, at += p.ldr) res[j / 2] = j < mine ? __ldg(at) : 0u;
 }
 
 template <int PASS, typename T, int ACT>
@@ -313,11 +318,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(MMA_THREADS, 1)
     constexpr bool A_K_MAJOR = PASS == PASS_FORWARD, B_K_MAJOR = PASS != PASS_WEIGHT;
     extern __shared__ unsigned char smem_raw[];
     // full, tempty, patched: the first CTA's are used; empty, tfull, landed: each CTA its own
-    __shared__ __align__(8) uint64_t full[MMA_MAX_STAGES], empty[MMA_MAX_STAGES], tfull[2], tempty[2], landed, patched, drained;
+    __shared__ __align__(8) uint64_t full[MMA_MAX_STAGES], empty[MMA_MAX_STAGES], tfull[2], tempty[2], sfull[MMA_TILES], sempty[MMA_TILES], landed, patched, drained;
     __shared__ uint32_t s_tmem;
     __shared__ int s_abort;
     __shared__ uint32_t s_issued;
     __shared__ int s_tiles;
+    __shared__ Tile s_tile[MMA_TILES];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int rank = blockIdx.x & 1, pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
     // the experts' tables, then the stages, each on a 1024-byte boundary
@@ -326,6 +332,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(MMA_THREADS, 1)
     const int stage_bytes = MMA_A_BYTES + p.bn / 2 * MMA_KB * 2;
     const volatile int* abort = &s_abort;
 
+    if (tid == 32) {
+        asm volatile("prefetch.tensormap [%0];" ::"l"(&map_a) : "memory");
+        asm volatile("prefetch.tensormap [%0];" ::"l"(&map_b) : "memory");
+    }
     if (warp == 2) {
         asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(saddr(&s_tmem)) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
@@ -334,6 +344,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(MMA_THREADS, 1)
         s_abort = 0;
         for (int s = 0; s < p.stages; ++s) { bar_init(&full[s], 1); bar_init(&empty[s], 1); }
         for (int b = 0; b < 2; ++b) { bar_init(&tfull[b], 1); bar_init(&tempty[b], 2 * 4 * MMA_GROUPS); }
+        for (int i = 0; i < MMA_TILES; ++i) { bar_init(&sfull[i], 1); bar_init(&sempty[i], 4 * MMA_GROUPS + 1 + (rank == 0)); }
         bar_init(&landed, 1);
         bar_init(&patched, 1);
         bar_init(&drained, 1);
@@ -367,13 +378,46 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(MMA_THREADS, 1)
         atomicExch(&g_expert_error, ELA_ERR_TIMEOUT);
     };
 
+    // The i-th tile of this pair from the scheduling warp; false: none left, or a wait gave up (ok).
+    auto fetch = [&](int i, Tile& t, bool& ok) {
+        const int slot = i % MMA_TILES;
+        int good = 0;
+        if (lane == 0) good = bar_wait(&sfull[slot], (i / MMA_TILES) & 1, p.wait_ns, abort);
+        ok = __shfl_sync(~0u, good, 0);
+        __syncwarp();
+        if (!ok) { if (lane == 0) give_up(); return false; }
+        t = s_tile[slot];
+        __syncwarp();
+        if (lane == 0) bar_arrive(&sempty[slot]);
+        return t.e >= 0;
+    };
+
     uint32_t issued = 0;  // stages loaded (by the loading lane)
-    if (warp == 0) {  // ---- loads of this CTA's features and its half of the columns
+    if (warp == 3) {  // ---- tiles, a few ahead: their index arithmetic would cost each role 1000 cycles a tile
+        bool ok = true, left = true;
+        for (int i = 0, n = pair; ok && left; ++i, n += pairs) {
+            const int slot = i % MMA_TILES;
+            Tile t;
+            left = get_tile<PASS>(p, plan, n, t);
+            int good = 0;
+            if (lane == 0) {
+                good = bar_wait(&sempty[slot], ((i / MMA_TILES) & 1) ^ 1, p.wait_ns, abort);
+                if (good) {
+                    if (!left) t.e = -1;
+                    s_tile[slot] = t;
+                    bar_arrive(&sfull[slot]);
+                } else {
+                    give_up();
+                }
+            }
+            ok = __shfl_sync(~0u, good, 0);
+        }
+    } else if (warp == 0) {  // ---- loads of this CTA's features and its half of the columns
         Tile t;
         int s = 0;
         uint32_t phase = 0, landings = 0;
         bool ok = true;
-        for (int n = pair; ok && get_tile<PASS>(p, plan, n, t); n += pairs) {
+        for (int i = 0; ok && fetch(i, t, ok); ++i) {
             const int f0 = t.f0 + rank * MMA_F;
             // column operand: boxes of p.bbox rows (K-major) or of 64 columns (MN-major)
             const int half = ((t.nc + 31) & ~31) >> 1, c0 = t.c0 + rank * half;
@@ -428,8 +472,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(MMA_THREADS, 1)
                 ++landings;
                 unsigned char* a = smem + (size_t)s * stage_bytes;
                 const int pieces = (16 - (tail & 15)) * 8;  // A's two boxes, then B's, 8192 bytes each
-                for (int i = lane; i < (2 + boxes) * pieces; i += 32)
-                    *reinterpret_cast<uint4*>(a + (size_t)(i / pieces) * 8192 + tail * 128 + i % pieces * 16) = make_uint4(0, 0, 0, 0);
+                for (int j = lane; j < (2 + boxes) * pieces; j += 32)
+                    *reinterpret_cast<uint4*>(a + (size_t)(j / pieces) * 8192 + tail * 128 + j % pieces * 16) = make_uint4(0, 0, 0, 0);
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                 __syncwarp();
                 if (lane == 0) {
@@ -456,7 +500,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(MMA_THREADS, 1)
         bool ok = true;
         const uint64_t a_desc = operand_desc(saddr(smem), A_K_MAJOR), b_desc = operand_desc(saddr(smem) + MMA_A_BYTES, B_K_MAJOR);
         constexpr int A_STEP = A_K_MAJOR ? 2 : 128, B_STEP = B_K_MAJOR ? 2 : 128;  // 16 k, in 16-byte units
-        for (int n = pair; ok && get_tile<PASS>(p, plan, n, t); n += pairs) {
+        for (int i = 0; ok && fetch(i, t, ok); ++i) {
             const int blocks = (t.nk + MMA_KB - 1) / MMA_KB;
             if (blocks == 0) continue;  // an expert without rows: the epilogue writes its zeros
             if (elect_one()) {
@@ -522,14 +566,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(MMA_THREADS, 1)
         };
         auto write = [&](float* v, float bias, const uint32_t* res, int64_t c, int f, int left) {
             if (with_z) {
-                if (with_res) finish<T, ACT, FWD, FWD>(v, bias, res, p, c, f, left);
-                else finish<T, ACT, FWD, false>(v, bias, res, p, c, f, left);
+                if (with_res) finish<T, ACT, FWD, FWD, FWD>(v, bias, res, p, c, f, left);
+                else finish<T, ACT, FWD, FWD, false>(v, bias, res, p, c, f, left);
             } else {
-                if (with_res) finish<T, ACT, false, FWD>(v, bias, res, p, c, f, left);
-                else finish<T, ACT, false, false>(v, bias, res, p, c, f, left);
+                if (with_res) finish<T, ACT, FWD, false, FWD>(v, bias, res, p, c, f, left);
+                else finish<T, ACT, FWD, false, false>(v, bias, res, p, c, f, left);
             }
         };
-        for (int n = pair; ok && get_tile<PASS>(p, plan, n, t); n += pairs) {
+        for (int i = 0; ok && fetch(i, t, ok); ++i) {
             const bool product = t.nk > 0;
             const int half = it & 1;
             const int f = t.f0 + rank * MMA_F + 32 * w + lane;
@@ -540,9 +584,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(MMA_THREADS, 1)
             if (with_res) load_residual<T>(res, p, c_base + group * MMA_CHUNK, f, t.nc - group * MMA_CHUNK);
             if (product && !accumulators(half, it)) break;
             for (int c = group * MMA_CHUNK; c < t.nc; c += MMA_GROUPS * MMA_CHUNK) {
-                float v[MMA_CHUNK] = {};
+                float v[MMA_CHUNK];
                 __syncwarp();
-                if (product) tmem_ld16(tmem + ((uint32_t)(32 * w) << 16) + half * MMA_C + c, v);
+                if (product) {
+                    tmem_ld16(tmem + ((uint32_t)(32 * w) << 16) + half * MMA_C + c, v);
+                } else {
+#pragma unroll
+                    for (int j = 0; j < MMA_CHUNK; ++j) v[j] = 0.f;
+                }
                 write(v, bias, res, c_base + c, f, t.nc - c);
                 const int next = c + MMA_GROUPS * MMA_CHUNK;
                 if (with_res && next < t.nc) load_residual<T>(res, p, c_base + next, f, t.nc - next);
