@@ -75,6 +75,7 @@ __global__ void __launch_bounds__(PLAN_THREADS, 1) plan_kernel(const Id* expert,
     __syncthreads();
     for (int b = tid; b < B; b += blockDim.x) {
         int sum = 0;
+#pragma unroll 8
         for (int w = 0; w < nwarps; ++w) sum += shared[w * B + b];
         total[b] = sum;
     }
@@ -82,9 +83,16 @@ __global__ void __launch_bounds__(PLAN_THREADS, 1) plan_kernel(const Id* expert,
     // buckets in runs, one run a thread: slots of lower buckets, and of this one in earlier CTAs
     const int run = (B + blockDim.x - 1) / blockDim.x;
     const int b0 = min(tid * run, B), b1 = min(b0 + run, B);
-    int sum = 0;
-    for (int b = b0; b < b1; ++b)
-        for (int r = 0; r < ctas; ++r) sum += r == rank ? total[b] : peer_read(total + b, r);
+    auto totals = [&](int b, int* c) {  // every CTA's, all reads in flight at once
+#pragma unroll
+        for (int r = 0; r < PLAN_CLUSTER; ++r) c[r] = r >= ctas ? 0 : r == rank ? total[b] : peer_read(total + b, r);
+    };
+    int sum = 0, c[PLAN_CLUSTER];
+    for (int b = b0; b < b1; ++b) {
+        totals(b, c);
+#pragma unroll
+        for (int r = 0; r < PLAN_CLUSTER; ++r) sum += c[r];
+    }
     int incl = sum;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -97,16 +105,18 @@ __global__ void __launch_bounds__(PLAN_THREADS, 1) plan_kernel(const Id* expert,
     for (int w = 0; w < warp; ++w) base += warp_sum[w];
     for (int b = b0; b < b1; ++b) {
         if (rank == 0) offsets[b] = base;
+        if (run > 1) totals(b, c);
         int at = base;
-        for (int r = 0; r < ctas; ++r) {
-            const int c = r == rank ? total[b] : peer_read(total + b, r);
-            if (r < rank) at += c;
-            base += c;
+#pragma unroll
+        for (int r = 0; r < PLAN_CLUSTER; ++r) {
+            if (r < rank) at += c[r];
+            base += c[r];
         }
+#pragma unroll 8
         for (int w = 0; w < nwarps; ++w) {
-            const int c = shared[w * B + b];
+            const int n = shared[w * B + b];
             shared[w * B + b] = at;
-            at += c;
+            at += n;
         }
     }
     if (ctas > 1) plan_cluster_sync(); else __syncthreads();  // (peers have read this CTA's totals)

@@ -289,6 +289,11 @@ int ela_expert_linear(const void* x, const void* weight, const void* bias, const
     if (rc != ELA_OK) return rc;
     MmaParams p = row_pass(offsets, R, E, N, K);
     p.bias = bias;
+    p.x = mx.p;
+    p.ldx = mx.ld;
+    p.weight = mw.p;
+    p.ldw = mw.ld;
+    p.stride_e = mw.stride_e;
     p.residual = residual;
     p.ldr = ldr;
     p.out = y;

@@ -16,6 +16,7 @@
 #include <torch/csrc/autograd/custom_function.h>
 #include <ATen/ATen.h>
 #include <ATen/core/dispatch/Dispatcher.h>
+#include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 
@@ -55,8 +56,15 @@ Tensor rows_of(const Tensor& t) {
 }
 int64_t ld(const Tensor& t) { return t.size(0) > 1 ? t.stride(0) : t.size(-1); }
 
+// An uninitialised tensor on like's device from the caching allocator (straight from it:
+// at::empty's dispatch costs as much again).
+Tensor fresh(at::IntArrayRef sizes, at::ScalarType type, const Tensor& like) {
+    return at::detail::empty_cuda(sizes, type, like.device(), std::nullopt);
+}
+Tensor fresh(at::IntArrayRef sizes, const Tensor& like) { return fresh(sizes, like.scalar_type(), like); }
+
 Tensor workspace(size_t bytes, const Tensor& like) {
-    return bytes ? at::empty({(int64_t)bytes}, like.options().dtype(at::kByte)) : Tensor();
+    return bytes ? fresh({(int64_t)bytes}, at::kByte, like) : Tensor();
 }
 
 void no_second_derivative() {
@@ -72,9 +80,8 @@ std::tuple<Tensor, Tensor, Tensor> plan(const Tensor& expert_in, int64_t E) {
     TORCH_CHECK_VALUE(expert_in.numel() <= INT32_MAX, "expert_plan: more than 2^31 - 1 choices");
     c10::cuda::CUDAGuard guard(expert_in.device());
     const Tensor expert = expert_in.contiguous();
-    const auto opt = expert.options().dtype(at::kInt);
-    Tensor offsets = at::empty({E + 1}, opt), source = at::empty({expert.numel()}, opt);
-    Tensor position = at::empty({expert.size(0), expert.dim() == 1 ? 1 : expert.size(1)}, opt);
+    Tensor offsets = fresh({E + 1}, at::kInt, expert), source = fresh({expert.numel()}, at::kInt, expert);
+    Tensor position = fresh({expert.size(0), expert.dim() == 1 ? 1 : expert.size(1)}, at::kInt, expert);
     const size_t bytes = ela_expert_plan_workspace_bytes(expert.numel(), E);
     Tensor ws = workspace(bytes, expert);
     check_rc(ela_expert_plan(expert.data_ptr(), (int)expert.element_size(), expert.numel(), E, offsets.data_ptr<int32_t>(),
@@ -99,7 +106,7 @@ Tensor dispatch_raw(const Tensor& x_in, const Tensor& position, const Tensor& of
     const int code = code_of(x_in);
     c10::cuda::CUDAGuard guard(x_in.device());
     const Tensor x = rows_of(x_in);
-    Tensor rows = at::empty({position.numel(), x.size(1)}, x.options());
+    Tensor rows = fresh({position.numel(), x.size(1)}, x);
     check_rc(ela_expert_dispatch(x.data_ptr(), code, x.size(0), position.size(1), x.size(1), ld(x),
                                  position.data_ptr<int32_t>(), offsets.data_ptr<int32_t>(), offsets.numel() - 1,
                                  rows.data_ptr(), stream_of(x)),
@@ -119,7 +126,7 @@ Tensor combine_raw(const Tensor& y_in, const Tensor& position, const Tensor& off
     c10::cuda::CUDAGuard guard(y_in.device());
     const Tensor y = rows_of(y_in);
     const OptTensor w = weights.has_value() ? OptTensor(weights->contiguous()) : OptTensor();
-    Tensor out = at::empty({position.size(0), y.size(1)}, y.options());
+    Tensor out = fresh({position.size(0), y.size(1)}, y);
     check_rc(ela_expert_combine(y.data_ptr(), code, position.size(0), position.size(1), y.size(1), ld(y),
                                 position.data_ptr<int32_t>(), offsets.data_ptr<int32_t>(), offsets.numel() - 1, ptr(w),
                                 w.has_value() ? code_of(*w) : ELA_DTYPE_F32, out.data_ptr(), stream_of(y)),
@@ -134,8 +141,8 @@ std::tuple<Tensor, Tensor> combine_grad_raw(const Tensor& dout_in, const OptTens
     const OptTensor y = y_in.has_value() ? OptTensor(rows_of(*y_in)) : OptTensor();
     const OptTensor w = weights.has_value() ? OptTensor(weights->contiguous()) : OptTensor();
     c10::cuda::CUDAGuard guard(dout.device());
-    Tensor dy = at::empty({need_y ? position.numel() : 0, dout.size(1)}, dout.options());
-    Tensor dw = need_w ? at::empty(w->sizes(), w->options()) : at::empty({0}, dout.options());
+    Tensor dy = fresh({need_y ? position.numel() : 0, dout.size(1)}, dout);
+    Tensor dw = need_w ? fresh(w->sizes(), *w) : fresh({0}, dout);
     check_rc(ela_expert_combine_grad(dout.data_ptr(), ptr(y), code_of(dout), position.size(0), position.size(1),
                                      dout.size(1), ld(dout), y.has_value() ? ld(*y) : 0, position.data_ptr<int32_t>(),
                                      offsets.data_ptr<int32_t>(), offsets.numel() - 1, ptr(w),
@@ -214,8 +221,8 @@ std::tuple<Tensor, Tensor> linear_raw(const Tensor& x, const Tensor& weight, con
     c10::cuda::CUDAGuard guard(x.device());
     const OptTensor b = bias.has_value() ? OptTensor(bias->contiguous()) : OptTensor();
     const OptTensor r = residual.has_value() ? OptTensor(rows_of(*residual)) : OptTensor();
-    Tensor y = at::empty({s.R, s.N}, s.x.options());
-    Tensor z = at::empty({want_z ? s.R : 0, s.N}, s.x.options());  // rows of no expert stay unwritten
+    Tensor y = fresh({s.R, s.N}, s.x);
+    Tensor z = fresh({want_z ? s.R : 0, s.N}, s.x);  // rows of no expert stay unwritten
     const int al = aligned(s.x, ld(s.x)) && aligned(s.w, s.ldw, s.stride_e);
     const size_t bytes = ela_expert_linear_workspace_bytes(ELA_LINEAR_FORWARD, s.R, s.E, s.K, s.N, al);
     Tensor ws = workspace(bytes, x);
@@ -236,13 +243,13 @@ std::tuple<Tensor, Tensor, Tensor> linear_grad_raw(const Tensor& dy_in, const Op
     const int64_t R = dy.size(0), N = dy.size(1), K = wsizes.back(), E = wsizes.size() == 3 ? wsizes[0] : 1;
     const int code = code_of(dy);
     void* stream = stream_of(dy);
-    Tensor dx = at::empty({need_x ? R : 0, K}, dy.options());
-    Tensor dw = need_w ? at::empty(wsizes, dy.options()) : at::empty({0}, dy.options());
-    Tensor db = need_b ? at::empty(bsizes, dy.options()) : at::empty({0}, dy.options());
+    Tensor dx = fresh({need_x ? R : 0, K}, dy);
+    Tensor dw = need_w ? fresh(wsizes, dy) : fresh({0}, dy);
+    Tensor db = need_b ? fresh(bsizes, dy) : fresh({0}, dy);
     Tensor dz = dy;
     if (need_b || act != ELA_ACT_NONE) {
         const bool write = act != ELA_ACT_NONE && (need_x || need_w);
-        if (write) dz = at::empty_like(dy);
+        if (write) dz = fresh(dy.sizes(), dy);
         const size_t bytes = ela_expert_linear_workspace_bytes(ELA_LINEAR_GRAD_ACT, R, E, K, N, 1);
         Tensor ws = workspace(bytes, dy);
         check_rc(ela_expert_linear_grad_act(dy.data_ptr(), ptr(z), off_ptr(offsets), code, R, E, N, (int)act,
