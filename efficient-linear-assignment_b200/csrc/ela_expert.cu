@@ -8,14 +8,14 @@ namespace ela_expert {
 
 // ------------------------------------------------------------------- plan
 // A stable counting sort by one cluster of CTAs.  Every warp of the cluster owns a
-// contiguous range of slots and walks it 32 at a time: the lanes of one bucket
-// (__match_any_sync) rank themselves in lane order behind the warp's counter of that
-// bucket, so a slot's rank inside its warp's range is known when the ranges have been
+// contiguous range of slots and walks it 32 at a time: the lanes of one bucket (found by
+// a ballot for each bit of it; __match_any_sync took 80 cycles of an SM a time, five
+// times as long) rank themselves in lane order behind the warp's counter of that bucket, so a slot's rank inside its warp's range is known when the ranges have been
 // read once.  The first row of bucket b for a warp is then the slots of lower buckets
 // anywhere, plus those of b in CTAs before this one (read from their shared memory),
 // plus those of b in warps before this one.  Ranges up to 32 * PLAN_ITEMS slots stay in
 // registers; longer ones park the rank in `position`.
-constexpr int PLAN_THREADS = 1024, PLAN_ITEMS = 8, PLAN_CLUSTER = 8;
+constexpr int PLAN_THREADS = 1024, PLAN_ITEMS = 8, PLAN_CLUSTER = 16;
 
 __device__ __forceinline__ int peer_read(const int* p, int rank) {
     uint32_t a;
@@ -28,9 +28,15 @@ __device__ __forceinline__ void plan_cluster_sync() {
     asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 
-// Rank of this lane's slot among the warp's slots of bucket b so far (all lanes call; b < 0: no slot).
-__device__ __forceinline__ int plan_rank(int* mine, int b, int lane) {
-    const unsigned same = __match_any_sync(~0u, b);
+// Rank of this lane's slot among the warp's slots of bucket b so far (all lanes call; b < 0:
+// no slot).  bits: of the largest bucket plus one, so that -1 is no bucket in them.
+__device__ __forceinline__ int plan_rank(int* mine, int b, int bits, int lane) {
+    unsigned same = ~0u;
+    for (int i = 0; i < bits; ++i) {
+        const bool one = (b >> i) & 1;
+        const unsigned with = __ballot_sync(~0u, one);
+        same &= one ? with : ~with;
+    }
     const int ahead = __popc(same & ((1u << lane) - 1));
     const int rank = b >= 0 ? mine[b] + ahead : 0;
     __syncwarp();
@@ -45,7 +51,7 @@ __global__ void __launch_bounds__(PLAN_THREADS, 1) plan_kernel(const Id* expert,
     extern __shared__ int shared[];  // [nwarps][E + 1] counts, [E + 1] totals of the CTA
     __shared__ int warp_sum[32];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, B = E + 1;
-    const int rank = blockIdx.x, ctas = gridDim.x;
+    const int rank = blockIdx.x, ctas = gridDim.x, bits = 32 - __clz(E + 1);
     int* total = shared + nwarps * B;
     for (int i = tid; i < nwarps * B; i += blockDim.x) shared[i] = 0;
     __syncthreads();
@@ -68,7 +74,7 @@ __global__ void __launch_bounds__(PLAN_THREADS, 1) plan_kernel(const Id* expert,
 #pragma unroll
         for (int i = 0; i < PLAN_ITEMS; ++i) {
             if (s + 32 * i >= s1) break;
-            local[i] = plan_rank(mine, bucket[i], lane);
+            local[i] = plan_rank(mine, bucket[i], bits, lane);
             if (!kept && bucket[i] >= 0) position[s + 32 * i + lane] = local[i];
         }
     }
@@ -155,9 +161,10 @@ __global__ void __launch_bounds__(PLAN_THREADS, 1) plan_kernel(const Id* expert,
 template <typename Id>
 int plan_launch(const Id* expert, int slots, int E, int32_t* offsets, int32_t* position, int32_t* source, cudaStream_t st) {
     const int fit = 200 * 1024 / (4 * (E + 1)) - 1, most = fit < 32 ? fit : 32;
-    // one CTA while its warps keep their slots in registers at two steps each, then more
+    // a CTA for every 1024 slots (a step of its warps), up to 16: the scattered stores of a CTA
+    // take as long as everything else, 32768 slots on 8 CTAs 9.5 us, a single CTA 52
     int ctas = 1;
-    while (ctas < PLAN_CLUSTER && slots > ctas * most * 64) ctas *= 2;
+    while (ctas < PLAN_CLUSTER && slots > ctas * most * 32) ctas *= 2;
     int nwarps = most;
     while (ctas == 1 && nwarps > 1 && (nwarps / 2) * 64 >= slots) nwarps /= 2;
     const int64_t all = (int64_t)ctas * nwarps;
@@ -173,6 +180,7 @@ int plan_launch(const Id* expert, int slots, int E, int32_t* offsets, int32_t* p
         kern<<<1, threads, smem, st>>>(expert, slots, E, nwarps, per, offsets, position, source);
         return launch_status();
     }
+    if (ctas > 8 && !allow_wide_cluster<&plan_kernel<Id>>()) return ELA_ERR_CUDA;
     cudaLaunchAttribute attr = {};
     attr.id = cudaLaunchAttributeClusterDimension;
     attr.val.clusterDim.x = ctas;

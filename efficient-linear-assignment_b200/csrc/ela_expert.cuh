@@ -67,6 +67,17 @@ template <auto KERNEL> __host__ inline bool allow_smem(int bytes) {
     return true;
 }
 
+// Lets a kernel run in clusters of 16 (8 is what every device of the architecture has).
+template <auto KERNEL> __host__ inline bool allow_wide_cluster() {
+    static std::atomic<bool> done[64];
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return false;
+    if (done[dev].load(std::memory_order_relaxed)) return true;
+    if (cudaFuncSetAttribute(KERNEL, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess) return false;
+    done[dev].store(true, std::memory_order_relaxed);
+    return true;
+}
+
 // Rows of expert e, kept inside [0, R] whatever the offsets hold.
 __device__ __forceinline__ int clampi(int v, int lo, int hi) { return v < lo ? lo : v > hi ? hi : v; }
 __device__ __forceinline__ void expert_rows(const int32_t* offsets, int e, int R, int& r0, int& r1) {
