@@ -210,13 +210,12 @@ inline MmaParams row_pass(const int32_t* offsets, int64_t R, int64_t E, int64_t 
     MmaParams p = {};
     p.offsets = offsets;
     p.R = (int)R; p.E = (int)E; p.F = (int)F; p.K = (int)K;
-    p.bn = columns_per_tile(R, E);
-    // boxes as tall as half an expert's share of the rows, so that few rows do not load many
-    int64_t share = (R + E - 1) / E;
-    p.bbox = 16;
-    while (p.bbox < p.bn / 2 && 2 * p.bbox < share) p.bbox *= 2;  // each CTA of a pair loads half
-    p.stages = stages_for(p.bn, E);
     p.f_tiles = (int)((F + MMA_PAIR_F - 1) / MMA_PAIR_F);
+    p.bn = columns_per_tile(R, E, p.f_tiles, (K + MMA_KB - 1) / MMA_KB);
+    // a CTA's half of a tile's columns is one box, or boxes of 64 where experts have fewer rows
+    // than that makes (a box is loaded whole)
+    p.bbox = p.bn % 128 == 0 && R < 256 * E ? 64 : p.bn / 2;
+    p.stages = stages_for(p.bn, E);
     p.wait_ns = LINEAR_WAIT_NS;
     return p;
 }
@@ -248,7 +247,7 @@ size_t ela_expert_linear_workspace_bytes(int pass, int64_t R, int64_t E, int64_t
         const int rows = act_block_rows(R, N);
         return (size_t)((R + rows - 1) / rows + E) * N * 4;
     }
-    if (aligned || (pass == ELA_LINEAR_FORWARD && few_rows(R, E))) return 0;
+    if (aligned || (pass == ELA_LINEAR_FORWARD && few_rows(R, E, N))) return 0;
     const Matrix x = {nullptr, 1, R, K, 0, 0}, w = {nullptr, E, N, K, 0, 0}, dz = {nullptr, 1, R, N, 0, 0};
     return pass == ELA_LINEAR_FORWARD ? x.padded_bytes() + w.padded_bytes()
          : pass == ELA_LINEAR_GRAD_INPUT ? dz.padded_bytes() + w.padded_bytes()
@@ -273,13 +272,13 @@ int ela_expert_linear(const void* x, const void* weight, const void* bias, const
     if (R == 0) return ELA_OK;
     if (!x || !weight || !y) return ELA_ERR_ARGUMENT;
     cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-    if (few_rows(R, E)) {
+    if (few_rows(R, E, N)) {
         StreamParams q = {x, weight, bias, residual, offsets, (int)R, (int)E, (int)K, (int)N, 0, ldx, stride_e, ldw, ldr, y, z};
         const uint64_t bits = reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(weight) | (uint64_t)(ldx * 2) | (uint64_t)(ldw * 2) |
                               (uint64_t)(E > 1 ? stride_e * 2 : 0) | (uint64_t)(K * 2);
         const int vb = bits % 32 == 0 ? 32 : bits % 16 == 0 ? 16 : bits % 4 == 0 ? 4 : 2;
         int rc = ELA_OK;
-        ELA_BY_TYPE(dtype, { ELA_BY_ACT(activation, rc = R <= 4 * E || (E == 1 && R <= 8) ? (stream_launch<T_, A_, 1>(q, vb, st)) : (stream_launch<T_, A_, 2>(q, vb, st))) })
+        ELA_BY_TYPE(dtype, { ELA_BY_ACT(activation, rc = R <= 4 * E || (E == 1 && R <= 8) ? (stream_launch<T_, A_, 1>(q, vb, st)) : R <= 16 * E ? (stream_launch<T_, A_, 2>(q, vb, st)) : (stream_launch<T_, A_, 4>(q, vb, st))) })
         return rc;
     }
     char* ws = reinterpret_cast<char*>(workspace);

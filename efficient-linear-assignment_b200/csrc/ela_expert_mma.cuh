@@ -734,14 +734,23 @@ int mma_launch(const CUtensorMap& a, const CUtensorMap& b, const MmaParams& p, i
     return launch_status();
 }
 
-// Columns per tile of the row passes: the least of 32, 64, 128, 256 that holds twice an
-// expert's share of the rows (loads are uneven, and an expert in two tiles has its
-// weights loaded twice).  A smaller tile leaves more of the shared memory to stages of
-// the weights (10 of 18 KB at 32, 6 or 7 of 32 KB at 256), which is what a few rows per
-// expert wait for.
-inline int columns_per_tile(int64_t R, int64_t E) {
-    const int64_t share = (R + E - 1) / E;
-    return share <= 16 ? 32 : share <= 32 ? 64 : share <= 64 ? 128 : 256;
+// Columns per tile of the row passes, a multiple of 32 up to 256: the one whose rounds of
+// tiles over the pairs take least.  A block of 64 k takes the longer of its products (2
+// cycles a column) and its loads (16 KB of weights and 64 bytes a column, at the 57
+// bytes a cycle that an SM gets from the L2); a tile some 500 cycles more.  Loads are
+// uneven, so an expert is taken to have half as many rows again as its share.  300 rows
+// by 4096 x 4096: 29 us with 32 tiles of 256 columns, 19 with 64 tiles of 96.
+inline int columns_per_tile(int64_t R, int64_t E, int64_t f_tiles, int64_t k_blocks) {
+    const int64_t share = (R + E - 1) / E, rows = E == 1 ? share : share + share / 2, pairs = sm_count() / 2 > 0 ? sm_count() / 2 : 1;
+    int best = 256;
+    int64_t least = INT64_MAX;
+    for (int bn = 256; bn >= 32; bn -= 32) {
+        const int64_t tiles = f_tiles * (E < R ? E : R) * ((rows + bn - 1) / bn), used = rows < bn ? (rows + 31) / 32 * 32 : bn;
+        const int64_t loads = (16384 + 64 * used) / 57, block = 2 * used > loads ? 2 * used : loads;
+        const int64_t time = (tiles + pairs - 1) / pairs * (k_blocks * block + 500);
+        if (time < least || (time == least && rows <= bn)) { least = time; best = bn; }  // (a smaller stage leaves room for more)
+    }
+    return best;
 }
 inline int stages_for(int bn, int64_t E) {
     const int64_t n = (MMA_SMEM - 1024 - MMA_SMEM_FIXED - 12 * E) / (MMA_A_BYTES + bn / 2 * MMA_KB * 2);

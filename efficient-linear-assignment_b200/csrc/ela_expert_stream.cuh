@@ -195,8 +195,11 @@ __global__ void __launch_bounds__(STREAM_WARPS * 32, 2) stream_kernel(const Stre
 }
 
 // Rows per expert up to which the weights' read is what the product costs: 16 rows for
-// each of 16 experts take 31 us here and 33 us by tiles, 32 rows 45 and 34.
-inline bool few_rows(int64_t R, int64_t E) { return R <= 16 * E; }
+// each of 16 experts take 31 us here and 33 us by tiles, 32 rows 45 and 34.  Where tiles
+// of 256 features leave half of the pairs idle, which then read at 44 GB/s an SM, up to 64.
+inline bool few_rows(int64_t R, int64_t E, int64_t N) {
+    return R <= 16 * E || (R <= 64 * E && E * ((N + 255) / 256) <= sm_count() / 4);
+}
 
 template <typename T, int ACT, int RG, int MT>
 int stream_launch_vb(StreamParams p, int vb, cudaStream_t st) {
