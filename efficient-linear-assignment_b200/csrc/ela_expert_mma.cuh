@@ -738,10 +738,11 @@ int mma_launch(const CUtensorMap& a, const CUtensorMap& b, const MmaParams& p, i
 // tiles over the pairs take least.  A block of 64 k takes the longer of its products (2
 // cycles a column) and its loads (16 KB of weights and 64 bytes a column, at the 57
 // bytes a cycle that an SM gets from the L2); a tile some 500 cycles more.  Loads are
-// uneven, so an expert is taken to have half as many rows again as its share.  300 rows
-// by 4096 x 4096: 29 us with 32 tiles of 256 columns, 19 with 64 tiles of 96.
+// uneven, so an expert is taken to have twice its share of the rows: 1003 rows of 8
+// experts of 2056 x 1032 take 22 us with tiles of 256 and 26 with 192.  300 rows by
+// 4096 x 4096: 29 us with 32 tiles of 256 columns, 27 with 64 tiles of 96.
 inline int columns_per_tile(int64_t R, int64_t E, int64_t f_tiles, int64_t k_blocks) {
-    const int64_t share = (R + E - 1) / E, rows = E == 1 ? share : share + share / 2, pairs = sm_count() / 2 > 0 ? sm_count() / 2 : 1;
+    const int64_t share = (R + E - 1) / E, rows = E == 1 ? share : 2 * share, pairs = sm_count() / 2 > 0 ? sm_count() / 2 : 1;
     int best = 256;
     int64_t least = INT64_MAX;
     for (int bn = 256; bn >= 32; bn -= 32) {

@@ -355,6 +355,39 @@ def test_linear_large_sums():
         check_linear(t, off, "gelu", dy, torch.bfloat16)
 
 
+@pytest.mark.parametrize("K,N", [(1024, 96), (264, 40), (130, 33), (97, 64), (2100, 20)])
+@pytest.mark.parametrize("counts", [[1, 0, 1, 1], [9, 8, 0, 3], [40, 2, 0, 1, 0, 0, 0, 0], [17, 16, 30, 1], [5]])
+def test_linear_few_rows(K, N, counts):
+    """The path that streams the weights once: rows past a group of 8, uneven loads, widths
+    that make loads of 32, 16, 4 and 2 bytes."""
+    for dtype in (torch.bfloat16, torch.float16):
+        t, off, dy = linear_case(sum(counts) + 3, len(counts), K, N, dtype, K + N, counts, first=2)
+        check_linear(t, off, "gelu", dy, dtype)
+
+
+def test_linear_one_matrix_few_rows():
+    for R in (1, 8, 9, 16, 17, 33, 64, 65):
+        t, off, dy = linear_case(R, 1, 520, 136, torch.bfloat16, R, [R])
+        check_linear(t, off, "silu", dy, torch.bfloat16, two_d=True, give_offsets=False)
+
+
+def test_linear_many_experts():
+    """More experts than a warp has lanes, most of them without rows; and the most there are."""
+    g = gen(77)
+    for E, R in ((70, 3000), (1000, 2000), (4096, 500)):
+        cut = torch.randint(0, R + 1, (E,), generator=g).sort().values
+        counts = torch.diff(torch.cat([torch.zeros(1, dtype=torch.long), cut])).tolist()
+        t, off, dy = linear_case(R, E, 72, 40, torch.bfloat16, E, counts)
+        check_linear(t, off, "relu", dy, torch.bfloat16)
+
+
+@pytest.mark.parametrize("R,E,K,N", [(300, 1, 512, 2048), (700, 1, 256, 4096), (1100, 2, 320, 1024), (90, 1, 128, 9000)])
+def test_linear_column_tiles(R, E, K, N):
+    """Sizes that choose tiles of other than 256 columns."""
+    t, off, dy = linear_case(R, E, K, N, torch.float16, R)
+    check_linear(t, off, "none", dy, torch.float16)
+
+
 def test_linear_rows_of_others_do_not_leak():
     """NaN and infinities in rows of no expert, and in one expert's rows, stay there."""
     R, E, K, N = 150, 3, 80, 72
@@ -554,6 +587,23 @@ def test_refusals():
     y = ela.expert_linear(a.requires_grad_(), w, offsets=off)
     with pytest.raises(RuntimeError, match="second derivative"):
         torch.autograd.grad(y.sum(), a, create_graph=True)
+
+
+def test_no_wait_gave_up():
+    """After everything above: no kernel ended a wait at its limit."""
+    ela.expert_check()
+
+
+def test_example_trains():
+    import importlib.util
+    import os
+    path = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "examples", "balanced_experts.py")
+    spec = importlib.util.spec_from_file_location("balanced_experts", path)
+    mod = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(mod)
+    losses = mod.train(steps=30, tokens=512, hidden=128, width=256, experts=8, verbose=False)
+    assert losses[-1] < 0.7 * losses[0]
+    assert mod.generate(steps=3, tokens=4, hidden=128, width=256, experts=8, verbose=False)
 
 
 def test_linear_without_rows():
