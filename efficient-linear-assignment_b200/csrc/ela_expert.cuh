@@ -45,15 +45,13 @@ __host__ inline bool aligned16(const void* p, int64_t ld_bytes = 0) {
 __host__ inline int launch_status() { return cudaGetLastError() == cudaSuccess ? ELA_OK : ELA_ERR_CUDA; }
 
 inline int sm_count() {
-    static int counts[64] = {};
-    int dev = 0;
+    static std::atomic<int> counts[64];
+    int dev = 0, n = 0;
     if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 0;
-    if (counts[dev] == 0) {
-        int n = 0;
-        if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) return 0;
-        counts[dev] = n;
-    }
-    return counts[dev];
+    if ((n = counts[dev].load(std::memory_order_relaxed)) != 0) return n;
+    if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) return 0;
+    counts[dev].store(n, std::memory_order_relaxed);
+    return n;
 }
 
 // Lets a kernel use this much dynamic shared memory; asked of the driver once per kernel and device.

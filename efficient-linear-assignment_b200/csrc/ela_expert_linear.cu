@@ -2,7 +2,8 @@
 // gradient (include/ela_expert.h).
 //
 // The three products (forward, input gradient, weight gradient) are one
-// tensor-core kernel, ela_expert_mma.cuh; here are their entry points, the copies
+// tensor-core kernel, ela_expert_mma.cuh; the forward product of a few rows per
+// expert streams the weights instead, ela_expert_stream.cuh; here are their entry points, the copies
 // of operands that TMA cannot address, and the gradient of the activation with the
 // bias gradient.
 
@@ -257,6 +258,7 @@ size_t ela_expert_linear_workspace_bytes(int pass, int64_t R, int64_t E, int64_t
 int ela_expert_status(int* status) {
     if (!status) return ELA_ERR_ARGUMENT;
     const int zero = ELA_OK;
+    if (cudaDeviceSynchronize() != cudaSuccess) return ELA_ERR_CUDA;
     if (cudaMemcpyFromSymbol(status, g_expert_error, sizeof(int)) != cudaSuccess) return ELA_ERR_CUDA;
     if (*status != ELA_OK && cudaMemcpyToSymbol(g_expert_error, &zero, sizeof(int)) != cudaSuccess) return ELA_ERR_CUDA;
     return ELA_OK;
@@ -273,6 +275,7 @@ int ela_expert_linear(const void* x, const void* weight, const void* bias, const
     if (!x || !weight || !y) return ELA_ERR_ARGUMENT;
     cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
     if (few_rows(R, E, N)) {
+        if (E * ((N + 15) / 16) > INT32_MAX) return ELA_ERR_UNSUPPORTED;
         StreamParams q = {x, weight, bias, residual, offsets, (int)R, (int)E, (int)K, (int)N, 0, ldx, stride_e, ldw, ldr, y, z};
         const uint64_t bits = reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(weight) | (uint64_t)(ldx * 2) | (uint64_t)(ldw * 2) |
                               (uint64_t)(E > 1 ? stride_e * 2 : 0) | (uint64_t)(K * 2);
