@@ -33,7 +33,7 @@
 //
 // Roles, in each CTA: warp 0 issues the TMA loads of the CTA's halves, which count on
 // the first CTA's barriers; warp 1 of the first CTA issues the MMAs of the pair; warp 2
-// owns the TMEM allocation; warp 3 works out the tiles; warps 4-19 run the epilogue
+// owns the TMEM allocation; warp 3 works out the tiles; warps 4-11 run the epilogue
 // while the next tile's MMAs fill the other half of TMEM (2 x 256 columns).  Loads and
 // MMAs are issued by one elected thread that runs the whole inner loop (a warp that
 // polls, broadcasts and reconverges each block took 40 % longer), and no arrival of the
@@ -61,7 +61,8 @@ constexpr int MMA_C = 256;              // most columns per tile
 constexpr int MMA_KB = 64;              // k per stage: 128 bytes, one swizzle span
 constexpr int MMA_A_BYTES = MMA_F * MMA_KB * 2;
 constexpr int MMA_CHUNK = 16;           // columns an epilogue warp takes at a time
-constexpr int MMA_GROUPS = 4;           // epilogue warps per 32 TMEM lanes
+constexpr int MMA_GROUPS = 2;           // epilogue warps per 32 TMEM lanes: 4 take 3 % less for the shortest
+                                        // sums, but 2-4 % more for long ones at the power limit
 constexpr int MMA_MAX_STAGES = 10;
 constexpr int MMA_THREADS = 128 + MMA_GROUPS * 128;
 constexpr int MMA_SMEM = 227 * 1024;
