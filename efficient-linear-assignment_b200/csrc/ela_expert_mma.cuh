@@ -270,23 +270,24 @@ template <> __device__ __forceinline__ float2 unpack2<__nv_bfloat16>(uint32_t p)
 // lane's residual words are those of swap_pair's layout (loaded by load_residual).
 // Addresses go from pair to pair of columns by one 64-bit addition: written as a product
 // with j they made most of the epilogue's instructions.
-template <typename T, int ACT, bool BIAS, bool Z, bool RES>
+template <typename T, int ACT, bool BIAS, bool Z, bool RES, bool ALL>
 __device__ __forceinline__ void finish(float* v, float bias, const uint32_t* res, const MmaParams& p, int64_t c, int f, int left) {
     const bool odd = threadIdx.x & 1;
     const uint32_t order = odd ? 0x3276 : 0x5410;
-    if (p.vec) {
+    if (ALL || p.vec) {
         const int64_t at = (c + odd) * p.F + (f & ~1);
         char* out = reinterpret_cast<char*>(reinterpret_cast<T*>(p.out) + at);
         char* zout = reinterpret_cast<char*>(reinterpret_cast<T*>(p.z) + at);
         const int64_t step = 4 * (int64_t)p.F;
-        const int mine = f < p.F ? left - odd : 0;  // (F is even: both lanes of a pair are in or out)
+        // (F is even: both lanes of a pair are in or out)
+        const int mine = ALL ? MMA_CHUNK : f < p.F ? left - odd : 0;
 #pragma unroll
         for (int j = 0; j < MMA_CHUNK; j += 2) {
             float a = v[j], b = v[j + 1];
             if (BIAS) { a += bias; b += bias; }
             if (Z) {
                 const uint32_t w = swap_pair(pack2<T>(a, b), order);
-                if (j < mine) *reinterpret_cast<uint32_t*>(zout) = w;
+                if (ALL || j < mine) *reinterpret_cast<uint32_t*>(zout) = w;
                 zout += step;
             }
             a = act_value<ACT>(a);
@@ -297,7 +298,7 @@ __device__ __forceinline__ void finish(float* v, float bias, const uint32_t* res
                 b += r.y;
             }
             const uint32_t w = swap_pair(pack2<T>(a, b), order);
-            if (j < mine) *reinterpret_cast<uint32_t*>(out) = w;
+            if (ALL || j < mine) *reinterpret_cast<uint32_t*>(out) = w;
             out += step;
         }
     } else if (f < p.F) {
@@ -638,11 +639,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(MMA_THREADS, 1)
         auto write = [&](float* v, float bias, const uint32_t* res, int64_t c, int f, int left) {
             if (with_z) {
                 if constexpr (FWD && ACT == ELA_ACT_RELU) note_near_zero<T>(v, bias, p, t.e, c, f, left, s_near, &s_near_count);
-                if (with_res) finish<T, ACT, FWD, FWD, FWD>(v, bias, res, p, c, f, left);
-                else finish<T, ACT, FWD, FWD, false>(v, bias, res, p, c, f, left);
+                if (with_res) finish<T, ACT, FWD, FWD, FWD, false>(v, bias, res, p, c, f, left);
+                else finish<T, ACT, FWD, FWD, false, false>(v, bias, res, p, c, f, left);
             } else {
-                if (with_res) finish<T, ACT, FWD, false, FWD>(v, bias, res, p, c, f, left);
-                else finish<T, ACT, FWD, false, false>(v, bias, res, p, c, f, left);
+                if (with_res) finish<T, ACT, FWD, false, FWD, false>(v, bias, res, p, c, f, left);
+                else if (p.vec && left >= MMA_CHUNK && (f | 31) < p.F) finish<T, ACT, FWD, false, false, true>(v, bias, res, p, c, f, left);
+                else finish<T, ACT, FWD, false, false, false>(v, bias, res, p, c, f, left);
             }
         };
         for (int i = 0; ok && fetch(i, t, ok); ++i) {

@@ -523,6 +523,21 @@ def test_layer_in_a_graph():
         assert torch.equal(out, layer(x, expert, E, w1, b1, w2, gate))
 
 
+def test_layer_in_a_compiled_graph():
+    """torch.compile traces the operators and their gradients (no graph break) to the same bits."""
+    x, expert, E, w1, b1, w2, gate = layer_inputs()
+    leaves = [v.requires_grad_() for v in (x, w1, b1, w2, gate)]
+
+    def f(x, w1, b1, w2, gate):
+        return layer(x, expert, E, w1, b1, w2, gate)
+
+    traced = torch.compile(f, backend="aot_eager", fullgraph=True)
+    want, got = f(*leaves), traced(*leaves)
+    assert torch.equal(want, got)
+    for a, b in zip(torch.autograd.grad(want, leaves, torch.ones_like(want)), torch.autograd.grad(got, leaves, torch.ones_like(got))):
+        assert torch.equal(a, b)
+
+
 def test_assignment_to_experts_end_to_end():
     """Tokens to expert slots by the solver, through the experts and back; tokens
     that the solver leaves out (max_iter) come back as zeros."""
