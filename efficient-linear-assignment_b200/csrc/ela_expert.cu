@@ -48,6 +48,8 @@ __device__ __forceinline__ int plan_rank(int* mine, int b, int bits, int lane) {
 template <typename Id>
 __global__ void __launch_bounds__(PLAN_THREADS, 1) plan_kernel(const Id* expert, int slots, int E, int nwarps, int per,
                                                                int32_t* offsets, int32_t* position, int32_t* source) {
+    next_may_start();
+    previous_done();
     extern __shared__ int shared[];  // [nwarps][E + 1] counts, [E + 1] totals of the CTA
     __shared__ int warp_sum[32];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, B = E + 1;
@@ -177,22 +179,25 @@ int plan_launch(const Id* expert, int slots, int E, int32_t* offsets, int32_t* p
     while (threads < PLAN_THREADS && threads < E + 1) threads *= 2;
     if (threads > PLAN_THREADS) threads = PLAN_THREADS;
     if (ctas == 1) {
-        kern<<<1, threads, smem, st>>>(expert, slots, E, nwarps, per, offsets, position, source);
-        return launch_status();
+        return launch(kern, 1, threads, smem, st, expert, slots, E, nwarps, per, offsets, position, source);
     }
     if (ctas > 8 && !allow_wide_cluster<&plan_kernel<Id>>()) return ELA_ERR_CUDA;
-    cudaLaunchAttribute attr = {};
-    attr.id = cudaLaunchAttributeClusterDimension;
-    attr.val.clusterDim.x = ctas;
-    attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+    cudaLaunchAttribute attr[2] = {};
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = ctas;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[1].val.programmaticStreamSerializationAllowed = 1;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(ctas);
     cfg.blockDim = dim3(threads);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = st;
-    cfg.attrs = &attr;
-    cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, kern, expert, slots, E, nwarps, per, offsets, position, source) == cudaSuccess ? ELA_OK : ELA_ERR_CUDA;
+    cfg.attrs = attr;
+    cfg.numAttrs = 2;
+    if (cudaLaunchKernelEx(&cfg, kern, expert, slots, E, nwarps, per, offsets, position, source) == cudaSuccess) return ELA_OK;
+    cudaGetLastError();
+    return ELA_ERR_CUDA;
 }
 
 // --------------------------------------------------------- dispatch, combine
@@ -276,6 +281,8 @@ template <typename T, int VB>
 __global__ void __launch_bounds__(ROUTE_THREADS) dispatch_kernel(const T* x, int T_, int k, int H, int64_t ldx, int G,
                                                                  const int32_t* position, const int32_t* offsets, int E,
                                                                  int rows, T* out) {
+    next_may_start();
+    previous_done();
     constexpr int N = VB / sizeof(T), U = Route<VB>::U;
     const int64_t t = (int64_t)blockIdx.x * (ROUTE_THREADS / G) + threadIdx.x / G;
     if (t >= T_) return;
@@ -304,6 +311,8 @@ __global__ void __launch_bounds__(ROUTE_THREADS, 4) combine_kernel(const T* y, i
                                                                             int G, const int32_t* position,
                                                                             const int32_t* offsets, int E, int rows,
                                                                             const Wt* weights, T* out) {
+    next_may_start();
+    previous_done();
     constexpr int N = VB / sizeof(T), U = Route<VB>::U;
     const int64_t t = (int64_t)blockIdx.x * (ROUTE_THREADS / G) + threadIdx.x / G;
     if (t >= T_) return;
@@ -348,6 +357,8 @@ __global__ void __launch_bounds__(ROUTE_THREADS, 6)
     combine_grad_kernel(const T* dout, const T* y, int T_, int k, int H, int64_t lddo, int64_t ldy, int G,
                         const int32_t* position, const int32_t* offsets, int E, int rows, const Wt* weights, T* dy,
                         Wt* dweights) {
+    next_may_start();
+    previous_done();
     constexpr int N = VB / sizeof(T);
     __shared__ float part[ROUTE_THREADS / 32][JC];
     const int64_t t = (int64_t)blockIdx.x * (ROUTE_THREADS / G) + threadIdx.x / G;
@@ -477,11 +488,12 @@ int ela_expert_dispatch(const void* x, int dtype, int64_t T, int64_t k, int64_t 
     const int es = dtype_bytes(dtype);
     const int vb = piece_bytes(address(x) | address(rows) | (uint64_t)(ldx * es) | (uint64_t)(H * es));
     const int G = group_threads(H, es, vb);
+    int rc = ELA_OK;
     ELA_BY_DTYPE(dtype, ELA_BY_PIECE(vb, {
-        dispatch_kernel<T_, V_><<<route_grid(T, G), ROUTE_THREADS, 0, st>>>((const T_*)x, (int)T, (int)k, (int)H, ldx, G, position, offsets,
+        rc = launch(dispatch_kernel<T_, V_>, route_grid(T, G), ROUTE_THREADS, 0, st, (const T_*)x, (int)T, (int)k, (int)H, ldx, G, position, offsets,
                                                                           (int)num_experts, (int)(T * k), (T_*)rows);
     }))
-    return launch_status();
+    return rc;
 }
 
 int ela_expert_combine(const void* y, int dtype, int64_t T, int64_t k, int64_t H, int64_t ldy,
@@ -496,15 +508,16 @@ int ela_expert_combine(const void* y, int dtype, int64_t T, int64_t k, int64_t H
     const int vb = piece_bytes(address(y) | address(out) | (uint64_t)(ldy * es) | (uint64_t)(H * es));
     const int G = group_threads(H, es, vb);
     const bool w32 = !weights || weights_dtype == ELA_DTYPE_F32;
+    int rc = ELA_OK;
     ELA_BY_DTYPE(dtype, ELA_BY_PIECE(vb, {
         if (w32)
-            combine_kernel<T_, float, V_><<<route_grid(T, G), ROUTE_THREADS, 0, st>>>((const T_*)y, (int)T, (int)k, (int)H, ldy, G, position, offsets,
+            rc = launch(combine_kernel<T_, float, V_>, route_grid(T, G), ROUTE_THREADS, 0, st, (const T_*)y, (int)T, (int)k, (int)H, ldy, G, position, offsets,
                                                                                      (int)num_experts, (int)(T * k), (const float*)weights, (T_*)out);
         else
-            combine_kernel<T_, T_, V_><<<route_grid(T, G), ROUTE_THREADS, 0, st>>>((const T_*)y, (int)T, (int)k, (int)H, ldy, G, position, offsets,
+            rc = launch(combine_kernel<T_, T_, V_>, route_grid(T, G), ROUTE_THREADS, 0, st, (const T_*)y, (int)T, (int)k, (int)H, ldy, G, position, offsets,
                                                                                   (int)num_experts, (int)(T * k), (const T_*)weights, (T_*)out);
     }))
-    return launch_status();
+    return rc;
 }
 
 int ela_expert_combine_grad(const void* dout, const void* y, int dtype, int64_t T, int64_t k, int64_t H,
@@ -521,17 +534,18 @@ int ela_expert_combine_grad(const void* dout, const void* y, int dtype, int64_t 
                                (uint64_t)(dweights ? ldy * es : 0) | (uint64_t)(H * es));
     const int G = group_threads(H, es, vb);
     const bool w32 = (!weights && !dweights) || weights_dtype == ELA_DTYPE_F32;
+    int rc = ELA_OK;
     ELA_BY_DTYPE(dtype, ELA_BY_PIECE(vb, {
         if (w32)
-            combine_grad_kernel<T_, float, V_><<<route_grid(T, G), ROUTE_THREADS, 0, st>>>(
+            rc = launch(combine_grad_kernel<T_, float, V_>, route_grid(T, G), ROUTE_THREADS, 0, st, 
                 (const T_*)dout, (const T_*)y, (int)T, (int)k, (int)H, lddo, ldy, G, position, offsets, (int)num_experts, (int)(T * k),
                 (const float*)weights, (T_*)dy, (float*)dweights);
         else
-            combine_grad_kernel<T_, T_, V_><<<route_grid(T, G), ROUTE_THREADS, 0, st>>>(
+            rc = launch(combine_grad_kernel<T_, T_, V_>, route_grid(T, G), ROUTE_THREADS, 0, st, 
                 (const T_*)dout, (const T_*)y, (int)T, (int)k, (int)H, lddo, ldy, G, position, offsets, (int)num_experts, (int)(T * k),
                 (const T_*)weights, (T_*)dy, (T_*)dweights);
     }))
-    return launch_status();
+    return rc;
 }
 
 }  // extern "C"

@@ -42,7 +42,6 @@ __host__ inline int dtype_bytes(int dtype) {
 __host__ inline bool aligned16(const void* p, int64_t ld_bytes = 0) {
     return (reinterpret_cast<uintptr_t>(p) & 15u) == 0 && ld_bytes % 16 == 0;
 }
-__host__ inline int launch_status() { return cudaGetLastError() == cudaSuccess ? ELA_OK : ELA_ERR_CUDA; }
 
 inline int sm_count() {
     static std::atomic<int> counts[64];
@@ -75,6 +74,29 @@ template <auto KERNEL> __host__ inline bool allow_wide_cluster() {
     done[dev].store(true, std::memory_order_relaxed);
     return true;
 }
+
+// Every kernel here is launched so that it may start while the one before it in the stream
+// ends (programmatic stream serialization): its prologue, and its CTAs' places on SMs that
+// are done, overlap that kernel's tail.  In return every kernel calls previous_done() before
+// it touches memory, which waits until the kernels before it are complete and visible.
+template <typename... P, typename... A>
+__host__ inline int launch(void (*kern)(P...), unsigned grid, unsigned block, size_t smem, cudaStream_t st, A... args) {
+    cudaLaunchAttribute attr = {};
+    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr.val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(grid);
+    cfg.blockDim = dim3(block);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    if (cudaLaunchKernelEx(&cfg, kern, static_cast<P>(args)...) == cudaSuccess) return ELA_OK;
+    cudaGetLastError();
+    return ELA_ERR_CUDA;
+}
+__device__ __forceinline__ void next_may_start() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+__device__ __forceinline__ void previous_done() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 
 // Rows of expert e, kept inside [0, R] whatever the offsets hold.
 __device__ __forceinline__ int clampi(int v, int lo, int hi) { return v < lo ? lo : v > hi ? hi : v; }

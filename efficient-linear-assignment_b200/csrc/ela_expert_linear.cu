@@ -21,6 +21,8 @@ constexpr unsigned long long LINEAR_WAIT_NS = 2000000000ull;  // limit of every 
 // around them (no word is touched that does not hold an element of the row).
 __global__ void __launch_bounds__(256) realign_kernel(const uint16_t* src, int64_t rows, int cols, int64_t ld,
                                                       int64_t rows_per_matrix, int64_t stride_e, uint16_t* dst, int64_t ldd) {
+    next_may_start();
+    previous_done();
     const int pieces = (cols + 7) / 8;
     const int64_t all = rows * pieces;
     for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < all; i += (int64_t)gridDim.x * blockDim.x) {
@@ -59,14 +61,13 @@ inline int readable(Matrix& m, char*& ws, size_t& left, cudaStream_t st) {
     if (!ws || left < need) return ELA_ERR_ARGUMENT;
     const int64_t rows = m.matrices * m.rows, ld = round8(m.cols);
     const int64_t blocks = (rows * (ld / 8) + 255) / 256, most = 8 * (int64_t)sm_count();
-    realign_kernel<<<(unsigned)(blocks < most ? blocks : most), 256, 0, st>>>((const uint16_t*)m.p, rows, (int)m.cols, m.ld, m.rows, m.stride_e,
-                                                                         (uint16_t*)ws, ld);
+    const int rc = launch(realign_kernel, (unsigned)(blocks < most ? blocks : most), 256, 0, st, (const uint16_t*)m.p, rows, (int)m.cols, m.ld, m.rows, m.stride_e, (uint16_t*)ws, ld);
     m.p = ws;
     m.ld = ld;
     m.stride_e = m.rows * ld;
     ws += need;
     left -= need;
-    return launch_status();
+    return rc;
 }
 inline bool map_of(CUtensorMap* map, int dtype, const Matrix& m, int box_cols, int box_rows, bool three) {
     const int64_t se = m.matrices > 1 ? m.stride_e : round8(m.ld * m.rows);
@@ -88,6 +89,8 @@ constexpr int ACT_COLS = 256, ACT_WARPS = 8, ACT_ROWS = 2;  // rows a lane has i
 template <typename T, int ACT, bool VEC>
 __global__ void __launch_bounds__(ACT_WARPS * 32, 4) grad_act_kernel(const T* dy, const T* z, const int32_t* offsets, int R,
                                                                   int E, int N, int block_rows, T* dz, float* partial) {
+    next_may_start();
+    previous_done();
     __shared__ float part[ACT_WARPS][ACT_COLS];
     const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
     const int strips = (N + ACT_COLS - 1) / ACT_COLS, strip = blockIdx.x % strips, block = blockIdx.x / strips;
@@ -173,6 +176,8 @@ __global__ void __launch_bounds__(ACT_WARPS * 32, 4) grad_act_kernel(const T* dy
 template <typename T>
 __global__ void __launch_bounds__(256) sum_kernel(const float* partial, const int32_t* offsets, int R, int N, int block_rows,
                                                   T* dbias) {
+    next_may_start();
+    previous_done();
     __shared__ float part[8][32];
     const int strips = (N + 31) / 32, e = blockIdx.x / strips;
     const int c = threadIdx.x & 31, w = threadIdx.x >> 5, n = blockIdx.x % strips * 32 + c;
@@ -320,17 +325,18 @@ int ela_expert_linear_grad_act(const void* dy, const void* z, const int32_t* off
     cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
     float* partial = dbias ? reinterpret_cast<float*>(workspace) : nullptr;
     const bool vec = aligned16(dy, N * 2) && (!z || aligned16(z)) && (!dz || aligned16(dz));
+    int rc = ELA_OK;
     ELA_BY_TYPE(dtype, {
         const unsigned grid = (unsigned)(blocks * ((N + ACT_COLS - 1) / ACT_COLS));  // strips of columns innermost
         if (R > 0)
             ELA_BY_ACT(activation, {
                 auto kern = vec ? grad_act_kernel<T_, A_, true> : grad_act_kernel<T_, A_, false>;
-                kern<<<grid, ACT_WARPS * 32, 0, st>>>((const T_*)dy, (const T_*)z, offsets, (int)R, (int)E, (int)N, rows, (T_*)dz, partial);
+                rc = launch(kern, grid, ACT_WARPS * 32, 0, st, (const T_*)dy, (const T_*)z, offsets, (int)R, (int)E, (int)N, rows, (T_*)dz, partial);
             })
-        if (dbias)
-            sum_kernel<T_><<<(unsigned)(E * ((N + 31) / 32)), 256, 0, st>>>(partial, offsets, (int)R, (int)N, rows, (T_*)dbias);
+        if (dbias && rc == ELA_OK)
+            rc = launch(sum_kernel<T_>, (unsigned)(E * ((N + 31) / 32)), 256, 0, st, (const float*)partial, offsets, (int)R, (int)N, rows, (T_*)dbias);
     })
-    return launch_status();
+    return rc;
 }
 
 int ela_expert_linear_grad_input(const void* dz, const void* weight, const int32_t* offsets, int dtype, int64_t R,

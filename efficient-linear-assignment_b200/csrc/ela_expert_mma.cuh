@@ -387,7 +387,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(MMA_THREADS, 1)
     constexpr bool A_K_MAJOR = PASS == PASS_FORWARD, B_K_MAJOR = PASS != PASS_WEIGHT;
     extern __shared__ unsigned char smem_raw[];
     // full, tempty, patched: the first CTA's are used; empty, tfull, landed: each CTA its own
-    __shared__ __align__(8) uint64_t full[MMA_MAX_STAGES], empty[MMA_MAX_STAGES], tfull[2], tempty[2], sfull[MMA_TILES], sempty[MMA_TILES], landed, patched, drained;
+    __shared__ __align__(8) uint64_t full[MMA_MAX_STAGES], empty[MMA_MAX_STAGES], tfull[2], tempty[2], sfull[MMA_TILES], sempty[MMA_TILES], patched[MMA_MAX_STAGES], landed, drained;
     __shared__ uint32_t s_tmem;
     __shared__ int s_abort;
     __shared__ uint32_t s_issued;
@@ -403,6 +403,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(MMA_THREADS, 1)
     const int stage_bytes = MMA_A_BYTES + p.bn / 2 * MMA_KB * 2;
     const volatile int* abort = &s_abort;
 
+    next_may_start();
     if (tid == 32) {
         asm volatile("prefetch.tensormap [%0];" ::"l"(&map_a) : "memory");
         asm volatile("prefetch.tensormap [%0];" ::"l"(&map_b) : "memory");
@@ -418,10 +419,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(MMA_THREADS, 1)
         for (int b = 0; b < 2; ++b) { bar_init(&tfull[b], 1); bar_init(&tempty[b], 2 * 4 * MMA_GROUPS); }
         for (int i = 0; i < MMA_TILES; ++i) { bar_init(&sfull[i], 1); bar_init(&sempty[i], 4 * MMA_GROUPS + 1 + (rank == 0)); }
         bar_init(&landed, 1);
-        bar_init(&patched, 1);
+        for (int s = 0; s < p.stages; ++s) bar_init(&patched[s], 1);
         bar_init(&drained, 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
+    previous_done();  // (no memory was touched before)
     for (int e = tid; e < p.E; e += MMA_THREADS) expert_rows(p.offsets, e, p.R, table[e], table[p.E + e]);
     __syncthreads();
     if (PASS != PASS_WEIGHT && warp == 3) {  // row tiles before each expert
@@ -487,7 +489,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(MMA_THREADS, 1)
     } else if (warp == 0) {  // ---- loads of this CTA's features and its half of the columns
         Tile t;
         int s = 0;
-        uint32_t phase = 0, landings = 0;
+        uint32_t phase = 0, landings = 0, patches = 0;  // patches: bit s, the parity of stage s's patches
         bool ok = true;
         for (int i = 0; ok && fetch(i, t, ok); ++i) {
             const int f0 = t.f0 + rank * MMA_F;
@@ -549,16 +551,19 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(MMA_THREADS, 1)
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                 __syncwarp();
                 if (lane == 0) {
+                    // (a barrier per stage: the second CTA may be as many patches ahead as there are
+                    // stages, and a phase of a single barrier would pass unseen)
                     if (rank == 1) {
-                        bar_arrive_at(leader_addr(&patched));
+                        bar_arrive_at(leader_addr(&patched[s]));
                     } else {
-                        ok = bar_wait(&patched, (landings - 1) & 1, p.wait_ns, abort);
+                        ok = bar_wait(&patched[s], (patches >> s) & 1, p.wait_ns, abort);
                         asm volatile("fence.acq_rel.cluster;" ::: "memory");
                         if (ok) bar_arrive(&full[s]);
                         else give_up();
                     }
                 }
                 ok = __shfl_sync(~0u, (int)ok, 0);
+                patches ^= 1u << s;
                 if (++s == p.stages) { s = 0; phase ^= 1; }
             }
         }
@@ -740,8 +745,7 @@ int mma_launch(const CUtensorMap& a, const CUtensorMap& b, const MmaParams& p, i
     const int sms = sm_count();
     if (sms == 0 || !allow_smem<&mma_kernel<PASS, T, ACT>>(MMA_SMEM - 1024)) return ELA_ERR_CUDA;
     const int grid = 2 * (int)(max_tiles < sms / 2 ? max_tiles : sms / 2);
-    kern<<<grid, MMA_THREADS, MMA_SMEM - 1024, st>>>(a, b, p);
-    return launch_status();
+    return launch(kern, grid, MMA_THREADS, MMA_SMEM - 1024, st, a, b, p);
 }
 
 // Columns per tile of the row passes, a multiple of 32 up to 256: the one whose rounds of

@@ -89,6 +89,8 @@ template <typename T> __device__ __forceinline__ void mma16816(float* d, uint32_
 // tiles of ela_expert_mma.cuh.  16-byte loads: 27 us.
 template <typename T, int ACT, int RG, int MT, int VB>
 __global__ void __launch_bounds__(STREAM_WARPS * 32, 2) stream_kernel(const StreamParams p) {
+    next_may_start();
+    previous_done();
     constexpr int F = 16 * MT, LOADS = RG == 1 ? 8 : 4, SUB = LOADS / (2 * MT), KB = 64 * SUB;  // features, steps of 64 k, k of a batch
     __shared__ float part[STREAM_WARPS][RG * 8][F + 1];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
@@ -206,11 +208,9 @@ int stream_launch_vb(StreamParams p, int vb, cudaStream_t st) {
     p.f_tiles = (p.N + 16 * MT - 1) / (16 * MT);
     const int64_t items = (int64_t)p.E * p.f_tiles, most = 2 * (int64_t)sm_count();
     const unsigned grid = (unsigned)(items < most ? items : most);
-    if (vb == 32) stream_kernel<T, ACT, RG, MT, 32><<<grid, STREAM_WARPS * 32, 0, st>>>(p);
-    else if (vb == 16) stream_kernel<T, ACT, RG, MT, 16><<<grid, STREAM_WARPS * 32, 0, st>>>(p);
-    else if (vb == 4) stream_kernel<T, ACT, RG, MT, 4><<<grid, STREAM_WARPS * 32, 0, st>>>(p);
-    else stream_kernel<T, ACT, RG, MT, 2><<<grid, STREAM_WARPS * 32, 0, st>>>(p);
-    return launch_status();
+    auto kern = vb == 32 ? stream_kernel<T, ACT, RG, MT, 32> : vb == 16 ? stream_kernel<T, ACT, RG, MT, 16>
+              : vb == 4 ? stream_kernel<T, ACT, RG, MT, 4> : stream_kernel<T, ACT, RG, MT, 2>;
+    return launch(kern, grid, STREAM_WARPS * 32, 0, st, p);
 }
 // Items of 16 features where 32 would leave CTAs without one.
 template <typename T, int ACT, int RG>

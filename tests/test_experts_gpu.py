@@ -381,6 +381,25 @@ def test_linear_many_experts():
         check_linear(t, off, "relu", dy, torch.bfloat16)
 
 
+def test_weight_gradient_of_many_short_sums():
+    """Hundreds of sums of 1 to 70 rows in a row, each ending inside a block of 16, again and
+    again: the two CTAs of a pair run apart by several of them."""
+    g = gen(78)
+    E, K, N = 700, 72, 40
+    counts = torch.randint(1, 71, (E,), generator=g)
+    counts[::3] = torch.randint(1, 4, counts[::3].shape, generator=g)
+    R = int(counts.sum())
+    t, off, dy = linear_case(R, E, K, N, torch.bfloat16, 78, counts.tolist(), bias=False, residual=False)
+    offsets = torch.tensor(off, dtype=torch.int32, device="cuda")
+    ref, bound = linear_definition(t, off, "none", dy, torch.bfloat16)
+    x, w, dyc = t["x"].cuda(), t["weight"].cuda().requires_grad_(), dy.cuda()
+    for _ in range(20):
+        y = ela.expert_linear(x, w, None, None, "none", offsets)
+        (dw,) = torch.autograd.grad(y, w, dyc)
+    close(dw, ref["weight"], bound["weight"], "dweight")
+    ela.expert_check()
+
+
 @pytest.mark.parametrize("R,E,K,N", [(300, 1, 512, 2048), (700, 1, 256, 4096), (1100, 2, 320, 1024), (90, 1, 128, 9000)])
 def test_linear_column_tiles(R, E, K, N):
     """Sizes that choose tiles of other than 256 columns."""
