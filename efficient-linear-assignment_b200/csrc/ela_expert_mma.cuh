@@ -12,8 +12,8 @@
 //   weight grad    input feature          output feature       row of the expert
 //
 // Why a pair: one CTA's 128 x 256 tile loads 48 KB per 64 k, of which a CTA of a pair
-// loads 32 KB for the same products: 4096^3 bf16 212 us by single CTAs, 99 us by pairs
-// with the rest below (1390 TFLOP/s, 0.84 of the measured 1658; the library's product
+// loads 32 KB for the same products: 4096^3 bf16 212 us by single CTAs, 97 us by pairs
+// with the rest below (1420 TFLOP/s, 0.86 of the measured 1658; the library's product
 // takes 93 us).  At full rounds a block of 64 k takes 386 ns against the 374 ns that the
 // library's burst rate means; the rest is the last round, 34 tiles for 74 pairs.  Long
 // products are held by the power limit, not by the schedule: the input gradient of 8192
