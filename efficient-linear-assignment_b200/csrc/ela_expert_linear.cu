@@ -322,7 +322,7 @@ int ela_expert_linear(const void* x, const void* weight, const void* bias, const
     p.vec = N % 2 == 0 && aligned4(y) && (!z || aligned4(z)) && (!residual || (aligned4(residual) && ldr % 2 == 0));
     CUtensorMap a, b;
     if (!map_of(&a, dtype, mw, MMA_KB, MMA_F, true) || !map_of(&b, dtype, mx, MMA_KB, p.bbox, false)) return ELA_ERR_CUDA;
-    ELA_BY_TYPE(dtype, { ELA_BY_ACT(activation, rc = (mma_launch<PASS_FORWARD, T_, A_>(a, b, p, row_tiles(p), st))) })
+    ELA_BY_TYPE(dtype, { ELA_BY_ACT(activation, rc = z ? (mma_launch<PASS_FORWARD, T_, A_, true>(a, b, p, row_tiles(p), st)) : (mma_launch<PASS_FORWARD, T_, A_>(a, b, p, row_tiles(p), st))) })
     return rc;
 }
 

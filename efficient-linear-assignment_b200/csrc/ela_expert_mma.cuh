@@ -33,8 +33,8 @@
 //
 // Roles, in each CTA: warp 0 issues the TMA loads of the CTA's halves, which count on
 // the first CTA's barriers; warp 1 of the first CTA issues the MMAs of the pair; warp 2
-// owns the TMEM allocation; warp 3 works out the tiles; warps 4-11 run the epilogue
-// while the next tile's MMAs fill the other half of TMEM (2 x 256 columns).  Loads and
+// owns the TMEM allocation and sums ReLU's z next to 0 again; warp 3 works out the tiles;
+// warps 4-11 run the epilogue while the next tile's MMAs fill the other half of TMEM (2 x 256 columns).  Loads and
 // MMAs are issued by one elected thread that runs the whole inner loop (a warp that
 // polls, broadcasts and reconverges each block took 40 % longer), and no arrival of the
 // inner loop crosses CTAs with cluster-scope ordering, whose fences cost 1000 cycles.  A warp reads 16 columns of its 32 features
@@ -78,7 +78,7 @@ struct MmaParams {
     int vec;                // two consecutive features may be loaded and stored together
     const void* bias;
     const void* residual;
-    const void* x;          // forward with z: the operands again, for resum
+    const void* x;          // forward with z: the operands again, for exact_z
     const void* weight;
     int64_t ldr, ldx, ldw, stride_e;
     void* out;
@@ -314,43 +314,68 @@ __device__ __forceinline__ void finish(float* v, float bias, const uint32_t* res
     }
 }
 
-// ReLU's slope jumps at 0, and the tensor cores' sums, which drop low bits at every step,
-// can leave a z near 0 on its other side: about one in eight million at K = 1024, each
-// of which moves a row of the weight gradient.  Where z is kept for the gradient, those
-// within the sums' error of 0 (K * 2^-28 of the lane's largest; about 1 in 100000) are
-// noted, and summed again in rounded fp32 when the CTA's tiles are done: by a warp each,
-// 32 partial sums and a tree (46 us against 42 without, 8192 rows of 64 experts of
-// 1024 x 1024).  An exact 0 is taken as it is; past NEAR_MOST of them, which only data
-// made so will have, they stay as they are.
-constexpr int NEAR_MOST = 32;  // (static shared memory stays under the 1024 bytes left beside the stages)
+// A z next to 0 (sign_band) to be summed again.  The epilogue warps leave them to warp 2,
+// which has nothing else to do, in a queue each, and only do themselves what finds its queue
+// full, and what is left when the tiles are done: done by the epilogue alone they held up the
+// tiles (8192 rows of 64 experts of 1024 x 1024 43 -> 56 us, 16384 of 8 of 8192 x 2048 402 ->
+// 564; so 43 and 427, and 37 and 369 without z).
 struct Near { int e, row, f; };
+constexpr int NEAR_QUEUE = 4;  // (static shared memory stays under the 1024 bytes left beside the stages)
+struct NearQueues {
+    Near at[4 * MMA_GROUPS][NEAR_QUEUE];
+    uint32_t head[4 * MMA_GROUPS], tail[4 * MMA_GROUPS];  // entries put in, and taken out
+    int ended[4 * MMA_GROUPS];                            // the epilogue warp has no more tiles
+    uint32_t tile;                                        // counts tiles: a sign of life
+};
 
-template <typename T>
-__device__ __forceinline__ float resum(const MmaParams& p, int e, int64_t row, int f) {
-    const T* x = reinterpret_cast<const T*>(p.x) + row * p.ldx;
-    const T* w = reinterpret_cast<const T*>(p.weight) + (int64_t)e * p.stride_e + (int64_t)f * p.ldw;
-    float sum = 0.f;
-    for (int k = (threadIdx.x & 31) * 8; k < p.K; k += 256) {  // (rows start on 16 bytes: TMA reads them too)
-        if (k + 8 <= p.K) {
-            const Pack<T> a = *reinterpret_cast<const Pack<T>*>(x + k), b = *reinterpret_cast<const Pack<T>*>(w + k);
-#pragma unroll
-            for (int i = 0; i < 8; ++i) sum = fmaf(El<T>::to(a.v[i]), El<T>::to(b.v[i]), sum);
-        } else {
-            for (int i = k; i < p.K; ++i) sum = fmaf(El<T>::to(x[i]), El<T>::to(w[i]), sum);
+template <bool SIGNS> struct Queues { typedef NearQueues Type; };
+template <> struct Queues<false> { typedef int Type; };
+
+// The whole warp: z of one row and feature, summed again.
+template <typename T> __device__ __forceinline__ double exact_z(const MmaParams& p, const Near& n) {
+    const double sum = exact_sum<T>(reinterpret_cast<const T*>(p.x) + (int64_t)n.row * p.ldx,
+                                    reinterpret_cast<const T*>(p.weight) + (int64_t)n.e * p.stride_e + (int64_t)n.f * p.ldw, p.K);
+    return sum + (p.bias ? (double)El<T>::to(reinterpret_cast<const T*>(p.bias)[(int64_t)n.e * p.F + n.f]) : 0.0);
+}
+template <typename T> __device__ __forceinline__ void settle_sign(const MmaParams& p, const Near& n) {
+    const double z = exact_z<T>(p, n);
+    if ((threadIdx.x & 31) == 0) reinterpret_cast<T*>(p.z)[(int64_t)n.row * p.F + n.f] = El<T>::from((float)z);
+}
+// Takes the oldest entry out of a queue and settles it; false: the queue is empty.  (The entry
+// is copied before it is claimed: only then may its place be filled again.)  The whole warp.
+template <typename T> __device__ __forceinline__ bool settle_oldest(const MmaParams& p, NearQueues& queues, int w) {
+    const int lane = threadIdx.x & 31;
+    Near n = {};
+    int got = 0;
+    if (lane == 0) {
+        for (;;) {  // (ends: another warp claimed an entry each time that this one did not)
+            const uint32_t tail = *(volatile uint32_t*)&queues.tail[w];
+            if (tail == *(volatile uint32_t*)&queues.head[w]) break;
+            __threadfence_block();
+            const volatile Near* at = &queues.at[w][tail % NEAR_QUEUE];
+            n.e = at->e; n.row = at->row; n.f = at->f;
+            __threadfence_block();
+            if (atomicCAS(&queues.tail[w], tail, tail + 1) == tail) { got = 1; break; }
         }
     }
-#pragma unroll
-    for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(~0u, sum, o);
-    return sum;
+    if (!__shfl_sync(~0u, got, 0)) return false;
+    n.e = __shfl_sync(~0u, n.e, 0);
+    n.row = __shfl_sync(~0u, n.row, 0);
+    n.f = __shfl_sync(~0u, n.f, 0);
+    settle_sign<T>(p, n);
+    return true;
 }
+
+// Whether a chunk may hold such a z, by the warp's largest: of |z| in its rounded form, two
+// columns at a time, 16 instructions a chunk.
 template <typename T> struct Two;
 template <> struct Two<__half> { typedef __half2 V; };
 template <> struct Two<__nv_bfloat16> { typedef __nv_bfloat162 V; };
 template <typename T>
-__device__ __forceinline__ void note_near_zero(const float* v, float bias, const MmaParams& p, int e, int64_t c, int f, int left, Near* list, int* count) {
-    if (left < MMA_CHUNK) return;  // (what lies past the columns is not z)
+__device__ __forceinline__ bool may_be_near_zero(const float* v, float bias, const MmaParams& p, int f, int left) {
+    if (left < MMA_CHUNK) return true;  // (what lies past the columns is not z)
     typedef typename Two<T>::V V;
-    V big, least;  // of |z|, two columns at a time in the rounded z: 16 instructions a chunk
+    V big, least;
 #pragma unroll
     for (int j = 0; j < MMA_CHUNK; j += 2) {
         const uint32_t w = pack2<T>(v[j] + bias, v[j + 1] + bias);
@@ -358,16 +383,74 @@ __device__ __forceinline__ void note_near_zero(const float* v, float bias, const
         big = j ? __hmax2(big, z) : z;
         least = j ? __hmin2(least, z) : z;
     }
-    const float most_z = fmaxf(El<T>::to(big.x), El<T>::to(big.y)), least_z = fminf(El<T>::to(least.x), El<T>::to(least.y));
-    // (an infinite z leaves no scale to compare with)
-    const float near = f < p.F && most_z < INFINITY ? most_z * (float)p.K * 3.7252902984619141e-9f : 0.f;
-    if (!__any_sync(~0u, least_z < near)) return;
+    const float most = f < p.F ? fmaxf(El<T>::to(big.x), El<T>::to(big.y)) + fabsf(bias) : 0.f;
+    // (numbers from 0 on compare as their bits do; a NaN or an infinity is not "above" the band and is looked at)
+    const float largest = __uint_as_float(__reduce_max_sync(~0u, __float_as_uint(most)));
+    const float z = fminf(El<T>::to(least.x), El<T>::to(least.y));
+    return __any_sync(~0u, f < p.F && !(z > sign_band(largest, p.K)));
+}
+
+// The lane's z within the band of their row, and its sums that are exactly 0, a bit a column.
+__device__ __forceinline__ void near_columns(const float* v, float bias, int K, bool in, unsigned features, int left, unsigned& near, unsigned& zero) {
+    const float bias_size = fabsf(bias) < INFINITY ? fabsf(bias) : 0.f;
+    const bool few = __popc(features) < 8;  // too few features to tell a row's size: the largest of all rows
+    float all = 0.f;
+    if (few) {
+#pragma unroll
+        for (int j = 0; j < MMA_CHUNK; ++j) {
+            const float z = fabsf(v[j] + bias);
+            if (in && j < left && z < INFINITY) all = fmaxf(all, z + bias_size);
+        }
+        all = __uint_as_float(__reduce_max_sync(~0u, __float_as_uint(all)));
+    }
+    near = zero = 0;
 #pragma unroll
     for (int j = 0; j < MMA_CHUNK; ++j) {
         const float z = fabsf(v[j] + bias);
-        if (z < near && z > 0.f) {
-            const int n = atomicAdd(count, 1);
-            if (n < NEAR_MOST) list[n] = {e, (int)c + j, f};
+        const bool here = in && j < left;
+        float row = all;
+        if (!few) row = __uint_as_float(__reduce_max_sync(~0u, __float_as_uint(here && z < INFINITY ? z + bias_size : 0.f)));
+        const float band = sign_band(row, K);
+        near |= (unsigned)(here && band > 0.f && z <= band) << j;
+        zero |= (unsigned)(here && v[j] == 0.f) << j;
+    }
+}
+
+// Hands the chunk's z next to 0 on to warp 2.  Exact zeros come by the hundred from rows of
+// zeros, from features whose weights are zeros, and from products that are mostly zeros or
+// small whole numbers; one by accident of rounding in 80000 chunks.  Whole rows and whole
+// features of them are taken as they are, and so are two and more where the first one is 0
+// summed again, too.
+template <typename T>
+__device__ __noinline__ void settle_signs(unsigned near, unsigned zero, const MmaParams& p, NearQueues& queues, int w, int e, int c, int f, int left) {
+    const int lane = threadIdx.x & 31;
+    const unsigned features = __ballot_sync(~0u, f < p.F), rows = left < MMA_CHUNK ? (1u << left) - 1 : (1u << MMA_CHUNK) - 1;
+    const unsigned empty = __reduce_and_sync(~0u, f < p.F ? zero : ~0u);
+    if (__popc(features) >= 8) near &= ~empty;
+    if (left >= 8 && zero == rows) near = 0;
+    if (__reduce_add_sync(~0u, __popc(near & zero)) >= 2) {
+        const int from = __ffs(__ballot_sync(~0u, (near & zero) != 0)) - 1;
+        const int j = __shfl_sync(~0u, __ffs(near & zero) - 1, from);
+        if (exact_sum<T>(reinterpret_cast<const T*>(p.x) + (int64_t)(c + j) * p.ldx,
+                         reinterpret_cast<const T*>(p.weight) + (int64_t)e * p.stride_e + (int64_t)(f - lane + from) * p.ldw, p.K) == 0.0)
+            near &= ~zero;
+    }
+    __syncwarp();  // finish()'s stores come before those that replace them
+    for (unsigned any = __reduce_or_sync(~0u, near); any; any &= any - 1) {
+        const int j = __ffs(any) - 1;
+        for (unsigned todo = __ballot_sync(~0u, near >> j & 1); todo; todo &= todo - 1) {
+            const Near n = {e, c + j, f - lane + __ffs(todo) - 1};
+            bool full = false;
+            if (lane == 0) {
+                const uint32_t head = queues.head[w];
+                full = head - *(volatile uint32_t*)&queues.tail[w] >= NEAR_QUEUE;
+                if (!full) {
+                    queues.at[w][head % NEAR_QUEUE] = n;
+                    __threadfence_block();
+                    *(volatile uint32_t*)&queues.head[w] = head + 1;
+                }
+            }
+            if (__any_sync(~0u, full)) settle_sign<T>(p, n);
         }
     }
 }
@@ -381,9 +464,11 @@ __device__ __forceinline__ void load_residual(uint32_t* res, const MmaParams& p,
     for (int j = 0; j < MMA_CHUNK; j += 2, at += p.ldr) res[j / 2] = j < mine ? __ldg(at) : 0u;
 }
 
-template <int PASS, typename T, int ACT>
+// Z: the forward pass keeps z for the gradient.
+template <int PASS, typename T, int ACT, bool Z>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(MMA_THREADS, 1)
-    mma_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const MmaParams p) {
+    mma_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
+               const __grid_constant__ MmaParams p) {
     constexpr bool A_K_MAJOR = PASS == PASS_FORWARD, B_K_MAJOR = PASS != PASS_WEIGHT;
     extern __shared__ unsigned char smem_raw[];
     // full, tempty, patched: the first CTA's are used; empty, tfull, landed: each CTA its own
@@ -393,8 +478,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(MMA_THREADS, 1)
     __shared__ uint32_t s_issued;
     __shared__ int s_tiles;
     __shared__ Tile s_tile[MMA_TILES];
-    __shared__ Near s_near[PASS == PASS_FORWARD && ACT == ELA_ACT_RELU ? NEAR_MOST : 1];
-    __shared__ int s_near_count;
+    constexpr bool SIGNS = Z && ACT == ELA_ACT_RELU;
+    __shared__ typename Queues<SIGNS>::Type s_near;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int rank = blockIdx.x & 1, pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
     // the experts' tables, then the stages, each on a 1024-byte boundary
@@ -414,7 +499,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(MMA_THREADS, 1)
     }
     if (tid == 0) {
         s_abort = 0;
-        s_near_count = 0;
         for (int s = 0; s < p.stages; ++s) { bar_init(&full[s], 1); bar_init(&empty[s], 1); }
         for (int b = 0; b < 2; ++b) { bar_init(&tfull[b], 1); bar_init(&tempty[b], 2 * 4 * MMA_GROUPS); }
         for (int i = 0; i < MMA_TILES; ++i) { bar_init(&sfull[i], 1); bar_init(&sempty[i], 4 * MMA_GROUPS + 1 + (rank == 0)); }
@@ -422,6 +506,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(MMA_THREADS, 1)
         for (int s = 0; s < p.stages; ++s) bar_init(&patched[s], 1);
         bar_init(&drained, 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if constexpr (SIGNS) {
+        if (tid < 4 * MMA_GROUPS) s_near.head[tid] = s_near.tail[tid] = s_near.ended[tid] = 0;
+        if (tid == 0) s_near.tile = 0;
     }
     previous_done();  // (no memory was touched before)
     for (int e = tid; e < p.E; e += MMA_THREADS) expert_rows(p.offsets, e, p.R, table[e], table[p.E + e]);
@@ -612,6 +700,32 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(MMA_THREADS, 1)
             phase = __shfl_sync(~0u, phase, who);
             ++it;
         }
+    } else if (SIGNS && warp == 2) {  // ---- z next to 0, as the epilogue finds them
+        if constexpr (SIGNS) {
+            const bool mine = lane < 4 * MMA_GROUPS;
+            uint32_t tile = 0;
+            unsigned long long t0 = 0, now;
+            for (;;) {
+                const bool ended = !mine || *(volatile int*)&s_near.ended[lane];
+                __threadfence_block();
+                const unsigned have = __ballot_sync(~0u, mine && *(volatile uint32_t*)&s_near.head[lane] != *(volatile uint32_t*)&s_near.tail[lane]);
+                if (have) {
+                    settle_oldest<T>(p, s_near, __ffs(have) - 1);
+                    t0 = 0;
+                    continue;
+                }
+                if (__all_sync(~0u, ended)) break;
+                __nanosleep(500);
+                asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(now));
+                const uint32_t seen = *(volatile uint32_t*)&s_near.tile;
+                if (t0 == 0 || seen != tile) { t0 = now; tile = seen; }
+                // (the epilogue's own waits end first: two of them at most between tiles)
+                if (__any_sync(~0u, now - t0 > 4 * p.wait_ns)) {
+                    if (lane == 0) give_up();
+                    break;
+                }
+            }
+        }
     } else if (warp >= 4) {  // ---- epilogue
         const int w = warp & 3, group = (warp - 4) >> 2;
         if constexpr (PASS != PASS_WEIGHT) {  // rows of no expert: the residual, or 0
@@ -627,7 +741,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(MMA_THREADS, 1)
         int it = 0;
         bool ok = true;
         constexpr bool FWD = PASS == PASS_FORWARD;
-        const bool with_z = PASS == PASS_FORWARD && p.z, with_res = PASS == PASS_FORWARD && p.residual;
+        const bool with_res = PASS == PASS_FORWARD && p.residual;
         auto accumulators = [&](int half, int it) {  // waits for the tile's products
             if (lane == 0) ok = bar_wait(&tfull[half], (it >> 1) & 1, p.wait_ns, abort);
             ok = __shfl_sync(~0u, (int)ok, 0);
@@ -642,10 +756,15 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(MMA_THREADS, 1)
             if (lane == 0) bar_arrive_relaxed_at(leader_addr(&tempty[half]));
         };
         auto write = [&](float* v, float bias, const uint32_t* res, int64_t c, int f, int left) {
-            if (with_z) {
-                if constexpr (FWD && ACT == ELA_ACT_RELU) note_near_zero<T>(v, bias, p, t.e, c, f, left, s_near, &s_near_count);
-                if (with_res) finish<T, ACT, FWD, FWD, FWD, false>(v, bias, res, p, c, f, left);
-                else finish<T, ACT, FWD, FWD, false, false>(v, bias, res, p, c, f, left);
+            if constexpr (Z) {
+                if (with_res) finish<T, ACT, FWD, true, FWD, false>(v, bias, res, p, c, f, left);
+                else finish<T, ACT, FWD, true, false, false>(v, bias, res, p, c, f, left);
+                if constexpr (SIGNS)
+                    if (may_be_near_zero<T>(v, bias, p, f, left)) {
+                        unsigned near, zero;
+                        near_columns(v, bias, p.K, f < p.F, __ballot_sync(~0u, f < p.F), left, near, zero);
+                        if (__any_sync(~0u, near != 0)) settle_signs<T>(near, zero, p, s_near, warp - 4, t.e, (int)c, f, left);
+                    }
             } else {
                 if (with_res) finish<T, ACT, FWD, false, FWD, false>(v, bias, res, p, c, f, left);
                 else if (p.vec && left >= MMA_CHUNK && (f | 31) < p.F) finish<T, ACT, FWD, false, false, true>(v, bias, res, p, c, f, left);
@@ -677,15 +796,18 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(MMA_THREADS, 1)
             }
             if (product) release(half);
             it += product;
-        }
-        if constexpr (FWD && ACT == ELA_ACT_RELU) {
-            asm volatile("barrier.cta.sync 1, %0;" ::"n"(MMA_GROUPS * 128) : "memory");
-            for (int i = warp - 4; with_z && i < min(s_near_count, NEAR_MOST); i += 4 * MMA_GROUPS) {
-                const Near at = s_near[i];
-                float z = resum<T>(p, at.e, at.row, at.f);
-                if (p.bias) z += El<T>::to(reinterpret_cast<const T*>(p.bias)[(int64_t)at.e * p.F + at.f]);
-                if (lane == 0) reinterpret_cast<T*>(p.z)[(int64_t)at.row * p.F + at.f] = El<T>::from(z);
+            if constexpr (SIGNS) {
+                if (tid == 128) *(volatile uint32_t*)&s_near.tile = i + 1;
+                // (off the tiles' path by now: the other half of TMEM is being filled)
+                while (__shfl_sync(~0u, s_near.head[warp - 4] - *(volatile uint32_t*)&s_near.tail[warp - 4], 0) > NEAR_QUEUE / 2)
+                    settle_oldest<T>(p, s_near, warp - 4);
             }
+        }
+        if constexpr (SIGNS) {
+            __syncwarp();
+            __threadfence_block();
+            if (lane == 0) *(volatile int*)&s_near.ended[warp - 4] = 1;
+            while (settle_oldest<T>(p, s_near, warp - 4)) {}
         }
     }
     __syncthreads();
@@ -739,11 +861,11 @@ inline bool make_map(CUtensorMap* map, int dtype, const void* base, int64_t d0, 
               CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-template <int PASS, typename T, int ACT>
+template <int PASS, typename T, int ACT, bool Z = false>
 int mma_launch(const CUtensorMap& a, const CUtensorMap& b, const MmaParams& p, int64_t max_tiles, cudaStream_t st) {
-    auto kern = mma_kernel<PASS, T, ACT>;
+    auto kern = mma_kernel<PASS, T, ACT, Z>;
     const int sms = sm_count();
-    if (sms == 0 || !allow_smem<&mma_kernel<PASS, T, ACT>>(MMA_SMEM - 1024)) return ELA_ERR_CUDA;
+    if (sms == 0 || !allow_smem<&mma_kernel<PASS, T, ACT, Z>>(MMA_SMEM - 1024)) return ELA_ERR_CUDA;
     const int grid = 2 * (int)(max_tiles < sms / 2 ? max_tiles : sms / 2);
     return launch(kern, grid, MMA_THREADS, MMA_SMEM - 1024, st, a, b, p);
 }

@@ -1,0 +1,88 @@
+"""GPU tests of the expert-layer operators where ordinary data does not lead:
+signs next to 0, the ends of fp16's range, sizes at a limit, derivatives that
+are not there."""
+import pytest
+import torch
+
+import efficient_linear_assignment_b200 as ela
+
+pytestmark = pytest.mark.gpu
+
+
+def gen(seed):
+    return torch.Generator().manual_seed(seed)
+
+
+def slopes_of(x, w, b, counts, act):
+    """act'(z) of every row and feature, as the operator rounds it: the rows get a
+    column each that no weight reads, dy is 1, and dW's entry there is that row's dz."""
+    R, E = x.shape[0], len(counts)
+    tag = torch.eye(R, dtype=x.dtype)
+    xt = torch.cat([x, tag], 1).cuda()
+    wt = torch.cat([w, torch.zeros(*w.shape[:2], R, dtype=w.dtype)], 2).cuda().requires_grad_()
+    off = torch.tensor([0] + list(counts)).cumsum(0)
+    y = ela.expert_linear(xt, wt, None if b is None else b.cuda(), None, act, off.int().cuda())
+    (dw,) = torch.autograd.grad(y, wt, torch.ones_like(y))
+    e = torch.repeat_interleave(torch.arange(E), torch.tensor(counts))
+    return dw.cpu()[e, :, x.shape[1] + torch.arange(R)]
+
+
+def exact_z(x, w, b, counts):
+    out = []
+    for e, part in enumerate(x.split(list(counts))):
+        out.append(part.double() @ w[e].double().t() + (0 if b is None else b[e].double()))
+    return torch.cat(out)
+
+
+def cancelling(counts, half, N, dtype, every, seed, bias=False):
+    """Every so-and-so-many-th feature's sum is the two halves of K against each other plus one
+    product of size 2^-23 to 2^-16 (with a bias: a sum that the bias takes away but for its
+    rounding): z is next to 0 with a sign that the order of an fp32 sum would decide."""
+    g = gen(seed)
+    R, E = sum(counts), len(counts)
+    p = torch.randn(R, half, generator=g)
+    sign = torch.randint(0, 2, (R, 1), generator=g) * 2.0 - 1
+    x = torch.cat([p, p, sign * 2.0 ** -6], 1).to(dtype)
+    w = (torch.randn(E, N, 2 * half + 1, generator=g) * half ** -0.5).to(dtype)
+    w[:, ::every, half:2 * half] = -w[:, ::every, :half]
+    w[:, ::every, 2 * half] = (torch.exp2(-torch.randint(10, 18, (E, w[:, ::every].shape[1]), generator=g).float())).to(dtype)
+    b = None
+    if bias:
+        b = torch.randn(E, N, generator=g).to(dtype)
+        # feature 1's sum: x's first column is 1, its weight there the bias's opposite
+        x[:, 0] = 1
+        x[:, half] = 1
+        w[:, ::every, 0] = -b[:, ::every]
+        w[:, ::every, half] = 0
+    return x, w, b
+
+
+# ---------------------------------------------------------------- ReLU's slope next to 0
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("bias", [False, True])
+@pytest.mark.parametrize("counts,half,N,every", [([100, 87, 63], 96, 136, 8), ([300], 500, 264, 32), ([70, 66, 65], 40, 520, 4),
+                                                 ([17] * 40, 64, 72, 8)])
+def test_relu_slope_next_to_zero(counts, half, N, every, bias, dtype):
+    """The slope is the sign of the 64-bit sum, in every row, the last of an expert's too."""
+    x, w, b = cancelling(counts, half, N, dtype, every, 5 * half + N, bias)
+    z = exact_z(x, w, b, counts)
+    near = z.abs() < 2.0 ** -15
+    assert near.float().mean() > 0.5 / every and (z[near] != 0).all()
+    got = slopes_of(x, w, b, counts, "relu")
+    assert torch.equal(got.double(), (z > 0).double())
+
+
+def test_relu_gradients_same_bits():
+    """More sums next to 0 than any CTA could list, the same gradients every time."""
+    counts = [700, 801, 523]
+    x, w, b = cancelling(counts, 120, 512, torch.bfloat16, 4, 3)
+    off = torch.tensor([0] + counts).cumsum(0).int().cuda()
+    leaf = [v.cuda().requires_grad_() for v in (x, w)]
+    dy = torch.randn(sum(counts), 512, generator=gen(4)).to(torch.bfloat16).cuda()
+    first = None
+    for _ in range(20):
+        y = ela.expert_linear(*leaf, None, None, "relu", off)
+        grads = torch.autograd.grad(y, leaf, dy)
+        first = first or grads
+        assert all(torch.equal(a, b) for a, b in zip(first, grads))
