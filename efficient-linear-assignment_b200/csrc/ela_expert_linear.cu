@@ -301,6 +301,7 @@ int ela_expert_linear(const void* x, const void* weight, const void* bias, const
         const int vb = bits % 32 == 0 ? 32 : bits % 16 == 0 ? 16 : bits % 4 == 0 ? 4 : 2;
         int rc = ELA_OK;
         ELA_BY_TYPE(dtype, { ELA_BY_ACT(activation, rc = R <= 4 * E || (E == 1 && R <= 8) ? (stream_launch<T_, A_, 1>(q, vb, st)) : R <= 16 * E ? (stream_launch<T_, A_, 2>(q, vb, st)) : (stream_launch<T_, A_, 4>(q, vb, st))) })
+        if (rc == ELA_OK && z && activation == ELA_ACT_RELU) ELA_BY_TYPE(dtype, { rc = settle_launch<T_>(q, st); })
         return rc;
     }
     char* ws = reinterpret_cast<char*>(workspace);

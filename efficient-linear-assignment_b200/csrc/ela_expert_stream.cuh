@@ -196,6 +196,70 @@ __global__ void __launch_bounds__(STREAM_WARPS * 32, 2) stream_kernel(const Stre
     }
 }
 
+// ReLU's z next to 0, summed again where z is kept (sign_band): a pass of its own over z, which
+// is small here, since the call of exact_sum cost the kernel above the registers of its loads
+// (16 rows of 16 experts of 4096 x 1024: 23 -> 45 us inside it, 27 as a pass; 16 rows each 29 -> 57, 36).  A warp
+// takes 256 features of a row, whose largest z is the scale.  Two and more exact zeros, which
+// rows of zeros make, are taken as they are where the first is 0 summed again, too.
+constexpr int SETTLE_GROUPS = 8;  // of 32 features
+template <typename T>
+__global__ void __launch_bounds__(256) settle_kernel(const StreamParams p) {
+    next_may_start();
+    previous_done();
+    const int lane = threadIdx.x & 31, segments = (p.N + 32 * SETTLE_GROUPS - 1) / (32 * SETTLE_GROUPS);
+    const int64_t unit = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
+    if (unit >= (int64_t)p.R * segments) return;
+    const int r = (int)(unit / segments), f0 = (int)(unit - (int64_t)r * segments) * 32 * SETTLE_GROUPS;
+    int e = 0, r0, r1;
+    for (int end = p.E; p.offsets && end - e > 1;) {  // the last expert that starts at or before r
+        const int mid = (e + end) >> 1;
+        if (clampi(p.offsets[mid], 0, p.R) <= r) e = mid; else end = mid;
+    }
+    expert_rows(p.offsets, e, p.R, r0, r1);
+    if (r < r0 || r >= r1) return;
+    T* zrow = reinterpret_cast<T*>(p.z) + (int64_t)r * p.N;
+    const T* bias = p.bias ? reinterpret_cast<const T*>(p.bias) + (int64_t)e * p.N : nullptr;
+    float z[SETTLE_GROUPS], b[SETTLE_GROUPS], largest = 0.f;
+#pragma unroll
+    for (int i = 0; i < SETTLE_GROUPS; ++i) {
+        const int f = f0 + 32 * i + lane;
+        z[i] = f < p.N ? fabsf(El<T>::to(zrow[f])) : INFINITY;
+        b[i] = f < p.N && bias ? El<T>::to(bias[f]) : 0.f;
+    }
+#pragma unroll
+    for (int i = 0; i < SETTLE_GROUPS; ++i)
+        if (z[i] < INFINITY) largest = fmaxf(largest, z[i] + (fabsf(b[i]) < INFINITY ? fabsf(b[i]) : 0.f));
+    // (numbers from 0 on compare as their bits do; 1.01: z is rounded)
+    const float band = 1.01f * sign_band(__uint_as_float(__reduce_max_sync(~0u, __float_as_uint(largest))), p.K);
+    if (!(band > 0.f)) return;
+    const T* x = reinterpret_cast<const T*>(p.x) + (int64_t)r * p.ldx;
+    const T* w = reinterpret_cast<const T*>(p.w) + (int64_t)e * p.stride_e;
+    unsigned near = 0, zero = 0;  // a bit a group
+#pragma unroll
+    for (int i = 0; i < SETTLE_GROUPS; ++i) {
+        near |= (unsigned)(z[i] <= band) << i;
+        zero |= (unsigned)(z[i] == 0.f && b[i] == 0.f) << i;
+    }
+    if (__reduce_add_sync(~0u, __popc(zero)) >= 2) {
+        const int from = __ffs(__ballot_sync(~0u, zero != 0)) - 1;
+        const int f = f0 + 32 * (__shfl_sync(~0u, __ffs(zero), from) - 1) + from;
+        if (exact_sum<T>(x, w + (int64_t)f * p.ldw, p.K) == 0.0) near &= ~zero;
+    }
+    for (unsigned any = __reduce_or_sync(~0u, near); any; any &= any - 1) {
+        const int i = __ffs(any) - 1;
+        for (unsigned todo = __ballot_sync(~0u, near >> i & 1); todo; todo &= todo - 1) {
+            const int f = f0 + 32 * i + __ffs(todo) - 1;
+            const double sum = exact_sum<T>(x, w + (int64_t)f * p.ldw, p.K);
+            if (lane == 0) zrow[f] = El<T>::from((float)(sum + (bias ? (double)El<T>::to(bias[f]) : 0.0)));
+        }
+    }
+}
+template <typename T> int settle_launch(const StreamParams& p, cudaStream_t st) {
+    const int64_t units = (int64_t)p.R * ((p.N + 32 * SETTLE_GROUPS - 1) / (32 * SETTLE_GROUPS)), blocks = (units + 7) / 8;
+    if (blocks > INT32_MAX) return ELA_ERR_UNSUPPORTED;
+    return launch(settle_kernel<T>, (unsigned)blocks, 256, 0, st, p);
+}
+
 // Rows per expert up to which the weights' read is what the product costs: 16 rows for
 // each of 16 experts take 31 us here and 33 us by tiles, 32 rows 45 and 34.  Where tiles
 // of 256 features leave half of the pairs idle, which then read at 44 GB/s an SM, up to 64.

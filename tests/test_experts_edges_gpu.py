@@ -73,6 +73,17 @@ def test_relu_slope_next_to_zero(counts, half, N, every, bias, dtype):
     assert torch.equal(got.double(), (z > 0).double())
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("bias", [False, True])
+@pytest.mark.parametrize("counts,half,N,every", [([1, 0, 2, 1], 96, 64, 8), ([9, 8, 20, 3], 250, 48, 8), ([4, 1], 33, 136, 16),
+                                                 ([40], 500, 96, 32)])
+def test_relu_slope_next_to_zero_few_rows(counts, half, N, every, bias, dtype):
+    x, w, b = cancelling(counts, half, N, dtype, every, 7 * half + N, bias)
+    z = exact_z(x, w, b, counts)
+    assert (z.abs() < 2.0 ** -15).any()
+    assert torch.equal(slopes_of(x, w, b, counts, "relu").double(), (z > 0).double())
+
+
 def test_relu_gradients_same_bits():
     """More sums next to 0 than any CTA could list, the same gradients every time."""
     counts = [700, 801, 523]
