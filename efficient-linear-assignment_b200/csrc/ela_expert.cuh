@@ -155,6 +155,13 @@ template <int ACT> __device__ __forceinline__ float act_slope(float z) {
 // sums, which leave no sum beside them to tell, keep the fp32 sum's sign.)
 __device__ __forceinline__ float sign_band(float largest, int K) { return largest * ((float)K + 64.f) * 5.587935447692871e-9f; }
 
+// z as it is kept for ReLU's gradient, which needs its sign alone: what rounds to 0 in fp16
+// (below 2^-25) is kept as the smallest number there is, so a positive z stays positive.
+template <typename T> __device__ __forceinline__ float sign_kept(float z) {
+    if constexpr (!El<T>::BF16) return z > 0.f ? fmaxf(z, 5.9604644775390625e-8f) : z;
+    return z;  // (bf16 has fp32's range)
+}
+
 // A sum in two floats: the rounding error of each addition, which is itself a float (Knuth's
 // two-sum), is added up beside it.  Products of 16-bit values are exact in fp32.
 struct TwoFloats {

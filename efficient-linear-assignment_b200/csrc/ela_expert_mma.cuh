@@ -286,7 +286,7 @@ __device__ __forceinline__ void finish(float* v, float bias, const uint32_t* res
             float a = v[j], b = v[j + 1];
             if (BIAS) { a += bias; b += bias; }
             if (Z) {
-                const uint32_t w = swap_pair(pack2<T>(a, b), order);
+                const uint32_t w = swap_pair(ACT == ELA_ACT_RELU ? pack2<T>(sign_kept<T>(a), sign_kept<T>(b)) : pack2<T>(a, b), order);
                 if (ALL || j < mine) *reinterpret_cast<uint32_t*>(zout) = w;
                 zout += step;
             }
@@ -307,7 +307,7 @@ __device__ __forceinline__ void finish(float* v, float bias, const uint32_t* res
             if (j < left) {
                 const float a = BIAS ? v[j] + bias : v[j];
                 const int64_t at = (c + j) * p.F + f;
-                if (Z) reinterpret_cast<T*>(p.z)[at] = El<T>::from(a);
+                if (Z) reinterpret_cast<T*>(p.z)[at] = El<T>::from(ACT == ELA_ACT_RELU ? sign_kept<T>(a) : a);
                 const float r = RES ? El<T>::to(reinterpret_cast<const T*>(p.residual)[(c + j) * p.ldr + f]) : 0.f;
                 reinterpret_cast<T*>(p.out)[at] = El<T>::from(act_value<ACT>(a) + r);
             }
@@ -339,7 +339,7 @@ template <typename T> __device__ __forceinline__ double exact_z(const MmaParams&
 }
 template <typename T> __device__ __forceinline__ void settle_sign(const MmaParams& p, const Near& n) {
     const double z = exact_z<T>(p, n);
-    if ((threadIdx.x & 31) == 0) reinterpret_cast<T*>(p.z)[(int64_t)n.row * p.F + n.f] = El<T>::from((float)z);
+    if ((threadIdx.x & 31) == 0) reinterpret_cast<T*>(p.z)[(int64_t)n.row * p.F + n.f] = El<T>::from(sign_kept<T>((float)z));
 }
 // Takes the oldest entry out of a queue and settles it; false: the queue is empty.  (The entry
 // is copied before it is claimed: only then may its place be filled again.)  The whole warp.

@@ -186,7 +186,7 @@ __global__ void __launch_bounds__(STREAM_WARPS * 32, 2) stream_kernel(const Stre
                 for (int w = 0; w < STREAM_WARPS; ++w) v += part[w][c][i % F];
                 if (p.bias) v += El<T>::to(reinterpret_cast<const T*>(p.bias)[(int64_t)done_e * p.N + f]);
                 const int64_t at = (int64_t)r * p.N + f;
-                if (p.z) reinterpret_cast<T*>(p.z)[at] = El<T>::from(v);
+                if (p.z) reinterpret_cast<T*>(p.z)[at] = El<T>::from(ACT == ELA_ACT_RELU ? sign_kept<T>(v) : v);
                 v = act_value<ACT>(v);
                 if (residual) v += El<T>::to(residual[r * p.ldr + f]);
                 y[at] = El<T>::from(v);
@@ -250,7 +250,7 @@ __global__ void __launch_bounds__(256) settle_kernel(const StreamParams p) {
         for (unsigned todo = __ballot_sync(~0u, near >> i & 1); todo; todo &= todo - 1) {
             const int f = f0 + 32 * i + __ffs(todo) - 1;
             const double sum = exact_sum<T>(x, w + (int64_t)f * p.ldw, p.K);
-            if (lane == 0) zrow[f] = El<T>::from((float)(sum + (bias ? (double)El<T>::to(bias[f]) : 0.0)));
+            if (lane == 0) zrow[f] = El<T>::from(sign_kept<T>((float)(sum + (bias ? (double)El<T>::to(bias[f]) : 0.0))));
         }
     }
 }

@@ -97,3 +97,19 @@ def test_relu_gradients_same_bits():
         grads = torch.autograd.grad(y, leaf, dy)
         first = first or grads
         assert all(torch.equal(a, b) for a, b in zip(first, grads))
+
+
+# ---------------------------------------------------------------- fp16's range
+
+@pytest.mark.parametrize("rows", [3, 300])
+def test_relu_slope_below_fp16(rows):
+    """A sum too small for fp16 still has its sign."""
+    g = gen(8)
+    x = torch.randn(rows, 64, generator=g).half()
+    w = torch.randn(1, 40, 64, generator=g).half()
+    w[0, ::4] = 0
+    x[:, 0] = 2.0 ** -12 * (torch.randint(0, 2, (rows,), generator=g) * 2 - 1)
+    w[0, ::4, 0] = 2.0 ** -14
+    z = exact_z(x, w, None, [rows])
+    assert (z[:, ::4].abs() == 2.0 ** -26).all()
+    assert torch.equal(slopes_of(x, w, None, [rows], "relu").double(), (z > 0).double())
