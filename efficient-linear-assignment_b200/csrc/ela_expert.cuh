@@ -155,6 +155,15 @@ template <int ACT> __device__ __forceinline__ float act_slope(float z) {
 // sums, which leave no sum beside them to tell, keep the fp32 sum's sign.)
 __device__ __forceinline__ float sign_band(float largest, int K) { return largest * ((float)K + 64.f) * 5.587935447692871e-9f; }
 
+// The type that z is kept in for the gradient: fp32 for GELU and SiLU, whose slope moves with
+// z's rounding and is NaN at the infinity that a finite z past fp16's range would become; 16
+// bits for ReLU, whose slope is z's sign.  Training 16384 rows through 8 experts of 8192 x 2048
+// took 1667 us with 16 bits for GELU, too, and takes 1728; its outputs were off by 0.0024 and
+// are by 0.0023, the rest of it dz's own rounding.
+template <typename T, int ACT> struct Kept { typedef T Type; };
+template <typename T> struct Kept<T, ELA_ACT_GELU> { typedef float Type; };
+template <typename T> struct Kept<T, ELA_ACT_SILU> { typedef float Type; };
+
 // z as it is kept for ReLU's gradient, which needs its sign alone: what rounds to 0 in fp16
 // (below 2^-25) is kept as the smallest number there is, so a positive z stays positive.
 template <typename T> __device__ __forceinline__ float sign_kept(float z) {

@@ -87,10 +87,12 @@ constexpr int ACT_COLS = 256, ACT_WARPS = 8, ACT_ROWS = 2;  // rows a lane has i
 // Two rows in flight at four CTAs an SM (64 registers): 155 us for 16384 x 8192 GELU with its
 // sums, against 179 for four rows at two CTAs and 208 for two rows at five (spills).
 template <typename T, int ACT, bool VEC>
-__global__ void __launch_bounds__(ACT_WARPS * 32, 4) grad_act_kernel(const T* dy, const T* z, const int32_t* offsets, int R,
+__global__ void __launch_bounds__(ACT_WARPS * 32, 4) grad_act_kernel(const T* dy, const typename Kept<T, ACT>::Type* z, const int32_t* offsets, int R,
                                                                   int E, int N, int block_rows, T* dz, float* partial) {
     next_may_start();
     previous_done();
+    typedef typename Kept<T, ACT>::Type Z;
+    struct alignas(16) Eight { Z v[8]; };
     __shared__ float part[ACT_WARPS][ACT_COLS];
     const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
     const int strips = (N + ACT_COLS - 1) / ACT_COLS, strip = blockIdx.x % strips, block = blockIdx.x / strips;
@@ -112,14 +114,15 @@ __global__ void __launch_bounds__(ACT_WARPS * 32, 4) grad_act_kernel(const T* dy
         if (r0 >= r1) continue;
         float sum[8] = {};
         if (VEC && n0 < N) {
-            const T *gp = dy + (int64_t)(r0 + w) * N + n0, *zp = z + (int64_t)(r0 + w) * N + n0;
+            const T* gp = dy + (int64_t)(r0 + w) * N + n0;
+            const Z* zp = z + (int64_t)(r0 + w) * N + n0;
             T* dp = dz + (int64_t)(r0 + w) * N + n0;
             const int64_t step = (int64_t)ACT_WARPS * N;
-            auto row = [&](Pack<T>& g, const Pack<T>& q, T* to) {
+            auto row = [&](Pack<T>& g, const Eight& q, T* to) {
 #pragma unroll
                 for (int c = 0; c < 8; ++c) {
                     float v = El<T>::to(g.v[c]);
-                    if (ACT != ELA_ACT_NONE) v *= act_slope<ACT>(El<T>::to(q.v[c]));
+                    if (ACT != ELA_ACT_NONE) v *= act_slope<ACT>(El<Z>::to(q.v[c]));
                     sum[c] += v;
                     g.v[c] = El<T>::from(v);
                 }
@@ -127,11 +130,12 @@ __global__ void __launch_bounds__(ACT_WARPS * 32, 4) grad_act_kernel(const T* dy
             };
             int r = r0 + w;
             for (; r + (ACT_ROWS - 1) * ACT_WARPS < r1; r += ACT_WARPS * ACT_ROWS) {
-                Pack<T> g[ACT_ROWS], q[ACT_ROWS];
+                Pack<T> g[ACT_ROWS];
+                Eight q[ACT_ROWS];
 #pragma unroll
                 for (int i = 0; i < ACT_ROWS; ++i) {
                     g[i] = *reinterpret_cast<const Pack<T>*>(gp + i * step);
-                    if (ACT != ELA_ACT_NONE) q[i] = *reinterpret_cast<const Pack<T>*>(zp + i * step);
+                    if (ACT != ELA_ACT_NONE) q[i] = *reinterpret_cast<const Eight*>(zp + i * step);
                 }
 #pragma unroll
                 for (int i = 0; i < ACT_ROWS; ++i) row(g[i], q[i], dp + i * step);
@@ -140,8 +144,9 @@ __global__ void __launch_bounds__(ACT_WARPS * 32, 4) grad_act_kernel(const T* dy
                 dp += ACT_ROWS * step;
             }
             for (; r < r1; r += ACT_WARPS) {
-                Pack<T> g = *reinterpret_cast<const Pack<T>*>(gp), q;
-                if (ACT != ELA_ACT_NONE) q = *reinterpret_cast<const Pack<T>*>(zp);
+                Pack<T> g = *reinterpret_cast<const Pack<T>*>(gp);
+                Eight q;
+                if (ACT != ELA_ACT_NONE) q = *reinterpret_cast<const Eight*>(zp);
                 row(g, q, dp);
                 gp += step;
                 zp += step;
@@ -149,7 +154,8 @@ __global__ void __launch_bounds__(ACT_WARPS * 32, 4) grad_act_kernel(const T* dy
             }
         } else if (!VEC) {
             for (int r = r0 + w; r < r1; r += 2 * ACT_WARPS) {  // two rows' loads before their stores: 4096 x 2051 33 -> 22 us, 300 x 1500 33 -> 15
-                T g[2][8] = {}, q[2][8] = {};
+                T g[2][8] = {};
+                Z q[2][8] = {};
 #pragma unroll
                 for (int i = 0; i < 2; ++i)
 #pragma unroll
@@ -165,7 +171,7 @@ __global__ void __launch_bounds__(ACT_WARPS * 32, 4) grad_act_kernel(const T* dy
                     for (int c = 0; c < 8; ++c)
                         if (r + i * ACT_WARPS < r1 && n0 + c * 32 < N) {
                             float v = El<T>::to(g[i][c]);
-                            if (ACT != ELA_ACT_NONE) v *= act_slope<ACT>(El<T>::to(q[i][c]));
+                            if (ACT != ELA_ACT_NONE) v *= act_slope<ACT>(El<Z>::to(q[i][c]));
                             sum[c] += v;
                             if (dz) dz[(int64_t)(r + i * ACT_WARPS) * N + n0 + c * 32] = El<T>::from(v);
                         }
@@ -320,7 +326,7 @@ int ela_expert_linear(const void* x, const void* weight, const void* bias, const
     p.ldr = ldr;
     p.out = y;
     p.z = z;
-    p.vec = N % 2 == 0 && aligned4(y) && (!z || aligned4(z)) && (!residual || (aligned4(residual) && ldr % 2 == 0));
+    p.vec = N % 2 == 0 && aligned4(y) && (!z || (reinterpret_cast<uintptr_t>(z) & 7) == 0) && (!residual || (aligned4(residual) && ldr % 2 == 0));
     CUtensorMap a, b;
     if (!map_of(&a, dtype, mw, MMA_KB, MMA_F, true) || !map_of(&b, dtype, mx, MMA_KB, p.bbox, false)) return ELA_ERR_CUDA;
     ELA_BY_TYPE(dtype, { ELA_BY_ACT(activation, rc = z ? (mma_launch<PASS_FORWARD, T_, A_, true>(a, b, p, row_tiles(p), st)) : (mma_launch<PASS_FORWARD, T_, A_>(a, b, p, row_tiles(p), st))) })
@@ -346,7 +352,7 @@ int ela_expert_linear_grad_act(const void* dy, const void* z, const int32_t* off
         if (R > 0)
             ELA_BY_ACT(activation, {
                 auto kern = vec ? grad_act_kernel<T_, A_, true> : grad_act_kernel<T_, A_, false>;
-                rc = launch(kern, grid, ACT_WARPS * 32, 0, st, (const T_*)dy, (const T_*)z, offsets, (int)R, (int)E, (int)N, rows, (T_*)dz, partial);
+                rc = launch(kern, grid, ACT_WARPS * 32, 0, st, (const T_*)dy, (const typename Kept<T_, A_>::Type*)z, offsets, (int)R, (int)E, (int)N, rows, (T_*)dz, partial);
             })
         if (dbias && rc == ELA_OK)
             rc = launch(sum_kernel<T_>, (unsigned)(E * ((N + 31) / 32)), 256, 0, st, (const float*)partial, offsets, (int)R, (int)N, rows, (T_*)dbias);

@@ -277,7 +277,8 @@ __device__ __forceinline__ void finish(float* v, float bias, const uint32_t* res
     if (ALL || p.vec) {
         const int64_t at = (c + odd) * p.F + (f & ~1);
         char* out = reinterpret_cast<char*>(reinterpret_cast<T*>(p.out) + at);
-        char* zout = reinterpret_cast<char*>(reinterpret_cast<T*>(p.z) + at);
+        typedef typename Kept<T, ACT>::Type K;
+        char* zout = reinterpret_cast<char*>(reinterpret_cast<K*>(p.z) + at);
         const int64_t step = 4 * (int64_t)p.F;
         // (F is even: both lanes of a pair are in or out)
         const int mine = ALL ? MMA_CHUNK : f < p.F ? left - odd : 0;
@@ -286,9 +287,14 @@ __device__ __forceinline__ void finish(float* v, float bias, const uint32_t* res
             float a = v[j], b = v[j + 1];
             if (BIAS) { a += bias; b += bias; }
             if (Z) {
-                const uint32_t w = swap_pair(ACT == ELA_ACT_RELU ? pack2<T>(sign_kept<T>(a), sign_kept<T>(b)) : pack2<T>(a, b), order);
-                if (ALL || j < mine) *reinterpret_cast<uint32_t*>(zout) = w;
-                zout += step;
+                if constexpr (sizeof(K) == 4) {  // the same exchange with one float each way
+                    const float other = __shfl_xor_sync(~0u, odd ? a : b, 1);
+                    if (ALL || j < mine) *reinterpret_cast<float2*>(zout) = odd ? make_float2(other, b) : make_float2(a, other);
+                } else {
+                    const uint32_t w = swap_pair(ACT == ELA_ACT_RELU ? pack2<T>(sign_kept<T>(a), sign_kept<T>(b)) : pack2<T>(a, b), order);
+                    if (ALL || j < mine) *reinterpret_cast<uint32_t*>(zout) = w;
+                }
+                zout += step * (sizeof(K) / 2);
             }
             a = act_value<ACT>(a);
             b = act_value<ACT>(b);
@@ -307,7 +313,8 @@ __device__ __forceinline__ void finish(float* v, float bias, const uint32_t* res
             if (j < left) {
                 const float a = BIAS ? v[j] + bias : v[j];
                 const int64_t at = (c + j) * p.F + f;
-                if (Z) reinterpret_cast<T*>(p.z)[at] = El<T>::from(ACT == ELA_ACT_RELU ? sign_kept<T>(a) : a);
+                typedef typename Kept<T, ACT>::Type K;
+                if (Z) reinterpret_cast<K*>(p.z)[at] = El<K>::from(ACT == ELA_ACT_RELU ? sign_kept<T>(a) : a);
                 const float r = RES ? El<T>::to(reinterpret_cast<const T*>(p.residual)[(c + j) * p.ldr + f]) : 0.f;
                 reinterpret_cast<T*>(p.out)[at] = El<T>::from(act_value<ACT>(a) + r);
             }

@@ -208,6 +208,11 @@ LinearSizes linear_sizes(const Tensor& x, const Tensor& weight, const OptTensor&
     return s;
 }
 
+// What z is kept in: the slope of GELU and SiLU is taken from an unrounded z, ReLU's from its sign.
+at::ScalarType kept_type(const Tensor& x, int64_t act) {
+    return act == ELA_ACT_GELU || act == ELA_ACT_SILU ? at::kFloat : x.scalar_type();
+}
+
 int aligned(const Tensor& t, int64_t ldt, int64_t stride_e = 0) {
     const int64_t es = t.element_size();
     return reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0 && ldt * es % 16 == 0 && stride_e * es % 16 == 0;
@@ -222,7 +227,7 @@ std::tuple<Tensor, Tensor> linear_raw(const Tensor& x, const Tensor& weight, con
     const OptTensor b = bias.has_value() ? OptTensor(bias->contiguous()) : OptTensor();
     const OptTensor r = residual.has_value() ? OptTensor(rows_of(*residual)) : OptTensor();
     Tensor y = fresh({s.R, s.N}, s.x);
-    Tensor z = fresh({want_z ? s.R : 0, s.N}, s.x);  // rows of no expert stay unwritten
+    Tensor z = fresh({want_z ? s.R : 0, s.N}, kept_type(x, act), s.x);  // rows of no expert stay unwritten
     const int al = aligned(s.x, ld(s.x)) && aligned(s.w, s.ldw, s.stride_e);
     const size_t bytes = ela_expert_linear_workspace_bytes(ELA_LINEAR_FORWARD, s.R, s.E, s.K, s.N, al);
     Tensor ws = workspace(bytes, x);

@@ -186,7 +186,8 @@ __global__ void __launch_bounds__(STREAM_WARPS * 32, 2) stream_kernel(const Stre
                 for (int w = 0; w < STREAM_WARPS; ++w) v += part[w][c][i % F];
                 if (p.bias) v += El<T>::to(reinterpret_cast<const T*>(p.bias)[(int64_t)done_e * p.N + f]);
                 const int64_t at = (int64_t)r * p.N + f;
-                if (p.z) reinterpret_cast<T*>(p.z)[at] = El<T>::from(ACT == ELA_ACT_RELU ? sign_kept<T>(v) : v);
+                typedef typename Kept<T, ACT>::Type Kt;
+                if (p.z) reinterpret_cast<Kt*>(p.z)[at] = El<Kt>::from(ACT == ELA_ACT_RELU ? sign_kept<T>(v) : v);
                 v = act_value<ACT>(v);
                 if (residual) v += El<T>::to(residual[r * p.ldr + f]);
                 y[at] = El<T>::from(v);

@@ -134,7 +134,8 @@ def _register_fakes() -> None:
 
     @torch.library.register_fake("ela_native::expert_linear_z")
     def _(x, weight, bias, residual, offsets, activation, want_z):
-        return x.new_empty((x.shape[0], weight.shape[-2])), x.new_empty((x.shape[0] if want_z else 0, weight.shape[-2]))
+        kept = torch.float32 if activation in (ACTIVATIONS["gelu"], ACTIVATIONS["silu"]) else x.dtype
+        return x.new_empty((x.shape[0], weight.shape[-2])), x.new_empty((x.shape[0] if want_z else 0, weight.shape[-2]), dtype=kept)
 
     @torch.library.register_fake("ela_native::expert_linear_grad")
     def _(dy, z, x, weight, offsets, activation, wsizes, bsizes, need_x, need_w, need_b):

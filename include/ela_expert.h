@@ -93,8 +93,10 @@ size_t ela_expert_linear_workspace_bytes(int pass, int64_t R, int64_t E, int64_t
  *   x (R,K) ldx; weight (E,N,K): expert distance stride_e, row distance ldw;
  *   bias (E,N) contiguous or NULL; residual (R,N) ldr or NULL; offsets int32[E+1],
  *   or NULL when E == 1 (every row is expert 0's);
- *   y (R,N) contiguous; z (R,N) contiguous or NULL: receives W_e x + b_e rounded to
- *   dtype, what the gradient of the activation needs (rows of no expert unwritten).
+ *   y (R,N) contiguous; z (R,N) contiguous or NULL: receives W_e x + b_e, what the
+ *   gradient of the activation needs (rows of no expert unwritten): float for
+ *   ELA_ACT_GELU and ELA_ACT_SILU; otherwise rounded to dtype, for ELA_ACT_RELU with
+ *   the sign of the sum (sums within rounding of 0 are formed again).
  * dtype: fp16 or bf16; products are summed in fp32 and y is rounded once.
  */
 int ela_expert_linear(const void* x, const void* weight, const void* bias, const void* residual,
@@ -104,7 +106,7 @@ int ela_expert_linear(const void* x, const void* weight, const void* bias, const
 
 /*
  * dz = dy * act'(z), and dbias[e] = sum of dz over the expert's rows (fp32 sums in a
- * fixed order).  dy, z, dz (R,N) contiguous.  dz NULL when only dbias is wanted;
+ * fixed order).  dy, z, dz (R,N) contiguous, z as ela_expert_linear writes it.  dz NULL when only dbias is wanted;
  * dbias (E,N) or NULL; z NULL for ELA_ACT_NONE.  Rows of no expert: dz unwritten.
  */
 int ela_expert_linear_grad_act(const void* dy, const void* z, const int32_t* offsets, int dtype, int64_t R,

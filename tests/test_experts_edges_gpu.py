@@ -8,6 +8,8 @@ import efficient_linear_assignment_b200 as ela
 
 pytestmark = pytest.mark.gpu
 
+U = {torch.bfloat16: 2.0 ** -8, torch.float16: 2.0 ** -11}
+
 
 def gen(seed):
     return torch.Generator().manual_seed(seed)
@@ -113,3 +115,51 @@ def test_relu_slope_below_fp16(rows):
     z = exact_z(x, w, None, [rows])
     assert (z[:, ::4].abs() == 2.0 ** -26).all()
     assert torch.equal(slopes_of(x, w, None, [rows], "relu").double(), (z > 0).double())
+
+
+@pytest.mark.parametrize("act", ["gelu", "silu"])
+@pytest.mark.parametrize("rows", [3, 300])
+def test_gradients_past_fp16_are_finite(rows, act):
+    """z beyond +-65504: the slope there is 0 or 1, as the forward pass's value says."""
+    g = gen(9)
+    x = torch.randn(rows, 64, generator=g).half()
+    w = (torch.randn(1, 48, 64, generator=g) * 0.125).half()
+    w[0, 5] = 0
+    w[0, 5, 3] = 300.0
+    x[:, 3] = torch.where(torch.arange(rows) % 2 == 0, 300.0, -300.0)  # z = +-90000
+    w[0, :5, 3] = w[0, 6:, 3] = 0
+    z = exact_z(x, w, None, [rows])
+    assert z[:, 5].abs().min() > 65504
+    got = slopes_of(x, w, None, [rows], act)
+    assert torch.isfinite(got).all()
+    assert torch.equal(got[:, 5].double(), (z[:, 5] > 0).double())
+    leaf = [v.cuda().requires_grad_() for v in (x, w)]
+    off = torch.tensor([0, rows], dtype=torch.int32, device="cuda")
+    y = ela.expert_linear(*leaf, None, None, act, off)
+    dy = torch.ones_like(y)
+    dy[:, 5] = 2.0 ** -10  # (dx holds 300 * dy)
+    for grad in torch.autograd.grad(y, leaf, dy):
+        assert torch.isfinite(grad).all()
+
+
+@pytest.mark.parametrize("act", ["gelu", "silu"])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("counts", [[3, 0, 4], [300, 301]])
+def test_slope_of_unrounded_z(counts, dtype, act):
+    """dz = dy * act'(z) is off by its own rounding, u |dz|, and not by the rounding of z, which
+    would be up to 0.8 u |z| (a sum's own error, 66 * 2^-22 of its terms, and the fast
+    exponential's 2^-20 besides)."""
+    g = gen(10)
+    x = torch.randn(sum(counts), 64, generator=g).to(dtype)
+    w = (torch.randn(len(counts), 40, 64, generator=g) * 0.3).to(dtype)
+    z = exact_z(x, w, None, counts)
+    if act == "gelu":
+        ref = torch.special.ndtr(z) + z * torch.exp(-z * z / 2) / (2 * torch.pi) ** 0.5
+    else:
+        ref = torch.sigmoid(z) * (1 + z * (1 - torch.sigmoid(z)))
+    terms = exact_z(x.abs(), w.abs(), None, counts)
+    bound = 1.01 * U[dtype] * ref.abs() + 0.8 * 66 * 2.0 ** -22 * terms + 2.0 ** -20 * (1 + z.abs())
+    if dtype == torch.float16:
+        bound += 2.0 ** -24
+    off = (slopes_of(x, w, None, counts, act).double() - ref).abs()
+    assert (off <= bound).all(), (off - bound).max()
