@@ -11,7 +11,7 @@
 // small call is bound by host time.  As in ela_torch_op.cpp: device guard, outputs and workspaces from the caching
 // allocator, the current stream, no synchronisation.  Autograd is here for
 // the same reason.  The backward passes launch kernels that autograd does not see, so asking for a gradient of
-// a gradient (create_graph) raises.
+// a gradient (create_graph) raises; so does a forward-mode derivative, whose tangents would be lost.
 #include <torch/library.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <ATen/ATen.h>
@@ -377,12 +377,20 @@ struct Linear : torch::autograd::Function<Linear> {
     }
 };
 
+// A tensor of a forward-mode derivative (a dual tensor) need not require a gradient.
+bool dual(const Tensor& t) { return t._fw_grad(/*level=*/0).defined(); }
+bool dual(const OptTensor& t) { return t.has_value() && dual(*t); }
+template <typename... Ts> void no_forward_mode(const Ts&... ts) {
+    TORCH_CHECK(!(dual(ts) || ...), "the expert operators have no forward-mode derivative");
+}
+
 // Without a gradient to prepare, the operator itself: the graph's bookkeeping costs more
 // host time than a small call's kernel.
 bool tracked(const Tensor& t) { return t.requires_grad() && at::GradMode::is_enabled(); }
 bool tracked(const OptTensor& t) { return t.has_value() && tracked(*t); }
 
 Tensor dispatch_autograd(const Tensor& x, const Tensor& position, const Tensor& offsets) {
+    no_forward_mode(x);
     if (!tracked(x)) {
         at::AutoDispatchBelowADInplaceOrView below;
         return call_dispatch(x, position, offsets);
@@ -390,6 +398,7 @@ Tensor dispatch_autograd(const Tensor& x, const Tensor& position, const Tensor& 
     return Dispatch::apply(x, position, offsets);
 }
 Tensor combine_autograd(const Tensor& y, const Tensor& position, const Tensor& offsets, const OptTensor& weights) {
+    no_forward_mode(y, weights);
     if (!tracked(y) && !tracked(weights)) {
         at::AutoDispatchBelowADInplaceOrView below;
         return call_combine(y, position, offsets, weights);
@@ -398,6 +407,7 @@ Tensor combine_autograd(const Tensor& y, const Tensor& position, const Tensor& o
 }
 Tensor linear_autograd(const Tensor& x, const Tensor& weight, const OptTensor& bias, const OptTensor& residual,
                        const OptTensor& offsets, int64_t act) {
+    no_forward_mode(x, weight, bias, residual);
     if (!tracked(x) && !tracked(weight) && !tracked(bias) && !tracked(residual)) {
         static auto f = op<Tensor(const Tensor&, const Tensor&, const OptTensor&, const OptTensor&, const OptTensor&,
                                   int64_t)>("ela_native::expert_linear");

@@ -13,7 +13,7 @@ All of them are C++ torch operators (csrc/ela_expert_op.cpp) over the C ABI of
 include/ela_expert.h, which also checks the arguments (TypeError, ValueError,
 RuntimeError for host tensors): current stream, no synchronisation, no data-dependent
 sizes, so the whole layer can be captured in a CUDA graph.  Dispatch, combine
-and linear are differentiable (once).  A choice outside [0, num_experts), such
+and linear are differentiable (once, in reverse mode).  A choice outside [0, num_experts), such
 as the solver's -1 for an unassigned row, belongs to no expert: it takes one of
 the last rows, is dispatched as zeros and adds nothing to the combined token.
 """

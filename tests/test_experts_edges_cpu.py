@@ -1,0 +1,29 @@
+"""CPU tests of the expert-layer operators' host side, with tensors that have no data."""
+import pytest
+import torch
+from torch._subclasses.fake_tensor import FakeTensorMode
+
+import efficient_linear_assignment_b200 as ela
+
+
+def fake_parts():
+    bf = torch.bfloat16
+    plan = ela.ExpertPlan(torch.empty(3, dtype=torch.int32, device="cuda"), torch.empty(4, 1, dtype=torch.int32, device="cuda"),
+                          torch.empty(4, dtype=torch.int32, device="cuda"))
+    x, w, g = torch.empty(4, 8, dtype=bf, device="cuda"), torch.empty(2, 16, 8, dtype=bf, device="cuda"), torch.empty(4, 1, device="cuda")
+    b, r = torch.empty(2, 16, dtype=bf, device="cuda"), torch.empty(4, 16, dtype=bf, device="cuda")
+    return [(lambda v: ela.expert_dispatch(v, plan), x), (lambda v: ela.expert_combine(v, plan, g), x),
+            (lambda v: ela.expert_combine(x, plan, v), g), (lambda v: ela.expert_linear(v, w, offsets=plan.offsets), x),
+            (lambda v: ela.expert_linear(x, v, offsets=plan.offsets), w),
+            (lambda v: ela.expert_linear(x, w, v, offsets=plan.offsets), b),
+            (lambda v: ela.expert_linear(x, w, None, v, offsets=plan.offsets), r)]
+
+
+def test_forward_mode_is_refused():
+    """A tangent is not dropped: forward-mode derivatives raise."""
+    import torch.autograd.forward_ad as fwd
+    with FakeTensorMode():
+        for f, v in fake_parts():
+            f(v)
+            with fwd.dual_level(), pytest.raises(RuntimeError, match="forward-mode"):
+                f(fwd.make_dual(v, torch.empty_like(v)))

@@ -163,3 +163,32 @@ def test_slope_of_unrounded_z(counts, dtype, act):
         bound += 2.0 ** -24
     off = (slopes_of(x, w, None, counts, act).double() - ref).abs()
     assert (off <= bound).all(), (off - bound).max()
+
+
+# ---------------------------------------------------------------- derivatives that are not there
+
+def layer_parts():
+    bf = torch.bfloat16
+    plan = ela.expert_plan(torch.tensor([[0], [1], [1], [-1]], device="cuda"), 2)
+    x, w = torch.randn(4, 8, device="cuda").to(bf), torch.randn(2, 16, 8, device="cuda").to(bf)
+    g = torch.rand(4, 1, device="cuda")
+    return [(lambda v: ela.expert_dispatch(v, plan), x), (lambda v: ela.expert_combine(v, plan, g), x),
+            (lambda v: ela.expert_combine(x, plan, v), g), (lambda v: ela.expert_linear(v, w, offsets=plan.offsets), x),
+            (lambda v: ela.expert_linear(x, v, offsets=plan.offsets), w),
+            (lambda v: ela.expert_linear(x, w, v, offsets=plan.offsets), w[:, :, 0].contiguous())]
+
+
+def test_forward_mode_is_refused():
+    """A tangent is not dropped: forward-mode derivatives raise."""
+    import torch.autograd.forward_ad as fwd
+    for f, v in layer_parts():
+        for needs in (False, True):
+            with fwd.dual_level():
+                dual = fwd.make_dual(v.clone().requires_grad_(needs), torch.ones_like(v))
+                with pytest.raises(RuntimeError, match="forward-mode"):
+                    f(dual)
+                with torch.no_grad(), pytest.raises(RuntimeError, match="forward-mode"):
+                    f(dual)
+        with pytest.raises(RuntimeError, match="forward-mode"):
+            torch.func.jvp(f, (v,), (torch.ones_like(v),))
+        f(v)  # (and nothing else does)
