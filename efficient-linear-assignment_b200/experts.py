@@ -130,7 +130,7 @@ def _register_fakes() -> None:
     @torch.library.register_fake("ela_native::expert_combine_grad")
     def _(dout, y, position, offsets, weights, need_y, need_w):
         return (dout.new_empty((position.numel() if need_y else 0, dout.shape[1])),
-                weights.new_empty(position.shape) if need_w else dout.new_empty((0,)))
+                weights.new_empty(weights.shape) if need_w else dout.new_empty((0,)))
 
     @torch.library.register_fake("ela_native::expert_linear_z")
     def _(x, weight, bias, residual, offsets, activation, want_z):

@@ -27,3 +27,14 @@ def test_forward_mode_is_refused():
             f(v)
             with fwd.dual_level(), pytest.raises(RuntimeError, match="forward-mode"):
                 f(fwd.make_dual(v, torch.empty_like(v)))
+
+
+@pytest.mark.parametrize("shape", [(4,), (4, 1)])
+def test_gradient_of_gates_has_their_shape(shape):
+    """What a traced graph sees of the gradient of the weights, (T,) or (T, 1)."""
+    with FakeTensorMode():
+        y, w = torch.empty(4, 8, device="cuda", requires_grad=True), torch.empty(shape, device="cuda", requires_grad=True)
+        plan = ela.ExpertPlan(torch.empty(3, dtype=torch.int32, device="cuda"),
+                              torch.empty(4, 1, dtype=torch.int32, device="cuda"), torch.empty(4, dtype=torch.int32, device="cuda"))
+        dy, dw = torch.ops.ela_native.expert_combine_grad(torch.empty(4, 8, device="cuda"), y, plan.position, plan.offsets, w, True, True)
+        assert dy.shape == y.shape and dw.shape == w.shape and dw.dtype == w.dtype

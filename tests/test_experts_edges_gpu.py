@@ -192,3 +192,18 @@ def test_forward_mode_is_refused():
         with pytest.raises(RuntimeError, match="forward-mode"):
             torch.func.jvp(f, (v,), (torch.ones_like(v),))
         f(v)  # (and nothing else does)
+
+
+def test_compiled_gradient_of_gates_without_a_second_dimension():
+    g = gen(12)
+    expert = torch.randint(-1, 4, (50,), generator=g).cuda()
+    plan = ela.expert_plan(expert, 4)
+    leaves = [torch.randn(50, 16, generator=g).cuda().requires_grad_(), torch.rand(50, generator=g).cuda().requires_grad_()]
+
+    def f(y, w):
+        return ela.expert_combine(y, plan, w) * 2
+
+    want, got = f(*leaves), torch.compile(f, backend="aot_eager", fullgraph=True)(*leaves)
+    assert torch.equal(want, got)
+    for a, b in zip(torch.autograd.grad(want, leaves, torch.ones_like(want)), torch.autograd.grad(got, leaves, torch.ones_like(got))):
+        assert a.shape == b.shape and torch.equal(a, b)
