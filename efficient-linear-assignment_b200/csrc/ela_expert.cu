@@ -286,22 +286,32 @@ __global__ void __launch_bounds__(ROUTE_THREADS) dispatch_kernel(const T* x, int
     constexpr int N = VB / sizeof(T), U = Route<VB>::U;
     const int64_t t = (int64_t)blockIdx.x * (ROUTE_THREADS / G) + threadIdx.x / G;
     if (t >= T_) return;
-    const int valid = __ldg(offsets + E);
+    const int valid = offsets[E];
     const int32_t* pos = position + t * k;
     const T* from = x + t * ldx;
     for (int i = threadIdx.x % G * N; i < H; i += G * N * U) {
         Piece<VB> v[U];
+        int at[4];  // positions (read before the stores, which might be to them for all the compiler knows)
+        auto next = [&](int j0) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) at[j] = j0 + j < k ? pos[j0 + j] : -1;
+        };
+        next(0);
 #pragma unroll
         for (int u = 0; u < U; ++u)
             if (i + u * G * N < H) v[u] = load_piece<VB>(from + i + u * G * N);
-        for (int j = 0; j < k; ++j) {
-            const int p = __ldg(pos + j);
-            if (p < 0 || p >= rows) continue;
-            T* to = out + (int64_t)p * H + i;
-            const Piece<VB> zero = {};
+        for (int j0 = 0; j0 < k; j0 += 4) {
+            if (j0) next(j0);
 #pragma unroll
-            for (int u = 0; u < U; ++u)
-                if (i + u * G * N < H) store_piece<VB>(to + u * G * N, p < valid ? v[u] : zero);
+            for (int j = 0; j < 4; ++j) {
+                const int p = at[j];
+                if (p < 0 || p >= rows) continue;
+                T* to = out + (int64_t)p * H + i;
+                const Piece<VB> zero = {};
+#pragma unroll
+                for (int u = 0; u < U; ++u)
+                    if (i + u * G * N < H) store_piece<VB>(to + u * G * N, p < valid ? v[u] : zero);
+            }
         }
     }
 }
@@ -316,7 +326,7 @@ __global__ void __launch_bounds__(ROUTE_THREADS, 4) combine_kernel(const T* y, i
     constexpr int N = VB / sizeof(T), U = Route<VB>::U;
     const int64_t t = (int64_t)blockIdx.x * (ROUTE_THREADS / G) + threadIdx.x / G;
     if (t >= T_) return;
-    const int valid = min(__ldg(offsets + E), rows);
+    const int valid = min(offsets[E], rows);
     for (int i = threadIdx.x % G * N; i < H; i += G * N * U) {
         float acc[U][N] = {};
         for (int j0 = 0; j0 < k; j0 += JC) {
@@ -325,7 +335,7 @@ __global__ void __launch_bounds__(ROUTE_THREADS, 4) combine_kernel(const T* y, i
             bool has[JC];
 #pragma unroll
             for (int j = 0; j < JC; ++j) {
-                const int p = j0 + j < k ? __ldg(position + t * k + j0 + j) : -1;
+                const int p = j0 + j < k ? position[t * k + j0 + j] : -1;
                 has[j] = p >= 0 && p < valid;
                 w[j] = has[j] && weights ? El<Wt>::to(weights[t * k + j0 + j]) : 1.f;
                 if (has[j])
@@ -364,13 +374,13 @@ __global__ void __launch_bounds__(ROUTE_THREADS, 6)
     const int64_t t = (int64_t)blockIdx.x * (ROUTE_THREADS / G) + threadIdx.x / G;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const bool in = t < T_;  // (no early return: the warps of a CTA share barriers)
-    const int valid = min(__ldg(offsets + E), rows);
+    const int valid = min(offsets[E], rows);
     for (int j0 = 0; j0 < k; j0 += JC) {
         int p[JC];
         float w[JC], dot[JC] = {};
 #pragma unroll
         for (int j = 0; j < JC; ++j) {
-            p[j] = in && j0 + j < k ? __ldg(position + t * k + j0 + j) : -1;
+            p[j] = in && j0 + j < k ? position[t * k + j0 + j] : -1;
             if (p[j] >= rows) p[j] = -1;
             w[j] = p[j] < 0 || p[j] >= valid ? 0.f : weights ? El<Wt>::to(weights[t * k + j0 + j]) : 1.f;
         }

@@ -78,7 +78,9 @@ template <auto KERNEL> __host__ inline bool allow_wide_cluster() {
 // Every kernel here is launched so that it may start while the one before it in the stream
 // ends (programmatic stream serialization): its prologue, and its CTAs' places on SMs that
 // are done, overlap that kernel's tail.  In return every kernel calls previous_done() before
-// it touches memory, which waits until the kernels before it are complete and visible.
+// it touches memory, which waits until the kernels before it are complete and visible, and
+// reads with ordinary loads: the non-coherent path is for data that does not change while the
+// kernel lives, which begins before the wait, and its loads may be moved above it.
 template <typename... P, typename... A>
 __host__ inline int launch(void (*kern)(P...), unsigned grid, unsigned block, size_t smem, cudaStream_t st, A... args) {
     cudaLaunchAttribute attr = {};
@@ -101,8 +103,8 @@ __device__ __forceinline__ void previous_done() { asm volatile("griddepcontrol.w
 // Rows of expert e, kept inside [0, R] whatever the offsets hold.
 __device__ __forceinline__ int clampi(int v, int lo, int hi) { return v < lo ? lo : v > hi ? hi : v; }
 __device__ __forceinline__ void expert_rows(const int32_t* offsets, int e, int R, int& r0, int& r1) {
-    r0 = offsets ? clampi(__ldg(offsets + e), 0, R) : 0;
-    r1 = offsets ? clampi(__ldg(offsets + e + 1), r0, R) : R;
+    r0 = offsets ? clampi(offsets[e], 0, R) : 0;
+    r1 = offsets ? clampi(offsets[e + 1], r0, R) : R;
 }
 
 // Complementary error function of x / sqrt(2) for x >= 0: Abramowitz and Stegun

@@ -25,21 +25,31 @@ __global__ void __launch_bounds__(256) realign_kernel(const uint16_t* src, int64
     previous_done();
     const int pieces = (cols + 7) / 8;
     const int64_t all = rows * pieces;
-    for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < all; i += (int64_t)gridDim.x * blockDim.x) {
-        const int64_t r = i / pieces;
-        const int c = (int)(i - r * pieces) * 8, left = cols - c;
-        const uint16_t* s = src + r / rows_per_matrix * stride_e + r % rows_per_matrix * ld + c;
-        const bool shift = (reinterpret_cast<uintptr_t>(s) & 3) != 0;
-        const uint32_t* w = reinterpret_cast<const uint32_t*>(s - shift);
-        uint32_t v[5];
+    const int64_t step = (int64_t)gridDim.x * blockDim.x;
+    for (int64_t i0 = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i0 < all; i0 += 2 * step) {
+        uint4 o[2];  // two pieces' loads before their stores
+        uint16_t* to[2];
 #pragma unroll
-        for (int k = 0; k < 5; ++k) v[k] = 2 * k - shift < left && (k < 4 || shift) ? __ldg(w + k) : 0u;
-        uint4 o;
-        o.x = shift ? __funnelshift_r(v[0], v[1], 16) : v[0];
-        o.y = shift ? __funnelshift_r(v[1], v[2], 16) : v[1];
-        o.z = shift ? __funnelshift_r(v[2], v[3], 16) : v[2];
-        o.w = shift ? __funnelshift_r(v[3], v[4], 16) : v[3];
-        *reinterpret_cast<uint4*>(dst + r * ldd + c) = o;  // (ldd is cols rounded up to 8)
+        for (int h = 0; h < 2; ++h) {
+            const int64_t i = i0 + h * step, r = i / pieces;
+            to[h] = nullptr;
+            if (i >= all) continue;
+            const int c = (int)(i - r * pieces) * 8, left = cols - c;
+            const uint16_t* s = src + r / rows_per_matrix * stride_e + r % rows_per_matrix * ld + c;
+            const bool shift = (reinterpret_cast<uintptr_t>(s) & 3) != 0;
+            const uint32_t* w = reinterpret_cast<const uint32_t*>(s - shift);
+            uint32_t v[5];
+#pragma unroll
+            for (int k = 0; k < 5; ++k) v[k] = 2 * k - shift < left && (k < 4 || shift) ? w[k] : 0u;
+            o[h].x = shift ? __funnelshift_r(v[0], v[1], 16) : v[0];
+            o[h].y = shift ? __funnelshift_r(v[1], v[2], 16) : v[1];
+            o[h].z = shift ? __funnelshift_r(v[2], v[3], 16) : v[2];
+            o[h].w = shift ? __funnelshift_r(v[3], v[4], 16) : v[3];
+            to[h] = dst + r * ldd + c;  // (ldd is cols rounded up to 8)
+        }
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+            if (to[h]) *reinterpret_cast<uint4*>(to[h]) = o[h];
     }
 }
 

@@ -468,7 +468,7 @@ __device__ __forceinline__ void load_residual(uint32_t* res, const MmaParams& p,
     const uint32_t* at = reinterpret_cast<const uint32_t*>(reinterpret_cast<const T*>(p.residual) + (c + odd) * p.ldr + (f & ~1));
     const int mine = p.vec && f < p.F ? left - odd : 0;
 #pragma unroll
-    for (int j = 0; j < MMA_CHUNK; j += 2, at += p.ldr) res[j / 2] = j < mine ? __ldg(at) : 0u;
+    for (int j = 0; j < MMA_CHUNK; j += 2, at += p.ldr) res[j / 2] = j < mine ? *at : 0u;
 }
 
 // Z: the forward pass keeps z for the gradient.

@@ -45,27 +45,27 @@ template <int VB, bool ONCE> __device__ __forceinline__ Sixteen load16(const uin
     if constexpr (VB == 32) {
         if (in && k < K) {
             if (ONCE)  // the weights: not kept in L1, fetched into the L2 256 bytes at a time
-                asm("ld.global.nc.L1::no_allocate.L2::256B.v8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
-                    : "=r"(v.w[0]), "=r"(v.w[1]), "=r"(v.w[2]), "=r"(v.w[3]), "=r"(v.w[4]), "=r"(v.w[5]), "=r"(v.w[6]), "=r"(v.w[7]) : "l"(row + k));
+                asm volatile("ld.global.L1::no_allocate.L2::256B.v8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+                    : "=r"(v.w[0]), "=r"(v.w[1]), "=r"(v.w[2]), "=r"(v.w[3]), "=r"(v.w[4]), "=r"(v.w[5]), "=r"(v.w[6]), "=r"(v.w[7]) : "l"(row + k) : "memory");
             else
-                asm("ld.global.nc.v8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
-                    : "=r"(v.w[0]), "=r"(v.w[1]), "=r"(v.w[2]), "=r"(v.w[3]), "=r"(v.w[4]), "=r"(v.w[5]), "=r"(v.w[6]), "=r"(v.w[7]) : "l"(row + k));
+                asm volatile("ld.global.v8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+                    : "=r"(v.w[0]), "=r"(v.w[1]), "=r"(v.w[2]), "=r"(v.w[3]), "=r"(v.w[4]), "=r"(v.w[5]), "=r"(v.w[6]), "=r"(v.w[7]) : "l"(row + k) : "memory");
         }
     } else if constexpr (VB == 16) {
 #pragma unroll
         for (int h = 0; h < 2; ++h)
             if (in && k + 8 * h < K) {
-                const uint4 q = __ldg(reinterpret_cast<const uint4*>(row + k + 8 * h));
+                const uint4 q = *reinterpret_cast<const uint4*>(row + k + 8 * h);
                 v.w[4 * h] = q.x; v.w[4 * h + 1] = q.y; v.w[4 * h + 2] = q.z; v.w[4 * h + 3] = q.w;
             }
     } else {
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
             if (VB == 4) {
-                if (in && k + 2 * i < K) v.w[i] = __ldg(reinterpret_cast<const uint32_t*>(row + k + 2 * i));
+                if (in && k + 2 * i < K) v.w[i] = *reinterpret_cast<const uint32_t*>(row + k + 2 * i);
             } else {
-                if (in && k + 2 * i < K) v.w[i] = __ldg(row + k + 2 * i);
-                if (in && k + 2 * i + 1 < K) v.w[i] |= (uint32_t)__ldg(row + k + 2 * i + 1) << 16;
+                if (in && k + 2 * i < K) v.w[i] = row[k + 2 * i];
+                if (in && k + 2 * i + 1 < K) v.w[i] |= (uint32_t)row[k + 2 * i + 1] << 16;
             }
         }
     }

@@ -1,4 +1,7 @@
 """CPU tests of the expert-layer operators' host side, with tensors that have no data."""
+import glob
+import os
+
 import pytest
 import torch
 from torch._subclasses.fake_tensor import FakeTensorMode
@@ -38,3 +41,16 @@ def test_gradient_of_gates_has_their_shape(shape):
                               torch.empty(4, 1, dtype=torch.int32, device="cuda"), torch.empty(4, dtype=torch.int32, device="cuda"))
         dy, dw = torch.ops.ela_native.expert_combine_grad(torch.empty(4, 8, device="cuda"), y, plan.position, plan.offsets, w, True, True)
         assert dy.shape == y.shape and dw.shape == w.shape and dw.dtype == w.dtype
+
+
+def test_kernels_that_start_early_read_coherently():
+    """Every expert kernel may begin before the one that writes its inputs has ended; loads by
+    the non-coherent path promise that nothing is written while the kernel lives."""
+    root = os.path.dirname(os.path.abspath(ela.experts.__file__))
+    files = glob.glob(os.path.join(root, "csrc", "ela_expert*.cu*"))
+    assert len(files) >= 4
+    for path in files:
+        with open(path) as f:
+            text = f.read()
+        for word in ("__ldg", "ld.global.nc", "__restrict__"):
+            assert word not in text, (path, word)
