@@ -173,7 +173,7 @@ int plan_launch(const Id* expert, int slots, int E, int32_t* offsets, int32_t* p
     const int per = (int)((((int64_t)slots + all - 1) / all + 31) / 32 * 32);
     const size_t smem = (size_t)(nwarps + 1) * (E + 1) * 4;
     auto kern = plan_kernel<Id>;
-    if (smem > 48 * 1024 && !allow_smem<&plan_kernel<Id>>(208 * 1024)) return ELA_ERR_CUDA;
+    if (!allow_smem<&plan_kernel<Id>>(208 * 1024)) return ELA_ERR_CUDA;  // (48 KB without, the static part included)
     // the scan takes a thread per bucket; few slots need few warps
     int threads = nwarps * 32;
     while (threads < PLAN_THREADS && threads < E + 1) threads *= 2;

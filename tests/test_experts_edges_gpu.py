@@ -1,6 +1,10 @@
 """GPU tests of the expert-layer operators where ordinary data does not lead:
 signs next to 0, the ends of fp16's range, sizes at a limit, derivatives that
 are not there."""
+import os
+import subprocess
+import sys
+
 import pytest
 import torch
 
@@ -8,6 +12,7 @@ import efficient_linear_assignment_b200 as ela
 
 pytestmark = pytest.mark.gpu
 
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 U = {torch.bfloat16: 2.0 ** -8, torch.float16: 2.0 ** -11}
 
 
@@ -163,6 +168,24 @@ def test_slope_of_unrounded_z(counts, dtype, act):
         bound += 2.0 ** -24
     off = (slopes_of(x, w, None, counts, act).double() - ref).abs()
     assert (off <= bound).all(), (off - bound).max()
+
+
+# ---------------------------------------------------------------- the plan's limits
+
+def test_plan_at_the_default_shared_memory():
+    """Counts that take 48 KB of shared memory but for the kernel's own, as the first plans of a
+    process (a larger one before them would have asked the driver for more)."""
+    code = """
+import torch, efficient_linear_assignment_b200 as ela
+for E, T in ((371, 2000), (720, 1000), (1363, 400), (2455, 200), (3070, 100), (4095, 100)):
+    for dtype in (torch.int32, torch.int64):
+        e = torch.randint(-1, E, (T,), generator=torch.Generator().manual_seed(1)).to(dtype)
+        p = ela.expert_plan(e.cuda(), E)
+        want = torch.sort(torch.where(e < 0, E, e), stable=True).indices
+        assert torch.equal(p.source.cpu().long(), want)
+"""
+    r = subprocess.run([sys.executable, "-c", code], cwd=ROOT, capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0, r.stderr[-2000:]
 
 
 # ---------------------------------------------------------------- derivatives that are not there
