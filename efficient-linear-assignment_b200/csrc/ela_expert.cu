@@ -58,15 +58,16 @@ __global__ void __launch_bounds__(PLAN_THREADS, 1) plan_kernel(const Id* expert,
     for (int i = tid; i < nwarps * B; i += blockDim.x) shared[i] = 0;
     __syncthreads();
     const int64_t first = ((int64_t)rank * nwarps + warp) * per;
-    const int s0 = warp < nwarps && first < slots ? (int)first : slots;
-    const int s1 = (int64_t)s0 + per < slots ? s0 + per : slots;
+    // (unsigned: a step past the end of 2^31 - 1 slots must not come out negative)
+    const unsigned s0 = warp < nwarps && first < slots ? (unsigned)first : slots;
+    const unsigned s1 = (int64_t)s0 + per < slots ? s0 + per : slots;
     int* mine = shared + (warp < nwarps ? warp : 0) * B;
     const bool kept = per <= 32 * PLAN_ITEMS;
     int bucket[PLAN_ITEMS], local[PLAN_ITEMS];
-    for (int s = s0; s < s1; s += 32 * PLAN_ITEMS) {
+    for (unsigned s = s0; s < s1; s += 32 * PLAN_ITEMS) {
 #pragma unroll
         for (int i = 0; i < PLAN_ITEMS; ++i) {
-            const int at = s + 32 * i + lane;
+            const unsigned at = s + 32 * i + lane;
             bucket[i] = -1;
             if (at < s1) {
                 const Id e = expert[at];
@@ -131,7 +132,7 @@ __global__ void __launch_bounds__(PLAN_THREADS, 1) plan_kernel(const Id* expert,
     if (kept) {
 #pragma unroll
         for (int i = 0; i < PLAN_ITEMS; ++i) {
-            const int at = s0 + 32 * i + lane;
+            const unsigned at = s0 + 32 * i + lane;
             if (at < s1) {
                 const int row = mine[bucket[i]] + local[i];
                 position[at] = row;
@@ -139,10 +140,10 @@ __global__ void __launch_bounds__(PLAN_THREADS, 1) plan_kernel(const Id* expert,
             }
         }
     } else {
-        for (int s = s0; s < s1; s += 32 * PLAN_ITEMS) {
+        for (unsigned s = s0; s < s1; s += 32 * PLAN_ITEMS) {
 #pragma unroll
             for (int i = 0; i < PLAN_ITEMS; ++i) {
-                const int at = s + 32 * i + lane;
+                const unsigned at = s + 32 * i + lane;
                 if (at < s1) {
                     const Id e = expert[at];
                     local[i] = mine[e >= 0 && e < (Id)E ? (int)e : E] + position[at];
@@ -150,7 +151,7 @@ __global__ void __launch_bounds__(PLAN_THREADS, 1) plan_kernel(const Id* expert,
             }
 #pragma unroll
             for (int i = 0; i < PLAN_ITEMS; ++i) {
-                const int at = s + 32 * i + lane;
+                const unsigned at = s + 32 * i + lane;
                 if (at < s1) {
                     position[at] = local[i];
                     source[local[i]] = at;

@@ -103,10 +103,12 @@ __global__ void __launch_bounds__(STREAM_WARPS * 32, 2) stream_kernel(const Stre
                 for (int f = threadIdx.x; f < p.N; f += STREAM_WARPS * 32)
                     y[(int64_t)r * p.N + f] = residual ? residual[r * p.ldr + f] : El<T>::from(0.f);
     }
-    const int items = p.E * p.f_tiles, rounds = (p.K + STREAM_WARPS * KB - 1) / (STREAM_WARPS * KB);
+    const unsigned items = (unsigned)p.E * p.f_tiles;  // (below 2^31: the step past the last does not wrap)
+    const int rounds = (p.K + STREAM_WARPS * KB - 1) / (STREAM_WARPS * KB);
 
     // the place of the next batch: item (expert e, features f0), rows rb.., round it
-    int item = blockIdx.x - gridDim.x, e = 0, f0 = 0, rb = 0, r1 = 0, it = 0;
+    unsigned item = blockIdx.x - gridDim.x;
+    int e = 0, f0 = 0, rb = 0, r1 = 0, it = 0;
     const uint16_t *wrow[2 * MT] = {}, *xrow[RG] = {};
     bool win[2 * MT] = {}, xin[RG] = {};
     auto rows = [&]() {
@@ -120,10 +122,10 @@ __global__ void __launch_bounds__(STREAM_WARPS * 32, 2) stream_kernel(const Stre
         do {
             item += gridDim.x;
             if (item >= items) return false;
-            e = item / p.f_tiles;
+            e = (int)(item / (unsigned)p.f_tiles);
             expert_rows(p.offsets, e, p.R, rb, r1);
         } while (rb >= r1);
-        f0 = (item - e * p.f_tiles) * F;
+        f0 = (int)(item - (unsigned)e * p.f_tiles) * F;
 #pragma unroll
         for (int h = 0; h < 2 * MT; ++h) {
             win[h] = f0 + g + 8 * h < p.N;

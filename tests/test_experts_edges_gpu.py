@@ -188,6 +188,25 @@ for E, T in ((371, 2000), (720, 1000), (1363, 400), (2455, 200), (3070, 100), (4
     assert r.returncode == 0, r.stderr[-2000:]
 
 
+def test_plan_of_the_most_choices():
+    """2^31 - 1 choices: the last step of a warp's range is inside the buffers and the plan right."""
+    n = 2 ** 31 - 1
+    e = torch.zeros(n, dtype=torch.int32, device="cuda")
+    e[0] = 1
+    e[-5:] = 1
+    plan = ela.expert_plan(e, 2)
+    del e
+    assert plan.offsets.tolist() == [0, n - 6, n]
+    pos = plan.position.view(-1)
+    assert pos[0].item() == n - 6 and pos[-5:].tolist() == list(range(n - 5, n))
+    assert plan.source[n - 6:].tolist() == [0] + list(range(n - 5, n))
+    for a in (1, n // 3, n - 2 ** 26 - 5):
+        want = torch.arange(a, a + 2 ** 26, device="cuda", dtype=torch.int32)
+        assert torch.equal(pos[a:a + 2 ** 26], want - 1) and torch.equal(plan.source[a - 1:a - 1 + 2 ** 26], want)
+    del plan, pos, want
+    torch.cuda.empty_cache()
+
+
 # ---------------------------------------------------------------- derivatives that are not there
 
 def layer_parts():
