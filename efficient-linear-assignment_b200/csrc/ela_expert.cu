@@ -482,7 +482,8 @@ size_t ela_expert_plan_workspace_bytes(int64_t, int64_t) { return 0; }
 int ela_expert_plan(const void* expert, int id_bytes, int64_t slots, int64_t num_experts, int32_t* offsets,
                     int32_t* position, int32_t* source, void*, size_t, void* stream) {
     if ((id_bytes != 4 && id_bytes != 8) || slots < 0 || slots > INT32_MAX || num_experts < 1 ||
-        num_experts > ELA_EXPERT_MAX || !offsets || (slots > 0 && (!expert || !position || !source)))
+        num_experts > ELA_EXPERT_MAX || !offsets || (slots > 0 && (!expert || !position || !source)) ||
+        !on_elements(id_bytes, expert) || !on_elements(4, offsets, position, source))
         return ELA_ERR_ARGUMENT;
     cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
     return id_bytes == 4 ? plan_launch((const int32_t*)expert, (int)slots, (int)num_experts, offsets, position, source, st)
@@ -494,7 +495,8 @@ int ela_expert_dispatch(const void* x, int dtype, int64_t T, int64_t k, int64_t 
                         void* stream) {
     if (!sizes_ok(dtype, T, k, H, num_experts) || ldx < 0) return ELA_ERR_ARGUMENT;
     if (T == 0 || k == 0 || H == 0) return ELA_OK;
-    if (!x || !position || !offsets || !rows) return ELA_ERR_ARGUMENT;
+    if (!x || !position || !offsets || !rows || !on_elements(dtype_bytes(dtype), x, rows) || !on_elements(4, position, offsets))
+        return ELA_ERR_ARGUMENT;
     cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
     const int es = dtype_bytes(dtype);
     const int vb = piece_bytes(address(x) | address(rows) | (uint64_t)(ldx * es) | (uint64_t)(H * es));
@@ -514,6 +516,9 @@ int ela_expert_combine(const void* y, int dtype, int64_t T, int64_t k, int64_t H
     if (weights && weights_dtype != ELA_DTYPE_F32 && weights_dtype != dtype) return ELA_ERR_ARGUMENT;
     if (T == 0 || H == 0) return ELA_OK;
     if (!out || !offsets || (k > 0 && (!y || !position))) return ELA_ERR_ARGUMENT;
+    if (!on_elements(dtype_bytes(dtype), y, out) || !on_elements(4, position, offsets) ||
+        (weights && !on_elements(dtype_bytes(weights_dtype), weights)))
+        return ELA_ERR_ARGUMENT;
     cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
     const int es = dtype_bytes(dtype);
     const int vb = piece_bytes(address(y) | address(out) | (uint64_t)(ldy * es) | (uint64_t)(H * es));
@@ -539,6 +544,9 @@ int ela_expert_combine_grad(const void* dout, const void* y, int dtype, int64_t 
     if ((weights || dweights) && weights_dtype != ELA_DTYPE_F32 && weights_dtype != dtype) return ELA_ERR_ARGUMENT;
     if (T == 0 || k == 0 || (!dy && !dweights)) return ELA_OK;
     if (!offsets || !position || (H > 0 && (!dout || (dweights && !y)))) return ELA_ERR_ARGUMENT;
+    if (!on_elements(dtype_bytes(dtype), dout, y, dy) || !on_elements(4, position, offsets) ||
+        ((weights || dweights) && !on_elements(dtype_bytes(weights_dtype), weights, dweights)))
+        return ELA_ERR_ARGUMENT;
     cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
     const int es = dtype_bytes(dtype);
     const int vb = piece_bytes(address(dout) | address(dy) | address(dweights ? y : nullptr) | (uint64_t)(lddo * es) |

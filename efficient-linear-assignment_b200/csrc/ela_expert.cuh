@@ -43,6 +43,11 @@ __host__ inline bool aligned16(const void* p, int64_t ld_bytes = 0) {
     return (reinterpret_cast<uintptr_t>(p) & 15u) == 0 && ld_bytes % 16 == 0;
 }
 
+// Pointers that the kernels may read and write elements of this size through (NULL is one).
+template <typename... P> __host__ inline bool on_elements(int size, P... p) {
+    return ((reinterpret_cast<uintptr_t>(p) | ...) & (uintptr_t)(size - 1)) == 0;
+}
+
 inline int sm_count() {
     static std::atomic<int> counts[64];
     int dev = 0, n = 0;

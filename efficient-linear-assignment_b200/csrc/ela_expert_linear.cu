@@ -68,7 +68,7 @@ struct Matrix {
 inline int readable(Matrix& m, char*& ws, size_t& left, cudaStream_t st) {
     if (m.ok()) return ELA_OK;
     const size_t need = m.padded_bytes();
-    if (!ws || left < need) return ELA_ERR_ARGUMENT;
+    if (!ws || left < need || !aligned16(ws)) return ELA_ERR_ARGUMENT;
     const int64_t rows = m.matrices * m.rows, ld = round8(m.cols);
     const int64_t blocks = (rows * (ld / 8) + 255) / 256, most = 8 * (int64_t)sm_count();
     const int rc = launch(realign_kernel, (unsigned)(blocks < most ? blocks : most), 256, 0, st, (const uint16_t*)m.p, rows, (int)m.cols, m.ld, m.rows, m.stride_e, (uint16_t*)ws, ld);
@@ -308,6 +308,9 @@ int ela_expert_linear(const void* x, const void* weight, const void* bias, const
         return ELA_ERR_ARGUMENT;
     if (R == 0) return ELA_OK;
     if (!x || !weight || !y) return ELA_ERR_ARGUMENT;
+    const bool wide_z = activation == ELA_ACT_GELU || activation == ELA_ACT_SILU;
+    if (!on_elements(2, x, weight, bias, residual, y) || !on_elements(wide_z ? 4 : 2, z) || !on_elements(4, offsets))
+        return ELA_ERR_ARGUMENT;
     cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
     if (few_rows(R, E, N)) {
         if (E * ((N + 15) / 16) > INT32_MAX) return ELA_ERR_UNSUPPORTED;
@@ -352,6 +355,9 @@ int ela_expert_linear_grad_act(const void* dy, const void* z, const int32_t* off
     if (R > 0 && (!dy || (!z && activation != ELA_ACT_NONE))) return ELA_ERR_ARGUMENT;
     const int rows = act_block_rows(R, N);
     const int64_t blocks = (R + rows - 1) / rows;
+    if (!on_elements(2, dy, dz, dbias) || !on_elements(activation == ELA_ACT_GELU || activation == ELA_ACT_SILU ? 4 : 2, z) ||
+        !on_elements(4, offsets) || (dbias && !on_elements(4, workspace)))
+        return ELA_ERR_ARGUMENT;
     if (dbias && (!workspace || workspace_bytes < (size_t)(blocks + E) * N * 4)) return ELA_ERR_ARGUMENT;
     cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
     float* partial = dbias ? reinterpret_cast<float*>(workspace) : nullptr;
@@ -375,7 +381,7 @@ int ela_expert_linear_grad_input(const void* dz, const void* weight, const int32
                                  void* workspace, size_t workspace_bytes, void* stream) {
     if (!linear_sizes_ok(dtype, R, E, K, N, offsets) || stride_e < 0 || ldw < 0) return ELA_ERR_ARGUMENT;
     if (R == 0) return ELA_OK;
-    if (!dz || !weight || !dx) return ELA_ERR_ARGUMENT;
+    if (!dz || !weight || !dx || !on_elements(2, dz, weight, dx) || !on_elements(4, offsets)) return ELA_ERR_ARGUMENT;
     cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
     char* ws = reinterpret_cast<char*>(workspace);
     Matrix mz = {dz, 1, R, N, N, 0}, mw = {weight, E, N, K, ldw, stride_e};
@@ -395,7 +401,7 @@ int ela_expert_linear_grad_weight(const void* dz, const void* x, const int32_t* 
                                   int64_t E, int64_t K, int64_t N, int64_t ldx, void* dweight, void* workspace,
                                   size_t workspace_bytes, void* stream) {
     if (!linear_sizes_ok(dtype, R, E, K, N, offsets) || ldx < 0) return ELA_ERR_ARGUMENT;
-    if (!dweight || (R > 0 && (!dz || !x))) return ELA_ERR_ARGUMENT;
+    if (!dweight || (R > 0 && (!dz || !x)) || !on_elements(2, dz, x, dweight) || !on_elements(4, offsets)) return ELA_ERR_ARGUMENT;
     cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
     if (R == 0) return cudaMemsetAsync(dweight, 0, (size_t)(E * N * K) * 2, st) == cudaSuccess ? ELA_OK : ELA_ERR_CUDA;
     char* ws = reinterpret_cast<char*>(workspace);

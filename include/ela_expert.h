@@ -6,7 +6,8 @@
  * Conventions as in ela_auction.h: plain pointers and sizes, device pointers on
  * the current CUDA device, work enqueued on `stream` and not waited for, status
  * codes ELA_*, element types ELA_DTYPE_*.  Matrices are row-major with unit
- * stride inside a row; `ld*` is the distance between rows in elements.
+ * stride inside a row; `ld*` is the distance between rows in elements.  Pointers lie on
+ * whole elements, workspaces on 16 bytes (ELA_ERR_ARGUMENT otherwise).
  *
  * Notation: T tokens, k choices per token, slots s = t*k + j; a slot's bucket is
  * its expert, or E when the expert is outside [0, E) (the solver's -1: no
