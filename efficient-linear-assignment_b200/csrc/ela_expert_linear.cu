@@ -13,7 +13,9 @@
 
 namespace ela_expert {
 
-constexpr unsigned long long LINEAR_WAIT_NS = 2000000000ull;  // limit of every device-side wait
+// Limit of every device-side wait: 2 s, and 4 us for each block of 64 k of a tile's sum, ten times
+// what one takes, so that a sum of hundreds of millions of terms is not given up on.
+inline unsigned long long wait_limit(int64_t k) { return 2000000000ull + 4000ull * (unsigned long long)(k / 64); }
 
 // Rows of any stride and alignment copied to rows a multiple of 16 bytes apart
 // (TMA's rule for strides and base).  Bits are moved, types do not matter.  A thread
@@ -252,7 +254,7 @@ inline MmaParams row_pass(const int32_t* offsets, int64_t R, int64_t E, int64_t 
     // than that makes (a box is loaded whole)
     p.bbox = p.bn % 128 == 0 && R < 256 * E ? 64 : p.bn / 2;
     p.stages = stages_for(p.bn, E);
-    p.wait_ns = LINEAR_WAIT_NS;
+    p.wait_ns = wait_limit(K);
     return p;
 }
 // At least as many tiles as the offsets can make.
@@ -418,7 +420,7 @@ int ela_expert_linear_grad_weight(const void* dz, const void* x, const int32_t* 
     p.c_tiles = (int)((N + MMA_C - 1) / MMA_C);
     p.out = dweight;
     p.vec = K % 2 == 0 && aligned4(dweight);
-    p.wait_ns = LINEAR_WAIT_NS;
+    p.wait_ns = wait_limit(R);
     CUtensorMap a, b;
     if (!map_of(&a, dtype, mx, 64, MMA_KB, false) || !map_of(&b, dtype, mz, 64, MMA_KB, false)) return ELA_ERR_CUDA;
     ELA_BY_TYPE(dtype, { rc = (mma_launch<PASS_WEIGHT, T_, ELA_ACT_NONE>(a, b, p, E * p.f_tiles * p.c_tiles, st)); })
