@@ -292,19 +292,19 @@ __global__ void __launch_bounds__(ROUTE_THREADS) dispatch_kernel(const T* x, int
     const T* from = x + t * ldx;
     for (int i = threadIdx.x % G * N; i < H; i += G * N * U) {
         Piece<VB> v[U];
-        int at[4];  // positions (read before the stores, which might be to them for all the compiler knows)
+        int at[2];  // positions (read before the stores, which might be to them for all the compiler knows)
         auto next = [&](int j0) {
 #pragma unroll
-            for (int j = 0; j < 4; ++j) at[j] = j0 + j < k ? pos[j0 + j] : -1;
+            for (int j = 0; j < 2; ++j) at[j] = j0 + j < k ? pos[j0 + j] : -1;
         };
         next(0);
 #pragma unroll
         for (int u = 0; u < U; ++u)
             if (i + u * G * N < H) v[u] = load_piece<VB>(from + i + u * G * N);
-        for (int j0 = 0; j0 < k; j0 += 4) {
+        for (int j0 = 0; j0 < k; j0 += 2) {
             if (j0) next(j0);
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
+            for (int j = 0; j < 2; ++j) {
                 const int p = at[j];
                 if (p < 0 || p >= rows) continue;
                 T* to = out + (int64_t)p * H + i;
