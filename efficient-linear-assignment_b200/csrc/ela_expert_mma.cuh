@@ -12,12 +12,13 @@
 //   weight grad    input feature          output feature       row of the expert
 //
 // Why a pair: one CTA's 128 x 256 tile loads 48 KB per 64 k, of which a CTA of a pair
-// loads 32 KB for the same products: 4096^3 bf16 212 us by single CTAs, 97 us by pairs
-// with the rest below (1420 TFLOP/s, 0.86 of the measured 1658; the library's product
-// takes 93 us).  At full rounds a block of 64 k takes 386 ns against the 374 ns that the
-// library's burst rate means; the rest is the last round, 34 tiles for 74 pairs.  Long
-// products are held by the power limit, not by the schedule: the input gradient of 8192
-// rows by 8 experts of 8192 x 2048 keeps the tensor pipe 91 % busy at 1.27 GHz.
+// loads 32 KB for the same products: 4096^3 bf16 212 us by single CTAs, 94 us by pairs
+// with the rest below, and 108 us in a loop at the power limit (1270 TFLOP/s, 0.92 of the
+// measured sustained 1384; the library's product 90.5 and 104).  At full rounds a block of
+// 64 k takes 386 ns against the 374 ns that the library's burst rate means; the rest is the
+// last round, 34 tiles for 74 pairs.  Long products are held by the power limit, not by the
+// schedule: 8192 rows by 8 experts of 8192 x 2048 take 203 us in a short run and 236 in a
+// loop, and their input gradient keeps the tensor pipe 91 % busy.
 //
 // The rows of an expert are the MMA's N side, whose extent is a multiple of 32
 // chosen per instruction: the last tile of an expert costs what its rows need, and
@@ -880,10 +881,11 @@ int mma_launch(const CUtensorMap& a, const CUtensorMap& b, const MmaParams& p, i
 // Columns per tile of the row passes, a multiple of 32 up to 256: the one whose rounds of
 // tiles over the pairs take least.  A block of 64 k takes the longer of its products (2
 // cycles a column) and its loads (16 KB of weights and 64 bytes a column, at the 57
-// bytes a cycle that an SM gets from the L2); a tile some 500 cycles more.  Loads are
-// uneven, so an expert is taken to have twice its share of the rows: 1003 rows of 8
-// experts of 2056 x 1032 take 22 us with tiles of 256 and 26 with 192.  300 rows by
-// 4096 x 4096: 29 us with 32 tiles of 256 columns, 27 with 64 tiles of 96.
+// bytes a cycle that an SM gets from the L2); a tile some 500 cycles more.  300 rows by
+// 4096 x 4096: 20.7 us with 64 tiles of 96 columns, 28.4 with 32 of 256; 1500 rows of 4 experts
+// of 1000 x 2048 16.8 and 20.0, 3000 of 64 of 1408 x 512 24.0 and 27.2.  Loads are uneven, so an
+// expert is taken to have twice its share of the rows; on six such shapes with skewed loads
+// that made 140 us in all, one and a half times 139, and the share itself 139.
 inline int columns_per_tile(int64_t R, int64_t E, int64_t f_tiles, int64_t k_blocks) {
     const int64_t share = (R + E - 1) / E, rows = E == 1 ? share : 2 * share, pairs = sm_count() / 2 > 0 ? sm_count() / 2 : 1;
     int best = 256;

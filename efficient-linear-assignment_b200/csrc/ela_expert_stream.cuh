@@ -266,6 +266,10 @@ template <typename T> int settle_launch(const StreamParams& p, cudaStream_t st) 
 // Rows per expert up to which the weights' read is what the product costs: 16 rows for
 // each of 16 experts take 31 us here and 33 us by tiles, 32 rows 45 and 34.  Where tiles
 // of 256 features leave half of the pairs idle, which then read at 44 GB/s an SM, up to 64.
+// The loads, which only the device knows, are taken to be equal, as an assignment makes them:
+// experts of 2048 x 1024 with half of all rows on one of them take, here and by tiles, 30 and
+// 18 us for 256 rows of 16 (equal loads: 14 and 14), 20 and 15 for 128 of 16 (13 and 15), 108
+// and 79 for 512 of 128 (80 and 86), 231 and 102 for 2048 of 128 (98 and 89).
 inline bool few_rows(int64_t R, int64_t E, int64_t N) {
     return R <= 16 * E || (R <= 64 * E && E * ((N + 255) / 256) <= sm_count() / 4);
 }
