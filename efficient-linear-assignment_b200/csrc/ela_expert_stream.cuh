@@ -202,8 +202,8 @@ __global__ void __launch_bounds__(STREAM_WARPS * 32, 2) stream_kernel(const Stre
 // ReLU's z next to 0, summed again where z is kept (sign_band): a pass of its own over z, which
 // is small here, since the call of exact_sum cost the kernel above the registers of its loads
 // (16 rows of 16 experts of 4096 x 1024: 23 -> 45 us inside it, 27 as a pass; 16 rows each 29 -> 57, 36).  A warp
-// takes 256 features of a row, whose largest z is the scale.  Two and more exact zeros, which
-// rows of zeros make, are taken as they are where the first is 0 summed again, too.
+// takes 256 features of a row, whose largest z is the scale.  Where every sum of them is 0, by
+// a row of zeros, z is taken as it is.
 constexpr int SETTLE_GROUPS = 8;  // of 32 features
 template <typename T>
 __global__ void __launch_bounds__(256) settle_kernel(const StreamParams p) {
@@ -223,31 +223,25 @@ __global__ void __launch_bounds__(256) settle_kernel(const StreamParams p) {
     T* zrow = reinterpret_cast<T*>(p.z) + (int64_t)r * p.N;
     const T* bias = p.bias ? reinterpret_cast<const T*>(p.bias) + (int64_t)e * p.N : nullptr;
     float z[SETTLE_GROUPS], b[SETTLE_GROUPS], largest = 0.f;
+    bool zeros = p.N - f0 >= 8;
 #pragma unroll
     for (int i = 0; i < SETTLE_GROUPS; ++i) {
         const int f = f0 + 32 * i + lane;
-        z[i] = f < p.N ? fabsf(El<T>::to(zrow[f])) : INFINITY;
+        z[i] = f < p.N ? El<T>::to(zrow[f]) : INFINITY;
         b[i] = f < p.N && bias ? El<T>::to(bias[f]) : 0.f;
+        zeros &= f >= p.N || z[i] == b[i];
     }
 #pragma unroll
     for (int i = 0; i < SETTLE_GROUPS; ++i)
-        if (z[i] < INFINITY) largest = fmaxf(largest, z[i] + (fabsf(b[i]) < INFINITY ? fabsf(b[i]) : 0.f));
+        if ((z[i] = fabsf(z[i])) < INFINITY) largest = fmaxf(largest, z[i] + (fabsf(b[i]) < INFINITY ? fabsf(b[i]) : 0.f));
     // (numbers from 0 on compare as their bits do; 1.01: z is rounded)
     const float band = 1.01f * sign_band(__uint_as_float(__reduce_max_sync(~0u, __float_as_uint(largest))), p.K);
-    if (!(band > 0.f)) return;
+    if (!(band > 0.f) || __all_sync(~0u, zeros)) return;
     const T* x = reinterpret_cast<const T*>(p.x) + (int64_t)r * p.ldx;
     const T* w = reinterpret_cast<const T*>(p.w) + (int64_t)e * p.stride_e;
-    unsigned near = 0, zero = 0;  // a bit a group
+    unsigned near = 0;  // a bit a group
 #pragma unroll
-    for (int i = 0; i < SETTLE_GROUPS; ++i) {
-        near |= (unsigned)(z[i] <= band) << i;
-        zero |= (unsigned)(z[i] == 0.f && b[i] == 0.f) << i;
-    }
-    if (__reduce_add_sync(~0u, __popc(zero)) >= 2) {
-        const int from = __ffs(__ballot_sync(~0u, zero != 0)) - 1;
-        const int f = f0 + 32 * (__shfl_sync(~0u, __ffs(zero), from) - 1) + from;
-        if (exact_sum<T>(x, w + (int64_t)f * p.ldw, p.K) == 0.0) near &= ~zero;
-    }
+    for (int i = 0; i < SETTLE_GROUPS; ++i) near |= (unsigned)(z[i] <= band) << i;
     for (unsigned any = __reduce_or_sync(~0u, near); any; any &= any - 1) {
         const int i = __ffs(any) - 1;
         for (unsigned todo = __ballot_sync(~0u, near >> i & 1); todo; todo &= todo - 1) {

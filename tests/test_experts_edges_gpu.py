@@ -91,6 +91,60 @@ def test_relu_slope_next_to_zero_few_rows(counts, half, N, every, bias, dtype):
     assert torch.equal(slopes_of(x, w, b, counts, "relu").double(), (z > 0).double())
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("counts", [[300, 61, 0, 150], [9, 1, 0, 5]])
+@pytest.mark.parametrize("kind", ["rows", "features", "blocks", "signs", "mixed"])
+def test_relu_slope_of_sums_that_are_zero(kind, counts, dtype):
+    """Sums of nothing but zeros, and of whole numbers that cancel, are 0 and have slope 0; what
+    is next to them, and next to 0, has its sign."""
+    g = gen(21)
+    x, w, b = cancelling(counts, 130, 72, dtype, 24, 22)
+    if kind == "rows":
+        x[::3] = 0
+    elif kind == "features":
+        w[:, 1::5] = 0
+    elif kind == "blocks":
+        x *= (torch.rand(x.shape[0], 9, generator=g) < 0.3).to(dtype).repeat_interleave(29, 1)[:, :261]
+        w *= (torch.rand(*w.shape[:2], 9, generator=g) < 0.3).to(dtype).repeat_interleave(29, 2)[:, :, :261]
+    elif kind == "signs":
+        x, w = x.sign(), w.sign()
+        x[:, -1] = 0  # (an even number of terms)
+    else:
+        x[::7] = 0
+        w[:, 2::9] = 0
+        b = torch.randn(w.shape[:2], generator=g).to(dtype)
+        b[:, ::2] = 0
+    z = exact_z(x, w, b, counts)
+    assert (z == 0).any()
+    assert torch.equal(slopes_of(x, w, b, counts, "relu").double(), (z > 0).double())
+
+
+@pytest.mark.parametrize("K,N", [(67, 1), (130, 3), (96, 7), (101, 33), (264, 131)])
+@pytest.mark.parametrize("rows", [5, 230])
+def test_relu_slope_next_to_zero_odd_sizes(rows, K, N):
+    """Operands off 16 bytes, features stored one by one, and too few of them to fill a warp."""
+    x, w, b = cancelling([rows], K // 2, N, torch.bfloat16, 4, K + N)
+    if N < 4:  # (a feature next to 0 needs one beside it that is not)
+        w[:, :1] = torch.randn(w[:, :1].shape, generator=gen(K)).to(w.dtype)
+    z = exact_z(x, w, b, [rows])
+    assert torch.equal(slopes_of(x, w, b, [rows], "relu").double(), (z > 0).double())
+
+
+@pytest.mark.parametrize("R,E,K,N", [(8192, 4, 512, 2048), (4096, 1, 2048, 4096)])
+def test_relu_signs_of_ordinary_values(R, E, K, N):
+    """Tens of millions of sums of normal values: every sign is that of the 64-bit sum."""
+    g = torch.Generator(device="cuda").manual_seed(R)
+    x = torch.randn(R, K, generator=g, device="cuda").to(torch.bfloat16)
+    w = (torch.randn(E, N, K, generator=g, device="cuda") * K ** -0.5).to(torch.bfloat16)
+    b = (torch.randn(E, N, generator=g, device="cuda") * 0.3).to(torch.bfloat16)
+    off = torch.arange(E + 1, device="cuda", dtype=torch.int32) * (R // E)
+    _, z = torch.ops.ela_native.expert_linear_z(x, w, b, None, off, 1, True)
+    for e in range(E):
+        a, c = e * (R // E), (e + 1) * (R // E)
+        want = x[a:c].double() @ w[e].double().t() + b[e].double()
+        assert torch.equal(z[a:c] > 0, want > 0)
+
+
 def test_relu_gradients_same_bits():
     """More sums next to 0 than any CTA could list, the same gradients every time."""
     counts = [700, 801, 523]
