@@ -203,7 +203,9 @@ __global__ void __launch_bounds__(STREAM_WARPS * 32, 2) stream_kernel(const Stre
 // is small here, since the call of exact_sum cost the kernel above the registers of its loads
 // (16 rows of 16 experts of 4096 x 1024: 23 -> 45 us inside it, 27 as a pass; 16 rows each 29 -> 57, 36).  A warp
 // takes 256 features of a row, whose largest z is the scale.  Where every sum of them is 0, by
-// a row of zeros, z is taken as it is.
+// a row of zeros, z is taken as it is, and so it is where a feature's sums are 0 in eight rows,
+// by weights of zeros (a quarter of the features so: 38 us, 232 with all of them summed; other
+// warps may be writing those rows, but no such z before or after).
 constexpr int SETTLE_GROUPS = 8;  // of 32 features
 template <typename T>
 __global__ void __launch_bounds__(256) settle_kernel(const StreamParams p) {
@@ -223,25 +225,36 @@ __global__ void __launch_bounds__(256) settle_kernel(const StreamParams p) {
     T* zrow = reinterpret_cast<T*>(p.z) + (int64_t)r * p.N;
     const T* bias = p.bias ? reinterpret_cast<const T*>(p.bias) + (int64_t)e * p.N : nullptr;
     float z[SETTLE_GROUPS], b[SETTLE_GROUPS], largest = 0.f;
-    bool zeros = p.N - f0 >= 8;
+    unsigned zeros = 0;  // a bit a group: the sum is 0 (or the bias hides it), or there is no feature
 #pragma unroll
     for (int i = 0; i < SETTLE_GROUPS; ++i) {
         const int f = f0 + 32 * i + lane;
         z[i] = f < p.N ? El<T>::to(zrow[f]) : INFINITY;
         b[i] = f < p.N && bias ? El<T>::to(bias[f]) : 0.f;
-        zeros &= f >= p.N || z[i] == b[i];
+        zeros |= (unsigned)(f >= p.N || z[i] == b[i]) << i;
     }
 #pragma unroll
     for (int i = 0; i < SETTLE_GROUPS; ++i)
         if ((z[i] = fabsf(z[i])) < INFINITY) largest = fmaxf(largest, z[i] + (fabsf(b[i]) < INFINITY ? fabsf(b[i]) : 0.f));
     // (numbers from 0 on compare as their bits do; 1.01: z is rounded)
     const float band = 1.01f * sign_band(__uint_as_float(__reduce_max_sync(~0u, __float_as_uint(largest))), p.K);
-    if (!(band > 0.f) || __all_sync(~0u, zeros)) return;
+    if (!(band > 0.f) || (p.N - f0 >= 8 && __all_sync(~0u, zeros == (1u << SETTLE_GROUPS) - 1))) return;
     const T* x = reinterpret_cast<const T*>(p.x) + (int64_t)r * p.ldx;
     const T* w = reinterpret_cast<const T*>(p.w) + (int64_t)e * p.stride_e;
     unsigned near = 0;  // a bit a group
 #pragma unroll
     for (int i = 0; i < SETTLE_GROUPS; ++i) near |= (unsigned)(z[i] <= band) << i;
+    if (r1 - r0 >= 8 && (near & zeros))
+#pragma unroll
+        for (int i = 0; i < SETTLE_GROUPS; ++i)
+            if ((near & zeros) >> i & 1) {
+                const T* column = reinterpret_cast<const T*>(p.z) + (int64_t)r0 * p.N + f0 + 32 * i + lane;
+                bool always = true;
+#pragma unroll
+                for (int q = 0; q < 8; ++q) always &= El<T>::to(column[(int64_t)q * p.N]) == b[i];
+                if (always) near &= ~(1u << i);
+            }
+    __syncwarp();
     for (unsigned any = __reduce_or_sync(~0u, near); any; any &= any - 1) {
         const int i = __ffs(any) - 1;
         for (unsigned todo = __ballot_sync(~0u, near >> i & 1); todo; todo &= todo - 1) {
