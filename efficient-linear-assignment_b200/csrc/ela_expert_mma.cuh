@@ -32,19 +32,20 @@
 // gradient, where rows are summed over, the last block's rows past the expert are
 // zeroed in shared memory, on both sides, since 0 * NaN is not 0.
 //
-// Roles, in each CTA: warp 0 issues the TMA loads of the CTA's halves, which count on
-// the first CTA's barriers; warp 1 of the first CTA issues the MMAs of the pair; warp 2
-// owns the TMEM allocation and sums ReLU's z next to 0 again; warp 3 works out the tiles;
-// warps 4-11 run the epilogue while the next tile's MMAs fill the other half of TMEM (2 x 256 columns).  Loads and
-// MMAs are issued by one elected thread that runs the whole inner loop (a warp that
-// polls, broadcasts and reconverges each block took 40 % longer), and no arrival of the
-// inner loop crosses CTAs with cluster-scope ordering, whose fences cost 1000 cycles.  A warp reads 16 columns of its 32 features
-// at a time, one feature a lane; bias, activation and residual are applied in fp32, and
-// two neighbouring lanes swap halves so that each stores two consecutive features of
-// one column: a store instruction writes 64 bytes of two columns, whole sectors, with
-// no staging in shared memory and no barrier between the warps (staging fp32 chunks to
-// store 256 bytes a row: 88 us instead of 46 for the weight gradient of 64 experts of
-// 1024 x 1024, whose tiles have two blocks of k each).  The residual of a chunk is loaded before its accumulators are waited for.
+// Roles, in each CTA: warp 0 issues the TMA loads of the CTA's halves, which count on the
+// first CTA's barriers; warp 1 of the first CTA issues the MMAs of the pair; warp 2 owns the
+// TMEM allocation and sums ReLU's z next to 0 again; warp 3 works out the tiles; warps 4-11
+// run the epilogue while the next tile's MMAs fill the other half of TMEM (2 x 256 columns).
+// Loads and MMAs are issued by one elected thread that runs the whole inner loop (a warp that
+// polls, broadcasts and reconverges each block took 40 % longer), and no arrival of the inner
+// loop crosses CTAs with cluster-scope ordering, whose fences cost 1000 cycles.  A warp reads
+// 16 columns of its 32 features at a time, one feature a lane; bias, activation and residual
+// are applied in fp32, and two neighbouring lanes swap halves so that each stores two
+// consecutive features of one column: a store instruction writes 64 bytes of two columns,
+// whole sectors, with no staging in shared memory and no barrier between the warps (staging
+// fp32 chunks to store 256 bytes a row: 88 us instead of 46 for the weight gradient of 64
+// experts of 1024 x 1024, whose tiles have two blocks of k each).  The residual of a chunk is
+// loaded before its accumulators are waited for.
 #pragma once
 
 #include <cuda.h>

@@ -201,8 +201,8 @@ __global__ void __launch_bounds__(STREAM_WARPS * 32, 2) stream_kernel(const Stre
 
 // ReLU's z next to 0, summed again where z is kept (sign_band): a pass of its own over z, which
 // is small here, since the call of exact_sum cost the kernel above the registers of its loads
-// (16 rows of 16 experts of 4096 x 1024: 23 -> 45 us inside it, 27 as a pass; 16 rows each 29 -> 57, 36).  A warp
-// takes 256 features of a row, whose largest z is the scale.  Where every sum of them is 0, by
+// (16 rows of 16 experts of 4096 x 1024: 23 -> 45 us inside it, 27 as a pass; 16 rows each
+// 29 -> 57, 36).  A warp takes 256 features of a row, whose largest z is the scale.  Where every sum of them is 0, by
 // a row of zeros, z is taken as it is, and so it is where a feature's sums are 0 in eight rows,
 // by weights of zeros (a quarter of the features so: 38 us, 232 with all of them summed; other
 // warps may be writing those rows, but no such z before or after).
