@@ -81,6 +81,23 @@ SIGNATURES = {
     "ela_expert_linear_grad_weight": (_c.c_int, [
         _c.c_void_p, _c.c_void_p, _c.c_void_p, _c.c_int, _c.c_int64, _c.c_int64, _c.c_int64, _c.c_int64, _c.c_int64,
         _c.c_void_p, _c.c_void_p, _c.c_size_t, _c.c_void_p]),
+    "ela_expert_route": (_c.c_int, [
+        _c.c_void_p, _c.c_int, _c.c_int64, _c.c_int64, _c.c_int64, _c.c_int64, _c.c_int, _c.c_void_p, _c.c_int64,
+        _c.c_int64, _c.c_int, _c.c_int, _c.c_float, _c.c_void_p, _c.c_void_p, _c.c_void_p]),
+    "ela_expert_route_grad": (_c.c_int, [
+        _c.c_void_p, _c.c_int, _c.c_int64, _c.c_int64, _c.c_int64, _c.c_int64, _c.c_int, _c.c_int, _c.c_float,
+        _c.c_void_p, _c.c_void_p, _c.c_void_p, _c.c_void_p]),
+    "ela_expert_quantize": (_c.c_int, [
+        _c.c_void_p, _c.c_int, _c.c_int64, _c.c_int64, _c.c_int64, _c.c_int64, _c.c_int64, _c.c_int64, _c.c_void_p,
+        _c.c_void_p, _c.c_void_p]),
+    "ela_expert_dequantize": (_c.c_int, [
+        _c.c_void_p, _c.c_void_p, _c.c_int, _c.c_int64, _c.c_int64, _c.c_int64, _c.c_int64, _c.c_void_p, _c.c_void_p]),
+    "ela_expert_linear_4bit_workspace_bytes": (_c.c_size_t, [
+        _c.c_int64, _c.c_int64, _c.c_int64, _c.c_int64, _c.c_int]),
+    "ela_expert_linear_4bit": (_c.c_int, [
+        _c.c_void_p, _c.c_void_p, _c.c_void_p, _c.c_void_p, _c.c_void_p, _c.c_void_p, _c.c_int, _c.c_int64, _c.c_int64,
+        _c.c_int64, _c.c_int64, _c.c_int64, _c.c_int64, _c.c_int64, _c.c_int, _c.c_void_p, _c.c_void_p, _c.c_size_t,
+        _c.c_void_p]),
     "ela_expert_status": (_c.c_int, [_c.POINTER(_c.c_int)]),
     "ela_auction_set_wait_limit_ns": (None, [_c.c_uint64]),
     "ela_auction_debug_skip_arrive": (None, [_c.c_int]),

@@ -17,6 +17,8 @@ CSRC = os.path.join(PKG_DIR, "csrc")
 SOURCES = {
     "ela_auction.cu": ["ela_implicit.cuh"],
     "ela_expert.cu": ["ela_expert.cuh"],
+    "ela_expert_route.cu": ["ela_expert.cuh"],
+    "ela_expert_4bit.cu": ["ela_expert.cuh", "ela_expert_mma.cuh", "ela_expert_stream.cuh", "ela_expert_4bit.cuh"],
     "ela_expert_linear.cu": ["ela_expert.cuh", "ela_expert_mma.cuh", "ela_expert_stream.cuh"],
 }
 OUT = os.path.join(PKG_DIR, "libela_auction.so")

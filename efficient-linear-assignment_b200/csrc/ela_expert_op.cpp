@@ -5,6 +5,10 @@
 //   ela_native::expert_dispatch(x, position, offsets) -> rows
 //   ela_native::expert_combine(y, position, offsets, weights?) -> out
 //   ela_native::expert_linear(x, weight, bias?, residual?, offsets?, activation) -> y
+//   ela_native::expert_route(logits, k, score, bias?, groups, kept, group_score, renormalize, scale) -> (expert, weights)
+//   ela_native::expert_quantize(weight, group) -> (packed, scales)
+//   ela_native::expert_dequantize(packed, scales, features, group) -> weight
+//   ela_native::expert_linear_4bit(x, packed, scales, features, group, bias?, residual?, offsets?, activation) -> y
 //
 // Arguments are checked here, with Python's TypeError and ValueError, and host tensors
 // are refused by CPU kernels that raise: the Python functions only forward, since a
@@ -20,6 +24,7 @@
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 
+#include <cmath>
 #include <tuple>
 
 #include "ela_expert.h"
@@ -289,6 +294,145 @@ Tensor linear_cuda(const Tensor& x, const Tensor& weight, const OptTensor& bias,
     return std::get<0>(linear_raw(x, weight, bias, residual, offsets, act, false));
 }
 
+// ---- route
+std::tuple<Tensor, Tensor> route_raw(const Tensor& logits_in, int64_t k, int64_t score, const OptTensor& bias, int64_t groups,
+                                     int64_t kept, int64_t group_score, bool renormalize, double scale) {
+    if (!logits_in.is_cuda()) refuse("expert_route");
+    const int code = code_of(logits_in);
+    TORCH_CHECK_TYPE(code >= 0, "expert_route: unsupported dtype ", logits_in.scalar_type());
+    TORCH_CHECK_VALUE(logits_in.dim() == 2, "expert_route: logits must be (T, E)");
+    const int64_t T = logits_in.size(0), E = logits_in.size(1);
+    TORCH_CHECK_VALUE(E >= 1 && E <= ELA_EXPERT_MAX, "expert_route: E must be 1..", ELA_EXPERT_MAX);
+    TORCH_CHECK_VALUE(groups >= 1 && E % groups == 0 && kept >= 1 && kept <= groups,
+                      "expert_route: groups must divide E, and 1 to all of them be kept");
+    TORCH_CHECK_VALUE(group_score != ELA_GROUP_TOP2 || groups == 1 || E / groups >= 2, "expert_route: top2 needs two experts in a group");
+    TORCH_CHECK_VALUE(k >= 1 && k <= ELA_ROUTE_MAX_K && k <= kept * (E / groups),
+                      "expert_route: k must be 1..", ELA_ROUTE_MAX_K, " and at most the experts of the kept groups");
+    TORCH_CHECK_VALUE(T <= INT32_MAX / k, "expert_route: more than 2^31 - 1 choices");
+    TORCH_CHECK_VALUE(std::isfinite((float)scale), "expert_route: scale must be finite");
+    if (bias.has_value()) {
+        TORCH_CHECK_TYPE(bias->scalar_type() == at::kFloat, "expert_route: bias must be float32, not ", bias->scalar_type());
+        TORCH_CHECK_VALUE(bias->dim() == 1 && bias->size(0) == E && bias->device() == logits_in.device(),
+                          "expert_route: bias must be (E,) on the logits' device");
+    }
+    c10::cuda::CUDAGuard guard(logits_in.device());
+    const Tensor logits = rows_of(logits_in);
+    const OptTensor b = bias.has_value() ? OptTensor(bias->contiguous()) : OptTensor();
+    Tensor expert = fresh({T, k}, at::kInt, logits), weights = fresh({T, k}, at::kFloat, logits);
+    check_rc(ela_expert_route(logits.data_ptr(), code, T, E, ld(logits), k, (int)score, static_cast<const float*>(ptr(b)), groups, kept,
+                              (int)group_score, renormalize, (float)scale, expert.data_ptr<int32_t>(), weights.data_ptr<float>(),
+                              stream_of(logits)),
+             "ela_expert_route");
+    return {expert, weights};
+}
+
+Tensor route_grad_raw(const Tensor& dweights_in, const Tensor& logits_in, const Tensor& expert, int64_t score, bool renormalize,
+                      double scale) {
+    c10::cuda::CUDAGuard guard(logits_in.device());
+    const Tensor logits = rows_of(logits_in), dweights = dweights_in.contiguous();
+    Tensor dlogits = fresh(logits.sizes(), logits);
+    check_rc(ela_expert_route_grad(logits.data_ptr(), code_of(logits), logits.size(0), logits.size(1), ld(logits), expert.size(1),
+                                   (int)score, renormalize, (float)scale, expert.data_ptr<int32_t>(), dweights.data_ptr<float>(),
+                                   dlogits.data_ptr(), stream_of(logits)),
+             "ela_expert_route_grad");
+    return dlogits;
+}
+
+// ---- 4-bit weights
+void check_group(const char* name, int64_t group) {
+    TORCH_CHECK_VALUE(group == 32 || group == 64 || group == 128, name, ": group must be 32, 64 or 128");
+}
+int64_t words_of(int64_t K) { return (K + 63) / 64 * 8; }
+
+std::tuple<Tensor, Tensor> quantize_raw(const Tensor& weight, int64_t group) {
+    TORCH_CHECK_TYPE(weight.scalar_type() == at::kHalf || weight.scalar_type() == at::kBFloat16,
+                     "expert_quantize: weight must be float16 or bfloat16, not ", weight.scalar_type());
+    check_group("expert_quantize", group);
+    TORCH_CHECK_VALUE((weight.dim() == 2 || weight.dim() == 3) && weight.numel() > 0 && (weight.dim() == 2 || weight.size(0) <= ELA_EXPERT_MAX),
+                      "expert_quantize: weight must be (E, N, K) or (N, K), E 1..", ELA_EXPERT_MAX, ", N and K at least 1");
+    c10::cuda::CUDAGuard guard(weight.device());
+    const Tensor w = weight_rows(weight);
+    const int64_t E = w.size(0), N = w.size(1), K = w.size(2), parts = (K + group - 1) / group;
+    const bool one = weight.dim() == 2;
+    Tensor packed = one ? fresh({N, words_of(K)}, at::kInt, w) : fresh({E, N, words_of(K)}, at::kInt, w);
+    Tensor scales = one ? fresh({parts, N}, w) : fresh({E, parts, N}, w);
+    check_rc(ela_expert_quantize(w.data_ptr(), code_of(w), E, K, N, E > 1 ? w.stride(0) : 0, N > 1 ? w.stride(1) : K, group,
+                                 packed.data_ptr<int32_t>(), scales.data_ptr(), stream_of(w)),
+             "ela_expert_quantize");
+    return {packed, scales};
+}
+
+// Packed rows and scales that belong together; contiguous, the words on 16 bytes.
+struct Packed {
+    int64_t E, N, K;
+    Tensor words, scales;
+};
+Packed packed_of(const char* name, const Tensor& packed, const Tensor& scales, int64_t K, int64_t group) {
+    if (!packed.is_cuda() || !scales.is_cuda()) refuse(name);
+    check_group(name, group);
+    TORCH_CHECK_TYPE(packed.scalar_type() == at::kInt && (scales.scalar_type() == at::kHalf || scales.scalar_type() == at::kBFloat16), name,
+                     ": packed weights are int32, scales float16 or bfloat16");
+    const bool one = packed.dim() == 2;
+    TORCH_CHECK_VALUE((one || packed.dim() == 3) && scales.dim() == packed.dim() && K >= 1 && packed.size(-1) == words_of(K) &&
+                          packed.numel() > 0 && scales.size(-1) == packed.size(-2) && scales.size(-2) == (K + group - 1) / group &&
+                          (one || (scales.size(0) == packed.size(0) && packed.size(0) <= ELA_EXPERT_MAX)) && scales.device() == packed.device(),
+                      name, ": packed (E, N, 8 ceil(K/64)) and scales (E, ceil(K/group), N), or both without E, on one device");
+    Packed p = {one ? 1 : packed.size(0), packed.size(-2), K, packed.contiguous(), scales.contiguous()};
+    if (reinterpret_cast<uintptr_t>(p.words.data_ptr()) % 16) p.words = p.words.clone();
+    return p;
+}
+
+Tensor dequantize_raw(const Tensor& packed, const Tensor& scales, int64_t K, int64_t group) {
+    c10::cuda::OptionalCUDAGuard guard;
+    if (packed.is_cuda()) guard.set_device(packed.device());
+    const Packed p = packed_of("expert_dequantize", packed, scales, K, group);
+    Tensor w = packed.dim() == 2 ? fresh({p.N, K}, p.scales) : fresh({p.E, p.N, K}, p.scales);
+    check_rc(ela_expert_dequantize(p.words.data_ptr<int32_t>(), p.scales.data_ptr(), code_of(w), p.E, K, p.N, group, w.data_ptr(), stream_of(w)),
+             "ela_expert_dequantize");
+    return w;
+}
+
+Tensor linear_4bit_raw(const Tensor& x_in, const Tensor& packed, const Tensor& scales, int64_t K, int64_t group, const OptTensor& bias,
+                       const OptTensor& residual, const OptTensor& offsets, int64_t act) {
+    const char* name = "expert_linear_4bit";
+    if (!x_in.is_cuda()) refuse(name);
+    c10::cuda::CUDAGuard guard(x_in.device());
+    const Packed p = packed_of(name, packed, scales, K, group);
+    const bool one = packed.dim() == 2;
+    auto operand = [&](const char* what, const Tensor& t) {
+        TORCH_CHECK_TYPE(t.scalar_type() == scales.scalar_type(), name, ": ", what, " must be the scales' ", scales.scalar_type(), ", not ", t.scalar_type());
+        TORCH_CHECK_VALUE(t.device() == packed.device(), name, ": ", what, " must be on the weights' device");
+    };
+    operand("x", x_in);
+    TORCH_CHECK_VALUE(x_in.dim() == 2 && x_in.size(1) == K, name, ": x must be (R, K)");
+    const int64_t R = x_in.size(0);
+    if (bias.has_value()) {
+        operand("bias", *bias);
+        TORCH_CHECK_VALUE(one ? bias->dim() == 1 && bias->size(0) == p.N : bias->dim() == 2 && bias->size(0) == p.E && bias->size(1) == p.N,
+                          name, ": bias must be (E, N), or (N,) for one matrix");
+    }
+    if (residual.has_value()) {
+        operand("residual", *residual);
+        TORCH_CHECK_VALUE(residual->dim() == 2 && residual->size(0) == R && residual->size(1) == p.N, name, ": residual must be (R, N)");
+    }
+    if (offsets.has_value())
+        TORCH_CHECK_VALUE(offsets->scalar_type() == at::kInt && offsets->is_contiguous() && offsets->dim() == 1 &&
+                              offsets->numel() == p.E + 1 && offsets->device() == x_in.device(),
+                          name, ": offsets must be contiguous int32 (E+1,) on x's device");
+    TORCH_CHECK_VALUE(offsets.has_value() || p.E == 1, name, ": offsets are needed for more than one expert");
+    const Tensor x = rows_of(x_in);
+    const OptTensor b = bias.has_value() ? OptTensor(bias->contiguous()) : OptTensor();
+    const OptTensor r = residual.has_value() ? OptTensor(rows_of(*residual)) : OptTensor();
+    Tensor y = fresh({R, p.N}, x);
+    const size_t bytes = ela_expert_linear_4bit_workspace_bytes(R, p.E, K, p.N, aligned(x, ld(x)));
+    Tensor ws = workspace(bytes, x);
+    check_rc(ela_expert_linear_4bit(x.data_ptr(), p.words.data_ptr<int32_t>(), p.scales.data_ptr(), ptr(b), ptr(r),
+                                    off_ptr(offsets), code_of(x), R, p.E, K, p.N, group, ld(x), r.has_value() ? ld(*r) : 0, (int)act, y.data_ptr(),
+                                    ptr(ws), bytes, stream_of(x)),
+             "ela_expert_linear_4bit");
+    return y;
+}
+
 // ---- autograd: every pass is a registered operator, so that traced graphs see them
 template <typename F> auto op(const char* name) {
     return c10::Dispatcher::singleton().findSchemaOrThrow(name, "").typed<F>();
@@ -377,6 +521,31 @@ struct Linear : torch::autograd::Function<Linear> {
     }
 };
 
+struct Route : torch::autograd::Function<Route> {
+    static variable_list forward(AutogradContext* ctx, const Tensor& logits, int64_t k, int64_t score, const OptTensor& bias, int64_t groups,
+                                 int64_t kept, int64_t group_score, bool renormalize, double scale) {
+        static auto f = op<std::tuple<Tensor, Tensor>(const Tensor&, int64_t, int64_t, const OptTensor&, int64_t, int64_t, int64_t, bool, double)>(
+            "ela_native::expert_route");
+        at::AutoDispatchBelowADInplaceOrView below;
+        auto out = f.call(logits, k, score, bias, groups, kept, group_score, renormalize, scale);
+        ctx->save_for_backward({logits, std::get<0>(out)});
+        ctx->saved_data["score"] = score;
+        ctx->saved_data["renormalize"] = renormalize;
+        ctx->saved_data["scale"] = scale;
+        ctx->mark_non_differentiable({std::get<0>(out)});
+        return {std::get<0>(out), std::get<1>(out)};
+    }
+    static variable_list backward(AutogradContext* ctx, variable_list grads) {
+        no_second_derivative();
+        static auto f = op<Tensor(const Tensor&, const Tensor&, const Tensor&, int64_t, bool, double)>("ela_native::expert_route_grad");
+        const auto saved = ctx->get_saved_variables();
+        variable_list out(9);
+        out[0] = f.call(grads[1], saved[0], saved[1], ctx->saved_data["score"].toInt(), ctx->saved_data["renormalize"].toBool(),
+                        ctx->saved_data["scale"].toDouble());
+        return out;
+    }
+};
+
 // A tensor of a forward-mode derivative (a dual tensor) need not require a gradient.
 bool dual(const Tensor& t) { return t._fw_grad(/*level=*/0).defined(); }
 bool dual(const OptTensor& t) { return t.has_value() && dual(*t); }
@@ -417,9 +586,55 @@ Tensor linear_autograd(const Tensor& x, const Tensor& weight, const OptTensor& b
     return Linear::apply(x, weight, bias, residual, offsets, act);
 }
 
+std::tuple<Tensor, Tensor> route_autograd(const Tensor& logits, int64_t k, int64_t score, const OptTensor& bias, int64_t groups, int64_t kept,
+                                          int64_t group_score, bool renormalize, double scale) {
+    no_forward_mode(logits, bias);
+    if (!tracked(logits)) {  // (the bias moves the choice alone: it has no gradient)
+        static auto f = op<std::tuple<Tensor, Tensor>(const Tensor&, int64_t, int64_t, const OptTensor&, int64_t, int64_t, int64_t, bool, double)>(
+            "ela_native::expert_route");
+        at::AutoDispatchBelowADInplaceOrView below;
+        return f.call(logits, k, score, bias, groups, kept, group_score, renormalize, scale);
+    }
+    auto out = Route::apply(logits, k, score, bias, groups, kept, group_score, renormalize, scale);
+    return {out[0], out[1]};
+}
+
+// The operators on 4-bit weights serve: a gradient that would be lost raises.
+template <typename... Ts> void no_gradient(const char* name, const Ts&... ts) {
+    no_forward_mode(ts...);
+    TORCH_CHECK(!(tracked(ts) || ...), name, " has no gradient: call it under torch.no_grad(), or detach its inputs");
+}
+std::tuple<Tensor, Tensor> quantize_autograd(const Tensor& weight, int64_t group) {
+    no_gradient("expert_quantize", weight);
+    static auto f = op<std::tuple<Tensor, Tensor>(const Tensor&, int64_t)>("ela_native::expert_quantize");
+    at::AutoDispatchBelowADInplaceOrView below;
+    return f.call(weight, group);
+}
+Tensor dequantize_autograd(const Tensor& packed, const Tensor& scales, int64_t K, int64_t group) {
+    no_gradient("expert_dequantize", scales);
+    static auto f = op<Tensor(const Tensor&, const Tensor&, int64_t, int64_t)>("ela_native::expert_dequantize");
+    at::AutoDispatchBelowADInplaceOrView below;
+    return f.call(packed, scales, K, group);
+}
+Tensor linear_4bit_autograd(const Tensor& x, const Tensor& packed, const Tensor& scales, int64_t K, int64_t group, const OptTensor& bias,
+                            const OptTensor& residual, const OptTensor& offsets, int64_t act) {
+    no_gradient("expert_linear_4bit", x, scales, bias, residual);
+    static auto f = op<Tensor(const Tensor&, const Tensor&, const Tensor&, int64_t, int64_t, const OptTensor&, const OptTensor&, const OptTensor&,
+                              int64_t)>("ela_native::expert_linear_4bit");
+    at::AutoDispatchBelowADInplaceOrView below;
+    return f.call(x, packed, scales, K, group, bias, residual, offsets, act);
+}
+
 }  // namespace
 
 TORCH_LIBRARY_FRAGMENT(ela_native, m) {
+    m.def("expert_route(Tensor logits, int k, int score, Tensor? bias, int groups, int groups_kept, int group_score, bool renormalize, "
+          "float scale) -> (Tensor, Tensor)");
+    m.def("expert_route_grad(Tensor dweights, Tensor logits, Tensor expert, int score, bool renormalize, float scale) -> Tensor");
+    m.def("expert_quantize(Tensor weight, int group) -> (Tensor, Tensor)");
+    m.def("expert_dequantize(Tensor packed, Tensor scales, int features, int group) -> Tensor");
+    m.def("expert_linear_4bit(Tensor x, Tensor packed, Tensor scales, int features, int group, Tensor? bias, Tensor? residual, "
+          "Tensor? offsets, int activation) -> Tensor");
     m.def("expert_plan(Tensor expert, int num_experts) -> (Tensor, Tensor, Tensor)");
     m.def("expert_dispatch(Tensor x, Tensor position, Tensor offsets) -> Tensor");
     m.def("expert_combine(Tensor y, Tensor position, Tensor offsets, Tensor? weights) -> Tensor");
@@ -440,6 +655,11 @@ TORCH_LIBRARY_IMPL(ela_native, CUDA, m) {
     m.impl("expert_linear", &linear_cuda);
     m.impl("expert_linear_z", &linear_raw);
     m.impl("expert_linear_grad", &linear_grad_raw);
+    m.impl("expert_route", &route_raw);
+    m.impl("expert_route_grad", &route_grad_raw);
+    m.impl("expert_quantize", &quantize_raw);
+    m.impl("expert_dequantize", &dequantize_raw);
+    m.impl("expert_linear_4bit", &linear_4bit_raw);
 }
 
 TORCH_LIBRARY_IMPL(ela_native, CPU, m) {
@@ -449,10 +669,21 @@ TORCH_LIBRARY_IMPL(ela_native, CPU, m) {
     m.impl("expert_linear", [](const Tensor&, const Tensor&, const OptTensor&, const OptTensor&, const OptTensor&, int64_t) -> Tensor {
         refuse("expert_linear");
     });
+    m.impl("expert_route", [](const Tensor&, int64_t, int64_t, const OptTensor&, int64_t, int64_t, int64_t, bool, double) -> std::tuple<Tensor, Tensor> {
+        refuse("expert_route");
+    });
+    m.impl("expert_quantize", [](const Tensor&, int64_t) -> std::tuple<Tensor, Tensor> { refuse("expert_quantize"); });
+    m.impl("expert_dequantize", [](const Tensor&, const Tensor&, int64_t, int64_t) -> Tensor { refuse("expert_dequantize"); });
+    m.impl("expert_linear_4bit", [](const Tensor&, const Tensor&, const Tensor&, int64_t, int64_t, const OptTensor&, const OptTensor&, const OptTensor&,
+                                    int64_t) -> Tensor { refuse("expert_linear_4bit"); });
 }
 
 TORCH_LIBRARY_IMPL(ela_native, AutogradCUDA, m) {
     m.impl("expert_dispatch", &dispatch_autograd);
     m.impl("expert_combine", &combine_autograd);
     m.impl("expert_linear", &linear_autograd);
+    m.impl("expert_route", &route_autograd);
+    m.impl("expert_quantize", &quantize_autograd);
+    m.impl("expert_dequantize", &dequantize_autograd);
+    m.impl("expert_linear_4bit", &linear_4bit_autograd);
 }

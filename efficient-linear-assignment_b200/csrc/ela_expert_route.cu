@@ -1,0 +1,497 @@
+// ela_expert_route.cu -- a router's logits to the experts of each token and their
+// weights, with the gradient (include/ela_expert.h).
+//
+// A row of logits belongs to a team of LANES threads, a part of a warp for up to 512
+// experts, so that 32 / LANES rows share a warp, and a block of 256 for more.  A thread holds
+// VPT consecutive experts in registers; one pass reads the row once, and everything else
+// (softmax, groups, k rounds of "largest key left", weights) stays in registers, shuffles
+// and a little shared memory.
+//
+// The choice is settled as in 64 bits.  Without a bias a score grows with its logit, so logits
+// are compared, which is exact.  Keys that are computed (score + bias, a group's sum) are
+// formed in fp32 with a bound on their error; a row in which two keys that decide something
+// lie closer than that is formed again in fp64.  That happens in a few rows of 10000, and
+// fp64 throughout would cost more than the rest of the kernel.
+#include "ela_expert.cuh"
+
+namespace ela_expert {
+
+constexpr int ROUTE_THREADS = 128, ROUTE_WIDE = 256;  // threads of a block; of a row's block past 512 experts
+
+struct RouteParams {
+    const void* logits;
+    int64_t T, ld;
+    int E, k, vec;  // vec: rows may be read 16 bytes at a time
+    const float* bias;
+    int groups, kept, top2;
+    int sigmoid, renormalize;
+    float scale;
+    int32_t* expert;
+    float* weights;
+};
+struct RouteGradParams {
+    const void* logits;
+    int64_t T, ld;
+    int E, k, vec;
+    int sigmoid, renormalize;
+    float scale;
+    const int32_t* expert;
+    const float* dweights;
+    void* dlogits;
+};
+
+// Numbers as unsigned whole numbers in the same order; NaN above all, -0 as 0.  0 is left
+// for "not to be chosen".
+__device__ __forceinline__ uint32_t ordered(float x) {
+    const uint32_t b = __float_as_uint(x + 0.f);
+    return x != x ? ~0u : b & 0x80000000u ? ~b : b | 0x80000000u;
+}
+__device__ __forceinline__ uint64_t ordered(double x) {
+    const uint64_t b = (uint64_t)__double_as_longlong(x + 0.0), top = 1ull << 63;
+    return x != x ? ~0ull : b & top ? ~b : b | top;
+}
+__device__ __forceinline__ float number(uint32_t u) { return __uint_as_float(u & 0x80000000u ? u & 0x7fffffffu : ~u); }
+__device__ __forceinline__ double number(uint64_t u) {
+    const uint64_t top = 1ull << 63;
+    return __longlong_as_double((long long)(u & top ? u & ~top : ~u));
+}
+template <typename F> struct Ordered { typedef uint32_t U; };
+template <> struct Ordered<double> { typedef uint64_t U; };
+
+// What the threads of a row do together.  Every thread of the warp (of the block) calls.
+template <int LANES> struct Team {
+    static constexpr bool WIDE = LANES > 32;
+    static constexpr int BLOCK = WIDE ? LANES : ROUTE_THREADS, ROWS = WIDE ? 1 : BLOCK / LANES;  // threads, rows of a block
+    static __device__ __forceinline__ int lane() { return threadIdx.x % LANES; }
+    static __device__ __forceinline__ int row() { return threadIdx.x / LANES; }
+    static __device__ __forceinline__ void sync() { if (WIDE) __syncthreads(); else __syncwarp(); }
+    static __device__ __forceinline__ bool any(bool v) { return WIDE ? __syncthreads_or(v) : __any_sync(~0u, v); }
+
+    template <typename V, typename Op> static __device__ __forceinline__ V reduce(V v, Op op) {
+#pragma unroll
+        for (int o = (WIDE ? 32 : LANES) / 2; o; o >>= 1) v = op(v, __shfl_xor_sync(~0u, v, o));
+        if constexpr (WIDE) {
+            __shared__ V part[LANES / 32];
+            __syncthreads();
+            if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = v;
+            __syncthreads();
+            v = part[0];
+            for (int i = 1; i < LANES / 32; ++i) v = op(v, part[i]);
+        }
+        return v;
+    }
+    template <typename V> static __device__ __forceinline__ V sum(V v) { return reduce(v, [](V a, V b) { return a + b; }); }
+    template <typename V> static __device__ __forceinline__ V most(V v) { return reduce(v, [](V a, V b) { return a > b ? a : b; }); }
+    template <typename V> static __device__ __forceinline__ V least(V v) { return reduce(v, [](V a, V b) { return a < b ? a : b; }); }
+    // The largest key and the first place that has it.
+    template <typename U> static __device__ __forceinline__ void first_most(U& key, int& at) {
+        auto op = [](U k, int a, U& key, int& at) { if (k > key || (k == key && a < at)) { key = k; at = a; } };
+#pragma unroll
+        for (int o = (WIDE ? 32 : LANES) / 2; o; o >>= 1) op(__shfl_xor_sync(~0u, key, o), __shfl_xor_sync(~0u, at, o), key, at);
+        if constexpr (WIDE) {
+            __shared__ U keys[LANES / 32];
+            __shared__ int ats[LANES / 32];
+            __syncthreads();
+            if ((threadIdx.x & 31) == 0) { keys[threadIdx.x >> 5] = key; ats[threadIdx.x >> 5] = at; }
+            __syncthreads();
+            for (int i = 0; i < LANES / 32; ++i) op(keys[i], ats[i], key, at);
+        }
+    }
+};
+
+// VPT logits of a row from expert e0 on; -inf past the last expert.
+template <typename T, int VPT> __device__ __forceinline__ void load_logits(float* l, const T* row, int e0, int E, bool vec, bool in) {
+#pragma unroll
+    for (int i = 0; i < VPT; ++i) l[i] = -INFINITY;
+    if (!in) return;
+    if (vec) {  // (E is a multiple of VPT: all of a thread's experts exist, or none)
+        if (e0 < E)
+#pragma unroll
+            for (int i = 0; i < VPT; i += El<T>::W) {
+                const Pack<T> q = *reinterpret_cast<const Pack<T>*>(row + e0 + i);
+#pragma unroll
+                for (int j = 0; j < El<T>::W; ++j) l[i + j] = El<T>::to(q.v[j]);
+            }
+    } else {
+#pragma unroll
+        for (int i = 0; i < VPT; ++i)
+            if (e0 + i < E) l[i] = El<T>::to(row[e0 + i]);
+    }
+}
+
+// A team's shared memory: the chosen experts and their logits, and with groups the experts'
+// values, the groups' and the groups kept.  (One word in 33 unused: threads that walk groups
+// of 32 side by side then hit different banks.)
+__host__ __device__ inline int route_slot(int e) { return e + (e >> 5); }
+struct RouteShared {
+    int* at;
+    float* logit;
+    void* value;
+    void* group;
+    unsigned char* kept;
+    static __host__ __device__ inline int bytes(int slots, int k, int groups) {
+        return 8 * ((k + 1) / 2 * 2) + (groups > 1 ? 8 * (route_slot(slots) + 1) + 8 * groups + (groups + 7) / 8 * 8 : 0);
+    }
+    __device__ __forceinline__ RouteShared(unsigned char* p, int slots, int k, int groups) {
+        const int even = (k + 1) / 2 * 2;
+        at = reinterpret_cast<int*>(p);
+        logit = reinterpret_cast<float*>(p + 4 * even);
+        value = p + 8 * even;
+        group = p + 8 * even + 8 * (route_slot(slots) + 1);
+        kept = p + 8 * even + 8 * (route_slot(slots) + 1) + 8 * groups;
+    }
+};
+
+__device__ __forceinline__ float exp_of(float x) { return expf(x); }
+__device__ __forceinline__ double exp_of(double x) { return exp(x); }
+
+// Chooses the row's experts, in F, and leaves them and their logits in s.  True: the choice is not sure in
+// fp32 (F double is always sure).  `mine`: the team has a row.
+template <typename F, int LANES, int VPT>
+__device__ __forceinline__ bool route_choose(const RouteParams& p, const float (&l)[VPT], const RouteShared& s) {
+    typedef Team<LANES> Tm;
+    typedef typename Ordered<F>::U U;
+    constexpr bool CHECK = sizeof(F) == 4;
+    const int lane = Tm::lane(), e0 = lane * VPT;
+    const bool computed = p.bias != nullptr;             // keys are scores and a bias, not logits
+    const bool scores = computed || p.top2;
+    F value[VPT];                                        // score + bias
+    F size = 0;                                          // the largest score, and value
+    if (scores) {
+        F m = 0, inv = 0;
+        if (!p.sigmoid) {
+            float most = -INFINITY;
+#pragma unroll
+            for (int i = 0; i < VPT; ++i) most = fmaxf(most, l[i]);
+            m = Tm::most(most);
+            if (m == -INFINITY) m = 0;  // (a row without experts)
+        }
+#pragma unroll
+        for (int i = 0; i < VPT; ++i) {
+            value[i] = p.sigmoid ? 1 / (1 + exp_of(-(F)l[i])) : exp_of((F)l[i] - m);
+            if (!p.sigmoid) inv += value[i];
+        }
+        if (!p.sigmoid) inv = Tm::sum(inv);
+        F most = 0;
+#pragma unroll
+        for (int i = 0; i < VPT; ++i) {
+            if (!p.sigmoid) value[i] = value[i] / inv;
+            if (CHECK) size = value[i] > size ? value[i] : size;
+            if (computed && e0 + i < p.E) value[i] += p.bias[e0 + i];
+            const F v = value[i] < 0 ? -value[i] : value[i];
+            if (CHECK && v > most && v < INFINITY) most = v;
+        }
+        // A score is off by at most 2^-19 of the largest: the exponent's rounding and the exponential
+        // by 2^-22, the row's sum, at most 29 additions one after the other, by 29 * 2^-24, the
+        // division by 2^-24.  Its sum with the bias is off by another 2^-24 of the value.  Two keys
+        // that differ by more than this (2^-17 and 2^-21) are in the right order.
+        if (CHECK) size = Tm::most(size) * (F)7.62939453125e-6 + Tm::most(most) * (F)4.76837158203125e-7;
+    }
+    U key[VPT];
+#pragma unroll
+    for (int i = 0; i < VPT; ++i) {
+        const bool there = e0 + i < p.E && l[i] != -INFINITY && !(computed && p.bias[e0 + i] == -INFINITY);
+        if (scores && !there) value[i] = -INFINITY;
+        key[i] = there ? ordered(computed ? value[i] : (F)l[i]) : 0;
+    }
+    bool unsure = false;
+    if (p.groups > 1) {
+        U* vals = reinterpret_cast<U*>(s.value);
+        U* group = reinterpret_cast<U*>(s.group);
+        const int S = p.E / p.groups;
+#pragma unroll
+        for (int i = 0; i < VPT; ++i)
+            if (e0 + i < p.E) vals[route_slot(e0 + i)] = p.top2 ? ordered(value[i]) : key[i] ? key[i] : ordered((F)-INFINITY);
+        Tm::sync();
+        for (int g = lane; g < p.groups; g += LANES) {
+            U a = 0, b = 0;  // the largest and the second
+            for (int i = 0; i < S; ++i) {
+                const U v = vals[route_slot(g * S + i)];
+                b = v > a ? a : v > b ? v : b;
+                a = v > a ? v : a;
+            }
+            group[g] = p.top2 ? ordered(number(a) + number(b)) : a;
+        }
+        Tm::sync();
+        F last = INFINITY, next = -INFINITY;  // the least kept group and the most one left out
+        for (int g = lane; g < p.groups; g += LANES) {
+            const U v = group[g];
+            int before = 0;
+            for (int h = 0; h < p.groups; ++h) before += group[h] > v || (group[h] == v && h < g);
+            s.kept[g] = before < p.kept;
+            if (CHECK) {
+                if (before < p.kept) last = number(v) < last ? number(v) : last;
+                else next = number(v) > next ? number(v) : next;
+            }
+        }
+        Tm::sync();
+        if (CHECK && scores) {
+            last = Tm::least(last);
+            next = Tm::most(next);
+            unsure = next > -INFINITY && last - next <= 2 * size;
+        }
+        int g = e0 / S, r = e0 - g * S;
+#pragma unroll
+        for (int i = 0; i < VPT; ++i) {
+            if (e0 + i < p.E && !s.kept[g]) key[i] = 0;
+            if (++r == S) { r = 0; ++g; }
+        }
+    }
+    F before = INFINITY;  // the choice before, its logit and place
+    float before_l = 0.f;
+    int before_at = 0;
+    for (int j = 0; j < p.k; ++j) {
+        U best = key[0];
+        int at = e0;
+#pragma unroll
+        for (int i = 1; i < VPT; ++i)
+            if (key[i] > best) { best = key[i]; at = e0 + i; }
+        Tm::first_most(best, at);
+#pragma unroll
+        for (int i = 0; i < VPT; ++i)
+            if (e0 + i == at) {
+                if (best) s.logit[j] = l[i];
+                key[i] = 0;
+            }
+        if (lane == 0) s.at[j] = best ? at : -1;
+        if (CHECK && computed) {
+            Tm::sync();
+            const float logit = s.logit[j];
+            const F v = number(best);
+            if (best && j > 0 && before - v <= size && !(logit == before_l && p.bias[at] == p.bias[before_at])) unsure = true;
+            if (best) { before = v; before_l = logit; before_at = at; }
+        }
+    }
+    if (CHECK && computed) {  // what is left next to the last choice
+        const float b = p.bias[before_at];
+#pragma unroll
+        for (int i = 0; i < VPT; ++i)
+            if (key[i] && before - number(key[i]) <= size && !(l[i] == before_l && p.bias[e0 + i] == b)) unsure = true;
+    }
+    Tm::sync();
+    return unsure;
+}
+
+// 64 bits, for the rows that need them (kept out of the kernel's registers).
+template <int LANES, int VPT>
+__device__ __noinline__ void route_settle(const RouteParams& p, const float (&l)[VPT], const RouteShared& s) {
+    route_choose<double, LANES, VPT>(p, l, s);
+}
+
+// Weights of the chosen experts, in place of their logits.  Ratios of the chosen scores are
+// formed from the exponents' differences, so that none is 0 / 0 however small the scores.
+template <int LANES, int VPT>
+__device__ __forceinline__ void route_weights(const RouteParams& p, const float (&l)[VPT], const RouteShared& s) {
+    typedef Team<LANES> Tm;
+    const int lane = Tm::lane();
+    if (p.renormalize) {
+        float most = -INFINITY, sum = 0.f;
+        for (int j = lane; j < p.k; j += LANES)
+            if (s.at[j] >= 0) most = fmaxf(most, p.sigmoid ? fminf(s.logit[j], 0.f) : s.logit[j]);
+        most = Tm::most(most);
+        auto part = [&](float x) { return p.sigmoid ? expf(fminf(x, 0.f) - most) / (1.f + expf(-fabsf(x))) : expf(x - most); };
+        for (int j = lane; j < p.k; j += LANES)
+            if (s.at[j] >= 0) sum += s.logit[j] = part(s.logit[j]);
+        sum = Tm::sum(sum);
+        if (!p.sigmoid && (p.bias || p.top2)) {  // a NaN or +inf that was not chosen: every score of its row is NaN
+            float spoiled = 0.f;
+#pragma unroll
+            for (int i = 0; i < VPT; ++i) spoiled = l[i] < INFINITY ? spoiled : NAN;
+            sum += Tm::sum(spoiled);
+        }
+        for (int j = lane; j < p.k; j += LANES) s.logit[j] = s.at[j] >= 0 ? p.scale * (s.logit[j] / sum) : 0.f;
+    } else {
+        float most = -INFINITY, sum = 0.f;
+        if (!p.sigmoid) {
+#pragma unroll
+            for (int i = 0; i < VPT; ++i) most = fmaxf(most, l[i]);
+            most = Tm::most(most);
+            if (most == -INFINITY) most = 0.f;
+#pragma unroll
+            for (int i = 0; i < VPT; ++i) sum += expf(l[i] - most);
+            sum = Tm::sum(sum);
+        }
+        for (int j = lane; j < p.k; j += LANES) {
+            const float x = s.logit[j];
+            s.logit[j] = s.at[j] < 0 ? 0.f : p.scale * (p.sigmoid ? 1.f / (1.f + expf(-x)) : expf(x - most) / sum);
+        }
+    }
+    Tm::sync();
+}
+
+template <typename T, int LANES, int VPT>
+__global__ void __launch_bounds__(Team<LANES>::BLOCK) route_kernel(const RouteParams p) {
+    next_may_start();
+    previous_done();
+    typedef Team<LANES> Tm;
+    extern __shared__ __align__(16) unsigned char shared[];
+    const int64_t first = (int64_t)blockIdx.x * Tm::ROWS, t = first + Tm::row();
+    const int bytes = RouteShared::bytes(LANES * VPT, p.k, p.groups);
+    const RouteShared s(shared + Tm::row() * bytes, LANES * VPT, p.k, p.groups);
+    float l[VPT];
+    load_logits<T, VPT>(l, reinterpret_cast<const T*>(p.logits) + (t < p.T ? t : 0) * p.ld, Tm::lane() * VPT, p.E, p.vec, t < p.T);
+    if (Tm::any(route_choose<float, LANES, VPT>(p, l, s))) route_settle<LANES, VPT>(p, l, s);
+    route_weights<LANES, VPT>(p, l, s);
+    if (t < p.T)
+        for (int j = Tm::lane(); j < p.k; j += LANES) {
+            p.expert[t * p.k + j] = s.at[j];
+            p.weights[t * p.k + j] = s.logit[j];
+        }
+}
+
+// Gradient.  With c_j = scale * dw_j and r_j the chosen ratios (p_i the softmax):
+//   softmax           dl_i = p_i (c_i - sum_j c_j p_j), c_i = 0 where i is not chosen
+//   softmax, ratios   dl_j = r_j (c_j - sum_j c_j r_j)
+//   sigmoid           dl_j = c_j s_j (1 - s_j)
+//   sigmoid, ratios   dl_j = r_j (c_j - sum_j c_j r_j) (1 - s_j)
+// Only the first reads the whole row.  A choice outside [0, E) has no gradient.
+template <typename T, int LANES, int VPT>
+__global__ void __launch_bounds__(Team<LANES>::BLOCK) route_grad_kernel(const RouteGradParams p) {
+    next_may_start();
+    previous_done();
+    typedef Team<LANES> Tm;
+    extern __shared__ __align__(16) unsigned char shared[];
+    const int lane = Tm::lane(), e0 = lane * VPT;
+    const int64_t t = (int64_t)blockIdx.x * Tm::ROWS + Tm::row();
+    const RouteShared s(shared + Tm::row() * RouteShared::bytes(LANES * VPT, p.k, 1), LANES * VPT, p.k, 1);
+    const T* row = reinterpret_cast<const T*>(p.logits) + (t < p.T ? t : 0) * p.ld;
+    const bool dense = !p.sigmoid && !p.renormalize;
+    float l[VPT], most = -INFINITY, sum = 0.f, mean = 0.f;
+    if (dense) {
+        load_logits<T, VPT>(l, row, e0, p.E, p.vec, t < p.T);
+#pragma unroll
+        for (int i = 0; i < VPT; ++i) most = fmaxf(most, l[i]);
+        most = Tm::most(most);
+        if (most == -INFINITY) most = 0.f;
+#pragma unroll
+        for (int i = 0; i < VPT; ++i) sum += l[i] = expf(l[i] - most);
+        sum = Tm::sum(sum);
+#pragma unroll
+        for (int i = 0; i < VPT; ++i) l[i] = sum > 0.f || sum != sum ? l[i] / sum : 0.f;
+    }
+    // the chosen experts, and what each adds to its logit's gradient
+    for (int j = lane; j < p.k; j += LANES) {
+        const int e = t < p.T ? p.expert[t * p.k + j] : -1;
+        s.at[j] = e >= 0 && e < p.E ? e : -1;
+        if (s.at[j] >= 0) {
+            s.logit[j] = El<T>::to(row[e]);
+            if (p.renormalize) most = fmaxf(most, p.sigmoid ? fminf(s.logit[j], 0.f) : s.logit[j]);
+        }
+    }
+    if (p.renormalize) {
+        most = Tm::most(most);
+        for (int j = lane; j < p.k; j += LANES)
+            if (s.at[j] >= 0) sum += p.sigmoid ? expf(fminf(s.logit[j], 0.f) - most) / (1.f + expf(-fabsf(s.logit[j]))) : expf(s.logit[j] - most);
+        sum = Tm::sum(sum);
+    }
+    auto ratio = [&](float x) {  // the weight, without scale
+        if (p.sigmoid) return p.renormalize ? expf(fminf(x, 0.f) - most) / (1.f + expf(-fabsf(x))) / sum : 1.f / (1.f + expf(-x));
+        return expf(x - most) / sum;
+    };
+    if (!p.sigmoid || p.renormalize) {
+        for (int j = lane; j < p.k; j += LANES)
+            if (s.at[j] >= 0) mean = fmaf(p.scale * p.dweights[t * p.k + j], ratio(s.logit[j]), mean);
+        mean = Tm::sum(mean);
+    }
+    for (int j = lane; j < p.k; j += LANES)
+        if (s.at[j] >= 0) {
+            const float x = s.logit[j], c = p.scale * p.dweights[t * p.k + j];
+            s.logit[j] = dense ? c : ratio(x) * (c - mean) * (p.sigmoid ? 1.f / (1.f + expf(x)) : 1.f);
+        }
+    Tm::sync();
+    float d[VPT] = {};
+    for (int j = 0; j < p.k; ++j) {
+        const int at = s.at[j];
+#pragma unroll
+        for (int i = 0; i < VPT; ++i)
+            if (e0 + i == at) d[i] += s.logit[j];
+    }
+    if (dense)
+#pragma unroll
+        for (int i = 0; i < VPT; ++i) d[i] = l[i] * (d[i] - mean);
+    if (t >= p.T) return;
+    T* out = reinterpret_cast<T*>(p.dlogits) + t * p.E;
+    if (p.vec) {
+        if (e0 < p.E)
+#pragma unroll
+            for (int i = 0; i < VPT; i += El<T>::W) {
+                Pack<T> q;
+#pragma unroll
+                for (int j = 0; j < El<T>::W; ++j) q.v[j] = El<T>::from(d[i + j]);
+                *reinterpret_cast<Pack<T>*>(out + e0 + i) = q;
+            }
+    } else {
+#pragma unroll
+        for (int i = 0; i < VPT; ++i)
+            if (e0 + i < p.E) out[e0 + i] = El<T>::from(d[i]);
+    }
+}
+
+template <typename T, int LANES, int VPT> int route_launch(const RouteParams& p, cudaStream_t st) {
+    typedef Team<LANES> Tm;
+    const int bytes = Tm::ROWS * RouteShared::bytes(LANES * VPT, p.k, p.groups);
+    const int64_t blocks = (p.T + Tm::ROWS - 1) / Tm::ROWS;
+    if (blocks > INT32_MAX) return ELA_ERR_UNSUPPORTED;
+    if (bytes > 48 * 1024 && !allow_smem<&route_kernel<T, LANES, VPT>>(100 * 1024)) return ELA_ERR_CUDA;
+    return launch(route_kernel<T, LANES, VPT>, (unsigned)blocks, Tm::BLOCK, bytes, st, p);
+}
+template <typename T, int LANES, int VPT> int route_launch(const RouteGradParams& p, cudaStream_t st) {
+    typedef Team<LANES> Tm;
+    const int64_t blocks = (p.T + Tm::ROWS - 1) / Tm::ROWS;
+    if (blocks > INT32_MAX) return ELA_ERR_UNSUPPORTED;
+    return launch(route_grad_kernel<T, LANES, VPT>, (unsigned)blocks, Tm::BLOCK, Tm::ROWS * RouteShared::bytes(LANES * VPT, p.k, 1), st, p);
+}
+
+// Eight experts a thread, so that a row of 16-bit logits is one load each, on as few threads
+// as that takes; sixteen past 256 experts.
+template <typename T, typename P> int route_by_size(P p, cudaStream_t st) {
+    const int per = p.E <= 256 ? 8 : 16;
+    p.vec = p.vec && p.E % per == 0;
+    return p.E <= 8 ? route_launch<T, 1, 8>(p, st) : p.E <= 16 ? route_launch<T, 2, 8>(p, st) : p.E <= 32 ? route_launch<T, 4, 8>(p, st)
+         : p.E <= 64 ? route_launch<T, 8, 8>(p, st) : p.E <= 128 ? route_launch<T, 16, 8>(p, st) : p.E <= 256 ? route_launch<T, 32, 8>(p, st)
+         : p.E <= 512 ? route_launch<T, 32, 16>(p, st) : route_launch<T, ROUTE_WIDE, 16>(p, st);
+}
+template <typename P> int route_by_type(const P& p, int dtype, cudaStream_t st) {
+    return dtype == ELA_DTYPE_F32 ? route_by_size<float>(p, st) : dtype == ELA_DTYPE_F16 ? route_by_size<__half>(p, st) : route_by_size<__nv_bfloat16>(p, st);
+}
+
+inline bool route_sizes_ok(int dtype, int64_t T, int64_t E, int64_t ld, int64_t k, int score, float scale) {
+    return dtype_bytes(dtype) != 0 && T >= 0 && E >= 1 && E <= ELA_EXPERT_MAX && ld >= 0 && k >= 1 && k <= E && k <= ELA_ROUTE_MAX_K &&
+           T <= INT32_MAX / k && (score == ELA_SCORE_SOFTMAX || score == ELA_SCORE_SIGMOID) && scale - scale == 0.f;
+}
+
+}  // namespace ela_expert
+
+using namespace ela_expert;
+
+extern "C" {
+
+int ela_expert_route(const void* logits, int dtype, int64_t T, int64_t E, int64_t ld, int64_t k, int score,
+                     const float* bias, int64_t groups, int64_t groups_kept, int group_score, int renormalize,
+                     float scale, int32_t* expert, float* weights, void* stream) {
+    if (!route_sizes_ok(dtype, T, E, ld, k, score, scale) || groups < 1 || E % groups != 0 || groups_kept < 1 ||
+        groups_kept > groups || k > groups_kept * (E / groups) ||
+        (group_score != ELA_GROUP_MAX && group_score != ELA_GROUP_TOP2) || (groups > 1 && group_score == ELA_GROUP_TOP2 && E / groups < 2))
+        return ELA_ERR_ARGUMENT;
+    if (T == 0) return ELA_OK;
+    if (!logits || !expert || !weights || !on_elements(dtype_bytes(dtype), logits) || !on_elements(4, bias, expert, weights)) return ELA_ERR_ARGUMENT;
+    if (groups == groups_kept) groups = groups_kept = 1;  // all stay
+    RouteParams p = {logits, T, ld, (int)E, (int)k, aligned16(logits, ld * dtype_bytes(dtype)), bias, (int)groups, (int)groups_kept,
+                     groups > 1 && group_score == ELA_GROUP_TOP2, score == ELA_SCORE_SIGMOID, renormalize != 0, scale, expert, weights};
+    return route_by_type(p, dtype, reinterpret_cast<cudaStream_t>(stream));
+}
+
+int ela_expert_route_grad(const void* logits, int dtype, int64_t T, int64_t E, int64_t ld, int64_t k, int score,
+                          int renormalize, float scale, const int32_t* expert, const float* dweights, void* dlogits,
+                          void* stream) {
+    if (!route_sizes_ok(dtype, T, E, ld, k, score, scale)) return ELA_ERR_ARGUMENT;
+    if (T == 0) return ELA_OK;
+    if (!logits || !expert || !dweights || !dlogits || !on_elements(dtype_bytes(dtype), logits, dlogits) || !on_elements(4, expert, dweights))
+        return ELA_ERR_ARGUMENT;
+    const int size = dtype_bytes(dtype);
+    RouteGradParams p = {logits, T, ld, (int)E, (int)k, aligned16(logits, ld * size) && aligned16(dlogits, E * size), score == ELA_SCORE_SIGMOID,
+                         renormalize != 0, scale, expert, dweights, dlogits};
+    return route_by_type(p, dtype, reinterpret_cast<cudaStream_t>(stream));
+}
+
+}  // extern "C"

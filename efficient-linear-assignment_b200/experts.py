@@ -9,11 +9,20 @@ these operators take the tokens there and back:
     h    = expert_linear(h, w2, b2, offsets=plan.offsets)
     out  = expert_combine(h, plan, weights)          # back, weighted and summed
 
+Beside the solver, ``expert_route`` makes the choices and their weights from a router's
+logits; for serving, ``expert_quantize`` brings the experts to 4 bits and
+``expert_linear_4bit`` multiplies with them:
+
+    expert, weights = expert_route(logits, 2)
+    w1 = expert_quantize(w1, group=64)               # once
+    h  = expert_linear_4bit(rows, w1, b1, activation="gelu", offsets=plan.offsets)
+
 All of them are C++ torch operators (csrc/ela_expert_op.cpp) over the C ABI of
 include/ela_expert.h, which also checks the arguments (TypeError, ValueError,
 RuntimeError for host tensors): current stream, no synchronisation, no data-dependent
-sizes, so the whole layer can be captured in a CUDA graph.  Dispatch, combine
-and linear are differentiable (once, in reverse mode).  A choice outside [0, num_experts), such
+sizes, so the whole layer can be captured in a CUDA graph.  Route, dispatch, combine
+and linear are differentiable (once, in reverse mode); the 4-bit operators serve, and raise
+where a gradient would be lost.  A choice outside [0, num_experts), such
 as the solver's -1 for an unassigned row, belongs to no expert: it takes one of
 the last rows, is dispatched as zeros and adds nothing to the combined token.
 """
@@ -28,6 +37,8 @@ from . import _lib
 from .solver import _native_op
 
 ACTIVATIONS = {"none": 0, "relu": 1, "gelu": 2, "silu": 3}
+SCORES = {"softmax": 0, "sigmoid": 1}
+GROUP_SCORES = {"max": 0, "top2": 1}
 MAX_EXPERTS = 4096  # ELA_EXPERT_MAX
 
 
@@ -43,6 +54,32 @@ class ExpertPlan(NamedTuple):
     source: torch.Tensor
 
 
+class ExpertRoute(NamedTuple):
+    """The experts of each token and their weights.
+
+    expert   int32 (T, k): the best first; -1 where none is left
+    weights  float32 (T, k): 0 where the expert is -1
+    """
+    expert: torch.Tensor
+    weights: torch.Tensor
+
+
+class Expert4Bit(NamedTuple):
+    """Experts' weights (E, N, K), or one matrix (N, K), in 4 bits: weight k of a row is
+    q * scale, q in -8..7, rounded to the scale's type; ``group`` inputs share a scale.
+
+    packed    int32 (E, N, W), W = 8 * ceil(K / 64): word i of a row holds q + 8 of the inputs
+              8 i + j at bits 4 * (j // 2) + 16 * (j % 2); inputs from K on are q = 0
+    scales    (E, ceil(K / group), N), float16 or bfloat16
+    features  K
+    group     32, 64 or 128
+    """
+    packed: torch.Tensor
+    scales: torch.Tensor
+    features: int
+    group: int
+
+
 _ops = None
 
 
@@ -52,7 +89,9 @@ def _native():
     if _ops is None:
         _native_op()  # loads the operator library
         n = torch.ops.ela_native
-        _ops = (n.expert_plan.default, n.expert_dispatch.default, n.expert_combine.default, n.expert_linear.default)
+        _ops = (n.expert_plan.default, n.expert_dispatch.default, n.expert_combine.default, n.expert_linear.default,
+                n.expert_route.default, n.expert_quantize.default, n.expert_dequantize.default,
+                n.expert_linear_4bit.default)
     return _ops
 
 
@@ -92,6 +131,55 @@ def expert_linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Te
     if code is None:
         raise ValueError(f"expert_linear: unknown activation '{activation}'. Options: {list(ACTIVATIONS)}")
     return (_ops or _native())[3](x, weight, bias, residual, offsets, code)
+
+
+def expert_route(logits: torch.Tensor, k: int, score: str = "softmax", bias: Optional[torch.Tensor] = None, groups: int = 1,
+                 groups_kept: Optional[int] = None, group_score: str = "max", renormalize: bool = True,
+                 scale: float = 1.0) -> ExpertRoute:
+    """The ``k`` best experts of each token and their weights, from ``logits`` (T, E).
+
+    Scores are the row's softmax or sigmoid.  Experts are chosen by score, or by
+    score + ``bias`` (float32 (E,), which balances the choice and does not touch the
+    weights); with ``groups`` > 1 only among the experts of the ``groups_kept`` best of
+    the equal runs of experts, ranked by their best expert ("max") or the sum of their two
+    best ("top2").  The weights are the chosen scores, divided by their sum with
+    ``renormalize``, times ``scale``.  Ties go to the lowest index, NaN counts as the
+    largest, and the order is that of 64-bit arithmetic.  An expert whose logit (or bias)
+    is -inf is never chosen: a token without enough of them gets expert -1, weight 0.
+    fp32, fp16 or bf16; k up to 64.  Backward: the gradient of the logits."""
+    code, by = SCORES.get(score), GROUP_SCORES.get(group_score)
+    if code is None:
+        raise ValueError(f"expert_route: unknown score '{score}'. Options: {list(SCORES)}")
+    if by is None:
+        raise ValueError(f"expert_route: unknown group_score '{group_score}'. Options: {list(GROUP_SCORES)}")
+    return ExpertRoute._make((_ops or _native())[4](logits, k, code, bias, groups, groups if groups_kept is None else groups_kept,
+                                                    by, renormalize, scale))
+
+
+def expert_quantize(weight: torch.Tensor, group: int = 64) -> Expert4Bit:
+    """``weight`` (E, N, K) or (N, K), fp16 or bf16, in 4 bits with a scale for every
+    ``group`` (32, 64 or 128) inputs of a row: scale = max|w| / 7, rounded to the weight's
+    type, q = w / scale rounded to even.  A group with a NaN or an infinity gets a scale
+    that is one.  No gradient."""
+    return Expert4Bit(*(_ops or _native())[5](weight, group), weight.shape[-1], group)
+
+
+def expert_dequantize(weight: Expert4Bit) -> torch.Tensor:
+    """The weights that ``weight`` stands for, (E, N, K) or (N, K), in the scales' type."""
+    return (_ops or _native())[6](*weight)
+
+
+def expert_linear_4bit(x: torch.Tensor, weight: Expert4Bit, bias: Optional[torch.Tensor] = None,
+                       residual: Optional[torch.Tensor] = None, activation: str = "none",
+                       offsets: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """``expert_linear`` with 4-bit weights: ``act(x W_e^T + b_e) + residual`` where W is what
+    ``expert_dequantize(weight)`` returns, without writing it.  x, bias and residual in the
+    scales' type; the other arguments, the rows of no expert and the sums in fp32 are as there.
+    No gradient: raises where one is asked for."""
+    code = ACTIVATIONS.get(activation)
+    if code is None:
+        raise ValueError(f"expert_linear_4bit: unknown activation '{activation}'. Options: {list(ACTIVATIONS)}")
+    return (_ops or _native())[7](x, *weight, bias, residual, offsets, code)
 
 
 def expert_check() -> None:
@@ -141,6 +229,30 @@ def _register_fakes() -> None:
     def _(dy, z, x, weight, offsets, activation, wsizes, bsizes, need_x, need_w, need_b):
         return (dy.new_empty((dy.shape[0] if need_x else 0, wsizes[-1])), dy.new_empty(wsizes if need_w else (0,)),
                 dy.new_empty(bsizes if need_b else (0,)))
+
+
+    @torch.library.register_fake("ela_native::expert_route")
+    def _(logits, k, score, bias, groups, groups_kept, group_score, renormalize, scale):
+        shape = (logits.shape[0], k)
+        return logits.new_empty(shape, dtype=torch.int32), logits.new_empty(shape, dtype=torch.float32)
+
+    @torch.library.register_fake("ela_native::expert_route_grad")
+    def _(dweights, logits, expert, score, renormalize, scale):
+        return logits.new_empty(logits.shape)
+
+    @torch.library.register_fake("ela_native::expert_quantize")
+    def _(weight, group):
+        *lead, n, k = weight.shape
+        return (weight.new_empty((*lead, n, (k + 63) // 64 * 8), dtype=torch.int32),
+                weight.new_empty((*lead, (k + group - 1) // group, n)))
+
+    @torch.library.register_fake("ela_native::expert_dequantize")
+    def _(packed, scales, features, group):
+        return scales.new_empty((*packed.shape[:-1], features))
+
+    @torch.library.register_fake("ela_native::expert_linear_4bit")
+    def _(x, packed, scales, features, group, bias, residual, offsets, activation):
+        return x.new_empty((x.shape[0], packed.shape[-2]))
 
 
 _register_fakes()

@@ -1,7 +1,8 @@
 /*
  * ela_expert.h -- C ABI of the expert-layer operators that follow a token-to-
  * expert assignment (libela_auction.so, built from
- * efficient-linear-assignment_b200/csrc/ela_expert.cu and ela_expert_linear.cu).
+ * efficient-linear-assignment_b200/csrc/ela_expert.cu, ela_expert_linear.cu,
+ * ela_expert_route.cu and ela_expert_4bit.cu).
  *
  * Conventions as in ela_auction.h: plain pointers and sizes, device pointers on
  * the current CUDA device, work enqueued on `stream` and not waited for, status
@@ -123,6 +124,71 @@ int ela_expert_linear_grad_input(const void* dz, const void* weight, const int32
 int ela_expert_linear_grad_weight(const void* dz, const void* x, const int32_t* offsets, int dtype, int64_t R,
                                   int64_t E, int64_t K, int64_t N, int64_t ldx, void* dweight, void* workspace,
                                   size_t workspace_bytes, void* stream);
+
+/* How a router's logits become scores, and what a group of experts is ranked by. */
+enum { ELA_SCORE_SOFTMAX = 0, ELA_SCORE_SIGMOID = 1 };
+enum { ELA_GROUP_MAX = 0, ELA_GROUP_TOP2 = 1 };
+
+/* Largest number of choices per token of ela_expert_route. */
+#define ELA_ROUTE_MAX_K 64
+
+/*
+ * The k experts of each token and their weights, from logits (T,E) with row distance
+ * ld; fp32, fp16 or bf16.
+ *   s_i = softmax or sigmoid of the row; key_i = l_i without a bias, s_i + bias_i with one
+ *   (float [E] or NULL; it moves the choice, not the weights)
+ *   groups > 1: the experts in `groups` equal runs; a group is ranked by its largest key, or
+ *   by the sum of its two largest s_i (+ bias_i), and only the experts of the
+ *   `groups_kept` best groups can be chosen
+ *   expert int32[T*k]: the experts of the k largest keys, the largest first; weights
+ *   float[T*k]: scale * s_e, or scale * s_e / (sum of the chosen s) with `renormalize`
+ * Equal keys and groups go to the lowest index, NaN counts as the largest.  An expert whose
+ * logit (or bias) is -inf is never chosen: where none is left, the choice is -1 with weight 0.
+ * The order is that of the keys in 64-bit arithmetic.  1 <= E <= ELA_EXPERT_MAX, k at most
+ * ELA_ROUTE_MAX_K and groups_kept * E / groups, T * k < 2^31.
+ */
+int ela_expert_route(const void* logits, int dtype, int64_t T, int64_t E, int64_t ld, int64_t k, int score,
+                     const float* bias, int64_t groups, int64_t groups_kept, int group_score, int renormalize,
+                     float scale, int32_t* expert, float* weights, void* stream);
+
+/*
+ * Gradient of the weights above: dlogits (T,E) contiguous, in the logits' type, from
+ * dweights float[T*k] and the choices (one outside [0, E) adds nothing).
+ */
+int ela_expert_route_grad(const void* logits, int dtype, int64_t T, int64_t E, int64_t ld, int64_t k, int score,
+                          int renormalize, float scale, const int32_t* expert, const float* dweights, void* dlogits,
+                          void* stream);
+
+/*
+ * 4-bit weights.  A row of K inputs is cut into groups of `group` (32, 64 or 128); a weight
+ * is q * scale with q in -8..7 and its group's scale, rounded to the scale's type.
+ *   packed: int32 words, eight inputs each, a row padded with zeros to a multiple of 64
+ *           inputs: W = 8 * ceil(K / 64) words.  Input 8 i + j of a row is the four bits of
+ *           word i from bit 4 (j / 2) + 16 (j % 2) on, and holds q + 8.
+ *   scales: (E, ceil(K / group), N), fp16 or bf16
+ * packed lies on 16 bytes.
+ */
+
+/* packed and scales from weight (E,N,K) with expert distance stride_e and row distance ldw:
+ * scale = max |w| / 7 of the group, rounded; q = w / scale, rounded to even, 0 where the scale is 0. */
+int ela_expert_quantize(const void* weight, int dtype, int64_t E, int64_t K, int64_t N, int64_t stride_e, int64_t ldw,
+                        int64_t group, int32_t* packed, void* scales, void* stream);
+
+/* weight (E,N,K) contiguous, in the scales' type. */
+int ela_expert_dequantize(const int32_t* packed, const void* scales, int dtype, int64_t E, int64_t K, int64_t N,
+                          int64_t group, void* weight, void* stream);
+
+/* Bytes of device workspace that ela_expert_linear_4bit needs at these sizes (`aligned`: as above, of x). */
+size_t ela_expert_linear_4bit_workspace_bytes(int64_t R, int64_t E, int64_t K, int64_t N, int aligned);
+
+/*
+ * ela_expert_linear with 4-bit weights, packed (E,N,W) and scales (E,ceil(K/group),N)
+ * contiguous, scales in x's type; the sums are over the weights that ela_expert_dequantize writes.
+ */
+int ela_expert_linear_4bit(const void* x, const int32_t* packed, const void* scales, const void* bias,
+                           const void* residual, const int32_t* offsets, int dtype, int64_t R, int64_t E, int64_t K,
+                           int64_t N, int64_t group, int64_t ldx, int64_t ldr, int activation, void* y,
+                           void* workspace, size_t workspace_bytes, void* stream);
 
 /*
  * Error of the linear kernels on the current device since the last call: ELA_OK, or
