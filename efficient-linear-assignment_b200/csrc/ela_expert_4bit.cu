@@ -2,6 +2,7 @@
 // (include/ela_expert.h): made from 16-bit weights, turned back into them, and multiplied.
 
 #include "ela_expert_4bit.cuh"
+#include "ela_expert_mma.cuh"
 
 namespace ela_expert {
 
@@ -108,9 +109,13 @@ inline int64_t pack_blocks(int64_t E, int64_t K, int64_t N) {
     return (q_words(K) * 8 + PACK_K - 1) / PACK_K * ((N + PACK_ROWS - 1) / PACK_ROWS) * E;
 }
 
-#define ELA_BY_TYPE(dtype, ...)                               \
-    if ((dtype) == ELA_DTYPE_F16) { typedef __half T_; __VA_ARGS__; } \
-    else { typedef __nv_bfloat16 T_; __VA_ARGS__; }
+// Error of the tiles' waits on the current device, read and cleared (for ela_expert_status).
+int status_4bit(int* status) {
+    const int zero = ELA_OK;
+    if (cudaMemcpyFromSymbol(status, g_expert_error, sizeof(int)) != cudaSuccess) return ELA_ERR_CUDA;
+    if (*status != ELA_OK && cudaMemcpyToSymbol(g_expert_error, &zero, sizeof(int)) != cudaSuccess) return ELA_ERR_CUDA;
+    return ELA_OK;
+}
 
 }  // namespace ela_expert
 
@@ -151,27 +156,47 @@ int ela_expert_dequantize(const int32_t* packed, const void* scales, int dtype, 
 }
 
 size_t ela_expert_linear_4bit_workspace_bytes(int64_t R, int64_t E, int64_t K, int64_t N, int aligned) {
-    (void)R; (void)E; (void)K; (void)N; (void)aligned;
-    return 0;
+    const Matrix x = {nullptr, 1, R, K, 0, 0};
+    return aligned || few_rows_4bit(R, E, N) ? 0 : x.padded_bytes();
 }
 
 int ela_expert_linear_4bit(const void* x, const int32_t* packed, const void* scales, const void* bias,
                            const void* residual, const int32_t* offsets, int dtype, int64_t R, int64_t E, int64_t K,
                            int64_t N, int64_t group, int64_t ldx, int64_t ldr, int activation, void* y,
                            void* workspace, size_t workspace_bytes, void* stream) {
-    if (!sizes_4bit_ok(dtype, E, K, N, group) || R < 0 || R > (1ll << 30) || (!offsets && E != 1) || activation < 0 ||
-        activation > ELA_ACT_SILU || ldx < 0 || ldr < 0)
+    if (!sizes_4bit_ok(dtype, E, K, N, group) || !linear_sizes_ok(dtype, R, E, K, N, offsets) || activation < 0 || activation > ELA_ACT_SILU ||
+        ldx < 0 || ldr < 0)
         return ELA_ERR_ARGUMENT;
     if (R == 0) return ELA_OK;
     if (!x || !packed || !scales || !y || !on_elements(2, x, scales, bias, residual, y) || !on_elements(4, offsets) || !aligned16(packed))
         return ELA_ERR_ARGUMENT;
-    (void)workspace; (void)workspace_bytes;
-    Stream4Params p = {x, (const uint32_t*)packed, scales, bias, residual, offsets, (int)R, (int)E, (int)K, (int)N, (int)q_words(K),
-                       (int)((K + group - 1) / group), group_shift(group), 0, activation, 0, ldx, ldr, y};
-    const bool vec = aligned16(x, ldx * 2) && K % 8 == 0;
-    int rc = ELA_OK;
     cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-    ELA_BY_TYPE(dtype, { rc = R <= 8 * E ? stream4_launch<T_, 1, 2, 2>(p, vec, st) : stream4_launch<T_, 4, 2, 2>(p, vec, st); })
+    const int words = (int)q_words(K), parts = (int)((K + group - 1) / group), shift = group_shift(group);
+    int rc = ELA_OK;
+    if (few_rows_4bit(R, E, N)) {
+        Stream4Params p = {x, (const uint32_t*)packed, scales, bias, residual, offsets, (int)R, (int)E, (int)K, (int)N, words, parts, shift, 0,
+                           activation, 0, ldx, ldr, y};
+        const bool vec = aligned16(x, ldx * 2) && K % 8 == 0;
+        ELA_BY_TYPE(dtype, { rc = R <= 8 * E ? stream4_launch<T_, 1, 2, 2>(p, vec, st) : stream4_launch<T_, 4, 2, 2>(p, vec, st); })
+        return rc;
+    }
+    char* ws = reinterpret_cast<char*>(workspace);
+    Matrix mx = {x, 1, R, K, ldx, 0};
+    if ((rc = readable(mx, ws, workspace_bytes, st)) != ELA_OK) return rc;
+    MmaParams p = row_pass(offsets, R, E, N, K, true);
+    p.bias = bias;
+    p.packed = (const uint32_t*)packed;
+    p.scales = scales;
+    p.words = words;
+    p.parts = parts;
+    p.shift = shift;
+    p.residual = residual;
+    p.ldr = ldr;
+    p.out = y;
+    p.vec = N % 2 == 0 && aligned4(y) && (!residual || (aligned4(residual) && ldr % 2 == 0));
+    CUtensorMap b;
+    if (!map_of(&b, dtype, mx, MMA_KB, p.bbox, false)) return ELA_ERR_CUDA;
+    ELA_BY_TYPE(dtype, { ELA_BY_ACT(activation, rc = (mma_launch<PASS_4BIT, T_, A_>(b, b, p, row_tiles(p), st))) })
     return rc;
 }
 

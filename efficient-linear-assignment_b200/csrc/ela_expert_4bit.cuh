@@ -1,50 +1,11 @@
-// ela_expert_4bit.cuh -- 4-bit weights: their words, and the forward product for a few rows
-// per expert (included by ela_expert_4bit.cu).
+// ela_expert_4bit.cuh -- the forward product with 4-bit weights for a few rows per expert
+// (included by ela_expert_4bit.cu).
 #pragma once
 
 #include "ela_expert.cuh"
 #include "ela_expert_stream.cuh"
 
 namespace ela_expert {
-
-constexpr int Q_PAD = 64;               // inputs that a packed row is padded to a multiple of
-constexpr uint32_t Q_ZERO = 0x88888888u;  // eight weights of 0
-__host__ __device__ inline int64_t q_words(int64_t K) { return (K + Q_PAD - 1) / Q_PAD * (Q_PAD / 8); }
-
-// Four pairs of weights from a word, in the order of the inputs.  The bits are placed as the
-// last ones of 128 (bf16) or 1024 (fp16), which makes that number plus q + 8; taking 136 or
-// 1032 away is exact, so the product with the scale is the one rounding.  Pair i sits in the
-// same bits of both halves of the word: one shift, one three-input logic operation, one
-// subtraction and one product for two weights.
-template <typename T> struct Nibbles;
-template <> struct Nibbles<__nv_bfloat16> {
-    typedef __nv_bfloat162 V;
-    static constexpr uint32_t ONE = 0x43004300u, OFF = 0x43084308u;  // 128, 136
-};
-template <> struct Nibbles<__half> {
-    typedef __half2 V;
-    static constexpr uint32_t ONE = 0x64006400u, OFF = 0x64086408u;  // 1024, 1032
-};
-template <typename T> __device__ __forceinline__ uint32_t scale_pair(T s) {
-    uint16_t b;
-    memcpy(&b, &s, 2);
-    return b * 0x10001u;
-}
-template <typename T> __device__ __forceinline__ void unpack(uint32_t word, uint32_t scales, uint32_t* out) {
-    typedef typename Nibbles<T>::V V;
-    constexpr uint32_t off = Nibbles<T>::OFF;
-    V o, s;
-    memcpy(&o, &off, 4);
-    memcpy(&s, &scales, 4);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const uint32_t bits = ((word >> (4 * i)) & 0x000f000fu) | Nibbles<T>::ONE;
-        V v;
-        memcpy(&v, &bits, 4);
-        v = __hmul2(__hsub2(v, o), s);
-        memcpy(out + i, &v, 4);
-    }
-}
 
 struct Stream4Params {
     const void* x;
@@ -237,5 +198,8 @@ template <typename T, int RG, int MT, int SUB> int stream4_launch(Stream4Params 
     return launch(vec ? stream4_kernel<T, RG, MT, SUB, 16> : stream4_kernel<T, RG, MT, SUB, 2>, (unsigned)(items < most ? items : most),
                   STREAM_WARPS * 32, 0, st, p);
 }
+
+// Rows per expert up to which the weights are streamed.
+inline bool few_rows_4bit(int64_t R, int64_t E, int64_t N) { return R <= 16 * E || (R <= 64 * E && E * ((N + 255) / 256) <= sm_count() / 4); }
 
 }  // namespace ela_expert

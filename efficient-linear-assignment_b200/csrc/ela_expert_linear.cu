@@ -13,78 +13,7 @@
 
 namespace ela_expert {
 
-// Limit of every device-side wait: 2 s, and 4 us for each block of 64 k of a tile's sum, ten times
-// what one takes, so that a sum of hundreds of millions of terms is not given up on.
-inline unsigned long long wait_limit(int64_t k) { return 2000000000ull + 4000ull * (unsigned long long)(k / 64); }
-
-// Rows of any stride and alignment copied to rows a multiple of 16 bytes apart
-// (TMA's rule for strides and base).  Bits are moved, types do not matter.  A thread
-// writes 16 bytes; where the source is off a 4-byte boundary it reads the five words
-// around them (no word is touched that does not hold an element of the row).
-__global__ void __launch_bounds__(256) realign_kernel(const uint16_t* src, int64_t rows, int cols, int64_t ld,
-                                                      int64_t rows_per_matrix, int64_t stride_e, uint16_t* dst, int64_t ldd) {
-    next_may_start();
-    previous_done();
-    const int pieces = (cols + 7) / 8;
-    const int64_t all = rows * pieces;
-    const int64_t step = (int64_t)gridDim.x * blockDim.x;
-    for (int64_t i0 = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i0 < all; i0 += 2 * step) {
-        uint4 o[2];  // two pieces' loads before their stores
-        uint16_t* to[2];
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            const int64_t i = i0 + h * step, r = i / pieces;
-            to[h] = nullptr;
-            if (i >= all) continue;
-            const int c = (int)(i - r * pieces) * 8, left = cols - c;
-            const uint16_t* s = src + r / rows_per_matrix * stride_e + r % rows_per_matrix * ld + c;
-            const bool shift = (reinterpret_cast<uintptr_t>(s) & 3) != 0;
-            const uint32_t* w = reinterpret_cast<const uint32_t*>(s - shift);
-            uint32_t v[5];
-#pragma unroll
-            for (int k = 0; k < 5; ++k) v[k] = 2 * k - shift < left && (k < 4 || shift) ? w[k] : 0u;
-            o[h].x = shift ? __funnelshift_r(v[0], v[1], 16) : v[0];
-            o[h].y = shift ? __funnelshift_r(v[1], v[2], 16) : v[1];
-            o[h].z = shift ? __funnelshift_r(v[2], v[3], 16) : v[2];
-            o[h].w = shift ? __funnelshift_r(v[3], v[4], 16) : v[3];
-            to[h] = dst + r * ldd + c;  // (ldd is cols rounded up to 8)
-        }
-#pragma unroll
-        for (int h = 0; h < 2; ++h)
-            if (to[h]) *reinterpret_cast<uint4*>(to[h]) = o[h];
-    }
-}
-
-inline int64_t round8(int64_t n) { return (n + 7) / 8 * 8; }
-inline size_t round256(size_t n) { return (n + 255) / 256 * 256; }
-
-// A matrix operand: (matrices, rows, cols), 16-bit.
-struct Matrix {
-    const void* p;
-    int64_t matrices, rows, cols, ld, stride_e;
-    size_t padded_bytes() const { return round256((size_t)(matrices * rows * round8(cols)) * 2); }
-    bool ok() const { return aligned16(p, ld * 2) && (matrices == 1 || stride_e * 2 % 16 == 0); }
-};
-
-// The matrix itself where TMA can read it, else its copy in the workspace.
-inline int readable(Matrix& m, char*& ws, size_t& left, cudaStream_t st) {
-    if (m.ok()) return ELA_OK;
-    const size_t need = m.padded_bytes();
-    if (!ws || left < need || !aligned16(ws)) return ELA_ERR_ARGUMENT;
-    const int64_t rows = m.matrices * m.rows, ld = round8(m.cols);
-    const int64_t blocks = (rows * (ld / 8) + 255) / 256, most = 8 * (int64_t)sm_count();
-    const int rc = launch(realign_kernel, (unsigned)(blocks < most ? blocks : most), 256, 0, st, (const uint16_t*)m.p, rows, (int)m.cols, m.ld, m.rows, m.stride_e, (uint16_t*)ws, ld);
-    m.p = ws;
-    m.ld = ld;
-    m.stride_e = m.rows * ld;
-    ws += need;
-    left -= need;
-    return rc;
-}
-inline bool map_of(CUtensorMap* map, int dtype, const Matrix& m, int box_cols, int box_rows, bool three) {
-    const int64_t se = m.matrices > 1 ? m.stride_e : round8(m.ld * m.rows);
-    return make_map(map, dtype, m.p, m.cols, m.rows, m.matrices, m.ld, se, box_cols, box_rows, three ? 3 : 2);
-}
+int status_4bit(int* status);  // ela_expert_4bit.cu
 
 // ------------------------------------- gradient of the activation and the bias
 // dz = dy * act'(z) in one pass over dy and z, with the column sums of dz (the bias
@@ -238,43 +167,6 @@ inline int act_block_rows(int64_t R, int64_t N) {
     return rows;
 }
 
-inline bool linear_sizes_ok(int dtype, int64_t R, int64_t E, int64_t K, int64_t N, const int32_t* offsets) {
-    return (dtype == ELA_DTYPE_F16 || dtype == ELA_DTYPE_BF16) && R >= 0 && R <= (1ll << 30) && E >= 1 &&
-           E <= ELA_EXPERT_MAX && K >= 1 && K <= (1ll << 30) && N >= 1 && N <= (1ll << 30) && (offsets || E == 1);
-}
-inline bool aligned4(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 3u) == 0; }
-
-// Parameters of a pass whose columns are the experts' rows: F features out, contraction length K.
-inline MmaParams row_pass(const int32_t* offsets, int64_t R, int64_t E, int64_t F, int64_t K) {
-    MmaParams p = {};
-    p.offsets = offsets;
-    p.R = (int)R; p.E = (int)E; p.F = (int)F; p.K = (int)K;
-    p.f_tiles = (int)((F + MMA_PAIR_F - 1) / MMA_PAIR_F);
-    p.bn = columns_per_tile(R, E, p.f_tiles, (K + MMA_KB - 1) / MMA_KB);
-    // a CTA's half of a tile's columns is one box, or boxes of 64 where experts have fewer rows
-    // than that makes (a box is loaded whole)
-    p.bbox = p.bn % 128 == 0 && R < 256 * E ? 64 : p.bn / 2;
-    p.stages = stages_for(p.bn, E);
-    p.wait_ns = wait_limit(K);
-    return p;
-}
-// At least as many tiles as the offsets can make.
-inline int64_t row_tiles(const MmaParams& p) {
-    const int64_t by_rows = p.R / p.bn + (p.E < p.R ? p.E : p.R);
-    return (by_rows > 0 ? by_rows : 1) * p.f_tiles;
-}
-
-#define ELA_BY_TYPE(dtype, ...)                               \
-    if ((dtype) == ELA_DTYPE_F16) { typedef __half T_; __VA_ARGS__; } \
-    else { typedef __nv_bfloat16 T_; __VA_ARGS__; }
-#define ELA_BY_ACT(act, ...)                                          \
-    switch (act) {                                                     \
-    case ELA_ACT_RELU: { constexpr int A_ = ELA_ACT_RELU; __VA_ARGS__; break; } \
-    case ELA_ACT_GELU: { constexpr int A_ = ELA_ACT_GELU; __VA_ARGS__; break; } \
-    case ELA_ACT_SILU: { constexpr int A_ = ELA_ACT_SILU; __VA_ARGS__; break; } \
-    default: { constexpr int A_ = ELA_ACT_NONE; __VA_ARGS__; break; }           \
-    }
-
 }  // namespace ela_expert
 
 using namespace ela_expert;
@@ -299,7 +191,10 @@ int ela_expert_status(int* status) {
     if (cudaDeviceSynchronize() != cudaSuccess) return ELA_ERR_CUDA;
     if (cudaMemcpyFromSymbol(status, g_expert_error, sizeof(int)) != cudaSuccess) return ELA_ERR_CUDA;
     if (*status != ELA_OK && cudaMemcpyToSymbol(g_expert_error, &zero, sizeof(int)) != cudaSuccess) return ELA_ERR_CUDA;
-    return ELA_OK;
+    int packed = ELA_OK;
+    const int rc = status_4bit(&packed);
+    if (*status == ELA_OK) *status = packed;
+    return rc;
 }
 
 int ela_expert_linear(const void* x, const void* weight, const void* bias, const void* residual,

@@ -1,5 +1,5 @@
-// ela_expert_mma.cuh -- the tensor-core product behind ela_expert_linear and its
-// gradients (included by ela_expert_linear.cu).
+// ela_expert_mma.cuh -- the tensor-core product behind ela_expert_linear, its gradients
+// (included by ela_expert_linear.cu) and ela_expert_linear_4bit (by ela_expert_4bit.cu).
 //
 // One persistent kernel computes out[c][f] = sum_k A(f,k) B(c,k), f contiguous in
 // memory.  A pair of CTAs (cluster of 2, tcgen05 cta_group::2) owns a tile of 256
@@ -8,6 +8,7 @@
 //
 //   pass           f (TMEM lanes)         c (MMA N)            k
 //   forward        output feature n       row of the expert    input feature
+//   4 bits         the same, the weights unpacked by eight warps instead of loaded by TMA
 //   input grad     input feature          row of the expert    output feature
 //   weight grad    input feature          output feature       row of the expert
 //
@@ -51,11 +52,13 @@
 #include <cuda.h>
 #include <cudaTypedefs.h>
 
+#include <algorithm>
+
 #include "ela_expert.cuh"
 
 namespace ela_expert {
 
-enum { PASS_FORWARD = 0, PASS_INPUT = 1, PASS_WEIGHT = 2 };
+enum { PASS_FORWARD = 0, PASS_INPUT = 1, PASS_WEIGHT = 2, PASS_4BIT = 3 };
 
 constexpr int MMA_F = 128;              // features per CTA (TMEM lanes)
 constexpr int MMA_PAIR_F = 256;         // features per tile
@@ -69,6 +72,7 @@ constexpr int MMA_MAX_STAGES = 10;
 constexpr int MMA_THREADS = 128 + MMA_GROUPS * 128;
 constexpr int MMA_SMEM = 227 * 1024;
 constexpr int MMA_SMEM_FIXED = 1024;    // alignment of the first stage
+constexpr int MMA_UNPACK = 8;            // warps that unpack 4-bit weights
 constexpr int MMA_TILES = 4;            // tiles the scheduling warp is ahead
 constexpr int MMA_GROUP = 16;           // column tiles walked together, for L2 reuse of both operands
 
@@ -83,13 +87,16 @@ struct MmaParams {
     const void* x;          // forward with z: the operands again, for exact_z
     const void* weight;
     int64_t ldr, ldx, ldw, stride_e;
+    const uint32_t* packed; // 4-bit weights: rows of words, groups of a row, log2 of a group's inputs
+    const void* scales;
+    int words, parts, shift;
     void* out;
     void* z;
     unsigned long long wait_ns;
 };
 
 // Sticky error of the kernels below (a wait that ran out), read by ela_expert_status.
-__device__ int g_expert_error;
+static __device__ int g_expert_error;
 
 // ------------------------------------------------------------- PTX wrappers
 __device__ __forceinline__ uint32_t saddr(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
@@ -473,12 +480,91 @@ __device__ __forceinline__ void load_residual(uint32_t* res, const MmaParams& p,
     for (int j = 0; j < MMA_CHUNK; j += 2, at += p.ldr) res[j / 2] = j < mine ? *at : 0u;
 }
 
+// ------------------------------------------------------------- 4-bit weights
+// Eight warps of each CTA write the weights' stages instead of TMA: four of them every other
+// stage, a thread one feature's 64 inputs, 32 bytes of words that come as eight 16-byte pieces of
+// the swizzled row (eight neighbouring lanes write eight different pieces: all banks once).
+// The words are loaded UNPACK_AHEAD of the warp's own stages before they are needed, across tiles.
+// A stage is handed over by an arrival at the first CTA's barrier after the fence that makes
+// the writes visible to the tensor core of this SM, which alone reads them.
+constexpr int UNPACK_AHEAD = 2;
+__device__ __forceinline__ void bar_arrive_leader(uint32_t addr) {
+    asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(addr) : "memory");
+}
+template <typename T, typename Fetch, typename GiveUp>
+__device__ __forceinline__ void unpack_stages(const MmaParams& p, unsigned char* smem, int stage_bytes, uint64_t* full, uint64_t* empty, int rank,
+                                              Fetch fetch, GiveUp give_up, const volatile int* abort) {
+    struct Words { uint4 v[2]; uint32_t s[2]; };
+    const int lane = threadIdx.x & 31, w = (threadIdx.x >> 5) - 4 - 4 * MMA_GROUPS, odd = w >> 2;
+    const int row = (w & 3) * 32 + lane;
+    const int blocks = (p.K + MMA_KB - 1) / MMA_KB;
+    Tile t = {};
+    int tile = -1, kb = odd - blocks;  // of the next load; the tile's number among the pair's
+    bool ok = true, more = true;
+    const uint32_t* words = nullptr;
+    const uint16_t* scales = nullptr;
+    auto load = [&](Words& q) {  // false: no stage left
+        while (more && (tile < 0 || kb >= blocks)) {
+            kb = tile < 0 ? odd : kb - blocks;
+            more = fetch(++tile, t, ok);
+            const int f = min(t.f0 + rank * MMA_F + row, p.F - 1);
+            words = p.packed + ((int64_t)t.e * p.F + f) * p.words;
+            scales = reinterpret_cast<const uint16_t*>(p.scales) + (int64_t)t.e * p.parts * p.F + f;
+        }
+        if (!more) return false;
+        const int k = kb * MMA_KB;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            asm volatile("ld.global.L1::no_allocate.L2::256B.v4.b32 {%0,%1,%2,%3}, [%4];"
+                : "=r"(q.v[h].x), "=r"(q.v[h].y), "=r"(q.v[h].z), "=r"(q.v[h].w) : "l"(words + k / 8 + 4 * h) : "memory");
+            q.s[h] = scales[(int64_t)min((k + 32 * h) >> p.shift, p.parts - 1) * p.F];
+        }
+        kb += 2;
+        return true;
+    };
+    Words q[UNPACK_AHEAD];
+    bool have[UNPACK_AHEAD];
+#pragma unroll
+    for (int i = 0; i < UNPACK_AHEAD; ++i) have[i] = load(q[i]);
+    int s = odd;
+    uint32_t phase = 0;
+    for (;;) {
+#pragma unroll
+        for (int i = 0; i < UNPACK_AHEAD; ++i) {
+            if (!have[i] || !ok) return;
+            int good = 0;
+            if (lane == 0) good = bar_wait(&empty[s], phase ^ 1, p.wait_ns, abort);
+            if (!__shfl_sync(~0u, good, 0)) {
+                if (lane == 0) give_up();
+                return;
+            }
+            unsigned char* to = smem + (size_t)s * stage_bytes + row * 128;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const uint4& v = q[i].v[j / 4];
+                uint32_t out[4];
+                unpack<T>(j % 4 == 0 ? v.x : j % 4 == 1 ? v.y : j % 4 == 2 ? v.z : v.w, q[i].s[j / 4] * 0x10001u, out);
+                *reinterpret_cast<uint4*>(to + ((j ^ (row & 7)) << 4)) = make_uint4(out[0], out[1], out[2], out[3]);
+            }
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            __syncwarp();
+            if (lane == 0) bar_arrive_leader(leader_addr(&full[s]));
+            if ((s += 2) >= p.stages) { s -= p.stages; phase ^= 1; }
+            have[i] = load(q[i]);
+        }
+    }
+}
+
+// Threads of a CTA.
+template <int PASS> constexpr int mma_threads() { return MMA_THREADS + (PASS == PASS_4BIT ? 32 * MMA_UNPACK : 0); }
+
 // Z: the forward pass keeps z for the gradient.
 template <int PASS, typename T, int ACT, bool Z>
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(MMA_THREADS, 1)
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(mma_threads<PASS>(), 1)
     mma_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
                const __grid_constant__ MmaParams p) {
-    constexpr bool A_K_MAJOR = PASS == PASS_FORWARD, B_K_MAJOR = PASS != PASS_WEIGHT;
+    constexpr bool PACKED = PASS == PASS_4BIT, FWD = PASS == PASS_FORWARD || PACKED;
+    constexpr bool A_K_MAJOR = FWD, B_K_MAJOR = PASS != PASS_WEIGHT;
     extern __shared__ unsigned char smem_raw[];
     // full, tempty, patched: the first CTA's are used; empty, tfull, landed: each CTA its own
     __shared__ __align__(8) uint64_t full[MMA_MAX_STAGES], empty[MMA_MAX_STAGES], tfull[2], tempty[2], sfull[MMA_TILES], sempty[MMA_TILES], patched[MMA_MAX_STAGES], landed, drained;
@@ -499,7 +585,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(MMA_THREADS, 1)
 
     next_may_start();
     if (tid == 32) {
-        asm volatile("prefetch.tensormap [%0];" ::"l"(&map_a) : "memory");
+        if (!PACKED) asm volatile("prefetch.tensormap [%0];" ::"l"(&map_a) : "memory");
         asm volatile("prefetch.tensormap [%0];" ::"l"(&map_b) : "memory");
     }
     if (warp == 2) {
@@ -508,9 +594,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(MMA_THREADS, 1)
     }
     if (tid == 0) {
         s_abort = 0;
-        for (int s = 0; s < p.stages; ++s) { bar_init(&full[s], 1); bar_init(&empty[s], 1); }
+        // full: the loads of the pair, and the weights of a stage that four warps of each CTA have unpacked
+        for (int s = 0; s < p.stages; ++s) { bar_init(&full[s], 1 + (PACKED ? MMA_UNPACK : 0)); bar_init(&empty[s], 1); }
         for (int b = 0; b < 2; ++b) { bar_init(&tfull[b], 1); bar_init(&tempty[b], 2 * 4 * MMA_GROUPS); }
-        for (int i = 0; i < MMA_TILES; ++i) { bar_init(&sfull[i], 1); bar_init(&sempty[i], 4 * MMA_GROUPS + 1 + (rank == 0)); }
+        for (int i = 0; i < MMA_TILES; ++i) { bar_init(&sfull[i], 1); bar_init(&sempty[i], 4 * MMA_GROUPS + 1 + (rank == 0) + (PACKED ? MMA_UNPACK : 0)); }
         bar_init(&landed, 1);
         for (int s = 0; s < p.stages; ++s) bar_init(&patched[s], 1);
         bar_init(&drained, 1);
@@ -521,7 +608,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(MMA_THREADS, 1)
         if (tid == 0) s_near.tile = 0;
     }
     previous_done();  // (no memory was touched before)
-    for (int e = tid; e < p.E; e += MMA_THREADS) expert_rows(p.offsets, e, p.R, table[e], table[p.E + e]);
+    for (int e = tid; e < p.E; e += mma_threads<PASS>()) expert_rows(p.offsets, e, p.R, table[e], table[p.E + e]);
     __syncthreads();
     if (PASS != PASS_WEIGHT && warp == 3) {  // row tiles before each expert
         int before = 0;
@@ -594,7 +681,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(MMA_THREADS, 1)
             const int half = ((t.nc + 31) & ~31) >> 1, c0 = t.c0 + rank * half;
             const int boxes = B_K_MAJOR ? (half + p.bbox - 1) / p.bbox : (half + 63) / 64;
             const int box_bytes = B_K_MAJOR ? p.bbox * MMA_KB * 2 : 64 * MMA_KB * 2;
-            const uint32_t bytes = MMA_A_BYTES + boxes * box_bytes;
+            const uint32_t bytes = (PACKED ? 0 : MMA_A_BYTES) + boxes * box_bytes;
             // Rows of the next expert in the last block of a sum over rows: that block's
             // loads land on a barrier of this CTA, the rows are zeroed, then the stage is full.
             const int tail = PASS == PASS_WEIGHT ? t.nk % MMA_KB : 0, blocks = (t.nk + MMA_KB - 1) / MMA_KB;
@@ -604,7 +691,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(MMA_THREADS, 1)
                 unsigned char* b = a + MMA_A_BYTES;
                 if (PASS == PASS_FORWARD) {
                     tma_3d(a, &map_a, k, f0, t.e, bar);
-                } else {
+                } else if (!PACKED) {
                     for (int h = 0; h < 2; ++h)
                         if (PASS == PASS_INPUT) tma_3d(a + h * 8192, &map_a, f0 + h * 64, k, t.e, bar);
                         else tma_2d(a + h * 8192, &map_a, f0 + h * 64, k, bar);
@@ -735,6 +822,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(MMA_THREADS, 1)
                 }
             }
         }
+    } else if (PACKED && warp >= 4 + 4 * MMA_GROUPS) {  // ---- weights out of 4 bits
+        if constexpr (PACKED) unpack_stages<T>(p, smem, stage_bytes, full, empty, rank, fetch, give_up, abort);
     } else if (warp >= 4) {  // ---- epilogue
         const int w = warp & 3, group = (warp - 4) >> 2;
         if constexpr (PASS != PASS_WEIGHT) {  // rows of no expert: the residual, or 0
@@ -749,8 +838,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(MMA_THREADS, 1)
         Tile t = {};
         int it = 0;
         bool ok = true;
-        constexpr bool FWD = PASS == PASS_FORWARD;
-        const bool with_res = PASS == PASS_FORWARD && p.residual;
+        const bool with_res = FWD && p.residual;
         auto accumulators = [&](int half, int it) {  // waits for the tile's products
             if (lane == 0) ok = bar_wait(&tfull[half], (it >> 1) & 1, p.wait_ns, abort);
             ok = __shfl_sync(~0u, (int)ok, 0);
@@ -784,7 +872,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(MMA_THREADS, 1)
             const bool product = t.nk > 0;
             const int half = it & 1;
             const int f = t.f0 + rank * MMA_F + 32 * w + lane;
-            const float bias = PASS == PASS_FORWARD && p.bias && f < p.F
+            const float bias = FWD && p.bias && f < p.F
                                    ? El<T>::to(reinterpret_cast<const T*>(p.bias)[(int64_t)t.e * p.F + f]) : 0.f;
             const int64_t c_base = PASS == PASS_WEIGHT ? (int64_t)t.e * p.C + t.c0 : t.c0;
             uint32_t res[MMA_CHUNK / 2];
@@ -822,7 +910,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(MMA_THREADS, 1)
     __syncthreads();
     if (s_abort) {  // loads and products in flight end before the CTA gives back its memory
         int never = 0;
-        if (tid == 0 && rank == 0) {
+        if (!PACKED && tid == 0 && rank == 0) {
             const uint32_t last = s_issued < (uint32_t)p.stages ? s_issued : p.stages;
             for (uint32_t i = s_issued - last; i < s_issued; ++i)
                 bar_wait(&full[i % p.stages], (i / p.stages) & 1, p.wait_ns, &never);
@@ -831,7 +919,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(MMA_THREADS, 1)
             mma_commit(&drained);
             bar_wait(&drained, 0, p.wait_ns, &never);
         }
-        if (tid == 0) {  // the other CTA's loads count on barriers that it cannot wait for
+        // the other CTA's loads count on barriers that it cannot wait for (nor can either where weights
+        // that nobody will unpack are waited for, too)
+        if (tid == 0) {
             unsigned long long t0, t1;
             asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t0));
             do asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t1)); while (t1 - t0 < 1000000ull);
@@ -876,7 +966,7 @@ int mma_launch(const CUtensorMap& a, const CUtensorMap& b, const MmaParams& p, i
     const int sms = sm_count();
     if (sms == 0 || !allow_smem<&mma_kernel<PASS, T, ACT, Z>>(MMA_SMEM - 1024)) return ELA_ERR_CUDA;
     const int grid = 2 * (int)(max_tiles < sms / 2 ? max_tiles : sms / 2);
-    return launch(kern, grid, MMA_THREADS, MMA_SMEM - 1024, st, a, b, p);
+    return launch(kern, grid, mma_threads<PASS>(), MMA_SMEM - 1024, st, a, b, p);
 }
 
 // Columns per tile of the row passes, a multiple of 32 up to 256: the one whose rounds of
@@ -887,13 +977,14 @@ int mma_launch(const CUtensorMap& a, const CUtensorMap& b, const MmaParams& p, i
 // of 1000 x 2048 16.8 and 20.0, 3000 of 64 of 1408 x 512 24.0 and 27.2.  Loads are uneven, so an
 // expert is taken to have twice its share of the rows; on six such shapes with skewed loads
 // that made 140 us in all, one and a half times 139, and the share itself 139.
-inline int columns_per_tile(int64_t R, int64_t E, int64_t f_tiles, int64_t k_blocks) {
+// 4-bit weights: 4 KB of a block, and some 200 cycles to unpack it.
+inline int columns_per_tile(int64_t R, int64_t E, int64_t f_tiles, int64_t k_blocks, bool packed = false) {
     const int64_t share = (R + E - 1) / E, rows = E == 1 ? share : 2 * share, pairs = sm_count() / 2 > 0 ? sm_count() / 2 : 1;
     int best = 256;
     int64_t least = INT64_MAX;
     for (int bn = 256; bn >= 32; bn -= 32) {
         const int64_t tiles = f_tiles * (E < R ? E : R) * ((rows + bn - 1) / bn), used = rows < bn ? (rows + 31) / 32 * 32 : bn;
-        const int64_t loads = (16384 + 64 * used) / 57, block = 2 * used > loads ? 2 * used : loads;
+        const int64_t loads = packed ? std::max<int64_t>((4096 + 64 * used) / 57, 200) : (16384 + 64 * used) / 57, block = 2 * used > loads ? 2 * used : loads;
         const int64_t time = (tiles + pairs - 1) / pairs * (k_blocks * block + 500);
         if (time < least || (time == least && rows <= bn)) { least = time; best = bn; }  // (a smaller stage leaves room for more)
     }
@@ -903,5 +994,115 @@ inline int stages_for(int bn, int64_t E) {
     const int64_t n = (MMA_SMEM - 1024 - MMA_SMEM_FIXED - 12 * E) / (MMA_A_BYTES + bn / 2 * MMA_KB * 2);
     return (int)(n < MMA_MAX_STAGES ? n : MMA_MAX_STAGES);
 }
+
+// Limit of every device-side wait: 2 s, and 4 us for each block of 64 k of a tile's sum, ten times
+// what one takes, so that a sum of hundreds of millions of terms is not given up on.
+inline unsigned long long wait_limit(int64_t k) { return 2000000000ull + 4000ull * (unsigned long long)(k / 64); }
+
+// Rows of any stride and alignment copied to rows a multiple of 16 bytes apart
+// (TMA's rule for strides and base).  Bits are moved, types do not matter.  A thread
+// writes 16 bytes; where the source is off a 4-byte boundary it reads the five words
+// around them (no word is touched that does not hold an element of the row).
+static __global__ void __launch_bounds__(256) realign_kernel(const uint16_t* src, int64_t rows, int cols, int64_t ld,
+                                                      int64_t rows_per_matrix, int64_t stride_e, uint16_t* dst, int64_t ldd) {
+    next_may_start();
+    previous_done();
+    const int pieces = (cols + 7) / 8;
+    const int64_t all = rows * pieces;
+    const int64_t step = (int64_t)gridDim.x * blockDim.x;
+    for (int64_t i0 = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i0 < all; i0 += 2 * step) {
+        uint4 o[2];  // two pieces' loads before their stores
+        uint16_t* to[2];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const int64_t i = i0 + h * step, r = i / pieces;
+            to[h] = nullptr;
+            if (i >= all) continue;
+            const int c = (int)(i - r * pieces) * 8, left = cols - c;
+            const uint16_t* s = src + r / rows_per_matrix * stride_e + r % rows_per_matrix * ld + c;
+            const bool shift = (reinterpret_cast<uintptr_t>(s) & 3) != 0;
+            const uint32_t* w = reinterpret_cast<const uint32_t*>(s - shift);
+            uint32_t v[5];
+#pragma unroll
+            for (int k = 0; k < 5; ++k) v[k] = 2 * k - shift < left && (k < 4 || shift) ? w[k] : 0u;
+            o[h].x = shift ? __funnelshift_r(v[0], v[1], 16) : v[0];
+            o[h].y = shift ? __funnelshift_r(v[1], v[2], 16) : v[1];
+            o[h].z = shift ? __funnelshift_r(v[2], v[3], 16) : v[2];
+            o[h].w = shift ? __funnelshift_r(v[3], v[4], 16) : v[3];
+            to[h] = dst + r * ldd + c;  // (ldd is cols rounded up to 8)
+        }
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+            if (to[h]) *reinterpret_cast<uint4*>(to[h]) = o[h];
+    }
+}
+
+inline int64_t round8(int64_t n) { return (n + 7) / 8 * 8; }
+inline size_t round256(size_t n) { return (n + 255) / 256 * 256; }
+
+// A matrix operand: (matrices, rows, cols), 16-bit.
+struct Matrix {
+    const void* p;
+    int64_t matrices, rows, cols, ld, stride_e;
+    size_t padded_bytes() const { return round256((size_t)(matrices * rows * round8(cols)) * 2); }
+    bool ok() const { return aligned16(p, ld * 2) && (matrices == 1 || stride_e * 2 % 16 == 0); }
+};
+
+// The matrix itself where TMA can read it, else its copy in the workspace.
+static inline int readable(Matrix& m, char*& ws, size_t& left, cudaStream_t st) {
+    if (m.ok()) return ELA_OK;
+    const size_t need = m.padded_bytes();
+    if (!ws || left < need || !aligned16(ws)) return ELA_ERR_ARGUMENT;
+    const int64_t rows = m.matrices * m.rows, ld = round8(m.cols);
+    const int64_t blocks = (rows * (ld / 8) + 255) / 256, most = 8 * (int64_t)sm_count();
+    const int rc = launch(realign_kernel, (unsigned)(blocks < most ? blocks : most), 256, 0, st, (const uint16_t*)m.p, rows, (int)m.cols, m.ld, m.rows, m.stride_e, (uint16_t*)ws, ld);
+    m.p = ws;
+    m.ld = ld;
+    m.stride_e = m.rows * ld;
+    ws += need;
+    left -= need;
+    return rc;
+}
+inline bool map_of(CUtensorMap* map, int dtype, const Matrix& m, int box_cols, int box_rows, bool three) {
+    const int64_t se = m.matrices > 1 ? m.stride_e : round8(m.ld * m.rows);
+    return make_map(map, dtype, m.p, m.cols, m.rows, m.matrices, m.ld, se, box_cols, box_rows, three ? 3 : 2);
+}
+
+inline bool linear_sizes_ok(int dtype, int64_t R, int64_t E, int64_t K, int64_t N, const int32_t* offsets) {
+    return (dtype == ELA_DTYPE_F16 || dtype == ELA_DTYPE_BF16) && R >= 0 && R <= (1ll << 30) && E >= 1 &&
+           E <= ELA_EXPERT_MAX && K >= 1 && K <= (1ll << 30) && N >= 1 && N <= (1ll << 30) && (offsets || E == 1);
+}
+inline bool aligned4(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 3u) == 0; }
+
+// Parameters of a pass whose columns are the experts' rows: F features out, contraction length K.
+inline MmaParams row_pass(const int32_t* offsets, int64_t R, int64_t E, int64_t F, int64_t K, bool packed = false) {
+    MmaParams p = {};
+    p.offsets = offsets;
+    p.R = (int)R; p.E = (int)E; p.F = (int)F; p.K = (int)K;
+    p.f_tiles = (int)((F + MMA_PAIR_F - 1) / MMA_PAIR_F);
+    p.bn = columns_per_tile(R, E, p.f_tiles, (K + MMA_KB - 1) / MMA_KB, packed);
+    // a CTA's half of a tile's columns is one box, or boxes of 64 where experts have fewer rows
+    // than that makes (a box is loaded whole)
+    p.bbox = p.bn % 128 == 0 && R < 256 * E ? 64 : p.bn / 2;
+    p.stages = stages_for(p.bn, E);
+    p.wait_ns = wait_limit(K);
+    return p;
+}
+// At least as many tiles as the offsets can make.
+inline int64_t row_tiles(const MmaParams& p) {
+    const int64_t by_rows = p.R / p.bn + (p.E < p.R ? p.E : p.R);
+    return (by_rows > 0 ? by_rows : 1) * p.f_tiles;
+}
+
+#define ELA_BY_TYPE(dtype, ...)                               \
+    if ((dtype) == ELA_DTYPE_F16) { typedef __half T_; __VA_ARGS__; } \
+    else { typedef __nv_bfloat16 T_; __VA_ARGS__; }
+#define ELA_BY_ACT(act, ...)                                          \
+    switch (act) {                                                     \
+    case ELA_ACT_RELU: { constexpr int A_ = ELA_ACT_RELU; __VA_ARGS__; break; } \
+    case ELA_ACT_GELU: { constexpr int A_ = ELA_ACT_GELU; __VA_ARGS__; break; } \
+    case ELA_ACT_SILU: { constexpr int A_ = ELA_ACT_SILU; __VA_ARGS__; break; } \
+    default: { constexpr int A_ = ELA_ACT_NONE; __VA_ARGS__; break; }           \
+    }
 
 }  // namespace ela_expert
