@@ -93,7 +93,7 @@ SIGNATURES = {
     "ela_expert_dequantize": (_c.c_int, [
         _c.c_void_p, _c.c_void_p, _c.c_int, _c.c_int64, _c.c_int64, _c.c_int64, _c.c_int64, _c.c_void_p, _c.c_void_p]),
     "ela_expert_linear_4bit_workspace_bytes": (_c.c_size_t, [
-        _c.c_int64, _c.c_int64, _c.c_int64, _c.c_int64, _c.c_int]),
+        _c.c_int64, _c.c_int64, _c.c_int64, _c.c_int64, _c.c_int64, _c.c_int]),
     "ela_expert_linear_4bit": (_c.c_int, [
         _c.c_void_p, _c.c_void_p, _c.c_void_p, _c.c_void_p, _c.c_void_p, _c.c_void_p, _c.c_int, _c.c_int64, _c.c_int64,
         _c.c_int64, _c.c_int64, _c.c_int64, _c.c_int64, _c.c_int64, _c.c_int, _c.c_void_p, _c.c_void_p, _c.c_size_t,

@@ -126,7 +126,7 @@ extern "C" {
 int ela_expert_quantize(const void* weight, int dtype, int64_t E, int64_t K, int64_t N, int64_t stride_e, int64_t ldw,
                         int64_t group, int32_t* packed, void* scales, void* stream) {
     if (!sizes_4bit_ok(dtype, E, K, N, group) || stride_e < 0 || ldw < 0 || !weight || !packed || !scales ||
-        !on_elements(2, weight, scales) || !aligned16(packed))
+        !on_elements(2, weight, scales) || !on_elements(32, packed))
         return ELA_ERR_ARGUMENT;
     const int64_t blocks = pack_blocks(E, K, N);
     if (blocks > INT32_MAX) return ELA_ERR_UNSUPPORTED;
@@ -142,7 +142,7 @@ int ela_expert_quantize(const void* weight, int dtype, int64_t E, int64_t K, int
 
 int ela_expert_dequantize(const int32_t* packed, const void* scales, int dtype, int64_t E, int64_t K, int64_t N,
                           int64_t group, void* weight, void* stream) {
-    if (!sizes_4bit_ok(dtype, E, K, N, group) || !weight || !packed || !scales || !on_elements(2, weight, scales) || !aligned16(packed))
+    if (!sizes_4bit_ok(dtype, E, K, N, group) || !weight || !packed || !scales || !on_elements(2, weight, scales) || !on_elements(32, packed))
         return ELA_ERR_ARGUMENT;
     const int64_t blocks = pack_blocks(E, K, N);
     if (blocks > INT32_MAX) return ELA_ERR_UNSUPPORTED;
@@ -155,9 +155,10 @@ int ela_expert_dequantize(const int32_t* packed, const void* scales, int dtype, 
     return rc;
 }
 
-size_t ela_expert_linear_4bit_workspace_bytes(int64_t R, int64_t E, int64_t K, int64_t N, int aligned) {
-    const Matrix x = {nullptr, 1, R, K, 0, 0};
-    return aligned || few_rows_4bit(R, E, N) ? 0 : x.padded_bytes();
+size_t ela_expert_linear_4bit_workspace_bytes(int64_t R, int64_t E, int64_t K, int64_t N, int64_t group, int aligned) {
+    if (few_rows_4bit(R, E, N) || group_shift(group) == 0) return 0;
+    const Matrix x = {nullptr, 1, R, K, 0, 0}, scales = {nullptr, 1, E * ((K + group - 1) / group), N, 0, 0};
+    return (aligned ? 0 : x.padded_bytes()) + (aligned && N % 8 == 0 ? 0 : scales.padded_bytes());
 }
 
 int ela_expert_linear_4bit(const void* x, const int32_t* packed, const void* scales, const void* bias,
@@ -168,7 +169,7 @@ int ela_expert_linear_4bit(const void* x, const int32_t* packed, const void* sca
         ldx < 0 || ldr < 0)
         return ELA_ERR_ARGUMENT;
     if (R == 0) return ELA_OK;
-    if (!x || !packed || !scales || !y || !on_elements(2, x, scales, bias, residual, y) || !on_elements(4, offsets) || !aligned16(packed))
+    if (!x || !packed || !scales || !y || !on_elements(2, x, scales, bias, residual, y) || !on_elements(4, offsets) || !on_elements(32, packed))
         return ELA_ERR_ARGUMENT;
     cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
     const int words = (int)q_words(K), parts = (int)((K + group - 1) / group), shift = group_shift(group);
@@ -181,22 +182,22 @@ int ela_expert_linear_4bit(const void* x, const int32_t* packed, const void* sca
         return rc;
     }
     char* ws = reinterpret_cast<char*>(workspace);
-    Matrix mx = {x, 1, R, K, ldx, 0};
-    if ((rc = readable(mx, ws, workspace_bytes, st)) != ELA_OK) return rc;
-    MmaParams p = row_pass(offsets, R, E, N, K, true);
+    Matrix mx = {x, 1, R, K, ldx, 0}, ms = {scales, 1, E * parts, N, N, 0};
+    if ((rc = readable(mx, ws, workspace_bytes, st)) != ELA_OK || (rc = readable(ms, ws, workspace_bytes, st)) != ELA_OK) return rc;
+    MmaParams4 p = {};
+    static_cast<MmaParams&>(p) = row_pass(offsets, R, E, N, K, true);
     p.bias = bias;
-    p.packed = (const uint32_t*)packed;
-    p.scales = scales;
-    p.words = words;
     p.parts = parts;
     p.shift = shift;
     p.residual = residual;
     p.ldr = ldr;
     p.out = y;
     p.vec = N % 2 == 0 && aligned4(y) && (!residual || (aligned4(residual) && ldr % 2 == 0));
-    CUtensorMap b;
-    if (!map_of(&b, dtype, mx, MMA_KB, p.bbox, false)) return ELA_ERR_CUDA;
-    ELA_BY_TYPE(dtype, { ELA_BY_ACT(activation, rc = (mma_launch<PASS_4BIT, T_, A_>(b, b, p, row_tiles(p), st))) })
+    CUtensorMap a, b;
+    if (!make_words_map(&a, packed, words, N, E) || !map_of(&b, dtype, mx, MMA_KB, p.bbox, false) ||
+        !make_scales_map(&p.map_scales, ms.p, N, E * parts, ms.ld, 128 / (int)group))
+        return ELA_ERR_CUDA;
+    ELA_BY_TYPE(dtype, { ELA_BY_ACT(activation, rc = (mma_launch<PASS_4BIT, T_, A_>(a, b, p, row_tiles(p), st))) })
     return rc;
 }
 

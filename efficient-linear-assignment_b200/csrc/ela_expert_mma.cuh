@@ -72,7 +72,7 @@ constexpr int MMA_MAX_STAGES = 10;
 constexpr int MMA_THREADS = 128 + MMA_GROUPS * 128;
 constexpr int MMA_SMEM = 227 * 1024;
 constexpr int MMA_SMEM_FIXED = 1024;    // alignment of the first stage
-constexpr int MMA_UNPACK = 8;            // warps that unpack 4-bit weights
+constexpr int MMA_UNPACK = 12;           // warps that unpack 4-bit weights
 constexpr int MMA_TILES = 4;            // tiles the scheduling warp is ahead
 constexpr int MMA_GROUP = 16;           // column tiles walked together, for L2 reuse of both operands
 
@@ -87,9 +87,7 @@ struct MmaParams {
     const void* x;          // forward with z: the operands again, for exact_z
     const void* weight;
     int64_t ldr, ldx, ldw, stride_e;
-    const uint32_t* packed; // 4-bit weights: rows of words, groups of a row, log2 of a group's inputs
-    const void* scales;
-    int words, parts, shift;
+    int parts, shift, ring; // 4-bit weights: groups of a row, log2 of a group's inputs, blocks of words in flight
     void* out;
     void* z;
     unsigned long long wait_ns;
@@ -151,10 +149,11 @@ __device__ __forceinline__ bool bar_wait(uint64_t* b, uint32_t parity, unsigned 
     }
 }
 // bar: shared::cluster address; it may be the pair's other CTA's.
-__device__ __forceinline__ void tma_2d(void* dst, const CUtensorMap* map, int x, int y, uint32_t bar) {
+__device__ __forceinline__ void tma_2d(uint32_t dst, const CUtensorMap* map, int x, int y, uint32_t bar) {
     asm volatile("cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];"
-                 ::"r"(saddr(dst)), "l"(map), "r"(bar), "r"(x), "r"(y) : "memory");
+                 ::"r"(dst), "l"(map), "r"(bar), "r"(x), "r"(y) : "memory");
 }
+__device__ __forceinline__ void tma_2d(void* dst, const CUtensorMap* map, int x, int y, uint32_t bar) { tma_2d(saddr(dst), map, x, y, bar); }
 __device__ __forceinline__ void tma_3d(void* dst, const CUtensorMap* map, int x, int y, int z, uint32_t bar) {
     asm volatile("cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];"
                  ::"r"(saddr(dst)), "l"(map), "r"(bar), "r"(x), "r"(y), "r"(z) : "memory");
@@ -279,7 +278,7 @@ template <> __device__ __forceinline__ float2 unpack2<__nv_bfloat16>(uint32_t p)
 // lane's residual words are those of swap_pair's layout (loaded by load_residual).
 // Addresses go from pair to pair of columns by one 64-bit addition: written as a product
 // with j they made most of the epilogue's instructions.
-template <typename T, int ACT, bool BIAS, bool Z, bool RES, bool ALL>
+template <typename T, int ACT, bool BIAS, bool Z, bool RES, bool ALL, bool LEAN>
 __device__ __forceinline__ void finish(float* v, float bias, const uint32_t* res, const MmaParams& p, int64_t c, int f, int left) {
     const bool odd = threadIdx.x & 1;
     const uint32_t order = odd ? 0x3276 : 0x5410;
@@ -305,8 +304,8 @@ __device__ __forceinline__ void finish(float* v, float bias, const uint32_t* res
                 }
                 zout += step * (sizeof(K) / 2);
             }
-            a = act_value<ACT>(a);
-            b = act_value<ACT>(b);
+            a = LEAN ? act_value_lean<ACT>(a) : act_value<ACT>(a);
+            b = LEAN ? act_value_lean<ACT>(b) : act_value<ACT>(b);
             if (RES) {
                 const float2 r = unpack2<T>(swap_pair(res[j / 2], order));
                 a += r.x;
@@ -325,7 +324,7 @@ __device__ __forceinline__ void finish(float* v, float bias, const uint32_t* res
                 typedef typename Kept<T, ACT>::Type K;
                 if (Z) reinterpret_cast<K*>(p.z)[at] = El<K>::from(ACT == ELA_ACT_RELU ? sign_kept<T>(a) : a);
                 const float r = RES ? El<T>::to(reinterpret_cast<const T*>(p.residual)[(c + j) * p.ldr + f]) : 0.f;
-                reinterpret_cast<T*>(p.out)[at] = El<T>::from(act_value<ACT>(a) + r);
+                reinterpret_cast<T*>(p.out)[at] = El<T>::from((LEAN ? act_value_lean<ACT>(a) : act_value<ACT>(a)) + r);
             }
     }
 }
@@ -481,77 +480,229 @@ __device__ __forceinline__ void load_residual(uint32_t* res, const MmaParams& p,
 }
 
 // ------------------------------------------------------------- 4-bit weights
-// Eight warps of each CTA write the weights' stages instead of TMA: four of them every other
-// stage, a thread one feature's 64 inputs, 32 bytes of words that come as eight 16-byte pieces of
-// the swizzled row (eight neighbouring lanes write eight different pieces: all banks once).
-// The words are loaded UNPACK_AHEAD of the warp's own stages before they are needed, across tiles.
-// A stage is handed over by an arrival at the first CTA's barrier after the fence that makes
-// the writes visible to the tensor core of this SM, which alone reads them.
-constexpr int UNPACK_AHEAD = 2;
+// The pass with 4-bit weights has roles of its own for the operands, and stages of 128 inputs:
+// a wait, a TMA instruction or a commit takes its thread some 100 cycles each, and with stages
+// of 64 the thread that loads was what all others waited for (700 cycles a stage).  Warp 0 loads
+// the columns, warp 2 the words, by TMA into a ring of their own, blocks of 128 features by 128
+// inputs with the scales of their groups.  Twelve warps unpack the blocks into the stages, half a
+// stage (64 inputs) by four of them in turn: a thread one feature's 64 inputs, which are eight
+// 16-byte pieces of the swizzled row (eight neighbouring lanes write eight different pieces: all
+// banks once).  A half is handed over by an arrival at the first CTA's barrier after the fence
+// that makes the writes visible to the tensor core of this SM, which alone reads them.  (The
+// fence waits for the thread's loads from memory, too: with the words loaded into registers
+// ahead, however far, 64 inputs took 900 cycles.)
+constexpr int PACK_KB = 2 * MMA_KB;  // inputs of a stage, and of a block of words
+constexpr int PACK_WORDS = MMA_F * PACK_KB / 2, PACK_BLOCK = PACK_WORDS + 1024;  // bytes of a block's words; with its scales
+constexpr int PACK_MAX_RING = 8;
+constexpr int PACK_TURNS = MMA_UNPACK / 4;  // groups of four warps
+struct MmaParams4 : MmaParams {
+    CUtensorMap map_scales;
+};
+template <int PASS> struct ParamsOf { typedef MmaParams Type; };
+template <> struct ParamsOf<PASS_4BIT> { typedef MmaParams4 Type; };
+
+// bar_wait by a whole warp that stays together: 70 cycles where nothing is to be waited for.
+// (bar_wait by all lanes takes 130, by one lane that then tells the others 290.)
+__device__ __forceinline__ bool bar_wait_warp(uint64_t* b, uint32_t parity, unsigned long long limit_ns, const volatile int* abort) {
+    const uint32_t a = saddr(b);
+    unsigned long long t0 = 0;
+    for (uint32_t spins = 1;; ++spins) {
+        uint32_t done;
+        asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+                     : "=r"(done) : "r"(a), "r"(parity), "r"(20000) : "memory");
+        if (__all_sync(~0u, done)) return true;
+        if ((spins & 15u) == 0) {
+            unsigned long long t;
+            asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));
+            if (t0 == 0) t0 = t;
+            if (__any_sync(~0u, *abort || t - t0 > limit_ns)) return false;
+        }
+    }
+}
+// An arrival at a barrier of the pair's first CTA.
 __device__ __forceinline__ void bar_arrive_leader(uint32_t addr) {
     asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(addr) : "memory");
 }
-template <typename T, typename Fetch, typename GiveUp>
-__device__ __forceinline__ void unpack_stages(const MmaParams& p, unsigned char* smem, int stage_bytes, uint64_t* full, uint64_t* empty, int rank,
-                                              Fetch fetch, GiveUp give_up, const volatile int* abort) {
-    struct Words { uint4 v[2]; uint32_t s[2]; };
-    const int lane = threadIdx.x & 31, w = (threadIdx.x >> 5) - 4 - 4 * MMA_GROUPS, odd = w >> 2;
-    const int row = (w & 3) * 32 + lane;
-    const int blocks = (p.K + MMA_KB - 1) / MMA_KB;
-    Tile t = {};
-    int tile = -1, kb = odd - blocks;  // of the next load; the tile's number among the pair's
-    bool ok = true, more = true;
-    const uint32_t* words = nullptr;
-    const uint16_t* scales = nullptr;
-    auto load = [&](Words& q) {  // false: no stage left
-        while (more && (tile < 0 || kb >= blocks)) {
-            kb = tile < 0 ? odd : kb - blocks;
-            more = fetch(++tile, t, ok);
-            const int f = min(t.f0 + rank * MMA_F + row, p.F - 1);
-            words = p.packed + ((int64_t)t.e * p.F + f) * p.words;
-            scales = reinterpret_cast<const uint16_t*>(p.scales) + (int64_t)t.e * p.parts * p.F + f;
-        }
-        if (!more) return false;
-        const int k = kb * MMA_KB;
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            asm volatile("ld.global.L1::no_allocate.L2::256B.v4.b32 {%0,%1,%2,%3}, [%4];"
-                : "=r"(q.v[h].x), "=r"(q.v[h].y), "=r"(q.v[h].z), "=r"(q.v[h].w) : "l"(words + k / 8 + 4 * h) : "memory");
-            q.s[h] = scales[(int64_t)min((k + 32 * h) >> p.shift, p.parts - 1) * p.F];
-        }
-        kb += 2;
-        return true;
-    };
-    Words q[UNPACK_AHEAD];
-    bool have[UNPACK_AHEAD];
-#pragma unroll
-    for (int i = 0; i < UNPACK_AHEAD; ++i) have[i] = load(q[i]);
-    int s = odd;
+__device__ __forceinline__ void tma_words(uint32_t dst, const CUtensorMap* map, int x, int y, int z, uint32_t bar) {
+    asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];"
+                 ::"r"(dst), "l"(map), "r"(bar), "r"(x), "r"(y), "r"(z) : "memory");
+}
+__device__ __forceinline__ void tma_scales(uint32_t dst, const CUtensorMap* map, int x, int y, uint32_t bar) {
+    asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];"
+                 ::"r"(dst), "l"(map), "r"(bar), "r"(x), "r"(y) : "memory");
+}
+
+// The place in a ring and the parity of its phase.
+struct Place {
+    int at = 0;
     uint32_t phase = 0;
-    for (;;) {
-#pragma unroll
-        for (int i = 0; i < UNPACK_AHEAD; ++i) {
-            if (!have[i] || !ok) return;
-            int good = 0;
-            if (lane == 0) good = bar_wait(&empty[s], phase ^ 1, p.wait_ns, abort);
-            if (!__shfl_sync(~0u, good, 0)) {
-                if (lane == 0) give_up();
-                return;
+    __device__ __forceinline__ void advance(int by, int size) {  // by at most size
+        if ((at += by) >= size) { at -= size; phase ^= 1; }
+    }
+    // from the elected lane to all (elect_one names the same lane again)
+    __device__ __forceinline__ void share(bool& ok) {
+        const int who = __ffs(__ballot_sync(~0u, elect_one())) - 1;
+        ok = __shfl_sync(~0u, (int)ok, who);
+        at = __shfl_sync(~0u, at, who);
+        phase = __shfl_sync(~0u, phase, who);
+        __syncwarp();
+    }
+};
+
+// One warp: the stages' columns, this CTA's half of them.
+template <typename Fetch, typename GiveUp>
+__device__ __forceinline__ void load_columns(const MmaParams4& p, const CUtensorMap& map, uint32_t stages, int stage_bytes, uint64_t* full, uint64_t* empty,
+                                             int rank, Fetch fetch, GiveUp give_up, const volatile int* abort) {
+    Tile t;
+    bool ok = true;
+    Place s;
+    const uint32_t ready = leader_addr(full), part = p.bn / 2 * MMA_KB * 2, box_bytes = p.bbox * MMA_KB * 2;
+    for (int i = 0; ok && fetch(i, t, ok); ++i) {
+        const int half = ((t.nc + 31) & ~31) >> 1, c0 = t.c0 + rank * half, boxes = (half + p.bbox - 1) / p.bbox;
+        if (elect_one()) {
+            for (int k = 0; k < p.K; k += PACK_KB) {
+                ok = bar_wait(&empty[s.at], s.phase ^ 1, p.wait_ns, abort);
+                if (!ok) break;
+                const bool two = k + MMA_KB < p.K;
+                if (rank == 0) bar_expect(&full[s.at], (two ? 4 : 2) * boxes * box_bytes);  // the pair's
+                uint32_t to = stages + s.at * stage_bytes + 2 * MMA_A_BYTES;
+                for (int b = 0; b < boxes; ++b, to += box_bytes) {
+                    tma_2d(to, &map, k, c0 + b * p.bbox, ready + 8 * s.at);
+                    if (two) tma_2d(to + part, &map, k + MMA_KB, c0 + b * p.bbox, ready + 8 * s.at);
+                }
+                s.advance(1, p.stages);
             }
-            unsigned char* to = smem + (size_t)s * stage_bytes + row * 128;
+            if (!ok) give_up();
+        }
+        s.share(ok);
+    }
+}
+
+// One warp: the blocks of this CTA's features, in the order of the stages.
+template <typename Fetch, typename GiveUp>
+__device__ __forceinline__ void load_words(const MmaParams4& p, const CUtensorMap& map, uint32_t ring, uint64_t* pfull, uint64_t* pempty, int rank,
+                                           Fetch fetch, GiveUp give_up, const volatile int* abort) {
+    Tile t;
+    bool ok = true;
+    Place s;
+    const uint32_t bytes = PACK_WORDS + (2 * MMA_F << (7 - p.shift));
+    for (int i = 0; ok && fetch(i, t, ok); ++i) {
+        const int f0 = t.f0 + rank * MMA_F;
+        if (elect_one()) {
+            for (int k = 0; k < p.K; k += PACK_KB) {
+                ok = bar_wait(&pempty[s.at], s.phase ^ 1, p.wait_ns, abort);
+                if (!ok) break;
+                bar_expect(&pfull[s.at], bytes);
+                const uint32_t to = ring + s.at * PACK_BLOCK, bar = saddr(&pfull[s.at]);
+                tma_words(to, &map, k / 8, f0, t.e, bar);
+                tma_scales(to + PACK_WORDS, &p.map_scales, f0, t.e * p.parts + (k >> p.shift), bar);
+                s.advance(1, p.ring);
+            }
+            if (!ok) give_up();
+        }
+        s.share(ok);
+    }
+}
+
+// One warp of the first CTA: the products of the pair.
+template <typename T, typename Fetch, typename GiveUp>
+__device__ __forceinline__ void issue_products(const MmaParams4& p, uint32_t stages, int stage_bytes, uint32_t tmem, uint64_t* full, uint64_t* empty,
+                                               uint64_t* tfull, uint64_t* tempty, Fetch fetch, GiveUp give_up, const volatile int* abort) {
+    Tile t;
+    bool ok = true;
+    Place s;
+    const uint64_t a0 = operand_desc(stages, true), b0 = operand_desc(stages + 2 * MMA_A_BYTES, true);
+    const uint32_t a_half = MMA_A_BYTES >> 4, b_half = p.bn / 2 * MMA_KB * 2 >> 4;
+    for (int i = 0; ok && fetch(i, t, ok); ++i) {
+        if (elect_one()) {
+            const int half = i & 1;
+            const uint32_t d = tmem + half * MMA_C, idesc = instr_desc<T>((t.nc + 31) & ~31, true, true);
+            ok = bar_wait(&tempty[half], ((i >> 1) & 1) ^ 1, p.wait_ns, abort);
+            fence_after();
+            for (int k = 0; k < p.K && ok; k += PACK_KB) {
+                ok = bar_wait(&full[s.at], s.phase, p.wait_ns, abort);
+                if (!ok) break;
+                fence_after();
+                const uint64_t off = (uint32_t)(s.at * stage_bytes) >> 4;
+                const int steps = min((p.K - k + 15) >> 4, PACK_KB / 16);
+                if (steps == PACK_KB / 16) {
+#pragma unroll
+                    for (int j = 0; j < PACK_KB / 16; ++j)
+                        mma_issue(d, a0 + off + (j >> 2) * a_half + (j & 3) * 2, b0 + off + (j >> 2) * b_half + (j & 3) * 2, idesc, k + j > 0);
+                } else {
+                    for (int j = 0; j < steps; ++j)
+                        mma_issue(d, a0 + off + (j >> 2) * a_half + (j & 3) * 2, b0 + off + (j >> 2) * b_half + (j & 3) * 2, idesc, k + j > 0);
+                }
+                mma_commit(&empty[s.at]);
+                s.advance(1, p.stages);
+            }
+            if (ok) mma_commit(&tfull[half]);
+            else give_up();
+        }
+        s.share(ok);
+    }
+}
+
+// Twelve warps: the halves of the stages of `tiles` tiles, in turn.  A half that the last stage
+// of a tile does not have is handed over as it is.  Four warps see two of three blocks; the
+// ring's size is a multiple of three, so that a slot is theirs every time or never, and no phase
+// of its barrier passes unseen.  (A stage's barrier may skip one: products end in order.)
+template <typename T, typename GiveUp>
+__device__ __forceinline__ void unpack_stages(const MmaParams4& p, uint32_t stages, int stage_bytes, uint32_t ring, uint64_t* full, uint64_t* empty,
+                                              uint64_t* pfull, uint64_t* pempty, int tiles, GiveUp give_up, const volatile int* abort) {
+    const int lane = threadIdx.x & 31, w = __shfl_sync(~0u, (threadIdx.x >> 5) - 4 - 4 * MMA_GROUPS, 0), row = (w & 3) * 32 + lane;
+    uint32_t at[8];  // where a piece goes in half a stage
+#pragma unroll
+    for (int j = 0; j < 8; ++j) at[j] = row * 128 + ((j ^ (row & 7)) << 4);
+    const uint32_t ready = leader_addr(full), second = p.shift == 5 ? 2 * MMA_F : 0;
+    const int blocks = (p.K + PACK_KB - 1) / PACK_KB, all = (p.K + MMA_KB - 1) / MMA_KB;
+    const int64_t count = 2 * (int64_t)tiles * blocks;
+    Place s, slot;
+    int kb = 0;  // the block's number in its tile
+    auto next_block = [&]() {
+        s.advance(1, p.stages);
+        slot.advance(1, p.ring);
+        if (++kb == blocks) kb = 0;
+    };
+    if (w >= 8) next_block();
+    for (int64_t n = w >> 2; n < count; n += PACK_TURNS) {
+        const int h = (int)(n & 1);
+        const bool there = 2 * kb + h < all;
+        uint32_t q[8];
+        uint16_t sc[2];
+        bool ok = bar_wait_warp(&pfull[slot.at], slot.phase, p.wait_ns, abort);
+        if (ok) {
+            // the row's 32 bytes of this half of a block (64-byte swizzle), and its groups' scales
+            const uint32_t from = ring + slot.at * PACK_BLOCK, words = from + row * 64 + ((2 * h ^ (row >> 1 & 3)) << 4);
+            const uint32_t scales = from + PACK_WORDS + row * 2 + (h * MMA_KB >> p.shift) * 2 * MMA_F;
+            asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];" : "=r"(q[0]), "=r"(q[1]), "=r"(q[2]), "=r"(q[3]) : "r"(words) : "memory");
+            asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];" : "=r"(q[4]), "=r"(q[5]), "=r"(q[6]), "=r"(q[7]) : "r"(words ^ 16) : "memory");
+            asm volatile("ld.shared.u16 %0, [%1];" : "=h"(sc[0]) : "r"(scales) : "memory");
+            asm volatile("ld.shared.u16 %0, [%1];" : "=h"(sc[1]) : "r"(scales + second) : "memory");
+            ok = bar_wait_warp(&empty[s.at], s.phase ^ 1, p.wait_ns, abort);
+        }
+        if (!ok) {
+            if (lane == 0) give_up();
+            return;
+        }
+        if (there) {
+            const uint32_t to = stages + s.at * stage_bytes + h * MMA_A_BYTES;
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
-                const uint4& v = q[i].v[j / 4];
                 uint32_t out[4];
-                unpack<T>(j % 4 == 0 ? v.x : j % 4 == 1 ? v.y : j % 4 == 2 ? v.z : v.w, q[i].s[j / 4] * 0x10001u, out);
-                *reinterpret_cast<uint4*>(to + ((j ^ (row & 7)) << 4)) = make_uint4(out[0], out[1], out[2], out[3]);
+                unpack<T>(q[j], sc[j / 4] * 0x10001u, out);
+                asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(to + at[j]), "r"(out[0]), "r"(out[1]), "r"(out[2]), "r"(out[3]) : "memory");
             }
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-            __syncwarp();
-            if (lane == 0) bar_arrive_leader(leader_addr(&full[s]));
-            if ((s += 2) >= p.stages) { s -= p.stages; phase ^= 1; }
-            have[i] = load(q[i]);
         }
+        __syncwarp();
+        if (lane == 0) {
+            bar_arrive_leader(ready + 8 * s.at);
+            bar_arrive(&pempty[slot.at]);
+        }
+        __syncwarp();
+        next_block();
+        if (h) next_block();
     }
 }
 
@@ -562,12 +713,13 @@ template <int PASS> constexpr int mma_threads() { return MMA_THREADS + (PASS == 
 template <int PASS, typename T, int ACT, bool Z>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(mma_threads<PASS>(), 1)
     mma_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
-               const __grid_constant__ MmaParams p) {
+               const __grid_constant__ typename ParamsOf<PASS>::Type p) {
     constexpr bool PACKED = PASS == PASS_4BIT, FWD = PASS == PASS_FORWARD || PACKED;
     constexpr bool A_K_MAJOR = FWD, B_K_MAJOR = PASS != PASS_WEIGHT;
     extern __shared__ unsigned char smem_raw[];
     // full, tempty, patched: the first CTA's are used; empty, tfull, landed: each CTA its own
     __shared__ __align__(8) uint64_t full[MMA_MAX_STAGES], empty[MMA_MAX_STAGES], tfull[2], tempty[2], sfull[MMA_TILES], sempty[MMA_TILES], patched[MMA_MAX_STAGES], landed, drained;
+    __shared__ __align__(8) uint64_t pfull[PACKED ? PACK_MAX_RING : 1], pempty[PACKED ? PACK_MAX_RING : 1];  // each CTA its own
     __shared__ uint32_t s_tmem;
     __shared__ int s_abort;
     __shared__ uint32_t s_issued;
@@ -580,12 +732,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(mma_threads<PASS>(),
     // the experts' tables, then the stages, each on a 1024-byte boundary
     int* table = reinterpret_cast<int*>(smem_raw);
     unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(table + 3 * p.E) + 1023) & ~(uintptr_t)1023);
-    const int stage_bytes = MMA_A_BYTES + p.bn / 2 * MMA_KB * 2;
+    const int stage_bytes = (MMA_A_BYTES + p.bn / 2 * MMA_KB * 2) * (PACKED ? 2 : 1);
+    const uint32_t ring = saddr(smem) + p.stages * stage_bytes;
     const volatile int* abort = &s_abort;
 
     next_may_start();
     if (tid == 32) {
-        if (!PACKED) asm volatile("prefetch.tensormap [%0];" ::"l"(&map_a) : "memory");
+        asm volatile("prefetch.tensormap [%0];" ::"l"(&map_a) : "memory");
         asm volatile("prefetch.tensormap [%0];" ::"l"(&map_b) : "memory");
     }
     if (warp == 2) {
@@ -594,10 +747,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(mma_threads<PASS>(),
     }
     if (tid == 0) {
         s_abort = 0;
-        // full: the loads of the pair, and the weights of a stage that four warps of each CTA have unpacked
-        for (int s = 0; s < p.stages; ++s) { bar_init(&full[s], 1 + (PACKED ? MMA_UNPACK : 0)); bar_init(&empty[s], 1); }
+        // full: the loads of the pair, and the two halves of the weights that four warps of each CTA unpack
+        for (int s = 0; s < p.stages; ++s) { bar_init(&full[s], 1 + (PACKED ? 16 : 0)); bar_init(&empty[s], 1); }
         for (int b = 0; b < 2; ++b) { bar_init(&tfull[b], 1); bar_init(&tempty[b], 2 * 4 * MMA_GROUPS); }
-        for (int i = 0; i < MMA_TILES; ++i) { bar_init(&sfull[i], 1); bar_init(&sempty[i], 4 * MMA_GROUPS + 1 + (rank == 0) + (PACKED ? MMA_UNPACK : 0)); }
+        for (int i = 0; i < MMA_TILES; ++i) { bar_init(&sfull[i], 1); bar_init(&sempty[i], 4 * MMA_GROUPS + 1 + (rank == 0) + PACKED); }
+        if constexpr (PACKED)
+            for (int s = 0; s < p.ring; ++s) { bar_init(&pfull[s], 1); bar_init(&pempty[s], 8); }
         bar_init(&landed, 1);
         for (int s = 0; s < p.stages; ++s) bar_init(&patched[s], 1);
         bar_init(&drained, 1);
@@ -650,6 +805,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(mma_threads<PASS>(),
         return t.e >= 0;
     };
 
+    // registers from the warps that need few to those of the epilogue (a block of 768 threads has 80 each:
+    // 128 * (64 + 2 * 112 + 3 * 64) of them)
+    if constexpr (PACKED) {
+        if (warp < 4) asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
+        else if (warp < 4 + 4 * MMA_GROUPS) asm volatile("setmaxnreg.inc.sync.aligned.u32 112;");
+        else asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
+    }
     uint32_t issued = 0;  // stages loaded (by the loading lane)
     if (warp == 3) {  // ---- tiles, a few ahead: their index arithmetic would cost each role 1000 cycles a tile
         bool ok = true, left = true;
@@ -670,6 +832,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(mma_threads<PASS>(),
             }
             ok = __shfl_sync(~0u, good, 0);
         }
+    } else if (PACKED && warp == 0) {  // ---- loads of this CTA's half of the columns
+        if constexpr (PACKED) load_columns(p, map_b, saddr(smem), stage_bytes, full, empty, rank, fetch, give_up, abort);
+    } else if (PACKED && warp == 1) {  // ---- products of the pair
+        if constexpr (PACKED)
+            if (rank == 0) issue_products<T>(p, saddr(smem), stage_bytes, tmem, full, empty, tfull, tempty, fetch, give_up, abort);
+    } else if (PACKED && warp == 2) {  // ---- loads of the words
+        if constexpr (PACKED) load_words(p, map_a, ring, pfull, pempty, rank, fetch, give_up, abort);
     } else if (warp == 0) {  // ---- loads of this CTA's features and its half of the columns
         Tile t;
         int s = 0;
@@ -681,7 +850,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(mma_threads<PASS>(),
             const int half = ((t.nc + 31) & ~31) >> 1, c0 = t.c0 + rank * half;
             const int boxes = B_K_MAJOR ? (half + p.bbox - 1) / p.bbox : (half + 63) / 64;
             const int box_bytes = B_K_MAJOR ? p.bbox * MMA_KB * 2 : 64 * MMA_KB * 2;
-            const uint32_t bytes = (PACKED ? 0 : MMA_A_BYTES) + boxes * box_bytes;
+            const uint32_t bytes = MMA_A_BYTES + boxes * box_bytes;
             // Rows of the next expert in the last block of a sum over rows: that block's
             // loads land on a barrier of this CTA, the rows are zeroed, then the stage is full.
             const int tail = PASS == PASS_WEIGHT ? t.nk % MMA_KB : 0, blocks = (t.nk + MMA_KB - 1) / MMA_KB;
@@ -691,7 +860,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(mma_threads<PASS>(),
                 unsigned char* b = a + MMA_A_BYTES;
                 if (PASS == PASS_FORWARD) {
                     tma_3d(a, &map_a, k, f0, t.e, bar);
-                } else if (!PACKED) {
+                } else {
                     for (int h = 0; h < 2; ++h)
                         if (PASS == PASS_INPUT) tma_3d(a + h * 8192, &map_a, f0 + h * 64, k, t.e, bar);
                         else tma_2d(a + h * 8192, &map_a, f0 + h * 64, k, bar);
@@ -823,7 +992,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(mma_threads<PASS>(),
             }
         }
     } else if (PACKED && warp >= 4 + 4 * MMA_GROUPS) {  // ---- weights out of 4 bits
-        if constexpr (PACKED) unpack_stages<T>(p, smem, stage_bytes, full, empty, rank, fetch, give_up, abort);
+        const int mine = plan.tiles > pair ? (plan.tiles - pair - 1) / pairs + 1 : 0;
+        if constexpr (PACKED) unpack_stages<T>(p, saddr(smem), stage_bytes, ring, full, empty, pfull, pempty, mine, give_up, abort);
     } else if (warp >= 4) {  // ---- epilogue
         const int w = warp & 3, group = (warp - 4) >> 2;
         if constexpr (PASS != PASS_WEIGHT) {  // rows of no expert: the residual, or 0
@@ -854,8 +1024,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(mma_threads<PASS>(),
         };
         auto write = [&](float* v, float bias, const uint32_t* res, int64_t c, int f, int left) {
             if constexpr (Z) {
-                if (with_res) finish<T, ACT, FWD, true, FWD, false>(v, bias, res, p, c, f, left);
-                else finish<T, ACT, FWD, true, false, false>(v, bias, res, p, c, f, left);
+                if (with_res) finish<T, ACT, FWD, true, FWD, false, PACKED>(v, bias, res, p, c, f, left);
+                else finish<T, ACT, FWD, true, false, false, PACKED>(v, bias, res, p, c, f, left);
                 if constexpr (SIGNS)
                     if (may_be_near_zero<T>(v, bias, p, f, left)) {
                         unsigned near, zero;
@@ -863,9 +1033,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(mma_threads<PASS>(),
                         if (__any_sync(~0u, near != 0)) settle_signs<T>(near, zero, p, s_near, warp - 4, t.e, (int)c, f, left);
                     }
             } else {
-                if (with_res) finish<T, ACT, FWD, false, FWD, false>(v, bias, res, p, c, f, left);
-                else if (p.vec && left >= MMA_CHUNK && (f | 31) < p.F) finish<T, ACT, FWD, false, false, true>(v, bias, res, p, c, f, left);
-                else finish<T, ACT, FWD, false, false, false>(v, bias, res, p, c, f, left);
+                if (with_res) finish<T, ACT, FWD, false, FWD, false, PACKED>(v, bias, res, p, c, f, left);
+                else if (p.vec && left >= MMA_CHUNK && (f | 31) < p.F) finish<T, ACT, FWD, false, false, true, PACKED>(v, bias, res, p, c, f, left);
+                else finish<T, ACT, FWD, false, false, false, PACKED>(v, bias, res, p, c, f, left);
             }
         };
         for (int i = 0; ok && fetch(i, t, ok); ++i) {
@@ -946,6 +1116,25 @@ inline PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
     return fn;
 }
 
+// Blocks of a packed weight (E, N, words): 16 words by 128 rows, 64-byte swizzle.
+inline bool make_words_map(CUtensorMap* map, const void* packed, int64_t words, int64_t N, int64_t E) {
+    const auto fn = encode_fn();
+    if (!fn) return false;
+    const cuuint64_t dims[3] = {(cuuint64_t)words, (cuuint64_t)N, (cuuint64_t)E}, strides[2] = {(cuuint64_t)words * 4, (cuuint64_t)(words * N) * 4};
+    const cuuint32_t box[3] = {2 * MMA_KB / 8, MMA_F, 1}, step[3] = {1, 1, 1};
+    return fn(map, CU_TENSOR_MAP_DATA_TYPE_INT32, 3, const_cast<void*>(packed), dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE,
+              CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+// Their scales, rows of N 16-bit values ld apart: 128 by as many rows as 128 inputs have groups.
+inline bool make_scales_map(CUtensorMap* map, const void* scales, int64_t N, int64_t rows, int64_t ld, int box_rows) {
+    const auto fn = encode_fn();
+    if (!fn) return false;
+    const cuuint64_t dims[2] = {(cuuint64_t)N, (cuuint64_t)rows}, strides[1] = {(cuuint64_t)ld * 2};
+    const cuuint32_t box[2] = {MMA_F, (cuuint32_t)box_rows}, step[2] = {1, 1};
+    return fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT16, 2, const_cast<void*>(scales), dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE,
+              CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 // A (d2, d1, d0) tensor of 16-bit elements, strides s1 and s2 in elements, read in
 // boxes of b0 x b1 with 128-byte swizzle; what lies outside reads as 0.
 inline bool make_map(CUtensorMap* map, int dtype, const void* base, int64_t d0, int64_t d1, int64_t d2, int64_t s1,
@@ -961,7 +1150,7 @@ inline bool make_map(CUtensorMap* map, int dtype, const void* base, int64_t d0, 
 }
 
 template <int PASS, typename T, int ACT, bool Z = false>
-int mma_launch(const CUtensorMap& a, const CUtensorMap& b, const MmaParams& p, int64_t max_tiles, cudaStream_t st) {
+int mma_launch(const CUtensorMap& a, const CUtensorMap& b, const typename ParamsOf<PASS>::Type& p, int64_t max_tiles, cudaStream_t st) {
     auto kern = mma_kernel<PASS, T, ACT, Z>;
     const int sms = sm_count();
     if (sms == 0 || !allow_smem<&mma_kernel<PASS, T, ACT, Z>>(MMA_SMEM - 1024)) return ELA_ERR_CUDA;
@@ -990,8 +1179,8 @@ inline int columns_per_tile(int64_t R, int64_t E, int64_t f_tiles, int64_t k_blo
     }
     return best;
 }
-inline int stages_for(int bn, int64_t E) {
-    const int64_t n = (MMA_SMEM - 1024 - MMA_SMEM_FIXED - 12 * E) / (MMA_A_BYTES + bn / 2 * MMA_KB * 2);
+inline int stages_for(int bn, int64_t E, int ring = 0) {
+    const int64_t n = (MMA_SMEM - 1024 - MMA_SMEM_FIXED - 12 * E - ring * PACK_BLOCK) / ((MMA_A_BYTES + bn / 2 * MMA_KB * 2) * (ring ? 2 : 1));
     return (int)(n < MMA_MAX_STAGES ? n : MMA_MAX_STAGES);
 }
 
@@ -1084,7 +1273,8 @@ inline MmaParams row_pass(const int32_t* offsets, int64_t R, int64_t E, int64_t 
     // a CTA's half of a tile's columns is one box, or boxes of 64 where experts have fewer rows
     // than that makes (a box is loaded whole)
     p.bbox = p.bn % 128 == 0 && R < 256 * E ? 64 : p.bn / 2;
-    p.stages = stages_for(p.bn, E);
+    p.ring = packed ? p.bn > 64 ? PACK_TURNS : 2 * PACK_TURNS : 0;
+    p.stages = stages_for(p.bn, E, p.ring);
     p.wait_ns = wait_limit(K);
     return p;
 }

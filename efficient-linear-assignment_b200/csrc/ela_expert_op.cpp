@@ -362,7 +362,7 @@ std::tuple<Tensor, Tensor> quantize_raw(const Tensor& weight, int64_t group) {
     return {packed, scales};
 }
 
-// Packed rows and scales that belong together; contiguous, the words on 16 bytes.
+// Packed rows and scales that belong together; contiguous, the words on 32 bytes.
 struct Packed {
     int64_t E, N, K;
     Tensor words, scales;
@@ -378,7 +378,7 @@ Packed packed_of(const char* name, const Tensor& packed, const Tensor& scales, i
                           (one || (scales.size(0) == packed.size(0) && packed.size(0) <= ELA_EXPERT_MAX)) && scales.device() == packed.device(),
                       name, ": packed (E, N, 8 ceil(K/64)) and scales (E, ceil(K/group), N), or both without E, on one device");
     Packed p = {one ? 1 : packed.size(0), packed.size(-2), K, packed.contiguous(), scales.contiguous()};
-    if (reinterpret_cast<uintptr_t>(p.words.data_ptr()) % 16) p.words = p.words.clone();
+    if (reinterpret_cast<uintptr_t>(p.words.data_ptr()) % 32) p.words = p.words.clone();
     return p;
 }
 
@@ -424,7 +424,7 @@ Tensor linear_4bit_raw(const Tensor& x_in, const Tensor& packed, const Tensor& s
     const OptTensor b = bias.has_value() ? OptTensor(bias->contiguous()) : OptTensor();
     const OptTensor r = residual.has_value() ? OptTensor(rows_of(*residual)) : OptTensor();
     Tensor y = fresh({R, p.N}, x);
-    const size_t bytes = ela_expert_linear_4bit_workspace_bytes(R, p.E, K, p.N, aligned(x, ld(x)));
+    const size_t bytes = ela_expert_linear_4bit_workspace_bytes(R, p.E, K, p.N, group, aligned(x, ld(x)) && aligned(p.scales, 0));
     Tensor ws = workspace(bytes, x);
     check_rc(ela_expert_linear_4bit(x.data_ptr(), p.words.data_ptr<int32_t>(), p.scales.data_ptr(), ptr(b), ptr(r),
                                     off_ptr(offsets), code_of(x), R, p.E, K, p.N, group, ld(x), r.has_value() ? ld(*r) : 0, (int)act, y.data_ptr(),

@@ -166,7 +166,7 @@ int ela_expert_route_grad(const void* logits, int dtype, int64_t T, int64_t E, i
  *           inputs: W = 8 * ceil(K / 64) words.  Input 8 i + j of a row is the four bits of
  *           word i from bit 4 (j / 2) + 16 (j % 2) on, and holds q + 8.
  *   scales: (E, ceil(K / group), N), fp16 or bf16
- * packed lies on 16 bytes.
+ * packed lies on 32 bytes.
  */
 
 /* packed and scales from weight (E,N,K) with expert distance stride_e and row distance ldw:
@@ -178,8 +178,11 @@ int ela_expert_quantize(const void* weight, int dtype, int64_t E, int64_t K, int
 int ela_expert_dequantize(const int32_t* packed, const void* scales, int dtype, int64_t E, int64_t K, int64_t N,
                           int64_t group, void* weight, void* stream);
 
-/* Bytes of device workspace that ela_expert_linear_4bit needs at these sizes (`aligned`: as above, of x). */
-size_t ela_expert_linear_4bit_workspace_bytes(int64_t R, int64_t E, int64_t K, int64_t N, int aligned);
+/*
+ * Bytes of device workspace that ela_expert_linear_4bit needs at these sizes (`aligned`: x and
+ * scales start on 16-byte boundaries and x has rows a multiple of 16 bytes apart).
+ */
+size_t ela_expert_linear_4bit_workspace_bytes(int64_t R, int64_t E, int64_t K, int64_t N, int64_t group, int aligned);
 
 /*
  * ela_expert_linear with 4-bit weights, packed (E,N,W) and scales (E,ceil(K/group),N)
