@@ -83,19 +83,25 @@ template <int LANES> struct Team {
     template <typename V> static __device__ __forceinline__ V sum(V v) { return reduce(v, [](V a, V b) { return a + b; }); }
     template <typename V> static __device__ __forceinline__ V most(V v) { return reduce(v, [](V a, V b) { return a > b ? a : b; }); }
     template <typename V> static __device__ __forceinline__ V least(V v) { return reduce(v, [](V a, V b) { return a < b ? a : b; }); }
-    // The largest key and the first place that has it.
-    template <typename U> static __device__ __forceinline__ void first_most(U& key, int& at) {
-        auto op = [](U k, int a, U& key, int& at) { if (k > key || (k == key && a < at)) { key = k; at = a; } };
-#pragma unroll
-        for (int o = (WIDE ? 32 : LANES) / 2; o; o >>= 1) op(__shfl_xor_sync(~0u, key, o), __shfl_xor_sync(~0u, at, o), key, at);
+    static __device__ __forceinline__ uint32_t most(uint32_t v) {
+        if constexpr (LANES == 32) return __reduce_max_sync(~0u, v);
+        return reduce(v, [](uint32_t a, uint32_t b) { return a > b ? a : b; });
+    }
+    // True in the first thread of the row in which v is.
+    static __device__ __forceinline__ bool first(bool v) {
+        unsigned has = __ballot_sync(~0u, v);
         if constexpr (WIDE) {
-            __shared__ U keys[LANES / 32];
-            __shared__ int ats[LANES / 32];
+            __shared__ unsigned warps[LANES / 32];
             __syncthreads();
-            if ((threadIdx.x & 31) == 0) { keys[threadIdx.x >> 5] = key; ats[threadIdx.x >> 5] = at; }
+            if ((threadIdx.x & 31) == 0) warps[threadIdx.x >> 5] = has;
             __syncthreads();
-            for (int i = 0; i < LANES / 32; ++i) op(keys[i], ats[i], key, at);
+            for (unsigned i = 0; i < threadIdx.x >> 5; ++i)
+                if (warps[i]) return false;
+        } else if constexpr (LANES < 32) {
+            has = has >> (threadIdx.x & 31 & ~(LANES - 1)) & ((1u << LANES) - 1);
+            return v && (has & ((1u << (threadIdx.x & (LANES - 1))) - 1)) == 0;
         }
+        return v && (has & ((1u << (threadIdx.x & 31)) - 1)) == 0;
     }
 };
 
@@ -119,31 +125,35 @@ template <typename T, int VPT> __device__ __forceinline__ void load_logits(float
     }
 }
 
-// A team's shared memory: the chosen experts and their logits, and with groups the experts'
-// values, the groups' and the groups kept.  (One word in 33 unused: threads that walk groups
+// A team's shared memory: the chosen experts, their logits and keys, and with groups the experts'
+// values (or each thread's two largest), the groups' and the groups kept.  (One word in 33 unused: threads that walk groups
 // of 32 side by side then hit different banks.)
 __host__ __device__ inline int route_slot(int e) { return e + (e >> 5); }
 struct RouteShared {
     int* at;
-    float* logit;
+    float *logit, *key;
     void* value;
     void* group;
     unsigned char* kept;
     static __host__ __device__ inline int bytes(int slots, int k, int groups) {
-        return 8 * ((k + 1) / 2 * 2) + (groups > 1 ? 8 * (route_slot(slots) + 1) + 8 * groups + (groups + 7) / 8 * 8 : 0);
+        return 12 * ((k + 1) / 2 * 2) + (groups > 1 ? 8 * (route_slot(slots) + 1) + 8 * groups + (groups + 7) / 8 * 8 : 0);
     }
     __device__ __forceinline__ RouteShared(unsigned char* p, int slots, int k, int groups) {
         const int even = (k + 1) / 2 * 2;
         at = reinterpret_cast<int*>(p);
         logit = reinterpret_cast<float*>(p + 4 * even);
-        value = p + 8 * even;
-        group = p + 8 * even + 8 * (route_slot(slots) + 1);
-        kept = p + 8 * even + 8 * (route_slot(slots) + 1) + 8 * groups;
+        key = reinterpret_cast<float*>(p + 8 * even);
+        value = p + 12 * even;
+        group = p + 12 * even + 8 * (route_slot(slots) + 1);
+        kept = p + 12 * even + 8 * (route_slot(slots) + 1) + 8 * groups;
     }
 };
 
-__device__ __forceinline__ float exp_of(float x) { return expf(x); }
+// For keys, whose error is allowed for: 2^-22 of the result and |x| 2^-24.
+__device__ __forceinline__ float exp_of(float x) { return exp2_fast(x * 1.4426950408889634f); }
 __device__ __forceinline__ double exp_of(double x) { return exp(x); }
+__device__ __forceinline__ float one_over(float x) { return reciprocal_fast(x); }
+__device__ __forceinline__ double one_over(double x) { return 1 / x; }
 
 // Chooses the row's experts, in F, and leaves them and their logits in s.  True: the choice is not sure in
 // fp32 (F double is always sure).  `mine`: the team has a row.
@@ -168,24 +178,25 @@ __device__ __forceinline__ bool route_choose(const RouteParams& p, const float (
         }
 #pragma unroll
         for (int i = 0; i < VPT; ++i) {
-            value[i] = p.sigmoid ? 1 / (1 + exp_of(-(F)l[i])) : exp_of((F)l[i] - m);
+            value[i] = p.sigmoid ? one_over(1 + exp_of(-(F)l[i])) : exp_of((F)l[i] - m);
             if (!p.sigmoid) inv += value[i];
         }
-        if (!p.sigmoid) inv = Tm::sum(inv);
+        if (!p.sigmoid) inv = one_over(Tm::sum(inv));
         F most = 0;
 #pragma unroll
         for (int i = 0; i < VPT; ++i) {
-            if (!p.sigmoid) value[i] = value[i] / inv;
+            if (!p.sigmoid) value[i] *= inv;
             if (CHECK) size = value[i] > size ? value[i] : size;
             if (computed && e0 + i < p.E) value[i] += p.bias[e0 + i];
             const F v = value[i] < 0 ? -value[i] : value[i];
             if (CHECK && v > most && v < INFINITY) most = v;
         }
-        // A score is off by at most 2^-19 of the largest: the exponent's rounding and the exponential
-        // by 2^-22, the row's sum, at most 29 additions one after the other, by 29 * 2^-24, the
-        // division by 2^-24.  Its sum with the bias is off by another 2^-24 of the value.  Two keys
-        // that differ by more than this (2^-17 and 2^-21) are in the right order.
-        if (CHECK) size = Tm::most(size) * (F)7.62939453125e-6 + Tm::most(most) * (F)4.76837158203125e-7;
+        // A sigmoid is off by at most 2^-22: the exponent's rounding moves it by s (1 - s) |x| 2^-24, the
+        // exponential's by s (1 - s) 2^-22, the reciprocal by s 2^-23.  A softmax is off by 2^-22 of the
+        // largest for its exponential, and by the row's sum, at most 29 additions one after the other of such
+        // terms, 2^-19.  A sum with the bias is off by another 2^-24 of the value.  Two keys that differ by
+        // more than this (2^-20 or 2^-17, and 2^-21) are in the right order.
+        if (CHECK) size = Tm::most(size) * (p.sigmoid ? (F)9.5367431640625e-7 : (F)7.62939453125e-6) + Tm::most(most) * (F)4.76837158203125e-7;
     }
     U key[VPT];
 #pragma unroll
@@ -199,17 +210,24 @@ __device__ __forceinline__ bool route_choose(const RouteParams& p, const float (
         U* vals = reinterpret_cast<U*>(s.value);
         U* group = reinterpret_cast<U*>(s.group);
         const int S = p.E / p.groups;
+        auto join = [](U v, U& a, U& b) {  // the largest and the second
+            b = v > a ? a : v > b ? v : b;
+            a = v > a ? v : a;
+        };
+        const bool whole = S % VPT == 0;  // a thread's experts are of one group: it joins them first
+        U a = 0, b = 0;
 #pragma unroll
-        for (int i = 0; i < VPT; ++i)
-            if (e0 + i < p.E) vals[route_slot(e0 + i)] = p.top2 ? ordered(value[i]) : key[i] ? key[i] : ordered((F)-INFINITY);
+        for (int i = 0; i < VPT; ++i) {
+            const U v = p.top2 ? ordered(value[i]) : key[i] ? key[i] : ordered((F)-INFINITY);
+            if (whole) join(v, a, b);
+            else if (e0 + i < p.E) vals[route_slot(e0 + i)] = v;
+        }
+        if (whole && e0 < p.E) { vals[2 * lane] = a; vals[2 * lane + 1] = b; }
         Tm::sync();
+        const int per = whole ? S / VPT * 2 : S;
         for (int g = lane; g < p.groups; g += LANES) {
-            U a = 0, b = 0;  // the largest and the second
-            for (int i = 0; i < S; ++i) {
-                const U v = vals[route_slot(g * S + i)];
-                b = v > a ? a : v > b ? v : b;
-                a = v > a ? v : a;
-            }
+            a = b = 0;
+            for (int i = 0; i < per; ++i) join(vals[whole ? g * per + i : route_slot(g * per + i)], a, b);
             group[g] = p.top2 ? ordered(number(a) + number(b)) : a;
         }
         Tm::sync();
@@ -231,44 +249,61 @@ __device__ __forceinline__ bool route_choose(const RouteParams& p, const float (
             unsure = next > -INFINITY && last - next <= 2 * size;
         }
         int g = e0 / S, r = e0 - g * S;
+        if (whole) {
+            const bool stays = e0 < p.E && s.kept[g];
 #pragma unroll
-        for (int i = 0; i < VPT; ++i) {
-            if (e0 + i < p.E && !s.kept[g]) key[i] = 0;
-            if (++r == S) { r = 0; ++g; }
-        }
-    }
-    F before = INFINITY;  // the choice before, its logit and place
-    float before_l = 0.f;
-    int before_at = 0;
-    for (int j = 0; j < p.k; ++j) {
-        U best = key[0];
-        int at = e0;
+            for (int i = 0; i < VPT; ++i) key[i] = stays ? key[i] : 0;
+        } else {
 #pragma unroll
-        for (int i = 1; i < VPT; ++i)
-            if (key[i] > best) { best = key[i]; at = e0 + i; }
-        Tm::first_most(best, at);
-#pragma unroll
-        for (int i = 0; i < VPT; ++i)
-            if (e0 + i == at) {
-                if (best) s.logit[j] = l[i];
-                key[i] = 0;
+            for (int i = 0; i < VPT; ++i) {
+                if (e0 + i < p.E && !s.kept[g]) key[i] = 0;
+                if (++r == S) { r = 0; ++g; }
             }
-        if (lane == 0) s.at[j] = best ? at : -1;
-        if (CHECK && computed) {
-            Tm::sync();
-            const float logit = s.logit[j];
-            const F v = number(best);
-            if (best && j > 0 && before - v <= size && !(logit == before_l && p.bias[at] == p.bias[before_at])) unsure = true;
-            if (best) { before = v; before_l = logit; before_at = at; }
         }
     }
-    if (CHECK && computed) {  // what is left next to the last choice
-        const float b = p.bias[before_at];
+    // k rounds: the row's largest key, taken out by the first thread that has it (whose experts
+    // are the lowest, and it takes its first), which looks for its next one
+    U best = key[0];
 #pragma unroll
-        for (int i = 0; i < VPT; ++i)
-            if (key[i] && before - number(key[i]) <= size && !(l[i] == before_l && p.bias[e0 + i] == b)) unsure = true;
+    for (int i = 1; i < VPT; ++i) best = key[i] > best ? key[i] : best;
+    for (int j = 0; j < p.k; ++j) {
+        const U top = Tm::most(best);
+        if (Tm::first(best == top)) {
+            U next = 0;
+            int at = 0;
+            float logit = 0.f;
+            bool found = false;
+#pragma unroll
+            for (int i = 0; i < VPT; ++i) {
+                if (!found && key[i] == top) {
+                    found = true;
+                    at = e0 + i;
+                    logit = l[i];
+                    key[i] = 0;
+                }
+                next = key[i] > next ? key[i] : next;
+            }
+            best = next;
+            s.at[j] = top ? at : -1;
+            s.logit[j] = logit;
+            if (CHECK) s.key[j] = (float)number(top);
+        }
+        if constexpr (!Tm::WIDE) __syncwarp();
     }
     Tm::sync();
+    if (CHECK && computed) {
+        auto close = [&](float a, int at, float la, float b, int bt, float lb) {  // (equal logits and biases make equal keys)
+            return a - b <= size && !(la == lb && p.bias[at] == p.bias[bt]);
+        };
+        for (int j = lane + 1; j < p.k; j += LANES)
+            if (s.at[j] >= 0) unsure |= close(s.key[j - 1], s.at[j - 1], s.logit[j - 1], s.key[j], s.at[j], s.logit[j]);
+        const int at = s.at[p.k - 1];  // and what is left next to the last choice
+        if (at >= 0 && best && s.key[p.k - 1] - number(best) <= size) {
+#pragma unroll
+            for (int i = 0; i < VPT; ++i)
+                if (key[i]) unsure |= close(s.key[p.k - 1], at, s.logit[p.k - 1], (float)number(key[i]), e0 + i, l[i]);
+        }
+    }
     return unsure;
 }
 
@@ -320,7 +355,7 @@ __device__ __forceinline__ void route_weights(const RouteParams& p, const float 
 }
 
 template <typename T, int LANES, int VPT>
-__global__ void __launch_bounds__(Team<LANES>::BLOCK) route_kernel(const RouteParams p) {
+__global__ void __launch_bounds__(Team<LANES>::BLOCK) route_kernel(const __grid_constant__ RouteParams p) {
     next_may_start();
     previous_done();
     typedef Team<LANES> Tm;
