@@ -4,14 +4,20 @@
 // A row of logits belongs to a team of LANES threads, a part of a warp for up to 512
 // experts, so that 32 / LANES rows share a warp, and a block of 256 for more.  A thread holds
 // VPT consecutive experts in registers; one pass reads the row once, and everything else
-// (softmax, groups, k rounds of "largest key left", weights) stays in registers, shuffles
-// and a little shared memory.
+// (softmax, groups, choice, weights) stays in registers, shuffles and a little shared memory.
+//
+// The k largest keys: the k-th largest of the threads' own largest keys is a bound that at
+// least k keys reach, and few others do (a dozen for 8 of 256).  Those that reach it are put
+// side by side in shared memory, in the order of the experts, and each counts the keys above
+// it, which is its rank.  8 of 256 experts take a third of the instructions of k rounds of
+// "largest key left", each with a search by the thread that had it.
 //
 // The choice is settled as in 64 bits.  Without a bias a score grows with its logit, so logits
 // are compared, which is exact.  Keys that are computed (score + bias, a group's sum) are
-// formed in fp32 with a bound on their error; a row in which two keys that decide something
-// lie closer than that is formed again in fp64.  That happens in a few rows of 10000, and
-// fp64 throughout would cost more than the rest of the kernel.
+// formed in fp32 with a bound on their error; where two keys that decide something lie closer
+// than that, the keys in question are formed again in fp64 (with all of the row's where groups
+// decide).  That happens in a row of a thousand, and fp64 throughout would cost more than the
+// rest of the kernel.
 #include "ela_expert.cuh"
 
 namespace ela_expert {
@@ -43,8 +49,8 @@ struct RouteGradParams {
 // Numbers as unsigned whole numbers in the same order; NaN above all, -0 as 0.  0 is left
 // for "not to be chosen".
 __device__ __forceinline__ uint32_t ordered(float x) {
-    const uint32_t b = __float_as_uint(x + 0.f);
-    return x != x ? ~0u : b & 0x80000000u ? ~b : b | 0x80000000u;
+    const uint32_t b = __float_as_uint(x + 0.f);  // (a sum that is NaN is 0x7fffffff)
+    return b ^ ((uint32_t)((int32_t)b >> 31) | 0x80000000u);
 }
 __device__ __forceinline__ uint64_t ordered(double x) {
     const uint64_t b = (uint64_t)__double_as_longlong(x + 0.0), top = 1ull << 63;
@@ -87,21 +93,29 @@ template <int LANES> struct Team {
         if constexpr (LANES == 32) return __reduce_max_sync(~0u, v);
         return reduce(v, [](uint32_t a, uint32_t b) { return a > b ? a : b; });
     }
-    // True in the first thread of the row in which v is.
-    static __device__ __forceinline__ bool first(bool v) {
-        unsigned has = __ballot_sync(~0u, v);
-        if constexpr (WIDE) {
-            __shared__ unsigned warps[LANES / 32];
-            __syncthreads();
-            if ((threadIdx.x & 31) == 0) warps[threadIdx.x >> 5] = has;
-            __syncthreads();
-            for (unsigned i = 0; i < threadIdx.x >> 5; ++i)
-                if (warps[i]) return false;
-        } else if constexpr (LANES < 32) {
-            has = has >> (threadIdx.x & 31 & ~(LANES - 1)) & ((1u << LANES) - 1);
-            return v && (has & ((1u << (threadIdx.x & (LANES - 1))) - 1)) == 0;
+    // The sum of v over the row's earlier threads, and over all.
+    static __device__ __forceinline__ int before(int v, int& all) {
+        constexpr int W = WIDE ? 32 : LANES;
+        const int mine = v, at = threadIdx.x & (W - 1);
+#pragma unroll
+        for (int o = 1; o < W; o <<= 1) {
+            const int u = __shfl_up_sync(~0u, v, o, W);
+            if (at >= o) v += u;
         }
-        return v && (has & ((1u << (threadIdx.x & 31)) - 1)) == 0;
+        all = __shfl_sync(~0u, v, W - 1, W);
+        int base = 0;
+        if constexpr (WIDE) {
+            __shared__ int part[LANES / 32];
+            __syncthreads();
+            if (at == 0) part[threadIdx.x >> 5] = all;
+            __syncthreads();
+            all = 0;
+            for (int i = 0; i < LANES / 32; ++i) {
+                if (i == (int)(threadIdx.x >> 5)) base = all;
+                all += part[i];
+            }
+        }
+        return base + v - mine;
     }
 };
 
@@ -125,27 +139,33 @@ template <typename T, int VPT> __device__ __forceinline__ void load_logits(float
     }
 }
 
-// A team's shared memory: the chosen experts, their logits and keys, and with groups the experts'
-// values (or each thread's two largest), the groups' and the groups kept.  (One word in 33 unused: threads that walk groups
-// of 32 side by side then hit different banks.)
+// A team's shared memory: the chosen experts, their logits and keys; the keys that reach the
+// bound with their experts, or before them the values that groups are ranked by (each
+// expert's, or each thread's two largest); with groups their ranks' values and the groups kept.
+// (One word in 33 of the values unused: threads that walk groups of 32 side by side then hit
+// different banks.)
 __host__ __device__ inline int route_slot(int e) { return e + (e >> 5); }
 struct RouteShared {
     int* at;
     float *logit, *key;
-    void* value;
+    void* value;       // [slots] keys of up to 8 bytes
+    int* value_at;     // [slots]
     void* group;
     unsigned char* kept;
+    static __host__ __device__ inline int even(int k) { return (k + 1) / 2 * 2; }
+    // (in the gradient: the list alone, slots 0)
     static __host__ __device__ inline int bytes(int slots, int k, int groups) {
-        return 12 * ((k + 1) / 2 * 2) + (groups > 1 ? 8 * (route_slot(slots) + 1) + 8 * groups + (groups + 7) / 8 * 8 : 0);
+        return 12 * even(k) + 12 * slots + (groups > 1 ? 8 * groups + (groups + 7) / 8 * 8 : 0);
     }
     __device__ __forceinline__ RouteShared(unsigned char* p, int slots, int k, int groups) {
-        const int even = (k + 1) / 2 * 2;
         at = reinterpret_cast<int*>(p);
-        logit = reinterpret_cast<float*>(p + 4 * even);
-        key = reinterpret_cast<float*>(p + 8 * even);
-        value = p + 12 * even;
-        group = p + 12 * even + 8 * (route_slot(slots) + 1);
-        kept = p + 12 * even + 8 * (route_slot(slots) + 1) + 8 * groups;
+        logit = reinterpret_cast<float*>(p + 4 * even(k));
+        key = reinterpret_cast<float*>(p + 8 * even(k));
+        p += 12 * even(k);
+        value = p;
+        value_at = reinterpret_cast<int*>(p + 8 * slots);
+        group = p + 12 * slots;
+        kept = p + 12 * slots + 8 * groups;
     }
 };
 
@@ -155,10 +175,62 @@ __device__ __forceinline__ double exp_of(double x) { return exp(x); }
 __device__ __forceinline__ float one_over(float x) { return reciprocal_fast(x); }
 __device__ __forceinline__ double one_over(double x) { return 1 / x; }
 
-// Chooses the row's experts, in F, and leaves them and their logits in s.  True: the choice is not sure in
-// fp32 (F double is always sure).  `mine`: the team has a row.
-template <typename F, int LANES, int VPT>
-__device__ __forceinline__ bool route_choose(const RouteParams& p, const float (&l)[VPT], const RouteShared& s) {
+// The ranks of the `all` keys in s.value (into the upper half of their s.value_at), and the k
+// experts of the first ranks with their logits and (fp32) keys.
+template <typename F, typename T, int LANES>
+__device__ __forceinline__ void route_ranks(int k, int all, const T* row, const RouteShared& s) {
+    typedef Team<LANES> Tm;
+    typedef typename Ordered<F>::U U;
+    const U* keys = reinterpret_cast<const U*>(s.value);
+    const int lane = Tm::lane();
+    for (int j = lane; j < k; j += LANES) s.at[j] = -1;
+    Tm::sync();
+    for (int c = lane; c < all; c += LANES) {
+        const U mine = keys[c];
+        const int at = s.value_at[c];
+        int rank = 0;
+#pragma unroll 4
+        for (int d = 0; d < all; ++d) rank += keys[d] > mine - (d < c);  // (of equal keys the first comes first; no key here is 0)
+        s.value_at[c] = at | rank << 16;
+        if (rank < k) {
+            s.at[rank] = at;
+            s.logit[rank] = El<T>::to(row[at]);
+            if (sizeof(F) == 4) s.key[rank] = number((uint32_t)mine);
+        }
+    }
+    Tm::sync();
+}
+
+// The keys in s.value formed again in 64 bits, and ranked.  (Kept out of the kernel's registers.)
+template <typename T, int LANES, int VPT>
+__device__ __noinline__ void route_settle(const RouteParams& p, int all, const T* row, const float (&l)[VPT], const RouteShared& s) {
+    typedef Team<LANES> Tm;
+    double m = 0, sum = 1;
+    if (!p.sigmoid) {
+        float most = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < VPT; ++i) most = fmaxf(most, l[i]);
+        m = Tm::most(most);
+        sum = 0;
+        for (int i = 0; i < VPT; ++i) sum += l[i] == -INFINITY ? 0 : exp((double)l[i] - m);
+        sum = Tm::sum(sum);
+    }
+    Tm::sync();
+    uint64_t* keys = reinterpret_cast<uint64_t*>(s.value);
+    for (int c = Tm::lane(); c < all; c += LANES) {
+        const int at = s.value_at[c] & 0xffff;
+        const double x = El<T>::to(row[at]);
+        keys[c] = ordered((p.sigmoid ? 1 / (1 + exp(-x)) : exp(x - m) / sum) + (double)p.bias[at]);
+        s.value_at[c] = at;
+    }
+    Tm::sync();
+    route_ranks<double, T, LANES>(p.k, all, row, s);
+}
+
+// Chooses the row's experts, in F, and leaves them in s, with their logits and (in fp32) keys.  True: the choice is
+// not sure in fp32 (F double is always sure).
+template <typename F, typename T, int LANES, int VPT>
+__device__ __forceinline__ bool route_choose(const RouteParams& p, const T* row, const float (&l)[VPT], const RouteShared& s) {
     typedef Team<LANES> Tm;
     typedef typename Ordered<F>::U U;
     constexpr bool CHECK = sizeof(F) == 4;
@@ -261,56 +333,47 @@ __device__ __forceinline__ bool route_choose(const RouteParams& p, const float (
             }
         }
     }
-    // k rounds: the row's largest key, taken out by the first thread that has it (whose experts
-    // are the lowest, and it takes its first), which looks for its next one
+    // the bound: the k-th of the threads' largest keys (equal ones leave together, which lowers it)
     U best = key[0];
 #pragma unroll
     for (int i = 1; i < VPT; ++i) best = key[i] > best ? key[i] : best;
+    U bound = 0;
     for (int j = 0; j < p.k; ++j) {
-        const U top = Tm::most(best);
-        if (Tm::first(best == top)) {
-            U next = 0;
-            int at = 0;
-            float logit = 0.f;
-            bool found = false;
-#pragma unroll
-            for (int i = 0; i < VPT; ++i) {
-                if (!found && key[i] == top) {
-                    found = true;
-                    at = e0 + i;
-                    logit = l[i];
-                    key[i] = 0;
-                }
-                next = key[i] > next ? key[i] : next;
-            }
-            best = next;
-            s.at[j] = top ? at : -1;
-            s.logit[j] = logit;
-            if (CHECK) s.key[j] = (float)number(top);
-        }
-        if constexpr (!Tm::WIDE) __syncwarp();
+        bound = Tm::most(best);
+        if (best == bound) best = 0;
+        if (LANES <= 32 && j >= LANES) break;  // (none left)
     }
-    Tm::sync();
-    if (CHECK && computed) {
-        auto close = [&](float a, int at, float la, float b, int bt, float lb) {  // (equal logits and biases make equal keys)
-            return a - b <= size && !(la == lb && p.bias[at] == p.bias[bt]);
-        };
-        for (int j = lane + 1; j < p.k; j += LANES)
-            if (s.at[j] >= 0) unsure |= close(s.key[j - 1], s.at[j - 1], s.logit[j - 1], s.key[j], s.at[j], s.logit[j]);
-        const int at = s.at[p.k - 1];  // and what is left next to the last choice
-        if (at >= 0 && best && s.key[p.k - 1] - number(best) <= size) {
+    if (CHECK && computed && bound != 0) bound = ordered(number(bound) - size);  // what may belong to them in 64 bits, too
+    if (bound == 0) bound = 1;
+    int reach = 0, all;
 #pragma unroll
-            for (int i = 0; i < VPT; ++i)
-                if (key[i]) unsure |= close(s.key[p.k - 1], at, s.logit[p.k - 1], (float)number(key[i]), e0 + i, l[i]);
+    for (int i = 0; i < VPT; ++i) reach += key[i] >= bound;
+    int to = Tm::before(reach, all);
+    U* keys = reinterpret_cast<U*>(s.value);
+#pragma unroll
+    for (int i = 0; i < VPT; ++i)
+        if (key[i] >= bound) {
+            keys[to] = key[i];
+            s.value_at[to++] = e0 + i;
         }
+    route_ranks<F, T, LANES>(p.k, all, row, s);
+    if (CHECK && computed) {
+        auto same = [&](int a, int b) { return El<T>::to(row[a]) == El<T>::to(row[b]) && p.bias[a] == p.bias[b]; };  // equal keys in any arithmetic
+        bool doubt = false;
+        for (int c = lane; c < all; c += LANES) {  // each against the choice before it, or the last one
+            const int rank = s.value_at[c] >> 16, at = s.value_at[c] & 0xffff, prev = min(rank, p.k) - 1;
+            if (prev >= 0) doubt |= s.key[prev] - number(keys[c]) <= size && !same(s.at[prev], at);
+        }
+        if (Tm::any(doubt)) route_settle<T, LANES, VPT>(p, all, row, l, s);
     }
     return unsure;
 }
 
-// 64 bits, for the rows that need them (kept out of the kernel's registers).
-template <int LANES, int VPT>
-__device__ __noinline__ void route_settle(const RouteParams& p, const float (&l)[VPT], const RouteShared& s) {
-    route_choose<double, LANES, VPT>(p, l, s);
+// 64 bits throughout, for the rows whose groups need them (kept out of the kernel's registers).
+template <typename T, int LANES, int VPT>
+__device__ __noinline__ void route_again(const RouteParams& p, const T* row, const float (&l)[VPT], const RouteShared& s) {
+    Team<LANES>::sync();
+    route_choose<double, T, LANES, VPT>(p, row, l, s);
 }
 
 // Weights of the chosen experts, in place of their logits.  Ratios of the chosen scores are
@@ -360,12 +423,13 @@ __global__ void __launch_bounds__(Team<LANES>::BLOCK) route_kernel(const __grid_
     previous_done();
     typedef Team<LANES> Tm;
     extern __shared__ __align__(16) unsigned char shared[];
-    const int64_t first = (int64_t)blockIdx.x * Tm::ROWS, t = first + Tm::row();
+    const int64_t t = (int64_t)blockIdx.x * Tm::ROWS + Tm::row();
     const int bytes = RouteShared::bytes(LANES * VPT, p.k, p.groups);
     const RouteShared s(shared + Tm::row() * bytes, LANES * VPT, p.k, p.groups);
     float l[VPT];
-    load_logits<T, VPT>(l, reinterpret_cast<const T*>(p.logits) + (t < p.T ? t : 0) * p.ld, Tm::lane() * VPT, p.E, p.vec, t < p.T);
-    if (Tm::any(route_choose<float, LANES, VPT>(p, l, s))) route_settle<LANES, VPT>(p, l, s);
+    const T* row = reinterpret_cast<const T*>(p.logits) + (t < p.T ? t : 0) * p.ld;
+    load_logits<T, VPT>(l, row, Tm::lane() * VPT, p.E, p.vec, t < p.T);
+    if (Tm::any(route_choose<float, T, LANES, VPT>(p, row, l, s))) route_again<T, LANES, VPT>(p, row, l, s);
     route_weights<LANES, VPT>(p, l, s);
     if (t < p.T)
         for (int j = Tm::lane(); j < p.k; j += LANES) {
@@ -381,14 +445,14 @@ __global__ void __launch_bounds__(Team<LANES>::BLOCK) route_kernel(const __grid_
 //   sigmoid, ratios   dl_j = r_j (c_j - sum_j c_j r_j) (1 - s_j)
 // Only the first reads the whole row.  A choice outside [0, E) has no gradient.
 template <typename T, int LANES, int VPT>
-__global__ void __launch_bounds__(Team<LANES>::BLOCK) route_grad_kernel(const RouteGradParams p) {
+__global__ void __launch_bounds__(Team<LANES>::BLOCK) route_grad_kernel(const __grid_constant__ RouteGradParams p) {
     next_may_start();
     previous_done();
     typedef Team<LANES> Tm;
     extern __shared__ __align__(16) unsigned char shared[];
     const int lane = Tm::lane(), e0 = lane * VPT;
     const int64_t t = (int64_t)blockIdx.x * Tm::ROWS + Tm::row();
-    const RouteShared s(shared + Tm::row() * RouteShared::bytes(LANES * VPT, p.k, 1), LANES * VPT, p.k, 1);
+    const RouteShared s(shared + Tm::row() * RouteShared::bytes(0, p.k, 1), 0, p.k, 1);
     const T* row = reinterpret_cast<const T*>(p.logits) + (t < p.T ? t : 0) * p.ld;
     const bool dense = !p.sigmoid && !p.renormalize;
     float l[VPT], most = -INFINITY, sum = 0.f, mean = 0.f;
@@ -474,16 +538,16 @@ template <typename T, int LANES, int VPT> int route_launch(const RouteGradParams
     typedef Team<LANES> Tm;
     const int64_t blocks = (p.T + Tm::ROWS - 1) / Tm::ROWS;
     if (blocks > INT32_MAX) return ELA_ERR_UNSUPPORTED;
-    return launch(route_grad_kernel<T, LANES, VPT>, (unsigned)blocks, Tm::BLOCK, Tm::ROWS * RouteShared::bytes(LANES * VPT, p.k, 1), st, p);
+    return launch(route_grad_kernel<T, LANES, VPT>, (unsigned)blocks, Tm::BLOCK, Tm::ROWS * RouteShared::bytes(0, p.k, 1), st, p);
 }
 
 // Eight experts a thread, so that a row of 16-bit logits is one load each, on as few threads
-// as that takes; sixteen past 256 experts.
+// as that takes; sixteen past 128 experts.
 template <typename T, typename P> int route_by_size(P p, cudaStream_t st) {
-    const int per = p.E <= 256 ? 8 : 16;
+    const int per = p.E <= 128 ? 8 : 16;
     p.vec = p.vec && p.E % per == 0;
     return p.E <= 8 ? route_launch<T, 1, 8>(p, st) : p.E <= 16 ? route_launch<T, 2, 8>(p, st) : p.E <= 32 ? route_launch<T, 4, 8>(p, st)
-         : p.E <= 64 ? route_launch<T, 8, 8>(p, st) : p.E <= 128 ? route_launch<T, 16, 8>(p, st) : p.E <= 256 ? route_launch<T, 32, 8>(p, st)
+         : p.E <= 64 ? route_launch<T, 8, 8>(p, st) : p.E <= 128 ? route_launch<T, 16, 8>(p, st) : p.E <= 256 ? route_launch<T, 16, 16>(p, st)
          : p.E <= 512 ? route_launch<T, 32, 16>(p, st) : route_launch<T, ROUTE_WIDE, 16>(p, st);
 }
 template <typename P> int route_by_type(const P& p, int dtype, cudaStream_t st) {
