@@ -23,7 +23,8 @@ __global__ void __launch_bounds__(PACK_WARPS * 32) quantize_kernel(const T* weig
     const int chunk = blockIdx.x % chunks, strip = blockIdx.x / chunks % strips, e = blockIdx.x / chunks / strips;
     const int k = chunk * PACK_K + 8 * lane, n0 = strip * PACK_ROWS, group_lanes = 1 << (shift - 3);
     constexpr int STEPS = PACK_ROWS / PACK_WARPS;
-    uint16_t w[STEPS][8];
+    constexpr float LEAST = El<T>::BF16 ? 1.17549435e-38f : 6.103515625e-5f;  // the least scale of full precision
+    uint32_t w[STEPS][4];
 #pragma unroll
     for (int i = 0; i < STEPS; ++i) {
         const int n = n0 + warp + PACK_WARPS * i;
@@ -34,22 +35,44 @@ __global__ void __launch_bounds__(PACK_WARPS * 32) quantize_kernel(const T* weig
 #pragma unroll
     for (int i = 0; i < STEPS; ++i) {
         const int r = warp + PACK_WARPS * i, n = n0 + r;
-        unsigned most = 0;
+        uint32_t most = 0;  // of both halves
 #pragma unroll
-        for (int j = 0; j < 8; ++j) most = max(most, w[i][j] & 0x7fffu);
-        for (int o = 1; o < group_lanes; o <<= 1) most = max(most, __shfl_xor_sync(~0u, most, o));
-        const uint16_t bits = (uint16_t)most;
+        for (int j = 0; j < 4; ++j) most = __vmaxu2(most, w[i][j] & 0x7fff7fffu);
+        for (int o = 1; o < group_lanes; o <<= 1) most = __vmaxu2(most, __shfl_xor_sync(~0u, most, o));
+        const uint16_t bits = (uint16_t)max(most >> 16, most & 0xffffu);
         T largest;
         memcpy(&largest, &bits, 2);
-        const T scale = El<T>::from(El<T>::to(largest) / 7.f);
+        // (a seventh is never halfway between two scales: 7 times an odd number has more bits than a
+        // weight; so the product with 1/7, off by 2^-23, is rounded as the quotient)
+        const T scale = El<T>::from(El<T>::to(largest) * 0.142857142857142857f);
         const float s = El<T>::to(scale);
         uint32_t word = 0;
+        if (s >= LEAST && s < INFINITY) {
+            // w / s by the reciprocal, onto multiples of 2^-14 and then onto whole numbers.  The product is
+            // off by 2^-20 at most; w / s is halfway between whole numbers or, both having 11 bits at most,
+            // 2^-12 and more away from there, so the second rounding decides as if on w / s.  The whole
+            // number plus 8 is left in the last bits of the float; what the float has above them adds up to
+            // the constant.
+            const float reciprocal = reciprocal_fast(s);
+            constexpr float GRID = 768.f, WHOLE = 12582912.f + 8.f;  // 1.5 * 2^9, 1.5 * 2^23
+            constexpr uint32_t ABOVE = 0x4b400000u;
+            uint32_t above = 0;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            T v;
-            memcpy(&v, &w[i][j], 2);
-            const float q = s > 0.f && s < INFINITY ? fminf(fmaxf(rintf(El<T>::to(v) / s), -8.f), 7.f) : 0.f;
-            word |= (uint32_t)((int)q + 8) << (4 * (j / 2) + 16 * (j % 2));
+            for (int j = 0; j < 4; ++j) {
+                const float2 v = unpack2<T>(w[i][j]);
+                const float q0 = __fadd_rn(__fadd_rn(__fmaf_rn(v.x, reciprocal, GRID), -GRID), WHOLE);
+                const float q1 = __fadd_rn(__fadd_rn(__fmaf_rn(v.y, reciprocal, GRID), -GRID), WHOLE);
+                word += (__float_as_uint(q0) << (4 * j)) + (__float_as_uint(q1) << (4 * j + 16));
+                above += (ABOVE << (4 * j)) + (ABOVE << (4 * j + 16));
+            }
+            word -= above;
+        } else {  // the scale is 0, has fewer bits (and |q| may pass 7), or is no number
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const float2 pair = unpack2<T>(w[i][j / 2]);
+                const float v = j & 1 ? pair.y : pair.x, q = s > 0.f && s < INFINITY ? fminf(fmaxf(rintf(v / s), -8.f), 7.f) : 0.f;
+                word |= (uint32_t)((int)q + 8) << (4 * (j / 2) + 16 * (j % 2));
+            }
         }
         if (n < N && k < words * 8) packed[((int64_t)e * N + n) * words + k / 8] = word;
         if ((lane & (group_lanes - 1)) == 0) s_scale[8 * lane >> shift][r] = scale;
@@ -62,23 +85,26 @@ __global__ void __launch_bounds__(PACK_WARPS * 32) quantize_kernel(const T* weig
     }
 }
 
+// Rows off their 16 bytes go through shared memory and are stored 4 bytes a lane, 128 in a row (1027 x 2051: 17 us
+// with eight 2-byte stores a lane).
 template <typename T, bool VEC>
 __global__ void __launch_bounds__(PACK_WARPS * 32) dequantize_kernel(const uint32_t* packed, const T* scales, int K, int N, int shift, int words,
                                                                      int parts, T* weight) {
     next_may_start();
     previous_done();
+    __shared__ __align__(16) uint16_t s_row[VEC ? 1 : PACK_WARPS][VEC ? 8 : PACK_K];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int chunks = (words * 8 + PACK_K - 1) / PACK_K, strips = (N + PACK_ROWS - 1) / PACK_ROWS;
     const int chunk = blockIdx.x % chunks, strip = blockIdx.x / chunks % strips, e = blockIdx.x / chunks / strips;
-    const int k = chunk * PACK_K + 8 * lane;
-    if (k >= K) return;
+    const int k0 = chunk * PACK_K, k = k0 + 8 * lane, count = min(K - k0, PACK_K);
+    if (count <= 0) return;
     constexpr int STEPS = PACK_ROWS / PACK_WARPS;
     uint32_t w[STEPS];
     T s[STEPS];
 #pragma unroll
     for (int i = 0; i < STEPS; ++i) {
         const int n = strip * PACK_ROWS + warp + PACK_WARPS * i;
-        if (n < N) {
+        if (n < N && k < K) {
             w[i] = packed[((int64_t)e * N + n) * words + k / 8];
             s[i] = scales[((int64_t)e * parts + (k >> shift)) * N + n];
         }
@@ -87,15 +113,21 @@ __global__ void __launch_bounds__(PACK_WARPS * 32) dequantize_kernel(const uint3
     for (int i = 0; i < STEPS; ++i) {
         const int n = strip * PACK_ROWS + warp + PACK_WARPS * i;
         if (n >= N) break;
-        T* out = weight + ((int64_t)e * N + n) * K + k;
-        uint32_t v[4];
-        unpack<T>(w[i], scale_pair(s[i]), v);
-        if (VEC) {
-            *reinterpret_cast<uint4*>(out) = make_uint4(v[0], v[1], v[2], v[3]);
+        uint16_t* out = reinterpret_cast<uint16_t*>(weight) + ((int64_t)e * N + n) * K + k0;
+        uint32_t v[4] = {};
+        if (k < K) unpack<T>(w[i], scale_pair(s[i]), v);
+        if constexpr (VEC) {
+            if (k < K) *reinterpret_cast<uint4*>(out + 8 * lane) = make_uint4(v[0], v[1], v[2], v[3]);
         } else {
-#pragma unroll
-            for (int j = 0; j < 8; ++j)
-                if (k + j < K) reinterpret_cast<uint16_t*>(out)[j] = (uint16_t)(v[j / 2] >> (16 * (j & 1)));
+            *reinterpret_cast<uint4*>(&s_row[warp][8 * lane]) = make_uint4(v[0], v[1], v[2], v[3]);
+            __syncwarp();
+            const int odd = reinterpret_cast<uintptr_t>(out) >> 1 & 1;  // words start at the element before
+            for (int j = 2 * lane - odd; j < count; j += 64) {
+                if (j >= 0 && j + 1 < count) *reinterpret_cast<uint32_t*>(out + j) = s_row[warp][j] | (uint32_t)s_row[warp][j + 1] << 16;
+                else if (j >= 0) out[j] = s_row[warp][j];
+                else out[0] = s_row[warp][0];
+            }
+            __syncwarp();
         }
     }
 }
