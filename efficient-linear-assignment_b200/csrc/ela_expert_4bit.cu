@@ -207,10 +207,10 @@ int ela_expert_linear_4bit(const void* x, const int32_t* packed, const void* sca
     const int words = (int)q_words(K), parts = (int)((K + group - 1) / group), shift = group_shift(group);
     int rc = ELA_OK;
     if (few_rows_4bit(R, E, N)) {
-        Stream4Params p = {x, (const uint32_t*)packed, scales, bias, residual, offsets, (int)R, (int)E, (int)K, (int)N, words, parts, shift, 0,
+        Stream4Params p = {x, (const uint32_t*)packed, scales, bias, residual, offsets, (int)R, (int)E, (int)K, (int)N, words, parts, shift, 0, 0,
                            activation, 0, ldx, ldr, y};
         const bool vec = aligned16(x, ldx * 2) && K % 8 == 0;
-        ELA_BY_TYPE(dtype, { rc = R <= 8 * E ? stream4_launch<T_, 1, 2, 2>(p, vec, st) : stream4_launch<T_, 4, 2, 2>(p, vec, st); })
+        ELA_BY_TYPE(dtype, { rc = stream4<T_>(p, vec, st); })
         return rc;
     }
     char* ws = reinterpret_cast<char*>(workspace);

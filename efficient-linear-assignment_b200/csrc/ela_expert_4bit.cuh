@@ -16,8 +16,8 @@ struct Stream4Params {
     const int32_t* offsets;
     int R, E, K, N;
     int words, parts, shift;  // of a packed row; groups of a row; log2(group)
-    int f_tiles, act;
-    int wide_scales;          // a lane's scales may be read at once
+    int k_warps, f_tiles;     // warps that share a contraction; items per expert
+    int act, wide_scales;     // a lane's scales may be read at once
     int64_t ldx, ldr;
     void* y;
 };
@@ -42,19 +42,30 @@ template <int VB> __device__ __forceinline__ uint4 load8(const uint16_t* row, in
     return v;
 }
 
-// As stream_kernel: items of 16 * MT features over the whole contraction, which the CTA's 8
-// warps share; a batch of loads is issued when the one before it has been taken.  A lane
-// (g = lane / 4, t = lane % 4) loads 32 consecutive inputs (16 bytes) of each of 2 * MT rows,
-// SUB times; a row's place among the MMA's 16 is free, so they are neighbouring features
-// (whose scales are neighbours too).  A group has at least 32 inputs: one scale for each load.
-// The token's inputs come from L1 when they are needed.
+// As stream_kernel, plain loads straight to registers: an item is a few features of an expert over
+// the whole contraction, which k_warps of the CTA's 8 warps share; the others take further
+// features, 16 * MT a warp.  A lane (g = lane / 4, t = lane % 4) loads 32 consecutive inputs (16
+// bytes) of each of 2 * MT rows, SUB times; a row's place among the MMA's 16 is free, so they are
+// neighbouring features (whose scales are neighbours too).  A group has at least 32 inputs: one
+// scale for each load.  For 8 tokens two loads are one of 32 bytes, so that a row's four lanes
+// read a whole line (16 experts of 4096 x 1024, a token each: 13.7 -> 12.0 us; the second token's
+// group would need the registers that hold the inputs of both halves).  The token's inputs come from L1 when they are needed, where a load that
+// nobody waits for has brought them a batch ahead; what an item's end reads is loaded ahead, too.
+//
+// Two rows' words are loaded again, for the lane's next batch (of the next item, after the
+// last), as soon as they have been multiplied, so that seven of the eight loads that a lane
+// has registers for are in flight all the time.
 template <typename T, int RG, int MT, int SUB, int VB>
 __global__ void __launch_bounds__(STREAM_WARPS * 32, 2) stream4_kernel(const Stream4Params p) {
     next_may_start();
     previous_done();
-    constexpr int F = 16 * MT, H = 2 * MT, KB = 128 * SUB;
-    __shared__ float part[STREAM_WARPS][RG * 8][F + 1];
+    constexpr int WF = 16 * MT, H = 2 * MT, KB = 128 * SUB;  // features of a warp, rows of a lane, inputs of a batch
+    constexpr int PAIR = RG == 1 ? 2 : 1;                    // 16-byte pieces of a load
+    auto input_of = [](int s) { return s % PAIR * 32 + s / PAIR * 128 * PAIR; };  // piece s of a lane, from its first input
+    __shared__ float parts[2][STREAM_WARPS][RG * 8][WF + 1];  // of this item and the one before: one barrier an item
+    int turn = 0;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
+    const int kw = warp % p.k_warps, fw = warp / p.k_warps, F = STREAM_WARPS / p.k_warps * WF;
     T* y = reinterpret_cast<T*>(p.y);
     const T* residual = reinterpret_cast<const T*>(p.residual);
     if (p.offsets) {  // rows of no expert: the residual, or 0
@@ -65,105 +76,145 @@ __global__ void __launch_bounds__(STREAM_WARPS * 32, 2) stream4_kernel(const Str
                     y[(int64_t)r * p.N + f] = residual ? residual[r * p.ldr + f] : El<T>::from(0.f);
     }
     const unsigned items = (unsigned)p.E * p.f_tiles;  // (below 2^31: the step past the last does not wrap)
-    const int rounds = (p.words * 8 + STREAM_WARPS * KB - 1) / (STREAM_WARPS * KB);
+    const int rounds = (p.words * 8 + p.k_warps * KB - 1) / (p.k_warps * KB);
 
+    // the place of a batch: item (expert e, features from f0 on), its rows rb.. of up to r1, round `it`
+    struct At { int e, f0, rb, r1, it; } next = {}, now;
     unsigned item = blockIdx.x - gridDim.x;
-    int e = 0, f0 = 0, rb = 0, r1 = 0, it = 0;
-    const uint32_t* wrow = nullptr;  // of the lane's first feature
-    const T* srow = nullptr;
-    const uint16_t* xrow[RG] = {};
-    bool xin[RG] = {};
-    int fin = 0;  // the lane's features that exist
-    auto rows = [&]() {
-#pragma unroll
-        for (int q = 0; q < RG; ++q) {
-            xin[q] = rb + 8 * q + g < r1;
-            xrow[q] = reinterpret_cast<const uint16_t*>(p.x) + (int64_t)(xin[q] ? rb + 8 * q + g : 0) * p.ldx;
-        }
-    };
     auto next_item = [&]() {  // false: none left
         do {
             item += gridDim.x;
             if (item >= items) return false;
-            e = (int)(item / (unsigned)p.f_tiles);
-            expert_rows(p.offsets, e, p.R, rb, r1);
-        } while (rb >= r1);
-        f0 = (int)(item - (unsigned)e * p.f_tiles) * F;
-        const int f = f0 + H * g;
-        fin = clampi(p.N - f, 0, H);
-        wrow = p.packed + ((int64_t)e * p.N + (fin ? f : 0)) * p.words;
-        srow = reinterpret_cast<const T*>(p.scales) + (int64_t)e * p.parts * p.N + (fin ? f : 0);
-        it = 0;
+            next.e = (int)(item / (unsigned)p.f_tiles);
+            expert_rows(p.offsets, next.e, p.R, next.rb, next.r1);
+        } while (next.rb >= next.r1);
+        next.f0 = (int)(item - (unsigned)next.e * p.f_tiles) * F;
+        next.it = 0;
         return true;
+    };
+    // where the lane reads the next batch
+    const uint32_t* words = nullptr;
+    const T* scales = nullptr;
+    int fin = 0, k_next = 0;  // the lane's features that exist; its first input
+    auto aim = [&]() {
+        const int f = next.f0 + WF * fw + H * g;
+        fin = clampi(p.N - f, 0, H);
+        k_next = (next.it * p.k_warps + kw) * KB + 32 * PAIR * t;
+        words = p.packed + ((int64_t)next.e * p.N + (fin ? f : 0)) * p.words + k_next / 8;
+        scales = reinterpret_cast<const T*>(p.scales) + (int64_t)next.e * p.parts * p.N + (fin ? f : 0);
+        // the batch's inputs of 8 tokens, a line of 64 a lane, into L1
+#pragma unroll
+        for (int q = 0; q < RG * KB / 256; ++q) {
+            const int r = next.rb + 8 * (q % RG) + g, k = (next.it * p.k_warps + kw) * KB + 64 * t + 256 * (q / RG);
+            if (r < next.r1 && k < p.K) {
+                uint16_t touched;
+                asm volatile("ld.global.b16 %0, [%1];" : "=h"(touched) : "l"(reinterpret_cast<const uint16_t*>(p.x) + (int64_t)r * p.ldx + k) : "memory");
+            }
+        }
     };
     uint4 a[SUB][H];
     uint32_t sc[SUB][MT];  // two features' scales each
-    int k_now = 0;
-    auto load = [&]() {
-        k_now = (it * STREAM_WARPS + warp) * KB + 32 * t;
+    auto load_words = [&](int s, int h) {  // PAIR pieces from s on
 #pragma unroll
-        for (int s = 0; s < SUB; ++s) {
-            const int k = k_now + 128 * s;
-            const bool in = k < p.words * 8;
+        for (int i = 0; i < PAIR; ++i) a[s + i][h] = make_uint4(Q_ZERO, Q_ZERO, Q_ZERO, Q_ZERO);
+        if (k_next + input_of(s) >= p.words * 8 || h >= fin) return;  // (rows are whole blocks of 64 inputs)
+        const uint32_t* from = words + (int64_t)h * p.words + input_of(s) / 8;
+        if constexpr (PAIR == 2)
+            asm volatile("ld.global.L1::no_allocate.L2::256B.v8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+                : "=r"(a[s][h].x), "=r"(a[s][h].y), "=r"(a[s][h].z), "=r"(a[s][h].w),
+                  "=r"(a[s + 1][h].x), "=r"(a[s + 1][h].y), "=r"(a[s + 1][h].z), "=r"(a[s + 1][h].w) : "l"(from) : "memory");
+        else
+            asm volatile("ld.global.L1::no_allocate.L2::256B.v4.b32 {%0,%1,%2,%3}, [%4];"
+                : "=r"(a[s][h].x), "=r"(a[s][h].y), "=r"(a[s][h].z), "=r"(a[s][h].w) : "l"(from) : "memory");
+    };
+    auto load_scales = [&](int s) {
+        const int k = k_next + input_of(s);
+        const T* from = scales + (int64_t)min(k >> p.shift, p.parts - 1) * p.N;
 #pragma unroll
-            for (int h = 0; h < H; ++h) {
-                a[s][h] = make_uint4(Q_ZERO, Q_ZERO, Q_ZERO, Q_ZERO);
-                if (in && h < fin)
-                    asm volatile("ld.global.L1::no_allocate.L2::256B.v4.b32 {%0,%1,%2,%3}, [%4];"
-                        : "=r"(a[s][h].x), "=r"(a[s][h].y), "=r"(a[s][h].z), "=r"(a[s][h].w) : "l"(wrow + (int64_t)h * p.words + k / 8) : "memory");
-            }
-            const int part_at = min(k >> p.shift, p.parts - 1);
-            const T* from = srow + (int64_t)part_at * p.N;
+        for (int m = 0; m < MT; ++m) sc[s][m] = 0;
+        if (k >= p.words * 8) return;
+        if (p.wide_scales) {
+            if constexpr (MT == 1) { if (fin) sc[s][0] = *reinterpret_cast<const uint32_t*>(from); }
+            if constexpr (MT == 2) { if (fin) { const uint2 v = *reinterpret_cast<const uint2*>(from); sc[s][0] = v.x; sc[s][1] = v.y; } }
+        } else {
 #pragma unroll
-            for (int m = 0; m < MT; ++m) sc[s][m] = 0;
-            if (in && p.wide_scales && fin) {
-                if constexpr (MT == 1) sc[s][0] = *reinterpret_cast<const uint32_t*>(from);
-                if constexpr (MT == 2) { const uint2 v = *reinterpret_cast<const uint2*>(from); sc[s][0] = v.x; sc[s][1] = v.y; }
-                if constexpr (MT == 4) {
-                    const uint4 v = *reinterpret_cast<const uint4*>(from);
-                    sc[s][0] = v.x; sc[s][1] = v.y; sc[s][2] = v.z; sc[s][3] = v.w;
-                }
-            } else if (in) {
-#pragma unroll
-                for (int h = 0; h < H; ++h)
-                    if (h < fin) sc[s][h / 2] |= (uint32_t)reinterpret_cast<const uint16_t*>(from)[h] << (16 * (h & 1));
-            }
+            for (int h = 0; h < H; ++h)
+                if (h < fin) sc[s][h / 2] |= (uint32_t)reinterpret_cast<const uint16_t*>(from)[h] << (16 * (h & 1));
         }
     };
     bool more = next_item();
-    if (more) { rows(); load(); }
+    if (more) {
+        aim();
+#pragma unroll
+        for (int s = 0; s < SUB; ++s) {
+            load_scales(s);
+            if (s % PAIR == 0)
+#pragma unroll
+                for (int h = 0; h < H; ++h) load_words(s, h);
+        }
+    }
     float acc[MT][RG][4] = {};
     while (more) {
+        now = next;
+        const int k_now = k_next;
+        if (++next.it == rounds) {
+            next.it = 0;
+            next.rb += 8 * RG;
+            if (next.rb >= next.r1) more = next_item();
+        }
+        if (more) aim();
+        const bool complete = now.it + 1 == rounds;
+        const int rows = min(RG * 8, now.r1 - now.rb);
+        float first = 0.f, first_res = 0.f;  // bias and residual of the thread's first value
+        if (complete && threadIdx.x < rows * F) {
+            const int c = threadIdx.x / F, f = now.f0 + threadIdx.x - c * F;
+            if (f < p.N) {
+                if (p.bias) first = El<T>::to(reinterpret_cast<const T*>(p.bias)[(int64_t)now.e * p.N + f]);
+                if (residual) first_res = El<T>::to(residual[(now.rb + c) * p.ldr + f]);
+            }
+        }
 #pragma unroll
-        for (int s = 0; s < SUB; ++s)
+        for (int s0 = 0; s0 < SUB; s0 += PAIR) {
+            uint4 b[PAIR][4][RG];
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                uint4 b[RG];
+            for (int q = 0; q < RG; ++q) {
+                const int r = now.rb + 8 * q + g;
+                const uint16_t* xrow = reinterpret_cast<const uint16_t*>(p.x) + (int64_t)(r < now.r1 ? r : 0) * p.ldx;
 #pragma unroll
-                for (int q = 0; q < RG; ++q) b[q] = load8<VB>(xrow[q], k_now + 128 * s + 8 * j, p.K, xin[q]);
+                for (int i = 0; i < PAIR; ++i)
 #pragma unroll
-                for (int m = 0; m < MT; ++m) {
-                    uint32_t lo[4], hi[4];
-                    const uint4 &u = a[s][2 * m], &v = a[s][2 * m + 1];
-                    unpack<T>(j == 0 ? u.x : j == 1 ? u.y : j == 2 ? u.z : u.w, __byte_perm(sc[s][m], 0, 0x1010), lo);
-                    unpack<T>(j == 0 ? v.x : j == 1 ? v.y : j == 2 ? v.z : v.w, __byte_perm(sc[s][m], 0, 0x3232), hi);
+                    for (int j = 0; j < 4; ++j) b[i][j][q] = load8<VB>(xrow, k_now + input_of(s0 + i) + 8 * j, p.K, r < now.r1);
+            }
 #pragma unroll
-                    for (int q = 0; q < RG; ++q) {
-                        mma16816<T>(acc[m][q], lo[0], hi[0], lo[1], hi[1], b[q].x, b[q].y);
-                        mma16816<T>(acc[m][q], lo[2], hi[2], lo[3], hi[3], b[q].z, b[q].w);
+            for (int m = 0; m < MT; ++m) {
+#pragma unroll
+                for (int i = 0; i < PAIR; ++i) {
+                    const uint32_t even = __byte_perm(sc[s0 + i][m], 0, 0x1010), odd = __byte_perm(sc[s0 + i][m], 0, 0x3232);
+                    const uint4 u = a[s0 + i][2 * m], v = a[s0 + i][2 * m + 1];
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        uint32_t lo[4], hi[4];
+                        unpack<T>(j == 0 ? u.x : j == 1 ? u.y : j == 2 ? u.z : u.w, even, lo);
+                        unpack<T>(j == 0 ? v.x : j == 1 ? v.y : j == 2 ? v.z : v.w, odd, hi);
+#pragma unroll
+                        for (int q = 0; q < RG; ++q) {
+                            mma16816<T>(acc[m][q], lo[0], hi[0], lo[1], hi[1], b[i][j][q].x, b[i][j][q].y);
+                            mma16816<T>(acc[m][q], lo[2], hi[2], lo[3], hi[3], b[i][j][q].z, b[i][j][q].w);
+                        }
                     }
                 }
+                if (more) {
+                    load_words(s0, 2 * m);
+                    load_words(s0, 2 * m + 1);
+                }
             }
-        // the next batch's loads, then what this one completes
-        const int done_e = e, done_f = f0, done_rb = rb, done_r1 = r1;
-        const bool complete = ++it == rounds;
-        if (complete) {
-            rb += 8 * RG;
-            if (rb < r1) it = 0; else more = next_item();
-            if (more) rows();
+            if (more)
+#pragma unroll
+                for (int i = 0; i < PAIR; ++i) load_scales(s0 + i);
         }
-        if (more) load();
         if (!complete) continue;
+        auto& part = parts[turn];
+        turn ^= 1;
 #pragma unroll
         for (int m = 0; m < MT; ++m)
 #pragma unroll
@@ -174,24 +225,31 @@ __global__ void __launch_bounds__(STREAM_WARPS * 32, 2) stream4_kernel(const Str
                     acc[m][q][i] = 0.f;
                 }
         __syncthreads();
-        for (int i = threadIdx.x; i < RG * 8 * F; i += STREAM_WARPS * 32) {
-            const int c = i / F, r = done_rb + c, f = done_f + i % F;
-            if (r < done_r1 && f < p.N) {
+        for (int i = threadIdx.x; i < rows * F; i += STREAM_WARPS * 32) {
+            const int c = i / F, of = i - c * F, r = now.rb + c, f = now.f0 + of;
+            if (f < p.N) {
                 float v = 0.f;
-#pragma unroll
-                for (int w = 0; w < STREAM_WARPS; ++w) v += part[w][c][i % F];
-                if (p.bias) v += El<T>::to(reinterpret_cast<const T*>(p.bias)[(int64_t)done_e * p.N + f]);
-                v = act_any(p.act, v);
-                if (residual) v += El<T>::to(residual[r * p.ldr + f]);
-                y[(int64_t)r * p.N + f] = El<T>::from(v);
+                for (int w = 0; w < p.k_warps; ++w) v += part[of / WF * p.k_warps + w][c][of % WF];
+                if (i >= STREAM_WARPS * 32) {
+                    first = p.bias ? El<T>::to(reinterpret_cast<const T*>(p.bias)[(int64_t)now.e * p.N + f]) : 0.f;
+                    first_res = residual ? El<T>::to(residual[r * p.ldr + f]) : 0.f;
+                }
+                y[(int64_t)r * p.N + f] = El<T>::from(act_any(p.act, v + first) + first_res);
             }
         }
-        __syncthreads();
     }
 }
 
+// As few warps share a contraction as leave no CTA without an item, since an item's end costs a
+// barrier: 16 experts of 4096 x 1024, a token each, take 12.0 us with one (256 items of 256
+// features), 14.0 with four; 4096 x 4096 alone 6.8 with eight, 24 with one.
 template <typename T, int RG, int MT, int SUB> int stream4_launch(Stream4Params p, bool vec, cudaStream_t st) {
-    p.f_tiles = (p.N + 16 * MT - 1) / (16 * MT);
+    const int64_t experts = p.E < p.R ? p.E : p.R;
+    const auto tiles = [&](int k_warps) { return (p.N + STREAM_WARPS / k_warps * 16 * MT - 1) / (STREAM_WARPS / k_warps * 16 * MT); };
+    p.k_warps = STREAM_WARPS;
+    while (p.k_warps > 1 && experts * tiles(p.k_warps / 2) >= 3 * sm_count() / 2) p.k_warps /= 2;
+    while (p.k_warps > 1 && p.k_warps / 2 * 128 * SUB >= p.words * 8) p.k_warps /= 2;  // (no batch for more)
+    p.f_tiles = tiles(p.k_warps);
     p.wide_scales = p.N % (2 * MT) == 0 && (reinterpret_cast<uintptr_t>(p.scales) & (4 * MT - 1)) == 0;
     const int64_t items = (int64_t)p.E * p.f_tiles, most = 2 * (int64_t)sm_count();
     if (items > INT32_MAX) return ELA_ERR_UNSUPPORTED;
@@ -199,7 +257,19 @@ template <typename T, int RG, int MT, int SUB> int stream4_launch(Stream4Params 
                   STREAM_WARPS * 32, 0, st, p);
 }
 
-// Rows per expert up to which the weights are streamed.
-inline bool few_rows_4bit(int64_t R, int64_t E, int64_t N) { return R <= 16 * E || (R <= 64 * E && E * ((N + 255) / 256) <= sm_count() / 4); }
+// Rows per expert up to which the weights are streamed (both ways in loops of 20): 16 rows for
+// each of 16 experts of 4096 x 1024 take 26.7 us here and 25.4 by tiles, of 4096 x 2048 40.7 and 41.3,
+// 8 rows 19.1 and 25.8, 31.1 and 41.2.  Where tiles of 256 features leave half of the pairs idle, up to
+// 32: 4096 x 4096 alone 15.7 and 23.1, with 64 rows 29.0 and 23.8.
+inline bool few_rows_4bit(int64_t R, int64_t E, int64_t N) { return R <= 16 * E || (R <= 32 * E && E * ((N + 255) / 256) <= sm_count() / 4); }
+
+// Eight tokens from one read of the weights, or sixteen.  Items of 16 features a warp where 32
+// would leave half of the CTAs without one.
+template <typename T> int stream4(const Stream4Params& p, bool vec, cudaStream_t st) {
+    const int64_t experts = p.E < p.R ? p.E : p.R;
+    const bool narrow = experts * ((p.N + 31) / 32) <= sm_count();
+    if (p.R <= 8 * p.E) return narrow ? stream4_launch<T, 1, 1, 4>(p, vec, st) : stream4_launch<T, 1, 2, 2>(p, vec, st);
+    return narrow ? stream4_launch<T, 2, 1, 4>(p, vec, st) : stream4_launch<T, 2, 2, 2>(p, vec, st);
+}
 
 }  // namespace ela_expert
