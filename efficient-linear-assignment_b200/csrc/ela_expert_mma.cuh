@@ -484,13 +484,13 @@ __device__ __forceinline__ void load_residual(uint32_t* res, const MmaParams& p,
 // a wait, a TMA instruction or a commit takes its thread some 100 cycles each, and with stages
 // of 64 the thread that loads was what all others waited for (700 cycles a stage).  Warp 0 loads
 // the columns, warp 2 the words, by TMA into a ring of their own, blocks of 128 features by 128
-// inputs with the scales of their groups.  Twelve warps unpack the blocks into the stages, half a
-// stage (64 inputs) by four of them in turn: a thread one feature's 64 inputs, which are eight
-// 16-byte pieces of the swizzled row (eight neighbouring lanes write eight different pieces: all
-// banks once).  A half is handed over by an arrival at the first CTA's barrier after the fence
-// that makes the writes visible to the tensor core of this SM, which alone reads them.  (The
-// fence waits for the thread's loads from memory, too: with the words loaded into registers
-// ahead, however far, 64 inputs took 900 cycles.)
+// inputs with the scales of their groups.  Twelve warps unpack the blocks into the stages, four
+// of them a stage in turn: a thread one feature's 128 inputs, which are twice eight 16-byte pieces
+// of a swizzled row (eight neighbouring lanes write eight different pieces: all banks once).  A
+// stage is handed over by an arrival at the first CTA's barrier after the fence that makes the
+// writes visible to the tensor core of this SM, which alone reads them.  (The fence waits for
+// the thread's loads from memory, too: with the words loaded into registers ahead, however far,
+// 64 inputs took 900 cycles.)
 constexpr int PACK_KB = 2 * MMA_KB;  // inputs of a stage, and of a block of words
 constexpr int PACK_WORDS = MMA_F * PACK_KB / 2, PACK_BLOCK = PACK_WORDS + 1024;  // bytes of a block's words; with its scales
 constexpr int PACK_MAX_RING = 8;
@@ -643,10 +643,11 @@ __device__ __forceinline__ void issue_products(const MmaParams4& p, uint32_t sta
     }
 }
 
-// Twelve warps: the halves of the stages of `tiles` tiles, in turn.  A half that the last stage
-// of a tile does not have is handed over as it is.  Four warps see two of three blocks; the
-// ring's size is a multiple of three, so that a slot is theirs every time or never, and no phase
-// of its barrier passes unseen.  (A stage's barrier may skip one: products end in order.)
+// Twelve warps: the stages of `tiles` tiles, every third by the same four.  The ring's size is a
+// multiple of three, so that a slot is theirs every time or never, and no phase of its barrier
+// passes unseen.  (A stage's barrier may skip one: products end in order.)  A turn's waits, fence
+// and hand-over take some 700 cycles beside 450 for each 64 inputs, so it is a whole stage: with
+// half a stage a turn the SM unpacked 64 inputs in 490 cycles.
 template <typename T, typename GiveUp>
 __device__ __forceinline__ void unpack_stages(const MmaParams4& p, uint32_t stages, int stage_bytes, uint32_t ring, uint64_t* full, uint64_t* empty,
                                               uint64_t* pfull, uint64_t* pempty, int tiles, GiveUp give_up, const volatile int* abort) {
@@ -654,55 +655,60 @@ __device__ __forceinline__ void unpack_stages(const MmaParams4& p, uint32_t stag
     uint32_t at[8];  // where a piece goes in half a stage
 #pragma unroll
     for (int j = 0; j < 8; ++j) at[j] = row * 128 + ((j ^ (row & 7)) << 4);
-    const uint32_t ready = leader_addr(full), second = p.shift == 5 ? 2 * MMA_F : 0;
-    const int blocks = (p.K + PACK_KB - 1) / PACK_KB, all = (p.K + MMA_KB - 1) / MMA_KB;
-    const int64_t count = 2 * (int64_t)tiles * blocks;
+    const uint32_t ready = leader_addr(full), second = p.shift == 5 ? 2 * MMA_F : 0, swap = row >> 1 & 3;
+    const int blocks = (p.K + PACK_KB - 1) / PACK_KB;
+    const bool odd = (p.K + MMA_KB - 1) / MMA_KB & 1;  // a tile's last stage has one half
+    const int64_t count = (int64_t)tiles * blocks;
     Place s, slot;
     int kb = 0;  // the block's number in its tile
-    auto next_block = [&]() {
-        s.advance(1, p.stages);
-        slot.advance(1, p.ring);
-        if (++kb == blocks) kb = 0;
+    auto advance = [&](int by) {
+        for (int i = 0; i < by; ++i) s.advance(1, p.stages);  // (there may be two)
+        slot.advance(by, p.ring);
+        kb += by;
+        while (kb >= blocks) kb -= blocks;
     };
-    if (w >= 8) next_block();
+    advance(w >> 2);
     for (int64_t n = w >> 2; n < count; n += PACK_TURNS) {
-        const int h = (int)(n & 1);
-        const bool there = 2 * kb + h < all;
-        uint32_t q[8];
-        uint16_t sc[2];
+        const bool two = !(odd && kb == blocks - 1);
         bool ok = bar_wait_warp(&pfull[slot.at], slot.phase, p.wait_ns, abort);
+        uint32_t q[2][8];
+        uint16_t sc[2][2];
         if (ok) {
-            // the row's 32 bytes of this half of a block (64-byte swizzle), and its groups' scales
-            const uint32_t from = ring + slot.at * PACK_BLOCK, words = from + row * 64 + ((2 * h ^ (row >> 1 & 3)) << 4);
-            const uint32_t scales = from + PACK_WORDS + row * 2 + (h * MMA_KB >> p.shift) * 2 * MMA_F;
-            asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];" : "=r"(q[0]), "=r"(q[1]), "=r"(q[2]), "=r"(q[3]) : "r"(words) : "memory");
-            asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];" : "=r"(q[4]), "=r"(q[5]), "=r"(q[6]), "=r"(q[7]) : "r"(words ^ 16) : "memory");
-            asm volatile("ld.shared.u16 %0, [%1];" : "=h"(sc[0]) : "r"(scales) : "memory");
-            asm volatile("ld.shared.u16 %0, [%1];" : "=h"(sc[1]) : "r"(scales + second) : "memory");
+            // the row's words (64-byte swizzle) and its groups' scales
+            const uint32_t from = ring + slot.at * PACK_BLOCK, words = from + row * 64, scales = from + PACK_WORDS + row * 2;
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];" : "=r"(q[h][0]), "=r"(q[h][1]), "=r"(q[h][2]), "=r"(q[h][3]) : "r"(words + ((2 * h ^ swap) << 4)) : "memory");
+                asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];" : "=r"(q[h][4]), "=r"(q[h][5]), "=r"(q[h][6]), "=r"(q[h][7]) : "r"(words + ((2 * h + 1 ^ swap) << 4)) : "memory");
+                const uint32_t group = scales + (h * MMA_KB >> p.shift) * 2 * MMA_F;
+                asm volatile("ld.shared.u16 %0, [%1];" : "=h"(sc[h][0]) : "r"(group) : "memory");
+                asm volatile("ld.shared.u16 %0, [%1];" : "=h"(sc[h][1]) : "r"(group + second) : "memory");
+            }
             ok = bar_wait_warp(&empty[s.at], s.phase ^ 1, p.wait_ns, abort);
         }
         if (!ok) {
             if (lane == 0) give_up();
             return;
         }
-        if (there) {
-            const uint32_t to = stages + s.at * stage_bytes + h * MMA_A_BYTES;
+        const uint32_t to = stages + s.at * stage_bytes;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            if (h && !two) break;
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
                 uint32_t out[4];
-                unpack<T>(q[j], sc[j / 4] * 0x10001u, out);
-                asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(to + at[j]), "r"(out[0]), "r"(out[1]), "r"(out[2]), "r"(out[3]) : "memory");
+                unpack<T>(q[h][j], sc[h][j / 4] * 0x10001u, out);
+                asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(to + h * MMA_A_BYTES + at[j]), "r"(out[0]), "r"(out[1]), "r"(out[2]), "r"(out[3]) : "memory");
             }
-            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         }
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         __syncwarp();
         if (lane == 0) {
             bar_arrive_leader(ready + 8 * s.at);
             bar_arrive(&pempty[slot.at]);
         }
         __syncwarp();
-        next_block();
-        if (h) next_block();
+        advance(PACK_TURNS);
     }
 }
 
@@ -747,12 +753,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(mma_threads<PASS>(),
     }
     if (tid == 0) {
         s_abort = 0;
-        // full: the loads of the pair, and the two halves of the weights that four warps of each CTA unpack
-        for (int s = 0; s < p.stages; ++s) { bar_init(&full[s], 1 + (PACKED ? 16 : 0)); bar_init(&empty[s], 1); }
+        // full: the loads of the pair, and the weights that four warps of each CTA unpack
+        for (int s = 0; s < p.stages; ++s) { bar_init(&full[s], 1 + (PACKED ? 8 : 0)); bar_init(&empty[s], 1); }
         for (int b = 0; b < 2; ++b) { bar_init(&tfull[b], 1); bar_init(&tempty[b], 2 * 4 * MMA_GROUPS); }
         for (int i = 0; i < MMA_TILES; ++i) { bar_init(&sfull[i], 1); bar_init(&sempty[i], 4 * MMA_GROUPS + 1 + (rank == 0) + PACKED); }
         if constexpr (PACKED)
-            for (int s = 0; s < p.ring; ++s) { bar_init(&pfull[s], 1); bar_init(&pempty[s], 8); }
+            for (int s = 0; s < p.ring; ++s) { bar_init(&pfull[s], 1); bar_init(&pempty[s], 4); }
         bar_init(&landed, 1);
         for (int s = 0; s < p.stages; ++s) bar_init(&patched[s], 1);
         bar_init(&drained, 1);
