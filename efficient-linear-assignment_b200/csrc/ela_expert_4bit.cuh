@@ -257,11 +257,13 @@ template <typename T, int RG, int MT, int SUB> int stream4_launch(Stream4Params 
                   STREAM_WARPS * 32, 0, st, p);
 }
 
-// Rows per expert up to which the weights are streamed (both ways in loops of 20): 16 rows for
-// each of 16 experts of 4096 x 1024 take 26.7 us here and 25.4 by tiles, of 4096 x 2048 40.7 and 41.3,
-// 8 rows 19.1 and 25.8, 31.1 and 41.2.  Where tiles of 256 features leave half of the pairs idle, up to
-// 32: 4096 x 4096 alone 15.7 and 23.1, with 64 rows 29.0 and 23.8.
-inline bool few_rows_4bit(int64_t R, int64_t E, int64_t N) { return R <= 16 * E || (R <= 32 * E && E * ((N + 255) / 256) <= sm_count() / 4); }
+// Rows per expert up to which the weights are streamed (both ways in loops of 20): 8 rows for
+// each of 16 experts of 4096 x 1024 take 19.1 us here and 22.9 by tiles, of 4096 x 2048 31.0 and
+// 34.5; 12 rows 37.3 and 34.6, 16 rows 26.6 and 22.4, 40.5 and 34.0.  Where tiles of 256 features
+// leave half of the pairs idle, up to 24: 4096 x 4096 alone with 16 rows 8.8 and 18.6, with 32 15.6
+// and 18.8, with 48 22.4 and 19.8; two of 2048 x 2048 with 16 rows each 8.9 and 13.1, with 32 15.6
+// and 13.3.
+inline bool few_rows_4bit(int64_t R, int64_t E, int64_t N) { return R <= 8 * E || (R <= 24 * E && E * ((N + 255) / 256) <= sm_count() / 4); }
 
 // Eight tokens from one read of the weights, or sixteen.  Items of 16 features a warp where 32
 // would leave half of the CTAs without one.
