@@ -20,6 +20,8 @@
 // rest of the kernel.
 #include "ela_expert.cuh"
 
+#include <type_traits>
+
 namespace ela_expert {
 
 constexpr int ROUTE_THREADS = 128, ROUTE_WIDE = 256;  // threads of a block; of a row's block past 512 experts
@@ -27,7 +29,7 @@ constexpr int ROUTE_THREADS = 128, ROUTE_WIDE = 256;  // threads of a block; of 
 struct RouteParams {
     const void* logits;
     int64_t T, ld;
-    int E, k, vec;  // vec: rows may be read 16 bytes at a time
+    int E, k, vec, vec_bias;  // vec: rows may be read 16 bytes at a time
     const float* bias;
     int groups, kept, top2;
     int sigmoid, renormalize;
@@ -237,6 +239,8 @@ __device__ __forceinline__ bool route_choose(const RouteParams& p, const T* row,
     const int lane = Tm::lane(), e0 = lane * VPT;
     const bool computed = p.bias != nullptr;             // keys are scores and a bias, not logits
     const bool scores = computed || p.top2;
+    float bias[VPT];
+    if (computed) load_logits<float, VPT>(bias, p.bias, e0, p.E, p.vec_bias, true);
     F value[VPT];                                        // score + bias
     F size = 0;                                          // the largest score, and value
     if (scores) {
@@ -259,7 +263,7 @@ __device__ __forceinline__ bool route_choose(const RouteParams& p, const T* row,
         for (int i = 0; i < VPT; ++i) {
             if (!p.sigmoid) value[i] *= inv;
             if (CHECK) size = value[i] > size ? value[i] : size;
-            if (computed && e0 + i < p.E) value[i] += p.bias[e0 + i];
+            if (computed && e0 + i < p.E) value[i] += bias[i];
             const F v = value[i] < 0 ? -value[i] : value[i];
             if (CHECK && v > most && v < INFINITY) most = v;
         }
@@ -273,7 +277,7 @@ __device__ __forceinline__ bool route_choose(const RouteParams& p, const T* row,
     U key[VPT];
 #pragma unroll
     for (int i = 0; i < VPT; ++i) {
-        const bool there = e0 + i < p.E && l[i] != -INFINITY && !(computed && p.bias[e0 + i] == -INFINITY);
+        const bool there = l[i] != -INFINITY && !(computed && bias[i] == -INFINITY);  // (past the last expert both are)
         if (scores && !there) value[i] = -INFINITY;
         key[i] = there ? ordered(computed ? value[i] : (F)l[i]) : 0;
     }
@@ -546,6 +550,7 @@ template <typename T, int LANES, int VPT> int route_launch(const RouteGradParams
 template <typename T, typename P> int route_by_size(P p, cudaStream_t st) {
     const int per = p.E <= 128 ? 8 : 16;
     p.vec = p.vec && p.E % per == 0;
+    if constexpr (std::is_same_v<P, RouteParams>) p.vec_bias = p.vec_bias && p.E % per == 0;
     return p.E <= 8 ? route_launch<T, 1, 8>(p, st) : p.E <= 16 ? route_launch<T, 2, 8>(p, st) : p.E <= 32 ? route_launch<T, 4, 8>(p, st)
          : p.E <= 64 ? route_launch<T, 8, 8>(p, st) : p.E <= 128 ? route_launch<T, 16, 8>(p, st) : p.E <= 256 ? route_launch<T, 16, 16>(p, st)
          : p.E <= 512 ? route_launch<T, 32, 16>(p, st) : route_launch<T, ROUTE_WIDE, 16>(p, st);
@@ -575,7 +580,7 @@ int ela_expert_route(const void* logits, int dtype, int64_t T, int64_t E, int64_
     if (T == 0) return ELA_OK;
     if (!logits || !expert || !weights || !on_elements(dtype_bytes(dtype), logits) || !on_elements(4, bias, expert, weights)) return ELA_ERR_ARGUMENT;
     if (groups == groups_kept) groups = groups_kept = 1;  // all stay
-    RouteParams p = {logits, T, ld, (int)E, (int)k, aligned16(logits, ld * dtype_bytes(dtype)), bias, (int)groups, (int)groups_kept,
+    RouteParams p = {logits, T, ld, (int)E, (int)k, aligned16(logits, ld * dtype_bytes(dtype)), aligned16(bias), bias, (int)groups, (int)groups_kept,
                      groups > 1 && group_score == ELA_GROUP_TOP2, score == ELA_SCORE_SIGMOID, renormalize != 0, scale, expert, weights};
     return route_by_type(p, dtype, reinterpret_cast<cudaStream_t>(stream));
 }
