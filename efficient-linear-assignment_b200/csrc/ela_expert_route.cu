@@ -6,8 +6,9 @@
 // VPT consecutive experts in registers; one pass reads the row once, and everything else
 // (softmax, groups, choice, weights) stays in registers, shuffles and a little shared memory.
 //
-// The k largest keys: the k-th largest of the threads' own largest keys is a bound that at
-// least k keys reach, and few others do (a dozen for 8 of 256).  Those that reach it are put
+// The k largest keys: the k-th largest of the threads' own two largest keys is a bound that at
+// least k keys reach, and few others do (one or two for 8 of 256; with each thread's largest
+// alone some 30 where groups leave half of the threads without a key).  Those that reach it are put
 // side by side in shared memory, in the order of the experts, and each counts the keys above
 // it, which is its rank.  8 of 256 experts take a third of the instructions of k rounds of
 // "largest key left", each with a search by the thread that had it.
@@ -267,12 +268,13 @@ __device__ __forceinline__ bool route_choose(const RouteParams& p, const T* row,
             const F v = value[i] < 0 ? -value[i] : value[i];
             if (CHECK && v > most && v < INFINITY) most = v;
         }
-        // A sigmoid is off by at most 2^-22: the exponent's rounding moves it by s (1 - s) |x| 2^-24, the
-        // exponential's by s (1 - s) 2^-22, the reciprocal by s 2^-23.  A softmax is off by 2^-22 of the
-        // largest for its exponential, and by the row's sum, at most 29 additions one after the other of such
-        // terms, 2^-19.  A sum with the bias is off by another 2^-24 of the value.  Two keys that differ by
-        // more than this (2^-20 or 2^-17, and 2^-21) are in the right order.
-        if (CHECK) size = Tm::most(size) * (p.sigmoid ? (F)9.5367431640625e-7 : (F)7.62939453125e-6) + Tm::most(most) * (F)4.76837158203125e-7;
+        // A sigmoid is off by at most 1.1 * 2^-22: the exponent's rounding moves it by s (1 - s) |x| 1.5 * 2^-24,
+        // under 2^-25, the exponential's by s (1 - s) 2^-22, at most 2^-24, the sum and the reciprocal by
+        // s (2^-24 + 2^-23).  A softmax is off by 2^-22 of the largest for its exponential, and by the row's
+        // sum, at most 29 additions one after the other of such terms, 2^-19.  A sum with the bias is off by
+        // another 2^-24 of the value.  Two keys that differ by more than this (1.4 * 2^-21 or 2^-17 of the
+        // largest score, and 1.25 * 2^-23 of the largest value) are in the right order.
+        if (CHECK) size = Tm::most(size) * (p.sigmoid ? (F)6.67572021484375e-7 : (F)7.62939453125e-6) + Tm::most(most) * (F)1.4901161193847656e-7;
     }
     U key[VPT];
 #pragma unroll
@@ -337,15 +339,19 @@ __device__ __forceinline__ bool route_choose(const RouteParams& p, const T* row,
             }
         }
     }
-    // the bound: the k-th of the threads' largest keys (equal ones leave together, which lowers it)
-    U best = key[0];
+    // the bound: the k-th of the threads' two largest keys each (equal ones leave together, which lowers it)
+    U best = key[0], second = 0;
 #pragma unroll
-    for (int i = 1; i < VPT; ++i) best = key[i] > best ? key[i] : best;
+    for (int i = 1; i < VPT; ++i) {
+        const U less = key[i] < best ? key[i] : best;
+        second = less > second ? less : second;
+        best = key[i] > best ? key[i] : best;
+    }
     U bound = 0;
     for (int j = 0; j < p.k; ++j) {
         bound = Tm::most(best);
-        if (best == bound) best = 0;
-        if (LANES <= 32 && j >= LANES) break;  // (none left)
+        if (best == bound) { best = second; second = 0; }
+        if (LANES <= 32 && j >= 2 * LANES) break;  // (none left)
     }
     if (CHECK && computed && bound != 0) bound = ordered(number(bound) - size);  // what may belong to them in 64 bits, too
     if (bound == 0) bound = 1;
