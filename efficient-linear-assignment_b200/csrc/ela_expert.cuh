@@ -174,8 +174,9 @@ template <int ACT> __device__ __forceinline__ float act_value_lean(float z) {
         q = fmaf(q, t, -0.142248368f);
         q = fmaf(q, t, 0.127414796f);
         const float tail = q * t * gauss;
-        // (NaN stays NaN by the tail; infinity times a tail of 0 must not make one)
-        return fmaf(-fminf(x, 1e18f), tail, fmaxf(z, 0.f));
+        // (NaN stays NaN by the tail; infinity times a tail of 0 must not make one; -infinity has none but NaN,
+        // as in act_value)
+        return fmaf(-fabsf(fminf(z, 1e18f)), tail, fmaxf(z, 0.f));
     }
     if (ACT == ELA_ACT_SILU) return z * reciprocal_fast(1.f + exp2_fast(z * -1.4426950408889634f));
     return act_value<ACT>(z);

@@ -213,6 +213,7 @@ int ela_expert_linear_4bit(const void* x, const int32_t* packed, const void* sca
         ELA_BY_TYPE(dtype, { rc = stream4<T_>(p, vec, st); })
         return rc;
     }
+    if (E * parts > INT32_MAX) return ELA_ERR_UNSUPPORTED;
     char* ws = reinterpret_cast<char*>(workspace);
     Matrix mx = {x, 1, R, K, ldx, 0}, ms = {scales, 1, E * parts, N, N, 0};
     if ((rc = readable(mx, ws, workspace_bytes, st)) != ELA_OK || (rc = readable(ms, ws, workspace_bytes, st)) != ELA_OK) return rc;

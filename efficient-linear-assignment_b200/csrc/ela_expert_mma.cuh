@@ -712,6 +712,11 @@ __device__ __forceinline__ void unpack_stages(const MmaParams4& p, uint32_t stag
     }
 }
 
+// Registers of a thread after the roles have shared them out anew: operands, epilogue, unpacking.
+// (setmaxnreg takes its numbers as they stand in the text: the statements below repeat them.)
+constexpr int PACK_REGS = 128 * (64 + MMA_GROUPS * 112 + PACK_TURNS * 64);
+static_assert(PACK_REGS <= 80 * (MMA_THREADS + 32 * MMA_UNPACK), "more than 80 registers a thread");
+
 // Threads of a CTA.
 template <int PASS> constexpr int mma_threads() { return MMA_THREADS + (PASS == PASS_4BIT ? 32 * MMA_UNPACK : 0); }
 
@@ -811,8 +816,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(mma_threads<PASS>(),
         return t.e >= 0;
     };
 
-    // registers from the warps that need few to those of the epilogue (a block of 768 threads has 80 each:
-    // 128 * (64 + 2 * 112 + 3 * 64) of them)
+    // registers from the warps that need few to those of the epilogue: PACK_REGS in all, which the
+    // launch has checked that the block has (the epilogue's warps would wait for ever for more)
     if constexpr (PACKED) {
         if (warp < 4) asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
         else if (warp < 4 + 4 * MMA_GROUPS) asm volatile("setmaxnreg.inc.sync.aligned.u32 112;");
@@ -1160,6 +1165,15 @@ int mma_launch(const CUtensorMap& a, const CUtensorMap& b, const typename Params
     auto kern = mma_kernel<PASS, T, ACT, Z>;
     const int sms = sm_count();
     if (sms == 0 || !allow_smem<&mma_kernel<PASS, T, ACT, Z>>(MMA_SMEM - 1024)) return ELA_ERR_CUDA;
+    if constexpr (PASS == PASS_4BIT) {
+        static std::atomic<bool> enough{false};
+        cudaFuncAttributes attr;
+        if (!enough.load(std::memory_order_relaxed)) {
+            if (cudaFuncGetAttributes(&attr, kern) != cudaSuccess) return ELA_ERR_CUDA;
+            if (attr.numRegs * mma_threads<PASS>() < PACK_REGS) return ELA_ERR_INTERNAL;
+            enough.store(true, std::memory_order_relaxed);
+        }
+    }
     const int grid = 2 * (int)(max_tiles < sms / 2 ? max_tiles : sms / 2);
     return launch(kern, grid, mma_threads<PASS>(), MMA_SMEM - 1024, st, a, b, p);
 }

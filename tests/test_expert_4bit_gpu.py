@@ -296,6 +296,69 @@ def test_offsets_out_of_range_stay_inside():
     ela.expert_check()
 
 
+@pytest.mark.parametrize("E,R", [(700, 9000), (4096, 40000)])
+def test_many_experts_in_tiles(E, R):
+    """More experts than fit beside many stages; every expert a few rows, some none."""
+    g = gen(E)
+    counts = torch.multinomial(torch.rand(E, generator=g) * (torch.rand(E, generator=g) < 0.9), R - 50, replacement=True, generator=g).bincount(minlength=E)
+    assert R > 8 * E
+    x, w, b, r, off = product_case(R, E, 200, 40, torch.bfloat16, 3, counts.tolist(), 20)
+    check(x, w, b, r, off, "silu")
+
+
+def test_wide_offsets_out_of_range_in_tiles():
+    x, w, _, r, _ = product_case(500, 3, 200, 300, torch.bfloat16, 6, [100, 100, 300])
+    for off in ([-5, 300, 2 ** 30, 2 ** 30], [300, 100, 50, 400], [2 ** 31 - 1] * 4, [-2 ** 31] * 4, [0, 0, 0, 0], [0, 500, 0, 500]):
+        y = ela.expert_linear_4bit(x.cuda(), w, None, r.cuda(), "none", torch.tensor(off, dtype=torch.int32, device="cuda"))
+        assert y.shape == (500, 300)
+    torch.cuda.synchronize()
+    ela.expert_check()
+
+
+def test_two_calls_at_once_with_workspaces():
+    """Odd widths, whose operands are copied into a workspace, on two streams, over and over."""
+    cases = []
+    for seed in (1, 2):
+        x, w, b, r, off = product_case(900, 3, 205, 333, torch.bfloat16, seed, [300, 0, 600])
+        cases.append((x.cuda(), w, b.cuda(), r.cuda(), "gelu", torch.tensor(off, dtype=torch.int32, device="cuda")))
+    want = [ela.expert_linear_4bit(*c) for c in cases]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in cases]
+    got = [[], []]
+    for _ in range(10):
+        for i, (s, c) in enumerate(zip(streams, cases)):
+            with torch.cuda.stream(s):
+                got[i].append(ela.expert_linear_4bit(*c))
+    torch.cuda.synchronize()
+    for i in range(2):
+        assert all(torch.equal(y, want[i]) for y in got[i])
+
+
+def test_activations_of_extreme_sums():
+    """Sums from the far tails: what rounds to 0 may be 0, infinities and NaN come out as the formula has them."""
+    K, N = 64, 32
+    w = ela.expert_quantize(torch.eye(N, K).to(torch.bfloat16).mul(7).cuda(), 32)  # feature n: 7 x_n
+    z = torch.tensor([0.0, -0.0, 1e-30, -1e-30, 0.5, -0.5, 3.0, -3.0, 6.0, -6.0, 12.0, -12.0, 14.0, -14.0, 80.0, -80.0, 100.0, -100.0, 1e4, -1e4,
+                      1e18, -1e18, 1e20, -1e20, 3e37, -3e37, math.inf, -math.inf, math.nan, 1.0, -1.0, 2.0])
+    x = torch.zeros(300, K)
+    x[:, :N] = z / 7
+    x[:, 26:29] = 0  # (an infinity times the other features' zeros would be NaN everywhere)
+    x = x.to(torch.bfloat16).cuda()
+    bias = torch.zeros(N)
+    bias[26:29] = z[26:29]
+    bias = bias.to(torch.bfloat16).cuda()
+    s = (x[0, :N].double() * 7 + bias.double()).cpu()
+    for act in ("relu", "gelu", "silu"):
+        want = act64(s, act)
+        for rows in (2, 300):
+            y = ela.expert_linear_4bit(x[:rows], w, bias, None, act).double().cpu()
+            assert torch.equal(y[0], y[-1]) or y[0].isnan().any()
+            y, fin = y[0], want.isfinite()
+            assert y[28].isnan() and y[26] == math.inf and (y[27] == 0 if act == "relu" else y[27].isnan())  # -inf * 0
+            own = torch.where(want != 0, 2.0 ** -20 * (1 + s.abs()), torch.zeros_like(s))[fin]  # (a product with 0 would be NaN at -inf)
+            assert ((y - want).abs()[fin] <= own + 2.0 ** -8 * 1.01 * want.abs()[fin] + 2.0 ** -20).all()
+
+
 def test_large_sums_and_large_values():
     """Values whose sums pass fp16's range come out as infinities, as rounding makes them."""
     x = torch.full((3, 256), 200.0).half()
