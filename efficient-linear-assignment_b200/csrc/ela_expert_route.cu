@@ -497,14 +497,16 @@ __global__ void __launch_bounds__(Team<LANES>::BLOCK) route_grad_kernel(const __
         if (p.sigmoid) return p.renormalize ? expf(fminf(x, 0.f) - most) / (1.f + expf(-fabsf(x))) / sum : 1.f / (1.f + expf(-x));
         return expf(x - most) / sum;
     };
+    // (rounded by itself: joined with the subtraction of the mean it left 2^-24 of a gradient that is 0)
+    auto weighted = [&](int j) { return __fmul_rn(p.scale, p.dweights[t * p.k + j]); };
     if (!p.sigmoid || p.renormalize) {
         for (int j = lane; j < p.k; j += LANES)
-            if (s.at[j] >= 0) mean = fmaf(p.scale * p.dweights[t * p.k + j], ratio(s.logit[j]), mean);
+            if (s.at[j] >= 0) mean = fmaf(weighted(j), ratio(s.logit[j]), mean);
         mean = Tm::sum(mean);
     }
     for (int j = lane; j < p.k; j += LANES)
         if (s.at[j] >= 0) {
-            const float x = s.logit[j], c = p.scale * p.dweights[t * p.k + j];
+            const float x = s.logit[j], c = weighted(j);
             s.logit[j] = dense ? c : ratio(x) * (c - mean) * (p.sigmoid ? 1.f / (1.f + expf(x)) : 1.f);
         }
     Tm::sync();

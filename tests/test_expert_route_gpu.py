@@ -280,6 +280,16 @@ def test_gradient_against_differences():
                     assert abs((q[0] - q[1]) / (2 * h) - d[t, e].item()) <= 1e-6 + 1e-6 * dw.abs().max()
 
 
+def test_gradient_of_one_renormalized_choice_is_zero():
+    """The weight of a single choice is the scale, whatever the logits."""
+    for score in ("softmax", "sigmoid"):
+        l = make(300, 216, torch.float32, 5, padding=4).cuda().requires_grad_()
+        w = ela.expert_route(l, 1, score, scale=2.5).weights
+        assert (w[:296] == 2.5).all() and (w[296:] == 0).all()
+        (d,) = torch.autograd.grad(w, l, torch.randn(300, 1, generator=gen(6)).cuda() * 5)
+        assert (d == 0).all()
+
+
 def test_strides_broadcast_gradients_and_offsets():
     wide = make(50, 64, torch.bfloat16, 11)
     for view in (wide[:, :31], wide[:, 1:33], wide[::2, :32], wide[:, ::2], wide.t()):
