@@ -645,7 +645,11 @@ __device__ __forceinline__ void issue_products(const MmaParams4& p, uint32_t sta
 
 // Twelve warps: the stages of `tiles` tiles, every third by the same four.  The ring's size is a
 // multiple of three, so that a slot is theirs every time or never, and no phase of its barrier
-// passes unseen.  (A stage's barrier may skip one: products end in order.)  A turn's waits, fence
+// passes unseen.  Of a stage's barrier they may miss phases, since with S stages the four see it
+// every S blocks of theirs and it passes one phase every S blocks of all.  Before block n they know
+// from block n - 3 that the product of n - 3 - S has ended, and with it all before; the parity
+// of the product of n - S, which they wait for, tells it from that of n - 2 S if that one has
+// ended: for S of three and more, which columns_per_tile leaves.  A turn's waits, fence
 // and hand-over take some 700 cycles beside 450 for each 64 inputs, so it is a whole stage: with
 // half a stage a turn the SM unpacked 64 inputs in 490 cycles.
 template <typename T, typename GiveUp>
@@ -662,7 +666,7 @@ __device__ __forceinline__ void unpack_stages(const MmaParams4& p, uint32_t stag
     Place s, slot;
     int kb = 0;  // the block's number in its tile
     auto advance = [&](int by) {
-        for (int i = 0; i < by; ++i) s.advance(1, p.stages);  // (there may be two)
+        s.advance(by, p.stages);
         slot.advance(by, p.ring);
         kb += by;
         while (kb >= blocks) kb -= blocks;
@@ -1178,6 +1182,17 @@ int mma_launch(const CUtensorMap& a, const CUtensorMap& b, const typename Params
     return launch(kern, grid, mma_threads<PASS>(), MMA_SMEM - 1024, st, a, b, p);
 }
 
+constexpr int ring_for(int bn) { return bn > 64 ? PACK_TURNS : 2 * PACK_TURNS; }  // 4-bit weights: blocks of words in flight
+constexpr int stages_for(int bn, int64_t E, int ring = 0) {
+    const int64_t n = (MMA_SMEM - 1024 - MMA_SMEM_FIXED - 12 * E - ring * PACK_BLOCK) / ((MMA_A_BYTES + bn / 2 * MMA_KB * 2) * (ring ? 2 : 1));
+    return (int)(n < MMA_MAX_STAGES ? n : MMA_MAX_STAGES);
+}
+// The 4-bit pass needs a stage for each turn of the warps that unpack (unpack_stages).  The experts'
+// tables take the place of some: 256 columns leave three up to 512 experts, 192 up to 2560, and these always.
+constexpr bool enough_stages(int bn, int64_t E) { return stages_for(bn, E, ring_for(bn)) >= PACK_TURNS; }
+static_assert(enough_stages(128, ELA_EXPERT_MAX) && enough_stages(96, ELA_EXPERT_MAX) && enough_stages(64, ELA_EXPERT_MAX) && enough_stages(32, ELA_EXPERT_MAX),
+              "too few stages for 4-bit weights");
+
 // Columns per tile of the row passes, a multiple of 32 up to 256: the one whose rounds of
 // tiles over the pairs take least.  A block of 64 k takes the longer of its products (2
 // cycles a column) and its loads (16 KB of weights and 64 bytes a column, at the 57
@@ -1192,16 +1207,13 @@ inline int columns_per_tile(int64_t R, int64_t E, int64_t f_tiles, int64_t k_blo
     int best = 256;
     int64_t least = INT64_MAX;
     for (int bn = 256; bn >= 32; bn -= 32) {
+        if (packed && !enough_stages(bn, E)) continue;
         const int64_t tiles = f_tiles * (E < R ? E : R) * ((rows + bn - 1) / bn), used = rows < bn ? (rows + 31) / 32 * 32 : bn;
         const int64_t loads = packed ? std::max<int64_t>((4096 + 64 * used) / 57, 200) : (16384 + 64 * used) / 57, block = 2 * used > loads ? 2 * used : loads;
         const int64_t time = (tiles + pairs - 1) / pairs * (k_blocks * block + 500);
         if (time < least || (time == least && rows <= bn)) { least = time; best = bn; }  // (a smaller stage leaves room for more)
     }
     return best;
-}
-inline int stages_for(int bn, int64_t E, int ring = 0) {
-    const int64_t n = (MMA_SMEM - 1024 - MMA_SMEM_FIXED - 12 * E - ring * PACK_BLOCK) / ((MMA_A_BYTES + bn / 2 * MMA_KB * 2) * (ring ? 2 : 1));
-    return (int)(n < MMA_MAX_STAGES ? n : MMA_MAX_STAGES);
 }
 
 // Limit of every device-side wait: 2 s, and 4 us for each block of 64 k of a tile's sum, ten times
@@ -1293,7 +1305,7 @@ inline MmaParams row_pass(const int32_t* offsets, int64_t R, int64_t E, int64_t 
     // a CTA's half of a tile's columns is one box, or boxes of 64 where experts have fewer rows
     // than that makes (a box is loaded whole)
     p.bbox = p.bn % 128 == 0 && R < 256 * E ? 64 : p.bn / 2;
-    p.ring = packed ? p.bn > 64 ? PACK_TURNS : 2 * PACK_TURNS : 0;
+    p.ring = packed ? ring_for(p.bn) : 0;
     p.stages = stages_for(p.bn, E, p.ring);
     p.wait_ns = wait_limit(K);
     return p;
