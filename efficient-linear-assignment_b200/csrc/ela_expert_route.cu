@@ -268,13 +268,21 @@ __device__ __forceinline__ bool route_choose(const RouteParams& p, const T* row,
             const F v = value[i] < 0 ? -value[i] : value[i];
             if (CHECK && v > most && v < INFINITY) most = v;
         }
-        // A sigmoid is off by at most 1.1 * 2^-22: the exponent's rounding moves it by s (1 - s) |x| 1.5 * 2^-24,
-        // under 2^-25, the exponential's by s (1 - s) 2^-22, at most 2^-24, the sum and the reciprocal by
-        // s (2^-24 + 2^-23).  A softmax is off by 2^-22 of the largest for its exponential, and by the row's
+        // A sigmoid's exponential is off by (1.5 |x| + 4) 2^-24 of itself (its exponent's rounding, its own error),
+        // which moves the sigmoid by 1 - s of that, and the sum and the reciprocal move it by 3 * 2^-24.  For
+        // x >= 0 that makes 3.4 * 2^-24, 5 * 2^-24 of the row's largest score S at most; below 0, where both the
+        // score and its error grow with x, (1.5 |x| (1 - S) + 4 (1 - S) + 3) 2^-24 of S for the largest x.  Where S lies
+        // in [2^e, 2^(e+1)), |x| is at most -0.7 e, and (5.6 + 2 (-1 - e)) 2^-24 is more for every e.  A score below
+        // 2^-126 comes out as 0.  A softmax is off by 2^-22 of the largest for its exponential, and by the row's
         // sum, at most 29 additions one after the other of such terms, 2^-19.  A sum with the bias is off by
-        // another 2^-24 of the value.  Two keys that differ by more than this (1.4 * 2^-21 or 2^-17 of the
-        // largest score, and 1.25 * 2^-23 of the largest value) are in the right order.
-        if (CHECK) size = Tm::most(size) * (p.sigmoid ? (F)6.67572021484375e-7 : (F)7.62939453125e-6) + Tm::most(most) * (F)1.4901161193847656e-7;
+        // another 2^-24 of the value.  Two keys that differ by more than twice all this (2^-17 of the largest score for
+        // a softmax, and 1.25 * 2^-23 of the largest value) are in the right order.
+        if (CHECK) {
+            size = Tm::most(size);
+            const float below = (float)(126 - (int)(__float_as_uint((float)size) >> 23));  // -1 - e
+            size = p.sigmoid ? fmaf((float)size, (5.6f + 2.f * fmaxf(below, 0.f)) * 1.1920928955078125e-7f, 2.3509887e-38f) : size * (F)7.62939453125e-6;
+            size += Tm::most(most) * (F)1.4901161193847656e-7;
+        }
     }
     U key[VPT];
 #pragma unroll
