@@ -243,7 +243,7 @@ __device__ __forceinline__ bool route_choose(const RouteParams& p, const T* row,
     float bias[VPT];
     if (computed) load_logits<float, VPT>(bias, p.bias, e0, p.E, p.vec_bias, true);
     F value[VPT];                                        // score + bias
-    F size = 0;                                          // the largest score, and value
+    F size = 0;                                          // what two keys' scores may be off by together
     if (scores) {
         F m = 0, inv = 0;
         if (!p.sigmoid) {
@@ -259,14 +259,11 @@ __device__ __forceinline__ bool route_choose(const RouteParams& p, const T* row,
             if (!p.sigmoid) inv += value[i];
         }
         if (!p.sigmoid) inv = one_over(Tm::sum(inv));
-        F most = 0;
 #pragma unroll
         for (int i = 0; i < VPT; ++i) {
             if (!p.sigmoid) value[i] *= inv;
             if (CHECK) size = value[i] > size ? value[i] : size;
             if (computed && e0 + i < p.E) value[i] += bias[i];
-            const F v = value[i] < 0 ? -value[i] : value[i];
-            if (CHECK && v > most && v < INFINITY) most = v;
         }
         // A sigmoid's exponential is off by (1.5 |x| + 4) 2^-24 of itself (its exponent's rounding, its own error),
         // which moves the sigmoid by 1 - s of that, and the sum and the reciprocal move it by 3 * 2^-24.  For
@@ -274,16 +271,18 @@ __device__ __forceinline__ bool route_choose(const RouteParams& p, const T* row,
         // score and its error grow with x, (1.5 |x| (1 - S) + 4 (1 - S) + 3) 2^-24 of S for the largest x.  Where S lies
         // in [2^e, 2^(e+1)), |x| is at most -0.7 e, and (5.6 + 2 (-1 - e)) 2^-24 is more for every e.  A score below
         // 2^-126 comes out as 0.  A softmax is off by 2^-22 of the largest for its exponential, and by the row's
-        // sum, at most 29 additions one after the other of such terms, 2^-19.  A sum with the bias is off by
-        // another 2^-24 of the value.  Two keys that differ by more than twice all this (2^-17 of the largest score for
-        // a softmax, and 1.25 * 2^-23 of the largest value) are in the right order.
+        // sum, at most 29 additions one after the other of such terms, 2^-19; two of them by 2^-17.  A sum with
+        // the bias is off by another 2^-24 of itself, which is allowed for key by key: one bias of -1e9
+        // for an expert that is out of the question leaves the others their digits (by the row's largest
+        // value every one was in doubt: 8192 x 256 took 120 and 260 us with and without groups, usual ones 17 and 14).
         if (CHECK) {
             size = Tm::most(size);
             const float below = (float)(126 - (int)(__float_as_uint((float)size) >> 23));  // -1 - e
             size = p.sigmoid ? fmaf((float)size, (5.6f + 2.f * fmaxf(below, 0.f)) * 1.1920928955078125e-7f, 2.3509887e-38f) : size * (F)7.62939453125e-6;
-            size += Tm::most(most) * (F)1.4901161193847656e-7;
         }
     }
+    // Two keys that differ by more than this are in the right order (of infinities: that differ).
+    auto apart = [&](float a, float b) { return fmaf(fminf(fmaxf(fabsf(a), fabsf(b)), 3.402823466e38f), 1.4901161193847656e-7f, (float)size); };
     U key[VPT];
 #pragma unroll
     for (int i = 0; i < VPT; ++i) {
@@ -295,6 +294,7 @@ __device__ __forceinline__ bool route_choose(const RouteParams& p, const T* row,
     if (p.groups > 1) {
         U* vals = reinterpret_cast<U*>(s.value);
         U* group = reinterpret_cast<U*>(s.group);
+        float* off = reinterpret_cast<float*>(group + p.groups);  // (in fp32, whose keys leave half of the place)
         const int S = p.E / p.groups;
         auto join = [](U v, U& a, U& b) {  // the largest and the second
             b = v > a ? a : v > b ? v : b;
@@ -315,24 +315,29 @@ __device__ __forceinline__ bool route_choose(const RouteParams& p, const T* row,
             a = b = 0;
             for (int i = 0; i < per; ++i) join(vals[whole ? g * per + i : route_slot(g * per + i)], a, b);
             group[g] = p.top2 ? ordered(number(a) + number(b)) : a;
+            if (CHECK && scores) {  // what it may be off by: its two keys, and their sum
+                const float x = number((uint32_t)a), y = p.top2 ? number((uint32_t)b) : 0.f;
+                off[g] = (p.top2 ? 1.f : 0.5f) * (float)size + (fabsf(x) + fabsf(y) + (p.top2 ? fabsf(x + y) : 0.f)) * 5.9604708e-8f;
+            }
         }
         Tm::sync();
-        F last = INFINITY, next = -INFINITY;  // the least kept group and the most one left out
+        float last = INFINITY, next = -INFINITY;  // the least that a kept group may be, the most that one left out may be
         for (int g = lane; g < p.groups; g += LANES) {
             const U v = group[g];
             int before = 0;
             for (int h = 0; h < p.groups; ++h) before += group[h] > v || (group[h] == v && h < g);
             s.kept[g] = before < p.kept;
-            if (CHECK) {
-                if (before < p.kept) last = number(v) < last ? number(v) : last;
-                else next = number(v) > next ? number(v) : next;
+            if (CHECK && scores) {  // (an infinite sum is off by infinity: no doubt where closed groups, -inf, are left out)
+                const float x = number((uint32_t)v);
+                if (before < p.kept) last = fminf(last, __fsub_rd(x, off[g]));
+                else next = fmaxf(next, __fadd_ru(x, off[g]));
             }
         }
         Tm::sync();
         if (CHECK && scores) {
             last = Tm::least(last);
             next = Tm::most(next);
-            unsure = next > -INFINITY && last - next <= 2 * size;
+            unsure = next > -INFINITY && last <= next;
         }
         int g = e0 / S, r = e0 - g * S;
         if (whole) {
@@ -361,7 +366,7 @@ __device__ __forceinline__ bool route_choose(const RouteParams& p, const T* row,
         if (best == bound) { best = second; second = 0; }
         if (LANES <= 32 && j >= 2 * LANES) break;  // (none left)
     }
-    if (CHECK && computed && bound != 0) bound = ordered(number(bound) - size);  // what may belong to them in 64 bits, too
+    if (CHECK && computed && bound != 0) bound = ordered(number(bound) - apart(number(bound), 0.f));  // what may belong to them in 64 bits, too
     if (bound == 0) bound = 1;
     int reach = 0, all;
 #pragma unroll
@@ -380,7 +385,7 @@ __device__ __forceinline__ bool route_choose(const RouteParams& p, const T* row,
         bool doubt = false;
         for (int c = lane; c < all; c += LANES) {  // each against the choice before it, or the last one
             const int rank = s.value_at[c] >> 16, at = s.value_at[c] & 0xffff, prev = min(rank, p.k) - 1;
-            if (prev >= 0) doubt |= s.key[prev] - number(keys[c]) <= size && !same(s.at[prev], at);
+            if (prev >= 0) doubt |= s.key[prev] - number(keys[c]) <= apart(s.key[prev], number(keys[c])) && !same(s.at[prev], at);
         }
         if (Tm::any(doubt)) route_settle<T, LANES, VPT>(p, all, row, l, s);
     }

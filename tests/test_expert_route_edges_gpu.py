@@ -3,6 +3,7 @@ of test_expert_route_gpu.py."""
 import pytest
 import torch
 
+import efficient_linear_assignment_b200 as ela
 from test_expert_route_gpu import check, gen
 
 pytestmark = pytest.mark.gpu
@@ -66,3 +67,59 @@ def test_sigmoids_below_the_normal_numbers():
         check(l, 6, "sigmoid", bias)
         check(l, 6, "sigmoid", bias, 4, 2, "top2")
     check(l, 6, "sigmoid", None, 4, 2, "top2")
+
+
+def logits_and_masks(T, E, seed, value):
+    """Usual logits and biases, a fifth of the experts closed by a large negative number."""
+    g = gen(seed)
+    bias = torch.randn(E, generator=g) * 0.1
+    bias[::5] = value
+    return torch.randn(T, E, generator=g) * 1.5, bias
+
+
+@pytest.mark.parametrize("value", [-30.0, -1e4, -1e9, torch.finfo(torch.float32).min])
+@pytest.mark.parametrize("score", ["softmax", "sigmoid"])
+def test_masks_that_are_finite(value, score):
+    """Experts closed by a finite bias: last in the order, and the others' order that of 64 bits."""
+    for T, E, k, groups, kept in ((60, 256, 8, 8, 4), (60, 40, 6, 5, 2), (12, 1000, 8, 1, 1), (60, 20, 20, 1, 1)):
+        l, bias = logits_and_masks(T, E, E, value)
+        for by in ("max", "top2"):
+            got = check(l, k, score, bias, groups, kept, by)
+            assert k == E or (got.expert % 5 != 0).all()
+    # close keys beside a mask
+    l, bias = torch.randn(200, 12, generator=gen(2)), torch.zeros(12)
+    bias[0], bias[2] = value, 0.01
+    l[:, 2] = logit((torch.special.expit(l[:, 1].double()) - bias[2].double()).clamp(1e-3, 1)).float()
+    s = torch.special.expit(l.double()) + bias.double()
+    row = told_apart(s[:, 1:2], s[:, 2:3])
+    check(l[row], 4, "sigmoid", bias)
+    check(l[row], 3, "sigmoid", bias, 4, 2, "max")
+
+
+def time_of(call, passes=10):
+    for _ in range(3):
+        call()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        for _ in range(passes):
+            call()
+    times = []
+    for _ in range(5):
+        a, b = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+        a.record()
+        graph.replay()
+        b.record()
+        b.synchronize()
+        times.append(a.elapsed_time(b))
+    return min(times)
+
+
+@pytest.mark.parametrize("T,E,groups,kept", [(8192, 256, 8, 4), (8192, 256, 1, 1), (1024, 4096, 1, 1)])
+@pytest.mark.parametrize("score", ["softmax", "sigmoid"])
+def test_a_finite_mask_costs_what_others_do(T, E, groups, kept, score):
+    """(The same takes as long; where every key was in doubt it took 7 to 300 times as long.)"""
+    times = []
+    for value in (0.0, -1e9):
+        l, bias = (v.cuda() for v in logits_and_masks(T, E, 5, value))
+        times.append(time_of(lambda: ela.expert_route(l, 8, score, bias, groups, kept, "top2" if groups > 1 else "max")))
+    assert times[1] < 3 * times[0], times
