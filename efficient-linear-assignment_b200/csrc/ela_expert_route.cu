@@ -314,7 +314,10 @@ __device__ __forceinline__ bool route_choose(const RouteParams& p, const T* row,
         for (int g = lane; g < p.groups; g += LANES) {
             a = b = 0;
             for (int i = 0; i < per; ++i) join(vals[whole ? g * per + i : route_slot(g * per + i)], a, b);
-            group[g] = p.top2 ? ordered(number(a) + number(b)) : a;
+            auto sum = number(a) + number(b);
+            if (CHECK && p.top2 && fabsf(sum) == INFINITY && fabsf(number((uint32_t)a)) < INFINITY && fabsf(number((uint32_t)b)) < INFINITY)
+                sum = sum > 0 ? 3.402823466e38f : -3.402823466e38f;  // (no infinity in 64 bits: in order with those, in doubt with its like)
+            group[g] = p.top2 ? ordered(sum) : a;
             if (CHECK && scores) {  // what it may be off by: its two keys, and their sum
                 const float x = number((uint32_t)a), y = p.top2 ? number((uint32_t)b) : 0.f;
                 off[g] = (p.top2 ? 1.f : 0.5f) * (float)size + (fabsf(x) + fabsf(y) + (p.top2 ? fabsf(x + y) : 0.f)) * 5.9604708e-8f;

@@ -123,3 +123,15 @@ def test_a_finite_mask_costs_what_others_do(T, E, groups, kept, score):
         l, bias = (v.cuda() for v in logits_and_masks(T, E, 5, value))
         times.append(time_of(lambda: ela.expert_route(l, 8, score, bias, groups, kept, "top2" if groups > 1 else "max")))
     assert times[1] < 3 * times[0], times
+
+
+def test_sums_of_groups_past_fp32s_range():
+    """Two biases whose sum is an infinity in fp32: in order among themselves, and not as closed groups are."""
+    inf, big = float("inf"), 3e38
+    l = torch.randn(6, 16, generator=gen(4))
+    for bias in ([2e38, 2e38, 0, 0, 3e38, 2e38, 0, 0, 2.5e38, 2e38, 0, 0, 0, 0, 0, 0], [-big] * 4 + [-2.9e38] * 4 + [-2.8e38] * 4 + [-3.1e38] * 4,
+                 [0, -inf, -inf, -inf] + [-big] * 4 + [-inf] * 4 + [-2.9e38] * 4, [big, -big, 0, 0] * 2 + [-big, -big, big, 1] * 2,
+                 [-inf] * 4 + [1, -inf, -inf, -inf] + [-big] * 4 + [-inf] * 4):
+        for score in ("softmax", "sigmoid"):
+            for kept in (1, 2, 3):
+                check(l, 2, score, torch.tensor(bias), 4, kept, "top2")
