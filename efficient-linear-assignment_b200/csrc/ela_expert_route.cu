@@ -178,6 +178,75 @@ __device__ __forceinline__ double exp_of(double x) { return exp(x); }
 __device__ __forceinline__ float one_over(float x) { return reciprocal_fast(x); }
 __device__ __forceinline__ double one_over(double x) { return 1 / x; }
 
+// Two keys that differ by more than this are in the right order (of infinities: that differ); size: what their
+// scores may be off by together.
+__device__ __forceinline__ float apart(float size, float a, float b) {
+    return fmaf(fminf(fmaxf(fabsf(a), fabsf(b)), 3.402823466e38f), 1.4901161193847656e-7f, size);
+}
+// A bound that also those keys reach that may do so in 64 bits.
+__device__ __forceinline__ uint32_t lowered(uint32_t bound, float size) { return ordered(number(bound) - apart(size, number(bound), 0.f)); }
+
+// Many keys reach the bound, as in a row of zeros: equal ones, which left the threads' two largest together
+// and lowered the bound, perhaps to nothing.  Here they are counted as they leave, and of those
+// that equal the first one at the bound in any arithmetic the first k alone stay in the list.  (Kept out of the
+// kernel's registers.)  8192 x 256 zeros with a bias 31 us, 192 by the ranks of all; 1024 x 4096 zeros 85 and 5530.
+template <typename F, typename T, int LANES>
+__device__ __noinline__ int route_thin(const RouteParams& p, int all, const T* row, float size, const RouteShared& s) {
+    typedef Team<LANES> Tm;
+    typedef typename Ordered<F>::U U;
+    U* keys = reinterpret_cast<U*>(s.value);
+    const int lane = Tm::lane();
+    Tm::sync();
+    U best = 0, second = 0, bound = 0;
+    for (int c = lane; c < all; c += LANES) {
+        const U v = keys[c];
+        second = v > best ? best : v > second ? v : second;
+        best = v > best ? v : best;
+    }
+    for (int taken = 0;;) {
+        const U most = Tm::most(best);
+        const bool open = taken < p.k && most != 0;
+        if (!Tm::any(open)) break;
+        if (open) bound = most;
+        const bool leaves = open && best == bound;
+        taken += Tm::sum((int)leaves);
+        if (leaves) { best = second; second = 0; }
+    }
+    U low = bound != 0 ? bound : 1;
+    bool by_key = true;  // equal keys are equal in any arithmetic
+    if constexpr (sizeof(F) == 4) {
+        if (p.bias && bound != 0) low = lowered(bound, size);
+        by_key = !p.bias || !(fabsf(number(bound)) < INFINITY);
+    }
+    int first = INT32_MAX;
+    for (int c = lane; c < all; c += LANES)
+        if (keys[c] == bound) { first = s.value_at[c]; break; }
+    first = Tm::least(first);  // (INT32_MAX: there are no keys)
+    float logit = 0.f, bias = 0.f;
+    if (first != INT32_MAX) {
+        logit = El<T>::to(row[first]);
+        if (p.bias) bias = p.bias[first];
+    }
+    int twins = 0, kept = 0, some;
+    for (int c = lane; Tm::any(c - lane < all); c += LANES) {
+        const U v = c < all ? keys[c] : 0;
+        const int at = c < all ? s.value_at[c] : 0;
+        const bool twin = c < all && v == bound && (by_key || (El<T>::to(row[at]) == logit && p.bias[at] == bias));
+        const int rank = twins + Tm::before(twin, some);
+        twins += some;
+        const bool stays = c < all && v >= low && !(twin && rank >= p.k);
+        const int to = kept + Tm::before(stays, some);
+        kept += some;
+        Tm::sync();
+        if (stays) {
+            keys[to] = v;
+            s.value_at[to] = at;
+        }
+        Tm::sync();
+    }
+    return kept;
+}
+
 // The ranks of the `all` keys in s.value (into the upper half of their s.value_at), and the k
 // experts of the first ranks with their logits and (fp32) keys.
 template <typename F, typename T, int LANES>
@@ -281,8 +350,6 @@ __device__ __forceinline__ bool route_choose(const RouteParams& p, const T* row,
             size = p.sigmoid ? fmaf((float)size, (5.6f + 2.f * fmaxf(below, 0.f)) * 1.1920928955078125e-7f, 2.3509887e-38f) : size * (F)7.62939453125e-6;
         }
     }
-    // Two keys that differ by more than this are in the right order (of infinities: that differ).
-    auto apart = [&](float a, float b) { return fmaf(fminf(fmaxf(fabsf(a), fabsf(b)), 3.402823466e38f), 1.4901161193847656e-7f, (float)size); };
     U key[VPT];
 #pragma unroll
     for (int i = 0; i < VPT; ++i) {
@@ -369,7 +436,7 @@ __device__ __forceinline__ bool route_choose(const RouteParams& p, const T* row,
         if (best == bound) { best = second; second = 0; }
         if (LANES <= 32 && j >= 2 * LANES) break;  // (none left)
     }
-    if (CHECK && computed && bound != 0) bound = ordered(number(bound) - apart(number(bound), 0.f));  // what may belong to them in 64 bits, too
+    if (CHECK && computed && bound != 0) bound = lowered(bound, (float)size);
     if (bound == 0) bound = 1;
     int reach = 0, all;
 #pragma unroll
@@ -382,13 +449,15 @@ __device__ __forceinline__ bool route_choose(const RouteParams& p, const T* row,
             keys[to] = key[i];
             s.value_at[to++] = e0 + i;
         }
+    constexpr int MANY = LANES < 16 ? 4 * LANES : 64;
+    if (Tm::any(all > MANY + 2 * p.k)) all = route_thin<F, T, LANES>(p, all, row, (float)size, s);
     route_ranks<F, T, LANES>(p.k, all, row, s);
     if (CHECK && computed) {
         auto same = [&](int a, int b) { return El<T>::to(row[a]) == El<T>::to(row[b]) && p.bias[a] == p.bias[b]; };  // equal keys in any arithmetic
         bool doubt = false;
         for (int c = lane; c < all; c += LANES) {  // each against the choice before it, or the last one
             const int rank = s.value_at[c] >> 16, at = s.value_at[c] & 0xffff, prev = min(rank, p.k) - 1;
-            if (prev >= 0) doubt |= s.key[prev] - number(keys[c]) <= apart(s.key[prev], number(keys[c])) && !same(s.at[prev], at);
+            if (prev >= 0) doubt |= s.key[prev] - number(keys[c]) <= apart((float)size, s.key[prev], number(keys[c])) && !same(s.at[prev], at);
         }
         if (Tm::any(doubt)) route_settle<T, LANES, VPT>(p, all, row, l, s);
     }
