@@ -578,7 +578,9 @@ __device__ __forceinline__ void load_columns(const MmaParams4& p, const CUtensor
     }
 }
 
-// One warp: the blocks of this CTA's features, in the order of the stages.
+// One warp: the blocks of this CTA's features, in the order of the stages.  It waits for the last
+// ones itself, so that none is in flight when the CTA leaves, also where a wait gave up and
+// nobody else will wait for them.
 template <typename Fetch, typename GiveUp>
 __device__ __forceinline__ void load_words(const MmaParams4& p, const CUtensorMap& map, uint32_t ring, uint64_t* pfull, uint64_t* pempty, int rank,
                                            Fetch fetch, GiveUp give_up, const volatile int* abort) {
@@ -602,6 +604,12 @@ __device__ __forceinline__ void load_words(const MmaParams4& p, const CUtensorMa
         }
         s.share(ok);
     }
+    if (elect_one()) {
+        int never = 0;
+        for (int j = 0; j < p.ring; ++j)  // the last load of each slot (one without any is in its first phase, which tells the same)
+            bar_wait(&pfull[j], s.phase ^ (j >= s.at), p.wait_ns, &never);
+    }
+    __syncwarp();
 }
 
 // One warp of the first CTA: the products of the pair.
@@ -1104,8 +1112,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(mma_threads<PASS>(),
             mma_commit(&drained);
             bar_wait(&drained, 0, p.wait_ns, &never);
         }
-        // the other CTA's loads count on barriers that it cannot wait for (nor can either where weights
-        // that nobody will unpack are waited for, too)
+        // the other CTA's loads count on barriers that it cannot wait for (with 4 bits neither CTA's columns
+        // can be waited for: their barriers wait for weights that nobody will unpack)
         if (tid == 0) {
             unsigned long long t0, t1;
             asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t0));
