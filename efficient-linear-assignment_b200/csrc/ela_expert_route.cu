@@ -338,8 +338,8 @@ __device__ __forceinline__ bool route_choose(const RouteParams& p, const T* row,
         // which moves the sigmoid by 1 - s of that, and the sum and the reciprocal move it by 3 * 2^-24.  For
         // x >= 0 that makes 3.4 * 2^-24, 5 * 2^-24 of the row's largest score S at most; below 0, where both the
         // score and its error grow with x, (1.5 |x| (1 - S) + 4 (1 - S) + 3) 2^-24 of S for the largest x.  Where S lies
-        // in [2^e, 2^(e+1)), |x| is at most -0.7 e, and (5.6 + 2 (-1 - e)) 2^-24 is more for every e.  A score below
-        // 2^-126 comes out as 0.  A softmax is off by 2^-22 of the largest for its exponential, and by the row's
+        // in [2^e, 2^(e+1)), |x| is at most -0.7 e, and (5.6 + 2 (-1 - e)) 2^-24 of S is more for every e; it never
+        // passes 3.4 * 2^-24.  A score below 2^-126 comes out as 0.  A softmax is off by 2^-22 of the largest for its exponential, and by the row's
         // sum, at most 29 additions one after the other of such terms, 2^-19; two of them by 2^-17.  A sum with
         // the bias is off by another 2^-24 of itself, which is allowed for key by key: one bias of -1e9
         // for an expert that is out of the question leaves the others their digits (by the row's largest
@@ -347,7 +347,7 @@ __device__ __forceinline__ bool route_choose(const RouteParams& p, const T* row,
         if (CHECK) {
             size = Tm::most(size);
             const float below = (float)(126 - (int)(__float_as_uint((float)size) >> 23));  // -1 - e
-            size = p.sigmoid ? fmaf((float)size, (5.6f + 2.f * fmaxf(below, 0.f)) * 1.1920928955078125e-7f, 2.3509887e-38f) : size * (F)7.62939453125e-6;
+            size = p.sigmoid ? fmaf(fminf((float)size * (5.6f + 2.f * fmaxf(below, 0.f)), 3.45f), 1.1920928955078125e-7f, 2.3509887e-38f) : size * (F)7.62939453125e-6;
         }
     }
     U key[VPT];
