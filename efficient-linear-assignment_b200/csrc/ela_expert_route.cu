@@ -189,7 +189,7 @@ __device__ __forceinline__ uint32_t lowered(uint32_t bound, float size) { return
 // Many keys reach the bound, as in a row of zeros: equal ones, which left the threads' two largest together
 // and lowered the bound, perhaps to nothing.  Here they are counted as they leave, and of those
 // that equal the first one at the bound in any arithmetic the first k alone stay in the list.  (Kept out of the
-// kernel's registers.)  8192 x 256 zeros with a bias 31 us, 192 by the ranks of all; 1024 x 4096 zeros 85 and 5530.
+// kernel's registers, and of rows of up to 16 experts, whose keys rank as fast.)  8192 x 256 zeros with a bias 31 us, 192 by the ranks of all; 1024 x 4096 zeros 85 and 5530.
 template <typename F, typename T, int LANES>
 __device__ __noinline__ int route_thin(const RouteParams& p, int all, const T* row, float size, const RouteShared& s) {
     typedef Team<LANES> Tm;
@@ -450,7 +450,7 @@ __device__ __forceinline__ bool route_choose(const RouteParams& p, const T* row,
             s.value_at[to++] = e0 + i;
         }
     constexpr int MANY = LANES < 16 ? 4 * LANES : 64;
-    if (Tm::any(all > MANY + 2 * p.k)) all = route_thin<F, T, LANES>(p, all, row, (float)size, s);
+    if (LANES >= 4 && Tm::any(all > MANY + 2 * p.k)) all = route_thin<F, T, LANES>(p, all, row, (float)size, s);
     route_ranks<F, T, LANES>(p.k, all, row, s);
     if (CHECK && computed) {
         auto same = [&](int a, int b) { return El<T>::to(row[a]) == El<T>::to(row[b]) && p.bias[a] == p.bias[b]; };  // equal keys in any arithmetic
