@@ -154,8 +154,9 @@ template <int ACT> __device__ __forceinline__ float act_slope(float z) {
 }
 
 // The same values in fewer instructions, for kernels whose warps have no issue slots to spare:
-// relu(z) - |z| tail(|z|) for GELU, and the approximate exponential and reciprocal as they are
-// (results below 2^-126 come out as 0).
+// relu(z) - |z| tail(|z|) for GELU, and the approximate exponential and reciprocal as they are (a
+// tail or a sigmoid below 2^-126 comes out as 0, and with it a result below |z| 2^-126: SiLU's from z = -87.4
+// on, 2^-119.5 and less in magnitude).
 __device__ __forceinline__ float exp2_fast(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
