@@ -8,7 +8,7 @@
 //
 //   pass           f (TMEM lanes)         c (MMA N)            k
 //   forward        output feature n       row of the expert    input feature
-//   4 bits         the same, the weights unpacked by eight warps instead of loaded by TMA
+//   4 bits         the same, the weights' words loaded by TMA into a ring and unpacked by twelve warps
 //   input grad     input feature          row of the expert    output feature
 //   weight grad    input feature          output feature       row of the expert
 //
