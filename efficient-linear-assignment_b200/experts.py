@@ -145,7 +145,9 @@ def expert_route(logits: torch.Tensor, k: int, score: str = "softmax", bias: Opt
     best ("top2").  The weights are the chosen scores, divided by their sum with
     ``renormalize``, times ``scale``.  Ties go to the lowest index, NaN counts as the
     largest, and the order is that of 64-bit arithmetic.  An expert whose logit (or bias)
-    is -inf is never chosen: a token without enough of them gets expert -1, weight 0.
+    is -inf is never chosen: a token without enough others in the groups that stay gets expert -1,
+    weight 0.  By "top2" a group with one open expert ranks with the closed ones, after every
+    group with two, so that its expert may be left out.
     fp32, fp16 or bf16; k up to 64.  Backward: the gradient of the logits."""
     code, by = SCORES.get(score), GROUP_SCORES.get(group_score)
     if code is None:

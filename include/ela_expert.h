@@ -143,7 +143,9 @@ enum { ELA_GROUP_MAX = 0, ELA_GROUP_TOP2 = 1 };
  *   expert int32[T*k]: the experts of the k largest keys, the largest first; weights
  *   float[T*k]: scale * s_e, or scale * s_e / (sum of the chosen s) with `renormalize`
  * Equal keys and groups go to the lowest index, NaN counts as the largest.  An expert whose
- * logit (or bias) is -inf is never chosen: where none is left, the choice is -1 with weight 0.
+ * logit (or bias) is -inf is never chosen: where none is left in the groups that stay, the choice is -1
+ * with weight 0.  By the sum of two, a group with one open expert ranks with the closed ones (-inf, by
+ * index), after every group with two: its expert may be left out though it is open.
  * The order is that of the keys in 64-bit arithmetic.  1 <= E <= ELA_EXPERT_MAX, k at most
  * ELA_ROUTE_MAX_K and groups_kept * E / groups, T * k < 2^31.
  */

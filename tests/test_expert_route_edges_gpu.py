@@ -180,3 +180,16 @@ def test_equal_keys_cost_what_others_do(T, E, groups, kept, biased):
         l = (torch.randn(T, E, generator=gen(5)) * spread).cuda()
         times.append(time_of(lambda: ela.expert_route(l, 8, "sigmoid", torch.zeros(E, device="cuda") if biased else None, groups, kept, "top2" if groups > 1 else "max")))
     assert times[1] < 6 * times[0], times
+
+
+@pytest.mark.parametrize("score", ["softmax", "sigmoid"])
+def test_groups_with_one_open_expert(score):
+    """By the sum of two such a group ranks with the closed ones, by index, and after every group with two."""
+    no = -float("inf")
+    l = torch.tensor([[no, no, 5.0, no, no, no], [no, no, 5.0, no, -3.0, -4.0], [5.0, no, 1.0, no, 2.0, no], [no, no, no, no, no, 1.0]])
+    for bias in (None, torch.zeros(6)):
+        top2 = check(l, 2, score, bias, 3, 1, "top2").expert.tolist()
+        assert top2 == [[-1, -1], [4, 5], [0, -1], [-1, -1]]
+        most = check(l, 2, score, bias, 3, 1, "max").expert.tolist()
+        assert most == [[2, -1], [2, -1], [0, -1], [5, -1]]
+        assert check(l, 2, score, bias, 3, 2, "top2").expert.tolist() == [[2, -1], [4, 5], [0, 2], [-1, -1]]
