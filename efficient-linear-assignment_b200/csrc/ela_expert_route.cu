@@ -198,12 +198,13 @@ __device__ __noinline__ int route_thin(const RouteParams& p, int all, const T* r
     const int lane = Tm::lane();
     Tm::sync();
     U best = 0, second = 0, bound = 0;
+    int taken = 0;
     for (int c = lane; c < all; c += LANES) {
         const U v = keys[c];
         second = v > best ? best : v > second ? v : second;
         best = v > best ? v : best;
     }
-    for (int taken = 0;;) {
+    while (true) {
         const U most = Tm::most(best);
         const bool open = taken < p.k && most != 0;
         if (!Tm::any(open)) break;
@@ -212,10 +213,11 @@ __device__ __noinline__ int route_thin(const RouteParams& p, int all, const T* r
         taken += Tm::sum((int)leaves);
         if (leaves) { best = second; second = 0; }
     }
-    U low = bound != 0 ? bound : 1;
+    const bool enough = taken >= p.k;  // (else the threads' two largest are fewer than k, and no bound: all stay but the surplus of the last one's equals)
+    U low = enough ? bound : 1;
     bool by_key = true;  // equal keys are equal in any arithmetic
     if constexpr (sizeof(F) == 4) {
-        if (p.bias && bound != 0) low = lowered(bound, size);
+        if (p.bias && enough) low = lowered(bound, size);
         by_key = !p.bias || !(fabsf(number(bound)) < INFINITY);
     }
     int first = INT32_MAX;

@@ -193,3 +193,19 @@ def test_groups_with_one_open_expert(score):
         most = check(l, 2, score, bias, 3, 1, "max").expert.tolist()
         assert most == [[2, -1], [2, -1], [0, -1], [5, -1]]
         assert check(l, 2, score, bias, 3, 2, "top2").expert.tolist() == [[2, -1], [4, 5], [0, 2], [-1, -1]]
+
+
+@pytest.mark.parametrize("E", [30, 64, 100, 193, 200, 230, 256, 320, 512])
+@pytest.mark.parametrize("k", [9, 17, 33, 40, 64])
+@pytest.mark.parametrize("score", ["softmax", "sigmoid"])
+def test_many_choices(E, k, score):
+    """More choices than a row's threads have largest keys, two each: usual rows, and rows with many equal keys."""
+    k = min(k, E)
+    g = gen(E + k)
+    l = torch.randn(20, E, generator=g) * 1.5
+    l[10:] = l[10:].round()
+    l[18], l[19] = 0.0, (torch.arange(E) % 2).float()
+    for bias in (None, torch.zeros(E), torch.randn(E, generator=g) * 0.1):
+        check(l, k, score, bias)
+        if E % 2 == 0 and k <= E // 2:
+            check(l, k, score, bias, 2, 1, "top2")
