@@ -326,10 +326,17 @@ std::tuple<Tensor, Tensor> route_raw(const Tensor& logits_in, int64_t k, int64_t
     return {expert, weights};
 }
 
-Tensor route_grad_raw(const Tensor& dweights_in, const Tensor& logits_in, const Tensor& expert, int64_t score, bool renormalize,
+Tensor route_grad_raw(const Tensor& dweights_in, const Tensor& logits_in, const Tensor& expert_in, int64_t score, bool renormalize,
                       double scale) {
+    // (reached through the gradient with what route made, but also by its name)
+    const char* name = "expert_route_grad";
+    TORCH_CHECK_TYPE(code_of(logits_in) >= 0 && expert_in.scalar_type() == at::kInt && dweights_in.scalar_type() == at::kFloat, name,
+                     ": logits as in expert_route, expert int32, dweights float32");
+    TORCH_CHECK_VALUE(logits_in.dim() == 2 && expert_in.dim() == 2 && expert_in.size(0) == logits_in.size(0) && dweights_in.sizes() == expert_in.sizes() &&
+                          expert_in.device() == logits_in.device() && dweights_in.device() == logits_in.device(),
+                      name, ": logits (T, E), expert and dweights (T, k) on one device");
     c10::cuda::CUDAGuard guard(logits_in.device());
-    const Tensor logits = rows_of(logits_in), dweights = dweights_in.contiguous();
+    const Tensor logits = rows_of(logits_in), dweights = dweights_in.contiguous(), expert = expert_in.contiguous();
     Tensor dlogits = fresh(logits.sizes(), logits);
     check_rc(ela_expert_route_grad(logits.data_ptr(), code_of(logits), logits.size(0), logits.size(1), ld(logits), expert.size(1),
                                    (int)score, renormalize, (float)scale, expert.data_ptr<int32_t>(), dweights.data_ptr<float>(),

@@ -209,3 +209,18 @@ def test_many_choices(E, k, score):
         check(l, k, score, bias)
         if E % 2 == 0 and k <= E // 2:
             check(l, k, score, bias, 2, 1, "top2")
+
+
+def test_the_gradient_operator_checks_its_arguments():
+    l, dw = torch.zeros(5, 8, device="cuda"), torch.ones(5, 3, device="cuda")
+    expert = ela.expert_route(l, 3).expert
+    grad = torch.ops.ela_native.expert_route_grad
+    want = grad(dw, l, expert, 0, False, 1.0)
+    assert torch.equal(grad(dw.t().contiguous().t(), l, expert.t().contiguous().t(), 0, False, 1.0), want)
+    for bad in ((dw[:4], l, expert), (dw, l, expert[:4]), (dw[:, :2], l, expert), (dw, l[:4], expert), (dw, l[0], expert), (dw[0], l, expert[0]),
+                (dw.cpu(), l, expert), (dw, l, expert.cpu())):
+        with pytest.raises(ValueError):
+            grad(*bad, 0, False, 1.0)
+    for bad in ((dw.double(), l, expert), (dw, l, expert.long()), (dw, l.double(), expert)):
+        with pytest.raises(TypeError):
+            grad(*bad, 0, False, 1.0)
