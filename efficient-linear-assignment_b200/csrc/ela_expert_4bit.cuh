@@ -262,7 +262,10 @@ template <typename T, int RG, int MT, int SUB> int stream4_launch(Stream4Params 
 // 34.5; 12 rows 37.3 and 34.6, 16 rows 26.6 and 22.4, 40.5 and 34.0.  Where tiles of 256 features
 // leave half of the pairs idle, up to 24: 4096 x 4096 alone with 16 rows 8.8 and 18.6, with 32 15.6
 // and 18.8, with 48 22.4 and 19.8; two of 2048 x 2048 with 16 rows each 8.9 and 13.1, with 32 15.6
-// and 13.3.
+// and 13.3.  The loads, which only the device knows, are taken to be equal.  Others cost here what the
+// busiest expert does, whose weights are read again for each 8 rows: 128 rows of 16 experts of 4096 x 1024 take 18.8
+// us, 102 with half of them on one expert and 181 with all, 1024 rows of 128 of 1024 x 512 24, 511 and 1130; by
+// tiles (136 and 1032 rows) 22.4, 22.5 and 13.8, and 24.5, 26.7 and 12.3.
 inline bool few_rows_4bit(int64_t R, int64_t E, int64_t N) { return R <= 8 * E || (R <= 24 * E && E * ((N + 255) / 256) <= sm_count() / 4); }
 
 // Eight tokens from one read of the weights, or sixteen.  Items of 16 features a warp where 32
