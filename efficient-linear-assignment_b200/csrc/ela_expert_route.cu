@@ -178,8 +178,9 @@ __device__ __forceinline__ double exp_of(double x) { return exp(x); }
 __device__ __forceinline__ float one_over(float x) { return reciprocal_fast(x); }
 __device__ __forceinline__ double one_over(double x) { return 1 / x; }
 
-// Two keys that differ by more than this are in the right order (of infinities: that differ); size: what their
-// scores may be off by together.
+// Two keys that differ by more than this are in the right order (of infinities: that differ).  size: what their
+// scores may be off by together; each sum with a bias is off by 2^-24 of itself, and half a step more is for the
+// arithmetic here.
 __device__ __forceinline__ float apart(float size, float a, float b) {
     return fmaf(fminf(fmaxf(fabsf(a), fabsf(b)), 3.402823466e38f), 1.4901161193847656e-7f, size);
 }
